@@ -28,6 +28,16 @@ DX_NOALLOC_SCRATCH_BYTES = 64 << 20
 _p = c_void_p
 _i32p = POINTER(c_int32)
 
+
+class Kv4Cache(ctypes.Structure):
+    """`dx_kv4_cache`."""
+
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("positions", _p), ("num_pages", c_int32),
+                ("num_kv_heads", c_int32), ("page_size", c_int32), ("head_dim", c_int32)]
+
+
+_cachep = POINTER(Kv4Cache)
+
 # Argument types of every entry point, in header order.
 SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "dx_version": (c_char_p, []),
@@ -113,6 +123,30 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     ),
     "dx_head_combine_f32": (c_int, [_p, _p, _p, _p, _p, c_int64, c_float, c_float, _p]),
     "dx_head_combine_scaled_f32": (c_int, [_p, _p, _p, _p, _p, _p, _p, _p, c_int64, _p]),
+    "dx_kv4_append": (
+        c_int,
+        [_cachep, _p, _p, _p, _p, c_int32, _p, _p, _p, c_int32, c_int32, c_int64, c_int64, c_int64, c_int32, _p],
+    ),
+    "dx_kv4_read": (
+        c_int, [_cachep, _p, _p, _p, c_int32, _p, _p, _p, c_int32, c_int32, c_int64, c_int64, c_int64, _p]),
+    "dx_attn_kv4": (
+        c_int,
+        [_cachep, _p, _p, _p, c_int32, _p, _p, _p, c_int32, c_int32, c_int32, c_int64, c_int32, c_int64, c_int64,
+         c_float, c_float, c_int32, _p, c_int64, c_int64, _p, c_int64, c_int64, c_int32, _p, c_int64, _p],
+    ),
+    "dx_attn_kv4_workspace": (
+        c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "dx_kv4_evict": (
+        c_int,
+        [_cachep, _p, c_int64, c_int64, _p, c_int32, _p, c_int32, c_int32, _p, c_int32, c_int32, c_int32, _p, c_int64,
+         c_int64, _p, _p, c_int64, _p],
+    ),
+    "dx_kv4_evict_workspace": (c_int64, [c_int32, c_int32, c_int32]),
+    "dx_token_logprobs": (
+        c_int,
+        [_p, _p, c_int64, c_int32, c_int64, c_float, c_int32, _p, _p, _p, _p, c_int32, _p, c_int64, _p],
+    ),
+    "dx_token_logprobs_workspace": (c_int64, [c_int64, c_int32, c_int32]),
 }
 
 _LIB: ctypes.CDLL | None = None

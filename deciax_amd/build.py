@@ -19,7 +19,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libdeciax_hip.so"
-SOURCES = ("abi.hip", "gemm.hip", "attention.hip", "rowwise.hip", "head.hip")
+SOURCES = ("abi.hip", "gemm.hip", "attention.hip", "rowwise.hip", "head.hip", "kv4_cache.hip",
+           "kv4_attention.hip", "logprobs.hip")
 ARCH = "gfx950"
 
 # Packed-fp32 VALU forms stay disabled in every device compile.

@@ -765,3 +765,237 @@ int dx_head_combine_scaled_f32(const float *prior, const float *cosine, const fl
                       "head_combine_scaled launch");
 }
 
+// ---------------------------------------------------------------------------- 4-bit cache, answers over it
+
+namespace {
+
+constexpr int32_t MOST_SLOTS = 1 << 30;  // of a sequence: spans of keys are counted in 32 bits
+
+int validate_cache(const dx_kv4_cache *c, Kv4Cache *out, const char *what) {
+  REQUIRE(c && c->k && c->v && c->k_scale && c->v_scale && c->positions, "%s: null cache array", what);
+  REQUIRE(c->num_pages >= 0 && c->num_kv_heads > 0, "%s: %d pages of %d heads", what, c->num_pages, c->num_kv_heads);
+  SUPPORTED(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim %d not in {64, 128, 256}", what,
+            c->head_dim);
+  SUPPORTED(c->page_size >= 64 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0,
+            "%s: page_size %d is no power of two in [64, 65536]", what, c->page_size);
+  SUPPORTED(c->num_kv_heads <= 65535, "%s: %d heads beyond the launch grid", what, c->num_kv_heads);
+  REQUIRE(aligned16(c->k) && aligned16(c->v) && aligned16(c->k_scale) && aligned16(c->v_scale) &&
+              aligned16(c->positions),
+          "%s: cache arrays must be 16-byte aligned", what);
+  int shift = 6;
+  while ((1 << shift) < c->page_size) ++shift;
+  *out = Kv4Cache{static_cast<uint8_t *>(c->k), static_cast<uint8_t *>(c->v), c->k_scale, c->v_scale, c->positions,
+                  c->num_pages, c->num_kv_heads, c->head_dim, shift};
+  return DX_OK;
+}
+
+int validate_batch(const Kv4Batch &q, const char *what) {
+  REQUIRE(q.table && q.seq_start && q.seq_len && q.ctx_len, "%s: null page table or lengths", what);
+  REQUIRE(q.num_seqs >= 0 && q.max_seq_len >= 0 && q.max_ctx >= 0 && q.rows >= 0 && q.table_width >= 0,
+          "%s: negative sequence count, length, rows or table width", what);
+  SUPPORTED(q.num_seqs <= 65535, "%s: %d sequences beyond the launch grid", what, q.num_seqs);
+  SUPPORTED(q.max_ctx <= MOST_SLOTS && q.max_seq_len <= MOST_SLOTS, "%s: sequences of more than 2^30 slots", what);
+  return DX_OK;
+}
+
+// Rows of k and v (append, read), `bytes` an element.
+int validate_kv_rows(const Kv4Cache &c, const Kv4Batch &q, const void *k, const void *v, int64_t ks, int64_t vs,
+                     int bytes, const char *what) {
+  REQUIRE(k && v, "%s: null k or v", what);
+  REQUIRE(aligned16(k) && aligned16(v), "%s: k and v must be 16-byte aligned", what);
+  const int64_t width = (int64_t)c.hkv * c.d;
+  REQUIRE(ks >= width && vs >= width && ks * bytes % 16 == 0 && vs * bytes % 16 == 0,
+          "%s: row strides must cover heads * head_dim and be multiples of %d elements", what, 16 / bytes);
+  SUPPORTED((int64_t)q.max_seq_len * (width / 8) < (INT64_C(1) << 31), "%s: %d tokens of %ld values a sequence", what,
+            q.max_seq_len, (long)width);
+  return DX_OK;
+}
+
+// Where the parts of dx_attn_kv4's workspace start, in bytes: spans' outputs, their statistics, the rows' log sums.
+struct Kv4Workspace {
+  int64_t stats, lse, total;
+};
+
+Kv4Workspace kv4_workspace(const Kv4Plan &p, int64_t units, int32_t d, bool weights) {
+  Kv4Workspace w;
+  w.stats = align_up(units * p.part_rows * d * 4, 256);
+  w.lse = w.stats + align_up(units * p.part_rows * 8, 256);
+  w.total = w.lse + (weights ? units * p.max_rows * 4 : 0);
+  return w;
+}
+
+}  // namespace
+
+int dx_kv4_append(const dx_kv4_cache *cache, const void *k, const void *v, const int32_t *positions,
+                  const int32_t *page_table, int32_t table_width, const int32_t *seq_start, const int32_t *seq_len,
+                  const int32_t *ctx_len, int32_t num_seqs, int32_t max_seq_len, int64_t rows, int64_t k_row_stride,
+                  int64_t v_row_stride, int32_t dtype, void *stream) {
+  Kv4Cache c;
+  const Kv4Batch q{page_table, seq_start, seq_len, ctx_len, table_width, num_seqs, max_seq_len, MOST_SLOTS, rows};
+  int st = validate_cache(cache, &c, "kv4_append");
+  if (!st) st = validate_batch(q, "kv4_append");
+  if (st) return st;
+  REQUIRE(dtype == DX_BF16 || dtype == DX_F32, "kv4_append: unknown dtype %d", dtype);
+  REQUIRE(positions, "kv4_append: null positions");
+  st = validate_kv_rows(c, q, k, v, k_row_stride, v_row_stride, dtype == DX_BF16 ? 2 : 4, "kv4_append");
+  if (st) return st;
+  if (num_seqs == 0 || max_seq_len == 0 || rows == 0) return DX_OK;
+  return check_launch(dx_kv4_append_launch(c, q, k, v, positions, k_row_stride, v_row_stride, dtype == DX_F32,
+                                           as_stream(stream)),
+                      "kv4_append launch");
+}
+
+int dx_kv4_read(const dx_kv4_cache *cache, void *k, void *v, const int32_t *page_table, int32_t table_width,
+                const int32_t *seq_start, const int32_t *seq_len, const int32_t *ctx_len, int32_t num_seqs,
+                int32_t max_seq_len, int64_t rows, int64_t k_row_stride, int64_t v_row_stride, void *stream) {
+  Kv4Cache c;
+  const Kv4Batch q{page_table, seq_start, seq_len, ctx_len, table_width, num_seqs, max_seq_len, MOST_SLOTS, rows};
+  int st = validate_cache(cache, &c, "kv4_read");
+  if (!st) st = validate_batch(q, "kv4_read");
+  if (!st) st = validate_kv_rows(c, q, k, v, k_row_stride, v_row_stride, 2, "kv4_read");
+  if (st) return st;
+  if (num_seqs == 0 || max_seq_len == 0 || rows == 0) return DX_OK;
+  return check_launch(dx_kv4_read_launch(c, q, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v), k_row_stride,
+                                         v_row_stride, as_stream(stream)),
+                      "kv4_read launch");
+}
+
+int64_t dx_attn_kv4_workspace(int32_t num_seqs, int32_t max_seq_len, int32_t max_ctx_len, int32_t num_q_heads,
+                              int32_t num_kv_heads, int32_t head_dim, int32_t window, int32_t with_weights) {
+  if (num_seqs <= 0 || max_seq_len < 0 || max_ctx_len < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || window < 0 ||
+      max_ctx_len > MOST_SLOTS || (int64_t)max_seq_len * (num_q_heads / num_kv_heads) > MOST_SLOTS / 32)
+    return 0;
+  const Kv4Plan p =
+      dx_kv4_attn_plan(max_seq_len, max_ctx_len, num_q_heads / num_kv_heads, in_range(window, max_ctx_len));
+  return kv4_workspace(p, (int64_t)num_seqs * num_kv_heads, head_dim, with_weights != 0).total;
+}
+
+int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32_t *page_table, int32_t table_width,
+                const int32_t *seq_start, const int32_t *seq_len, const int32_t *ctx_len, int32_t num_seqs,
+                int32_t max_seq_len, int32_t max_ctx_len, int64_t rows, int32_t num_q_heads, int64_t q_row_stride,
+                int64_t out_row_stride, float scale, float softcap, int32_t window, const float *weights_in,
+                int64_t weights_in_seq_stride, int64_t weights_in_head_stride, float *weights_out,
+                int64_t weights_out_seq_stride, int64_t weights_out_head_stride, int32_t dtype, void *workspace,
+                int64_t workspace_bytes, void *stream) {
+  Kv4Attn a{};
+  a.q = Kv4Batch{page_table, seq_start, seq_len, ctx_len, table_width, num_seqs, max_seq_len, max_ctx_len, rows};
+  int st = validate_cache(cache, &a.c, "attn_kv4");
+  if (!st) st = validate_batch(a.q, "attn_kv4");
+  if (st) return st;
+  REQUIRE(q && out, "attn_kv4: null q or out");
+  REQUIRE(dtype == DX_BF16 || dtype == DX_F32, "attn_kv4: unknown dtype %d", dtype);
+  REQUIRE(num_q_heads > 0 && num_q_heads % a.c.hkv == 0,
+          "attn_kv4: num_q_heads %d must be a positive multiple of num_kv_heads %d", num_q_heads, a.c.hkv);
+  REQUIRE(window >= 0, "attn_kv4: window must be >= 0, got %d", window);
+  REQUIRE(softcap >= 0.f && softcap < INFINITY && scale > 0.f && scale < INFINITY,
+          "attn_kv4: need a finite scale > 0 and softcap >= 0");
+  const int64_t vec = dtype == DX_BF16 ? 8 : 4, width = (int64_t)num_q_heads * a.c.d;
+  REQUIRE(q_row_stride >= width && out_row_stride >= width && q_row_stride % vec == 0 && out_row_stride % vec == 0,
+          "attn_kv4: row strides must cover heads * head_dim and be multiples of %ld elements", (long)vec);
+  REQUIRE(aligned16(q) && aligned16(out), "attn_kv4: pointers must be 16-byte aligned");
+  REQUIRE(!weights_out || weights_in, "attn_kv4: weights_out needs weights_in");
+  if (weights_out)
+    REQUIRE(weights_in_head_stride >= max_ctx_len && weights_out_head_stride >= max_ctx_len &&
+                weights_in_seq_stride >= 0 && weights_out_seq_stride >= 0,
+            "attn_kv4: weight rows shorter than max_ctx_len %d", max_ctx_len);
+  const int group = num_q_heads / a.c.hkv;
+  SUPPORTED((int64_t)max_seq_len * group <= MOST_SLOTS / 32, "attn_kv4: %d tokens of %d heads beyond the launch grid",
+            max_seq_len, group);
+  if (num_seqs == 0 || ((rows == 0 || max_seq_len == 0) && !weights_out)) return DX_OK;
+  a.window = window;
+  a.slots = in_range(window, max_ctx_len);
+  const Kv4Plan p = dx_kv4_attn_plan(max_seq_len, max_ctx_len, group, a.slots);
+  const Kv4Workspace w = kv4_workspace(p, (int64_t)num_seqs * a.c.hkv, a.c.d, weights_out != nullptr);
+  REQUIRE(workspace_bytes >= w.total, "attn_kv4: workspace of %ld bytes, need %ld", (long)workspace_bytes,
+          (long)w.total);
+  REQUIRE(w.total == 0 || (workspace && aligned16(workspace)), "attn_kv4: needs a 16-byte aligned workspace");
+  char *ws = static_cast<char *>(workspace);
+  a.partial = reinterpret_cast<float *>(ws);
+  a.stats = reinterpret_cast<float *>(ws + w.stats);
+  a.lse = reinterpret_cast<float *>(ws + w.lse);
+  a.part_rows = p.part_rows;
+  a.max_rows = p.max_rows;
+  a.max_splits = p.max_splits;
+  a.query = q;
+  a.out = out;
+  a.q_stride = q_row_stride;
+  a.out_stride = out_row_stride;
+  a.hq = num_q_heads;
+  a.scale = scale;
+  a.softcap = softcap;
+  a.w_in = weights_in;
+  a.w_out = weights_out;
+  a.wi_seq = weights_in_seq_stride;
+  a.wi_head = weights_in_head_stride;
+  a.wo_seq = weights_out_seq_stride;
+  a.wo_head = weights_out_head_stride;
+  return check_launch(dx_kv4_attn_launch(a, dtype == DX_F32, as_stream(stream)), "attn_kv4 launch");
+}
+
+int64_t dx_kv4_evict_workspace(int32_t num_seqs, int32_t num_kv_heads, int32_t keep) {
+  return num_seqs > 0 && num_kv_heads > 0 && keep > 0 ? (int64_t)num_seqs * num_kv_heads * keep * 4 : 0;
+}
+
+int dx_kv4_evict(const dx_kv4_cache *cache, const float *weights, int64_t weights_seq_stride,
+                 int64_t weights_head_stride, const int32_t *page_table, int32_t table_width, const int32_t *ctx_len,
+                 int32_t num_seqs, int32_t max_ctx_len, const int32_t *out_table, int32_t out_table_width, int32_t keep,
+                 int32_t recent, float *weights_out, int64_t weights_out_seq_stride, int64_t weights_out_head_stride,
+                 int32_t *out_len, void *workspace, int64_t workspace_bytes, void *stream) {
+  Kv4Cache c;
+  int st = validate_cache(cache, &c, "kv4_evict");
+  if (st) return st;
+  REQUIRE(weights && page_table && ctx_len && out_table && weights_out && out_len, "kv4_evict: null pointer argument");
+  REQUIRE(num_seqs >= 0 && max_ctx_len >= 0 && table_width >= 0 && out_table_width >= 0,
+          "kv4_evict: negative sequence count, length or table width");
+  REQUIRE(keep >= 1 && recent >= 0 && recent <= keep, "kv4_evict: keep %d with %d recent", keep, recent);
+  SUPPORTED(num_seqs <= 65535, "kv4_evict: %d sequences beyond the launch grid", num_seqs);
+  SUPPORTED(max_ctx_len <= MOST_SLOTS && keep <= MOST_SLOTS, "kv4_evict: sequences of more than 2^30 slots");
+  const int64_t slots = (int64_t)table_width * cache->page_size, room = (int64_t)out_table_width * cache->page_size;
+  const int32_t ctx = (int32_t)(slots < max_ctx_len ? slots : max_ctx_len), most = keep < ctx ? keep : ctx;
+  REQUIRE(room >= most, "kv4_evict: out_table holds %ld slots a sequence, need %d", (long)room, most);
+  REQUIRE(weights_seq_stride >= 0 && weights_head_stride >= ctx && weights_out_seq_stride >= 0 &&
+              weights_out_head_stride >= keep,
+          "kv4_evict: weight rows shorter than the slots they are for");
+  const int64_t need = dx_kv4_evict_workspace(num_seqs, c.hkv, keep);
+  REQUIRE(workspace_bytes >= need, "kv4_evict: workspace of %ld bytes, need %ld", (long)workspace_bytes, (long)need);
+  if (num_seqs == 0) return DX_OK;
+  REQUIRE(workspace && aligned16(workspace), "kv4_evict: needs a 16-byte aligned workspace");
+  return check_launch(dx_kv4_evict_launch(c, page_table, table_width, out_table, out_table_width, ctx_len, num_seqs, ctx,
+                                          keep, recent, weights, weights_seq_stride, weights_head_stride, weights_out,
+                                          weights_out_seq_stride, weights_out_head_stride, out_len,
+                                          static_cast<int32_t *>(workspace), as_stream(stream)),
+                      "kv4_evict launch");
+}
+
+int64_t dx_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top) {
+  if (rows <= 0 || vocab <= 0) return 0;
+  // three numbers for every 2048 logits, and the largest of every 32
+  return rows * 4 * (dx_ceil_div(vocab, 2048) * INT64_C(3) + (top > 0 ? dx_ceil_div(vocab, 32) : 0));
+}
+
+int dx_token_logprobs(const void *logits, const int32_t *targets, int64_t rows, int32_t vocab, int64_t row_stride,
+                      float softcap, int32_t top, float *logprobs, float *entropy, int32_t *top_ids,
+                      float *top_logprobs, int32_t dtype, void *workspace, int64_t workspace_bytes, void *stream) {
+  REQUIRE(logits && targets && logprobs && entropy, "token_logprobs: null pointer argument");
+  REQUIRE(dtype == DX_BF16 || dtype == DX_F32, "token_logprobs: unknown dtype %d", dtype);
+  REQUIRE(rows >= 0 && rows <= INT32_MAX && vocab > 0 && row_stride >= vocab,
+          "token_logprobs: %ld rows of %d (stride %ld)", (long)rows, vocab, (long)row_stride);
+  SUPPORTED(vocab <= MOST_SLOTS, "token_logprobs: vocabulary of %d", vocab);
+  REQUIRE(softcap >= 0.f && softcap < INFINITY, "token_logprobs: softcap must be >= 0 and finite");
+  REQUIRE(top >= 0 && top <= vocab, "token_logprobs: %d alternatives of %d", top, vocab);
+  SUPPORTED(top <= 64, "token_logprobs: %d alternatives, 64 at most", top);
+  REQUIRE(top == 0 || (top_ids && top_logprobs), "token_logprobs: null output of the alternatives");
+  REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == DX_BF16 ? 2 : 4) == 0,
+          "token_logprobs: logits not aligned to their type");
+  const int64_t need = dx_token_logprobs_workspace(rows, vocab, top);
+  REQUIRE(workspace_bytes >= need, "token_logprobs: workspace of %ld bytes, need %ld", (long)workspace_bytes,
+          (long)need);
+  if (rows == 0) return DX_OK;
+  REQUIRE(workspace && aligned16(workspace), "token_logprobs: needs a 16-byte aligned workspace");
+  float *parts = static_cast<float *>(workspace);
+  return check_launch(dx_token_logprobs_launch(logits, targets, rows, vocab, row_stride, softcap, top, logprobs, entropy,
+                                               top_ids, top_logprobs, parts,
+                                               parts + rows * dx_ceil_div(vocab, 2048) * 3, dtype == DX_F32,
+                                               as_stream(stream)),
+                      "token_logprobs launch");
+}

@@ -125,3 +125,53 @@ hipError_t dx_combine_scaled_f32_launch(const float *prior, const float *cosine,
                                         const uint8_t *option_mask, const float *prior_logit_scale,
                                         const float *joint_logit_scale, const float *residual_gate, float *out, long n,
                                         hipStream_t s);
+
+// The paged 4-bit cache (kv4.h): codes [pages][hkv][1 << shift][d / 2], scale bytes [..][d / 32], positions [..].
+struct Kv4Cache {
+  uint8_t *k, *v, *ks, *vs;
+  int32_t *pos;
+  int pages, hkv, d, shift;
+};
+
+// The newest seq_len[b] tokens of each sequence: packed rows from seq_start[b] (of `rows`), slots up to ctx_len[b].
+struct Kv4Batch {
+  const int32_t *table, *seq_start, *seq_len, *ctx_len;
+  int table_width, num_seqs, max_seq_len, max_ctx;
+  long rows;
+};
+
+hipError_t dx_kv4_append_launch(const Kv4Cache &c, const Kv4Batch &q, const void *k, const void *v,
+                                const int32_t *positions, long k_stride, long v_stride, bool f32, hipStream_t s);
+hipError_t dx_kv4_read_launch(const Kv4Cache &c, const Kv4Batch &q, uint16_t *k, uint16_t *v, long k_stride,
+                              long v_stride, hipStream_t s);
+hipError_t dx_kv4_evict_launch(const Kv4Cache &c, const int32_t *table, int width, const int32_t *out_table,
+                               int out_width, const int32_t *ctx_len, int num_seqs, int max_ctx, int keep, int recent,
+                               const float *weights, long w_seq, long w_head, float *out_weights, long o_seq,
+                               long o_head, int32_t *out_len, int32_t *list, hipStream_t s);
+
+struct Kv4Attn {
+  Kv4Cache c;
+  Kv4Batch q;
+  const void *query;
+  void *out;
+  long q_stride, out_stride;
+  int hq;
+  float scale, softcap;
+  int window, slots;  // window of positions, and of slots: cut to the longest sequence, so that it adds in 32 bits
+  const float *w_in;  // accumulated weights [seqs][hkv][slots], strides below; null without them
+  float *w_out;
+  long wi_seq, wi_head, wo_seq, wo_head;
+  float *partial, *stats, *lse;  // workspace, laid out by dx_kv4_attn_plan
+  int part_rows, max_rows, max_splits;
+};
+// Sizes that depend on the largest lengths alone: partial rows per (sequence, kv head), rows, splits.
+struct Kv4Plan {
+  int part_rows, max_rows, max_splits;
+};
+Kv4Plan dx_kv4_attn_plan(int max_seq_len, int max_ctx, int group, int window);
+hipError_t dx_kv4_attn_launch(const Kv4Attn &a, bool f32, hipStream_t s);
+
+// Log probabilities (logprobs.hip). groups: largest logit of each 32 of the vocabulary; parts: per 2048, see there.
+hipError_t dx_token_logprobs_launch(const void *logits, const int32_t *targets, long rows, int vocab, long ld, float cap,
+                                    int top, float *logprobs, float *entropy, int32_t *ids, float *top_logprobs,
+                                    float *parts, float *groups, bool f32, hipStream_t s);

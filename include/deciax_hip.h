@@ -489,6 +489,130 @@ int dx_head_combine_scaled_f32(const float *prior, const float *cosine,
                                const float *residual_gate, float *logits,
                                int64_t n, void *stream);
 
+/* ------------------------------------------------------------------------ */
+/* A cache of keys and values in 4 bits, and answers over it                  */
+/* ------------------------------------------------------------------------ */
+
+/* The state of one layer's cache, read by the host during a call. `k` and `v`
+ * hold [num_pages][num_kv_heads][page_size][head_dim / 2] bytes, the scales
+ * [num_pages][num_kv_heads][page_size][head_dim / 32] bytes, `positions`
+ * [num_pages][num_kv_heads][page_size] int32. 32 neighbouring values of a head
+ * share a scale 2^e, e the smallest integer with amax <= 6 2^e, kept in
+ * [-119, 125] and stored as the byte e + 127; a value is the nearest of 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6 (a tie takes the even code) with its sign in bit 3, the
+ * even dimension in the low half of its byte. A block that holds an infinity or
+ * a NaN has the scale byte 255 and reads as NaN. head_dim in {64, 128, 256};
+ * page_size a power of two in [64, 65536]; 16-byte aligned arrays. */
+typedef struct dx_kv4_cache {
+  void *k, *v;
+  uint8_t *k_scale, *v_scale;
+  int32_t *positions;
+  int32_t num_pages, num_kv_heads, page_size, head_dim;
+} dx_kv4_cache;
+
+/* What the calls below share: slot j of sequence b is row j % page_size of page
+ * page_table[b * table_width + j / page_size]; ctx_len[b] slots are in use (at
+ * most max_ctx_len and table_width * page_size; longer ones are cut), the last
+ * seq_len[b] of them (at most max_seq_len) those of its newest tokens, whose
+ * packed rows start at row seq_start[b] of `rows`. Rows outside [0, rows), slots
+ * below 0 and pages outside [0, num_pages) are never touched: such a slot is not
+ * written, reads as zeros and is not seen. All of it is device int32. */
+
+/* Write the newest tokens' rows of k and v (bf16 or fp32, head g at g *
+ * head_dim) and their positions into their slots. The reference has no cache: it
+ * repeats a state's whole forward for every call (src/deciax/runtime/clef.py:23-40).
+ * Slots must not be shared with a call that overlaps. */
+int dx_kv4_append(const dx_kv4_cache *cache, const void *k, const void *v,
+                  const int32_t *positions, const int32_t *page_table,
+                  int32_t table_width, const int32_t *seq_start,
+                  const int32_t *seq_len, const int32_t *ctx_len,
+                  int32_t num_seqs, int32_t max_seq_len, int64_t rows,
+                  int64_t k_row_stride, int64_t v_row_stride, int32_t dtype,
+                  void *stream);
+
+/* The newest tokens' rows as the cache holds them, in bf16 (exact, but for
+ * NaN's bits): the inverse of dx_kv4_append. No counterpart in the reference. */
+int dx_kv4_read(const dx_kv4_cache *cache, void *k, void *v,
+                const int32_t *page_table, int32_t table_width,
+                const int32_t *seq_start, const int32_t *seq_len,
+                const int32_t *ctx_len, int32_t num_seqs, int32_t max_seq_len,
+                int64_t rows, int64_t k_row_stride, int64_t v_row_stride,
+                void *stream);
+
+/* Attention of the newest tokens (appended before) over their sequences' slots:
+ * dx_attn_prefill's scores and softmax (src/deciax/kernels/attention/blocked.py:9-32,
+ * with soft-cap and window), the keys and values as the cache holds them. Token i
+ * of n sees slot j <= own = ctx_len - n + i and, with a window, j > own - window
+ * and position[j] > position[own] - window. q and out: bf16, or fp32 with three
+ * bf16 products for each fp32 one. A row that sees nothing is written as zeros;
+ * rows that belong to no sequence are not written. num_q_heads is any multiple
+ * of the cache's heads.
+ *
+ * With weights_out, every slot below ctx_len gets its accumulated attention
+ * weight: weights_in (0 for the newest tokens' slots, whatever it holds there)
+ * plus the softmax weights of all rows and query heads of the KV head that saw
+ * it. weights are fp32 at b * seq_stride + g * head_stride + slot; weights_in may
+ * be weights_out; slots from ctx_len on are not written. Sums have one order:
+ * the same call gives the same bits, alone or in a batch. Workspace size from
+ * dx_attn_kv4_workspace with the same sizes. */
+int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out,
+                const int32_t *page_table, int32_t table_width,
+                const int32_t *seq_start, const int32_t *seq_len,
+                const int32_t *ctx_len, int32_t num_seqs, int32_t max_seq_len,
+                int32_t max_ctx_len, int64_t rows, int32_t num_q_heads,
+                int64_t q_row_stride, int64_t out_row_stride, float scale,
+                float softcap, int32_t window, const float *weights_in,
+                int64_t weights_in_seq_stride, int64_t weights_in_head_stride,
+                float *weights_out, int64_t weights_out_seq_stride,
+                int64_t weights_out_head_stride, int32_t dtype,
+                void *workspace, int64_t workspace_bytes, void *stream);
+
+int64_t dx_attn_kv4_workspace(int32_t num_seqs, int32_t max_seq_len,
+                              int32_t max_ctx_len, int32_t num_q_heads,
+                              int32_t num_kv_heads, int32_t head_dim,
+                              int32_t window, int32_t with_weights);
+
+/* Cut every sequence to its `keep` most useful slots, copied to the pages of
+ * out_table (which must hold keep slots a sequence and share no page with
+ * page_table: the old pages stay as they are, for sequences that share them). A
+ * KV head keeps the last `recent` slots and, of the others, the heaviest by
+ * `weights`, the lower slot first where weights are equal (a NaN is above all);
+ * what is kept stays in slot order, with its position. weights_out[b, g, 0..keep)
+ * gets the kept slots' weights and zeros behind them, out_len[b] = min(ctx_len,
+ * keep). 0 <= recent <= keep, 1 <= keep. No counterpart in the reference.
+ * Workspace size from dx_kv4_evict_workspace. */
+int dx_kv4_evict(const dx_kv4_cache *cache, const float *weights,
+                 int64_t weights_seq_stride, int64_t weights_head_stride,
+                 const int32_t *page_table, int32_t table_width,
+                 const int32_t *ctx_len, int32_t num_seqs, int32_t max_ctx_len,
+                 const int32_t *out_table, int32_t out_table_width,
+                 int32_t keep, int32_t recent, float *weights_out,
+                 int64_t weights_out_seq_stride, int64_t weights_out_head_stride,
+                 int32_t *out_len, void *workspace, int64_t workspace_bytes,
+                 void *stream);
+
+int64_t dx_kv4_evict_workspace(int32_t num_seqs, int32_t num_kv_heads,
+                               int32_t keep);
+
+/* Per row of logits [rows, vocab] (bf16 or fp32, any row stride), with t = logit
+ * or softcap * tanh(logit / softcap): logprobs = log softmax(t)[target], entropy
+ * = -sum p log p (nats), and the `top` (0 to 64, at most vocab) best tokens,
+ * ranked by their logits as given, the lower token first where they are equal,
+ * with their log probabilities. Scores given tokens as dx_readout scores options
+ * (src/deciax/models/laya/heads.py:74-91), over the whole vocabulary.
+ * A logit of -inf is no alternative, soft-capped or not: probability 0, and
+ * token -1 with -inf where fewer than `top` others exist. A row of nothing but
+ * -inf: logprob -inf, entropy 0. A row with a NaN (or, without soft-cap, +inf):
+ * NaN, tokens -1. target -1: logprob 0 (no token asked for); another target
+ * outside the vocabulary: NaN. Workspace size from dx_token_logprobs_workspace. */
+int dx_token_logprobs(const void *logits, const int32_t *targets, int64_t rows,
+                      int32_t vocab, int64_t row_stride, float softcap,
+                      int32_t top, float *logprobs, float *entropy,
+                      int32_t *top_ids, float *top_logprobs, int32_t dtype,
+                      void *workspace, int64_t workspace_bytes, void *stream);
+
+int64_t dx_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top);
+
 #ifdef __cplusplus
 }
 #endif

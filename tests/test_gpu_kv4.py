@@ -1,0 +1,534 @@
+"""The 4-bit cache on the GPU: writing, reading, attention over it and eviction, against the 64-bit oracle.
+
+Tolerances count roundings (u = half a step of a type). Attention of bf16 queries: each weight is rounded to bf16 once
+and the output once, 2^-8 each; a score t is off by at most D sums of fp32 products, the conversion to base 2 and the
+soft-cap's arithmetic, `score_error`; that moves a weight, relative to the others, by at most twice as much. fp32
+queries: weights and queries in three bf16 parts keep 2^-24; sums run over 32 keys a step.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import kv4 as oracle
+from tests.conftest import i32, rng, say
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+
+
+class Case:
+    """A cache with random contents, its sequences' page table and the host's copy of all of it."""
+
+    def __init__(self, seed: int, new: list[int], ctx: list[int], hq: int, hkv: int, d: int, page: int = 64,
+                 dtype: str = "bf16", garbage: bool = True) -> None:
+        import torch
+
+        from deciax_amd import kernels as K
+
+        r = rng(seed)
+        self.new, self.ctx, self.hq, self.hkv, self.d, self.page, self.dtype = new, ctx, hq, hkv, d, page, dtype
+        counts = [max(1, -(-c // page)) for c in ctx]
+        self.pages = sum(counts) + 3
+        order = r.permutation(self.pages)
+        self.table = np.full((len(ctx), max(counts) + 1), -1, np.int64)  # unused entries name no page
+        at = 0
+        for b, n in enumerate(counts):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+        shape = (self.pages, hkv, page)
+        # whatever a fresh page holds: every byte, the NaN scale among them
+        raw = {n: r.integers(0, 256, (*shape, w)).astype(np.uint8) if garbage else np.zeros((*shape, w), np.uint8)
+               for n, w in (("k", d // 2), ("v", d // 2), ("k_scale", d // 32), ("v_scale", d // 32))}
+        if garbage:
+            for n in ("k_scale", "v_scale"):
+                raw[n][r.random(raw[n].shape) < 0.3] = 255
+        self.raw = raw
+        self.pos = r.integers(0, 1 << 30, shape).astype(np.int32)
+        self.cache = K.KV4Cache(*(torch.from_numpy(raw[n].copy()).cuda() for n in ("k", "v", "k_scale", "v_scale")),
+                                torch.from_numpy(self.pos.copy()).cuda())
+        self.d_table, self.d_new, self.d_ctx = i32(self.table), i32(new), i32(ctx)
+        self.starts = np.concatenate([[0], np.cumsum(new)[:-1]]).astype(np.int64)
+        self.d_starts = i32(self.starts)
+        self.rows, self.max_new, self.max_ctx = sum(new), max(new), max(ctx)
+        t = torch.bfloat16 if dtype == "bf16" else torch.float32
+        self.t = t
+        # columns of one packed buffer, as a projection leaves them, with a margin between
+        self.qkv = torch.from_numpy(r.normal(size=(self.rows, (hq + 2 * hkv) * d + 16)).astype(np.float32)).cuda().to(t)
+        self.q, self.k = self.qkv[:, :hq * d], self.qkv[:, hq * d:(hq + hkv) * d]
+        self.v = self.qkv[:, (hq + hkv) * d + 16:]
+        self.positions = i32(np.concatenate([np.arange(c - n, c) for n, c in zip(new, ctx)] or [[]]))
+
+    def fill(self, seed: int, std: float = 1.0) -> None:
+        """Proper old slots: quantised normals, positions in order."""
+        import torch
+
+        r = rng(seed)
+        for b, c in enumerate(self.ctx):
+            for j in range(c):
+                p = self.table[b, j // self.page]
+                self.pos[p, :, j % self.page] = j
+            pages = self.table[b, :max(1, -(-c // self.page))]
+            for n in ("k", "v"):
+                x = r.normal(size=(len(pages), self.hkv, self.page, self.d)) * std
+                code, scale = oracle.quantise(x)
+                keep = np.arange(len(pages) * self.page).reshape(len(pages), 1, self.page, 1) < c
+                self.raw[n][pages] = np.where(keep, oracle.pack(code), self.raw[n][pages])
+                self.raw[n + "_scale"][pages] = np.where(keep, scale, self.raw[n + "_scale"][pages])
+        for n in ("k", "v", "k_scale", "v_scale"):
+            getattr(self.cache, n).copy_(torch.from_numpy(self.raw[n]))
+        self.cache.positions.copy_(torch.from_numpy(self.pos))
+
+    def host(self, name: str) -> np.ndarray:
+        return getattr(self.cache, name).cpu().numpy()
+
+    def held(self, name: str, b: int, table: np.ndarray | None = None, ctx: int | None = None) -> np.ndarray:
+        """[hkv, ctx, d] values of a sequence, from the device's bytes."""
+        c = self.ctx[b] if ctx is None else ctx
+        pages = (self.table if table is None else table)[b, :-(-c // self.page)]
+        code = oracle.unpack(self.host(name)[pages])
+        v = oracle.values(code, self.host(name + "_scale")[pages])
+        return v.transpose(1, 0, 2, 3).reshape(self.hkv, len(pages) * self.page, self.d)[:, :c]
+
+    def held_positions(self, b: int, table: np.ndarray | None = None, ctx: int | None = None) -> np.ndarray:
+        c = self.ctx[b] if ctx is None else ctx
+        pages = (self.table if table is None else table)[b, :-(-c // self.page)]
+        return self.host("positions")[pages].transpose(1, 0, 2).reshape(self.hkv, len(pages) * self.page)[:, :c].astype(np.int64)
+
+    def append(self) -> None:
+        from deciax_amd import kernels as K
+
+        K.kv4_append(self.cache, self.k, self.v, self.positions, self.d_table, self.d_starts, self.d_new, self.d_ctx,
+                     self.max_new)
+
+    def attend(self, **kw):
+        from deciax_amd import kernels as K
+
+        return K.attention_kv4(self.q, self.cache, self.d_table, self.d_starts, self.d_new, self.d_ctx, self.max_new,
+                               self.max_ctx, num_q_heads=self.hq, **kw)
+
+    def check(self, out, weights_out=None, weights_in=None, *, scale: float, softcap: float, window: int) -> None:
+        """Device results against the oracle on the device's own cache."""
+        got = out.float().cpu().numpy().astype(np.float64)
+        q = self.q.float().cpu().numpy().astype(np.float64)
+        for b, (n, c) in enumerate(zip(self.new, self.ctx)):
+            k, v, pos = self.held("k", b), self.held("v", b), self.held_positions(b)
+            rows = slice(self.starts[b], self.starts[b] + n)
+            qb = q[rows].reshape(n, self.hq, self.d)
+            want, wsum, mass = oracle.attention(qb, k, v, pos, scale=scale, softcap=softcap, window=window)
+            finite = np.nan_to_num(k)
+            biggest = max((np.abs(qb) @ np.abs(finite).reshape(-1, self.d).T).max(initial=0.0) * scale, 1.0)
+            seen = min(biggest, softcap) if softcap else biggest
+            score_error = self.d * U32 * biggest + 8 * U32 * max(seen, softcap)
+            moved = 2 * score_error + 8 * U32
+            g = got[rows].reshape(n, self.hq, self.d)
+            nan = np.isnan(want)
+            assert (np.isnan(g) == nan).all(), f"sequence {b}: NaN at other places"
+            steps = 32 + c / 32 + 64
+            if self.dtype == "bf16":
+                tol = (2.0 ** -8 + moved + steps * U32) * mass + 2.0 ** -8 * np.abs(want)
+            else:
+                tol = (moved + (steps + 4) * U32) * mass + U32 * np.abs(want)
+            err = np.abs(np.where(nan, 0, g) - np.where(nan, 0, want))
+            assert (err <= np.where(nan, 0, tol) + 1e-30).all(), \
+                f"sequence {b}: {np.nanmax(err - np.where(nan, 0, tol)):.3e} beyond the bound, error {err.max():.3e}"
+            if weights_out is not None:
+                w = weights_out[b, :, :c].cpu().numpy().astype(np.float64)
+                old = weights_in[b, :, :c].astype(np.float64).copy()
+                old[:, c - n if c > n else 0:] = 0
+                group_rows = n * (self.hq // self.hkv)
+                wtol = (moved + (16 + group_rows) * U32) * wsum + U32 * np.abs(old + wsum) + 1e-30
+                wn = np.isnan(wsum)
+                assert (np.isnan(w) == wn).all()
+                assert (np.abs(np.where(wn, 0, w - old - wsum)) <= np.where(wn, 0, wtol)).all(), \
+                    f"sequence {b}: weights off by {np.nanmax(np.abs(w - old - wsum)):.3e}"
+
+
+# ------------------------------------------------------------------------------------------ append and read
+
+
+@pytest.mark.parametrize("d,hkv,page,dtype", [(64, 1, 64, "bf16"), (128, 3, 64, "bf16"), (256, 8, 128, "f32"),
+                                              (64, 5, 256, "f32"), (256, 1, 64, "bf16")])
+def test_append_and_read_are_exact(d: int, hkv: int, page: int, dtype: str) -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    new, ctx = [1, 70, 0, 129, 5], [1, 70, 9, 300, 3]  # the last: more new tokens than slots
+    say(f"kv4 append d={d} hkv={hkv} page={page} {dtype}")
+    c = Case(d + hkv, new, ctx, hkv, hkv, d, page, dtype)
+    r = rng(5)
+    x = c.qkv.float().cpu().numpy()
+    # the whole range, ties, zeros, and what no 4-bit number can hold
+    x *= np.exp2(r.integers(-40, 40, (x.shape[0], 1))).astype(np.float32)
+    x[0, :] = 0
+    x[1] *= np.float32(1e-38)
+    x[2, hkv * d + 3] = np.inf
+    x[3, hkv * d + 40] = np.nan
+    x[4, hkv * d:hkv * d + 32] = np.float32(3e38)
+    x[5, hkv * d:hkv * d + 32] = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 6] * 4, np.float32) * np.float32(0.125)
+    c.qkv.copy_(torch.from_numpy(x).to(c.t))
+    before = {n: c.host(n).copy() for n in ("k", "v", "k_scale", "v_scale", "positions")}
+    c.append()
+    torch.cuda.synchronize()
+    touched = np.zeros((c.pages, page), bool)
+    for b, (n, m) in enumerate(zip(new, ctx)):
+        for i in range(n):
+            slot = m - n + i
+            if slot < 0:
+                continue
+            p, at = c.table[b, slot // page], slot % page
+            touched[p, at] = True
+            row = c.starts[b] + i
+            for name, t in (("k", c.k), ("v", c.v)):
+                code, scale = oracle.quantise(t[row].float().cpu().numpy().reshape(hkv, d))
+                np.testing.assert_array_equal(c.host(name)[p, :, at], oracle.pack(code))
+                np.testing.assert_array_equal(c.host(name + "_scale")[p, :, at], scale)
+            assert (c.host("positions")[p, :, at] == slot).all()
+    for n, old in before.items():  # nothing else was written
+        np.testing.assert_array_equal(c.host(n).transpose(0, 2, 1, *range(3, old.ndim))[~touched],
+                                      old.transpose(0, 2, 1, *range(3, old.ndim))[~touched])
+    k, v = K.kv4_read(c.cache, c.d_table, c.d_starts, c.d_new, c.d_ctx, c.max_new, rows=c.rows)
+    for name, t in (("k", k), ("v", v)):
+        t = t.float().cpu().numpy()
+        for b, (n, m) in enumerate(zip(new, ctx)):
+            held = c.held(name, b)
+            for i in range(n):
+                want = held[:, m - n + i].reshape(-1) if m - n + i >= 0 else np.zeros(hkv * d)
+                np.testing.assert_array_equal(t[c.starts[b] + i], want.astype(np.float32))
+
+
+def test_pages_and_rows_out_of_range_are_not_touched() -> None:
+    """A table entry outside the pool, and a sequence whose rows leave the packed buffer: nothing is written for them."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("kv4 with bad pages and rows")
+    c = Case(3, [40, 10], [100, 10], 2, 2, 64, garbage=False)
+    c.table[0, 1] = c.pages + 7
+    c.d_table = i32(c.table)
+    c.d_starts = i32([0, 45])  # rows 50.. of the second do not exist
+    c.append()
+    k, v = K.kv4_read(c.cache, c.d_table, c.d_starts, c.d_new, c.d_ctx, c.max_new, rows=c.rows)
+    torch.cuda.synchronize()
+    used = c.table[1, 0]
+    held = c.host("k_scale")
+    assert (held[used, :, :5] != 0).all() and (held[used, :, 5:] == 0).all()
+    assert (k[36:40].float().cpu().numpy() == 0).all()  # slots 96.. lie in the page that is not there
+    out = c.attend(scale=0.125)
+    torch.cuda.synchronize()
+    assert torch.isfinite(out[:40].float()).all()
+
+
+# ------------------------------------------------------------------------------------------ attention
+
+
+SHAPES = [  # new, ctx, hq, hkv, d, page
+    ([1], [1], 1, 1, 64, 64),
+    ([1, 1, 1], [2, 63, 65], 2, 1, 64, 64),
+    ([1, 1, 1, 1], [33, 700, 257, 0], 16, 8, 256, 64),
+    ([1, 1], [2100, 129], 8, 2, 128, 128),
+    ([5, 1, 3], [64, 300, 3], 3, 1, 128, 64),
+    ([40, 1, 0, 17], [40, 600, 50, 1000], 4, 2, 256, 256),
+    ([150, 33], [500, 33], 8, 8, 64, 64),
+    ([3, 2], [1, 2], 8, 1, 128, 64),       # a sequence with more new tokens than slots: its first rows see nothing
+    ([20], [9000], 16, 1, 64, 64),
+]
+
+
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (50.0, 0), (50.0, 70), (0.0, 1)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention(shape: int, dtype: str, softcap: float, window: int) -> None:
+    import torch
+
+    new, ctx, hq, hkv, d, page = SHAPES[shape]
+    say(f"attention_kv4 new={new} ctx={ctx} hq={hq} hkv={hkv} d={d} page={page} {dtype} cap={softcap} window={window}")
+    c = Case(17 * shape + d, new, ctx, hq, hkv, d, page, dtype)
+    c.fill(shape)
+    c.append()
+    r = rng(shape)
+    w = np.abs(r.normal(size=(len(new), hkv, max(ctx) + 3))).astype(np.float32)
+    for b, (n, m) in enumerate(zip(new, ctx)):
+        w[b, :, max(m - n, 0):m] = np.nan  # the newest slots' old weights are not read
+    w_in = torch.from_numpy(w.copy()).cuda()
+    w_out = torch.full_like(w_in, -7.0)
+    kw = dict(scale=d ** -0.5 * 2, softcap=softcap, window=window)
+    plain = c.attend(**kw)
+    out = c.attend(weights=w_in, weights_out=w_out, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(plain, out), "weights change no output"
+    c.check(out, w_out, w, **kw)
+    for b, m in enumerate(ctx):
+        assert (w_out[b, :, m:] == -7.0).all(), "slots behind the sequence were written"
+    again = c.attend(weights=w_in, **kw)  # in place
+    torch.cuda.synchronize()
+    assert torch.equal(again, out)
+    for b, m in enumerate(ctx):
+        assert torch.equal(w_in[b, :, :m], w_out[b, :, :m])
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "bf16"), (128, "f32"), (256, "bf16")])
+def test_values_and_keys_that_are_nan_reach_only_rows_that_see_them(d: int, dtype: str) -> None:
+    import torch
+
+    new, ctx, hq, hkv = [20, 1], [90, 200], 4, 2
+    say(f"attention_kv4 with NaN, d={d} {dtype}")
+    c = Case(d, new, ctx, hq, hkv, d, 64, dtype)
+    c.fill(1)
+    c.v[7, 33] = float("nan")   # token 7 of sequence 0: one block of one head
+    c.v[15, 0] = float("inf")
+    c.k[11, 5] = float("nan")
+    c.append()
+    out = c.attend(scale=0.2, softcap=50.0)
+    torch.cuda.synchronize()
+    got = out.float().cpu().numpy().reshape(-1, hq, d)
+    assert np.isfinite(got[:7]).all() and np.isfinite(got[20]).all()
+    assert np.isnan(got[7, 0, 32:64]).all() and np.isfinite(got[7, 0, :32]).all() and np.isfinite(got[7, 2:]).all()
+    c.check(out, scale=0.2, softcap=50.0, window=0)
+
+
+def test_infinite_and_nan_queries_stay_in_their_rows() -> None:
+    import torch
+
+    say("attention_kv4 with NaN and infinite queries")
+    c = Case(2, [4, 1], [100, 50], 4, 2, 128)
+    c.fill(2)
+    c.q[1, 5] = float("nan")
+    c.q[2, 140] = float("inf")
+    c.append()
+    for cap in (0.0, 50.0):
+        out = c.attend(scale=0.1, softcap=cap).float().cpu().numpy().reshape(5, 4, 128)
+        assert np.isnan(out[1, 0]).all() and np.isfinite(out[1, 1:]).all()
+        assert np.isfinite(out[0]).all() and np.isfinite(out[3:]).all() and np.isfinite(out[2, [0, 2, 3]]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_sequence_does_not_depend_on_its_batch(dtype: str) -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    new, ctx, hq, hkv, d = [1, 60, 7, 1], [3000, 400, 9000, 64], 8, 2, 128
+    say(f"attention_kv4 alone and in a batch {dtype}")
+    c = Case(9, new, ctx, hq, hkv, d, 64, dtype)
+    c.fill(4)
+    c.append()
+    w = torch.rand((4, hkv, max(ctx)), device="cuda")
+    for window in (0, 500):
+        kw = dict(num_q_heads=hq, scale=0.1, softcap=50.0, window=window)
+        w_all = torch.empty_like(w)
+        whole = K.attention_kv4(c.q, c.cache, c.d_table, c.d_starts, c.d_new, c.d_ctx, c.max_new, c.max_ctx, weights=w,
+                                weights_out=w_all, **kw)
+        for b, (n, m) in enumerate(zip(new, ctx)):
+            rows = slice(c.starts[b], c.starts[b] + n)
+            w_one = torch.empty((1, hkv, m), device="cuda")
+            one = K.attention_kv4(c.q[rows], c.cache, c.d_table[b:b + 1].contiguous(), i32([0]), i32([n]), i32([m]), n, m,
+                                  weights=w[b:b + 1], weights_out=w_one, **kw)
+            torch.cuda.synchronize()
+            assert torch.equal(one, whole[rows]), f"sequence {b} window {window}"
+            assert torch.equal(w_one[0], w_all[b, :, :m])
+
+
+def test_window_goes_by_positions_after_eviction_left_gaps() -> None:
+    """Positions with gaps: fewer slots than the window spans are seen."""
+    import torch
+
+    say("attention_kv4 window over positions with gaps")
+    c = Case(6, [2, 1], [300, 150], 4, 2, 64)
+    c.fill(3)
+    c.append()
+    r = rng(0)
+    for b, m in enumerate(c.ctx):
+        for g in range(c.hkv):
+            p = np.sort(r.choice(4 * m, m, replace=False))
+            for j in range(m):
+                c.pos[c.table[b, j // 64], g, j % 64] = p[j]
+    c.cache.positions.copy_(torch.from_numpy(c.pos))
+    for window in (1, 100, 100000):
+        kw = dict(scale=0.2, softcap=0.0, window=window)
+        w = torch.zeros((2, 2, 300), device="cuda")
+        out = c.attend(weights=w, **kw)
+        torch.cuda.synchronize()
+        c.check(out, w, np.zeros((2, 2, 300), np.float32), **kw)
+
+
+def test_other_streams_and_graph_replays() -> None:
+    """A decoding step (append, attend with weights) on a side stream, and captured and replayed with other eager
+    calls between the replays."""
+    import torch
+
+    say("kv4 step on a side stream and in a graph")
+    c = Case(8, [1, 1, 1], [700, 65, 3000], 16, 8, 256)
+    c.fill(5)
+    kw = dict(scale=1 / 16, softcap=50.0)
+    w0 = torch.rand((3, 8, 3000), device="cuda")
+    w = w0.clone()
+    c.append()
+    want = c.attend(weights=w, **kw)
+    torch.cuda.synchronize()
+    w_want = w.clone()
+
+    side = torch.cuda.Stream()
+    w_side = w0.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.append()
+        out_side = c.attend(weights=w_side, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(out_side, want) and torch.equal(w_side, w_want)
+
+    out = torch.empty_like(want)
+    wg = w0.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.append()
+        c.attend(weights=wg, out=out, **kw)
+    other = Case(11, [1, 1], [500, 20], 16, 8, 256)
+    other.fill(6)
+    for i in range(4):
+        out.fill_(float("nan"))
+        wg.copy_(w0)
+        other.attend(**kw)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(wg, w_want), f"replay {i} differs"
+
+
+def test_pages_beyond_32_bit_offsets() -> None:
+    """A pool whose arrays pass 4 GiB: pages at its end are addressed in 64 bits."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("kv4 pages beyond 4 GiB")
+    hkv, d, page = 8, 256, 1024
+    pages = (5 << 30) // (hkv * page * d // 2)
+    cache = K.kv4_cache(pages, hkv, d, page_size=page)
+    r = rng(4)
+    n, m = 3, 1500
+    x = torch.from_numpy(r.normal(size=(m, 3 * hkv * d)).astype(np.float32)).cuda().bfloat16()
+    q, k, v = (x[:, i * hkv * d:(i + 1) * hkv * d] for i in range(3))
+    pos = i32(np.arange(m))
+    outs = []
+    for table in ([0, 1], [pages - 1, pages - 2]):
+        t = i32([table])
+        K.kv4_append(cache, k, v, pos, t, i32([0]), i32([m]), i32([m]), m)
+        outs.append(K.attention_kv4(q[:n], cache, t, i32([0]), i32([n]), i32([m]), n, m, num_q_heads=hkv, scale=1 / 16))
+        got = K.kv4_read(cache, t, i32([0]), i32([m]), i32([m]), m, rows=m)
+        outs.extend(got)
+    torch.cuda.synchronize()
+    for a, b in zip(outs[:3], outs[3:]):
+        assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------ eviction
+
+
+@pytest.mark.parametrize("ctx,keep,recent,d,hkv,page", [
+    ([1], 1, 0, 64, 1, 64), ([100, 64, 3, 0], 40, 8, 128, 2, 64), ([1000, 5000, 400], 400, 0, 64, 3, 64),
+    ([2900], 1000, 1000, 256, 2, 128), ([20000, 17000], 4097, 100, 64, 1, 256), ([300], 299, 1, 64, 2, 64),
+    ([70001], 30000, 500, 64, 1, 1024)])
+def test_evict(ctx: list[int], keep: int, recent: int, d: int, hkv: int, page: int) -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"kv4_evict ctx={ctx} keep={keep} recent={recent} d={d} hkv={hkv} page={page}")
+    extra = sum(-(-keep // page) for _ in ctx)
+    c = Case(keep, [0] * len(ctx), [*ctx], hkv, hkv, d, page)
+    r = rng(keep)
+    per = -(-keep // page)
+    big = K.kv4_cache(c.pages + extra, hkv, d, page_size=page)
+    for n in c.cache._fields:
+        getattr(big, n)[:c.pages] = getattr(c.cache, n)
+    c.cache = big
+    out_table = c.pages + r.permutation(extra).reshape(len(ctx), per)
+    w = np.exp(r.normal(size=(len(ctx), hkv, max(ctx) + 1)) * 3).astype(np.float32)
+    w[r.random(w.shape) < 0.3] = 0.0          # many ties
+    w[r.random(w.shape) < 0.1] = np.float32(0.5)
+    if max(ctx) > 500:
+        w[0, 0, 11], w[0, 0, 12], w[0, 0, 13] = np.nan, np.inf, -0.0
+    w_dev = torch.from_numpy(w).cuda()
+    before = c.host("k").copy()
+    w_out, length = K.kv4_evict(c.cache, w_dev, c.d_table, c.d_ctx, max(ctx), i32(out_table), keep=keep, recent=recent)
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(c.host("k")[:c.pages], before[:c.pages])
+    assert length.cpu().tolist() == [min(n, keep) for n in ctx]
+    for b, m in enumerate(ctx):
+        n = min(m, keep)
+        for g in range(hkv):
+            slots = oracle.evict(w[b, g, :m], keep, recent)
+            np.testing.assert_array_equal(w_out[b, g, :n].cpu().numpy(), w[b, g, slots])
+            assert (w_out[b, g, n:] == 0).all()
+            for name in ("k", "v", "k_scale", "v_scale", "positions"):
+                a = c.host(name)
+                src = a[c.table[b, slots // page], g, slots % page]
+                j = np.arange(n)
+                np.testing.assert_array_equal(a[out_table[b, j // page], g, j % page], src)
+
+
+# ------------------------------------------------------------------------------------------ together
+
+
+def test_a_state_is_kept_cut_and_answered_over() -> None:
+    """Append a state, attend while weights accumulate, cut it, append and attend over what is left with a window, and
+    score the answer's tokens: every stage against the oracle on the device's own data."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("kv4: append, attend, evict, attend, score")
+    hq, hkv, d, page, hidden, vocab = 4, 2, 128, 64, 512, 1024
+    lengths = [400, 130]
+    c = Case(21, lengths, [*lengths], hq, hkv, d, page)
+    c.append()
+    w = torch.zeros((2, hkv, 448), device="cuda")
+    kw = dict(scale=0.1, softcap=50.0, window=0)
+    out = c.attend(weights=w, **kw)
+    torch.cuda.synchronize()
+    c.check(out, w, np.zeros((2, hkv, 448), np.float32), **kw)
+
+    keep = 100
+    per = 3  # room for the answer behind what is kept
+    big = K.kv4_cache(c.pages + 2 * per, hkv, d, page_size=page)
+    for n in c.cache._fields:
+        getattr(big, n)[:c.pages] = getattr(c.cache, n)
+    old_w = w[:, :, :].cpu().numpy()
+    c.cache = big
+    table = c.pages + np.arange(2 * per).reshape(2, per)
+    w2, length = K.kv4_evict(big, w, c.d_table, c.d_ctx, max(lengths), i32(table), keep=keep, recent=16)
+    torch.cuda.synchronize()
+    for b in range(2):
+        for g in range(hkv):
+            slots = oracle.evict(old_w[b, g, :lengths[b]], keep, 16)
+            np.testing.assert_array_equal(c.held_positions(b, table, keep)[g], slots)
+
+    n = 9  # the answer, positions going on from the state's
+    a = Case(22, [n, n], [keep + n, keep + n], hq, hkv, d, page)
+    a.cache, a.table, a.d_table, a.pages = big, table, i32(table), c.pages + 2 * per
+    a.positions = i32(np.concatenate([np.arange(m, m + n) for m in lengths]))
+    room = torch.zeros((2, hkv, keep + n), device="cuda")
+    room[:, :, :keep] = w2
+    a.append()
+    kw = dict(scale=0.1, softcap=50.0, window=200)
+    out = a.attend(weights=room, **kw)
+    torch.cuda.synchronize()
+    a.check(out, room, np.concatenate([w2.cpu().numpy(), np.zeros((2, hkv, n), np.float32)], 2), **kw)
+
+    r = rng(3)
+    table_w = torch.from_numpy((r.normal(size=(vocab, hidden)) * 0.5).astype(np.float32)).cuda().bfloat16()
+    logits = K.linear(out, table_w, out_dtype=torch.float32)
+    targets = i32(r.integers(0, vocab, 2 * n))
+    lp, ent, ids, tops = K.token_logprobs(logits, targets, top=5, softcap=30.0)
+    torch.cuda.synchronize()
+    x, t = logits.cpu().numpy(), targets.cpu().numpy()
+    for i in range(2 * n):
+        want = oracle.token_logprobs(x[i], int(t[i]), 5, 30.0)
+        assert abs(lp[i].item() - want[0]) < 1e-4 and abs(ent[i].item() - want[1]) < 1e-4
+        assert ids[i].cpu().tolist() == want[2].tolist()

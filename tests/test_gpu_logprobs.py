@@ -1,0 +1,144 @@
+"""`kernels.token_logprobs` on the GPU against the 64-bit oracle.
+
+Tolerance (u = 2^-24): with a soft-cap a capped logit is off by at most 6 u cap on the way (product, exponential,
+reciprocal, scale), without one the difference to the largest by u |x| and its conversion to base 2 by as much; a sum of
+positive terms by its depth, 32 + 6 + 8 + 2 + chunk joins < 96; the logarithm and the last difference by u of their size.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import kv4 as oracle
+from tests.conftest import i32, rng, say
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def check(x: np.ndarray, targets: np.ndarray, top: int, cap: float, got) -> None:
+    lp, ent, ids, tops = (t.cpu().numpy().astype(np.float64) for t in got)
+    for i in range(len(x)):
+        want = oracle.token_logprobs(x[i], int(targets[i]), top, cap)
+        finite = np.abs(x[i][np.isfinite(x[i])])
+        size = cap if cap else finite.max(initial=1.0)
+        tol = 2 * (12 * size + 96 + 8) * U
+        for g, w, what in ((lp[i], want[0], "log probability"), (ent[i], want[1], "entropy")):
+            assert np.isnan(g) == np.isnan(w) and np.isinf(g) == np.isinf(w), (i, what, g, w)
+            if np.isfinite(w):
+                scale = 1 + abs(want[1]) if what == "entropy" else 1.0
+                assert abs(g - w) <= tol * scale + 4 * U * abs(w), (i, what, g, w, tol)
+        assert ids[i].tolist() == want[2].tolist(), (i, ids[i], want[2])
+        t = want[3]
+        assert (np.isnan(tops[i]) == np.isnan(t)).all() and (np.isneginf(tops[i]) == np.isneginf(t)).all()
+        f = np.isfinite(t)
+        assert (np.abs(tops[i][f] - t[f]) <= tol + 4 * U * np.abs(t[f])).all(), (i, tops[i], t)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 31, 31), (2, 64, 64), (5, 2047, 3), (4, 2048, 0),
+                                            (3, 2049, 1), (2, 32001, 20), (2, 50257, 64), (1, 256000, 8)])
+def test_logprobs(rows: int, vocab: int, top: int, cap: float, dtype: str) -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"token_logprobs rows={rows} vocab={vocab} top={top} cap={cap} {dtype}")
+    r = rng(vocab + rows)
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    buf = torch.full((rows, vocab + 5), 77.0, device="cuda", dtype=t)  # rows of an odd stride, larger values beside them
+    x = torch.from_numpy((r.normal(size=(rows, vocab)) * 4).astype(np.float32)).cuda().to(t)
+    logits = buf[:, 1:vocab + 1]
+    logits.copy_(x)
+    targets = r.integers(0, vocab, rows)
+    targets[0] = vocab - 1
+    got = K.token_logprobs(logits, i32(targets), top=top, softcap=cap)
+    torch.cuda.synchronize()
+    check(x.float().cpu().numpy(), targets, top, cap, got)
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_masks_ties_and_lost_rows(cap: float) -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"token_logprobs special rows cap={cap}")
+    vocab, top = 5000, 6
+    r = rng(1)
+    x = r.normal(size=(12, vocab)).astype(np.float32)
+    x[0] = -np.inf
+    x[1] = -np.inf
+    x[1, 4321] = -29.0                    # one token left
+    x[2, :4990] = -np.inf
+    x[3] = 1.5                            # all equal: the lowest tokens
+    x[4, 2500] = np.nan
+    x[5, 7] = np.inf
+    x[6] = np.float32(torch.finfo(torch.float32).min)
+    x[7] = np.arange(vocab) * 1e-3        # rising: every group is better than the last
+    x[8] = -0.0
+    x[8, 1::2] = 0.0                      # the two zeros are equal
+    x[9] = 1e30
+    x[9, 100:] = -1e30
+    x[10] = np.where(np.arange(vocab) % 7 == 3, 2.0, 1.0)
+    targets = np.array([5, 4321, 3, 4999, 1, 7, 0, 4999, 2, 50, -1, 10])
+    got = K.token_logprobs(torch.from_numpy(x).cuda(), i32(targets), top=top, softcap=cap)
+    torch.cuda.synchronize()
+    # rows of huge logits without a cap: differences of 2e30 underflow to weight 0, the rest are exact
+    check(x, targets, top, cap, got)
+    bad = K.token_logprobs(torch.from_numpy(x[10:]).cuda(), i32([vocab, -2]), top=0, softcap=cap)
+    assert torch.isnan(bad[0]).all() and torch.isfinite(bad[1]).all()
+
+
+def test_rows_do_not_depend_on_the_batch_and_streams_and_graphs() -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("token_logprobs alone, on a side stream, in a graph")
+    r = rng(2)
+    x = torch.from_numpy((r.normal(size=(70, 32001)) * 3).astype(np.float32)).cuda()
+    targets = i32(r.integers(0, 32001, 70))
+    want = K.token_logprobs(x, targets, top=7, softcap=30.0)
+    torch.cuda.synchronize()
+    for i in (0, 33, 69):
+        one = K.token_logprobs(x[i:i + 1], targets[i:i + 1], top=7, softcap=30.0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a[0], b[i]) for a, b in zip(one, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = K.token_logprobs(x, targets, top=7, softcap=30.0)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = K.token_logprobs(x, targets, top=7, softcap=30.0)
+    for _ in range(4):
+        for t in kept:
+            t.fill_(3)
+        K.token_logprobs(x[:5], targets[:5], top=3)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, want))
+
+
+def test_many_rows() -> None:
+    """More rows than a grid's y dimension holds."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("token_logprobs 70000 rows")
+    r = rng(5)
+    x = torch.from_numpy(r.normal(size=(70000, 40)).astype(np.float32)).cuda()
+    targets = i32(r.integers(0, 40, 70000))
+    lp, ent, ids, _ = K.token_logprobs(x, targets, top=2)
+    torch.cuda.synchronize()
+    want = torch.log_softmax(x.double().cpu(), 1)
+    assert (lp.cpu().double() - want.gather(1, targets.cpu().long()[:, None])[:, 0]).abs().max() < 1e-5
+    assert (ids[:, 0].cpu() == x.cpu().argmax(1)).all()

@@ -1,0 +1,154 @@
+"""Refusals of the 4-bit cache's and the log probabilities' entry points, on the CPU: every call here is rejected (or is
+empty) before the library touches the device."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from deciax_amd import _lib
+
+P = ctypes.c_void_p(0x10000)  # an aligned, non-null stand-in; never dereferenced by these calls
+ODD = ctypes.c_void_p(0x10008)
+F = ctypes.c_float
+INVALID, UNSUPPORTED, OK = _lib.DX_ERR_INVALID, _lib.DX_ERR_UNSUPPORTED, _lib.DX_OK
+BIG = 1 << 40
+
+
+def cache(k=0x10000, v=0x10000, ks=0x10000, vs=0x10000, pos=0x10000, pages=8, hkv=2, page=64, d=128):
+    return ctypes.byref(_lib.Kv4Cache(k, v, ks, vs, pos, pages, hkv, page, d))
+
+
+CACHES = [(dict(k=None), INVALID), (dict(v=None), INVALID), (dict(ks=None), INVALID), (dict(vs=None), INVALID),
+          (dict(pos=None), INVALID), (dict(pages=-1), INVALID), (dict(hkv=0), INVALID), (dict(d=96), UNSUPPORTED),
+          (dict(d=512), UNSUPPORTED), (dict(page=32), UNSUPPORTED), (dict(page=96), UNSUPPORTED),
+          (dict(page=1 << 17), UNSUPPORTED), (dict(hkv=70000), UNSUPPORTED), (dict(k=0x10008), INVALID),
+          (dict(ks=0x10004), INVALID), (dict(pos=0x10004), INVALID)]
+
+
+def append(c=None, k=P, v=P, pos=P, table=P, width=4, start=P, new=P, ctx=P, seqs=2, max_new=8, rows=16, ks=256, vs=256,
+           dtype=_lib.DX_BF16):
+    return "dx_kv4_append", (c or cache(), k, v, pos, table, width, start, new, ctx, seqs, max_new, rows, ks, vs, dtype, None)
+
+
+def read(c=None, k=P, v=P, table=P, width=4, start=P, new=P, ctx=P, seqs=2, max_new=8, rows=16, ks=256, vs=256):
+    return "dx_kv4_read", (c or cache(), k, v, table, width, start, new, ctx, seqs, max_new, rows, ks, vs, None)
+
+
+def attend(c=None, q=P, out=P, table=P, width=4, start=P, new=P, ctx=P, seqs=2, max_new=8, max_ctx=256, rows=16, hq=4,
+           qs=512, os=512, scale=0.1, cap=50.0, window=0, w_in=None, wi=(512, 256), w_out=None, wo=(512, 256),
+           dtype=_lib.DX_BF16, ws=P, ws_bytes=BIG):
+    return "dx_attn_kv4", (c or cache(), q, out, table, width, start, new, ctx, seqs, max_new, max_ctx, rows, hq, qs, os,
+                           F(scale), F(cap), window, w_in, *wi, w_out, *wo, dtype, ws, ws_bytes, None)
+
+
+def evict(c=None, w=P, wi=(512, 256), table=P, width=4, ctx=P, seqs=2, max_ctx=256, out_table=P, out_width=2, keep=100,
+          recent=10, w_out=P, wo=(200, 100), out_len=P, ws=P, ws_bytes=BIG):
+    return "dx_kv4_evict", (c or cache(), w, *wi, table, width, ctx, seqs, max_ctx, out_table, out_width, keep, recent,
+                            w_out, *wo, out_len, ws, ws_bytes, None)
+
+
+def score(x=P, t=P, rows=3, vocab=100, ld=100, cap=30.0, top=5, lp=P, ent=P, ids=P, tops=P, dtype=_lib.DX_BF16, ws=P,
+          ws_bytes=BIG):
+    return "dx_token_logprobs", (x, t, rows, vocab, ld, F(cap), top, lp, ent, ids, tops, dtype, ws, ws_bytes, None)
+
+
+def status(call) -> int:
+    name, args = call
+    return getattr(_lib.lib(), name)(*args)
+
+
+def check(call, want: int) -> None:
+    got = status(call)
+    assert got == want, (call[0], got, want, _lib.lib().dx_last_error())
+    if want != OK:
+        assert call[0].removeprefix("dx_").encode() in _lib.lib().dx_last_error()
+
+
+@pytest.mark.parametrize("make", [append, read, attend, evict], ids=lambda f: f.__name__)
+@pytest.mark.parametrize("bad,want", CACHES)
+def test_malformed_caches_are_refused(make, bad, want) -> None:
+    check(make(c=cache(**bad)), want)
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(k=None), INVALID), (dict(v=ODD), INVALID), (dict(pos=None), INVALID), (dict(table=None), INVALID),
+    (dict(start=None), INVALID), (dict(new=None), INVALID), (dict(ctx=None), INVALID), (dict(seqs=-1), INVALID),
+    (dict(seqs=70000), UNSUPPORTED), (dict(max_new=-1), INVALID), (dict(max_new=(1 << 30) + 1), UNSUPPORTED),
+    (dict(max_new=1 << 27), UNSUPPORTED), (dict(rows=-1), INVALID), (dict(width=-1), INVALID), (dict(ks=255), INVALID),
+    (dict(vs=260), INVALID), (dict(dtype=7), INVALID), (dict(seqs=0), OK), (dict(max_new=0), OK), (dict(rows=0), OK)])
+def test_append(bad, want) -> None:
+    check(append(**bad), want)
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(k=ODD), INVALID), (dict(v=None), INVALID), (dict(table=None), INVALID), (dict(ks=128), INVALID),
+    (dict(vs=260), INVALID), (dict(max_new=1 << 27), UNSUPPORTED), (dict(seqs=0), OK), (dict(rows=0), OK)])
+def test_read(bad, want) -> None:
+    check(read(**bad), want)
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(q=None), INVALID), (dict(out=ODD), INVALID), (dict(table=None), INVALID), (dict(hq=3), INVALID),
+    (dict(hq=0), INVALID), (dict(qs=256), INVALID), (dict(os=516), INVALID), (dict(scale=0.0), INVALID),
+    (dict(scale=float("nan")), INVALID), (dict(cap=-1.0), INVALID), (dict(window=-1), INVALID), (dict(dtype=3), INVALID),
+    (dict(max_ctx=-1), INVALID), (dict(max_ctx=(1 << 30) + 1), UNSUPPORTED), (dict(max_new=1 << 26), UNSUPPORTED),
+    (dict(w_out=P), INVALID), (dict(w_in=P, w_out=P, wi=(512, 255)), INVALID),
+    (dict(w_in=P, w_out=P, wo=(512, 100)), INVALID), (dict(ws=None, max_ctx=256, w_in=P, w_out=P), INVALID),
+    (dict(ws=ctypes.c_void_p(0x10004), max_ctx=9000), INVALID), (dict(ws_bytes=16, max_ctx=9000), INVALID),
+    (dict(seqs=70000), UNSUPPORTED), (dict(seqs=0), OK), (dict(max_new=0), OK), (dict(rows=0), OK)])
+def test_attention(bad, want) -> None:
+    check(attend(**bad), want)
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(w=None), INVALID), (dict(table=None), INVALID), (dict(ctx=None), INVALID), (dict(out_table=None), INVALID),
+    (dict(w_out=None), INVALID), (dict(out_len=None), INVALID), (dict(keep=0, recent=0), INVALID),
+    (dict(recent=101), INVALID), (dict(recent=-1), INVALID), (dict(out_width=1), INVALID), (dict(wi=(512, 255)), INVALID),
+    (dict(wo=(200, 99)), INVALID), (dict(ws=None), INVALID), (dict(ws_bytes=100), INVALID), (dict(max_ctx=-1), INVALID),
+    (dict(max_ctx=(1 << 30) + 1), UNSUPPORTED), (dict(seqs=70000), UNSUPPORTED), (dict(seqs=0), OK)])
+def test_evict(bad, want) -> None:
+    check(evict(**bad), want)
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(x=None), INVALID), (dict(t=None), INVALID), (dict(lp=None), INVALID), (dict(ent=None), INVALID),
+    (dict(ids=None), INVALID), (dict(tops=None), INVALID), (dict(rows=-1), INVALID), (dict(rows=1 << 31), INVALID),
+    (dict(vocab=0), INVALID), (dict(ld=99), INVALID), (dict(cap=-1.0), INVALID), (dict(top=-1), INVALID),
+    (dict(top=101), INVALID), (dict(top=65), UNSUPPORTED), (dict(dtype=9), INVALID),
+    (dict(x=ctypes.c_void_p(0x10001)), INVALID), (dict(x=ctypes.c_void_p(0x10002), dtype=_lib.DX_F32), INVALID),
+    (dict(ws=None), INVALID), (dict(ws_bytes=10), INVALID), (dict(vocab=(1 << 30) + 1, ld=1 << 31), UNSUPPORTED),
+    (dict(rows=0), OK)])
+def test_token_logprobs(bad, want) -> None:
+    check(score(**bad), want)
+
+
+def test_workspaces_are_host_arithmetic() -> None:
+    lib = _lib.lib()
+    assert lib.dx_kv4_evict_workspace(3, 2, 100) == 2400
+    assert lib.dx_token_logprobs_workspace(2, 2049, 0) == 2 * 4 * 2 * 3
+    assert lib.dx_token_logprobs_workspace(2, 2049, 1) == 2 * 4 * (2 * 3 + 65)
+    assert lib.dx_attn_kv4_workspace(0, 1, 1, 4, 2, 128, 0, 1) == 0
+    assert lib.dx_attn_kv4_workspace(2, 1, 256, 4, 2, 128, 0, 0) == 0      # one span: no parts to join
+    short = lib.dx_attn_kv4_workspace(2, 1, 9000, 4, 2, 128, 0, 0)
+    assert 0 < short <= lib.dx_attn_kv4_workspace(2, 300, 9000, 4, 2, 128, 0, 0)
+    assert lib.dx_attn_kv4_workspace(2, 1, 9000, 4, 2, 128, 64, 0) < short  # a window splits less
+
+
+def test_tensors_in_host_memory_are_refused() -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    c = K.kv4_cache(4, 2, 64, device="cpu")
+    assert c.k.shape == (4, 2, 64, 32) and c.k_scale.shape == (4, 2, 64, 2) and c.positions.dtype == torch.int32
+    x = torch.zeros((3, 128), dtype=torch.bfloat16)
+    i = torch.zeros(1, dtype=torch.int32)
+    t = torch.zeros((1, 2), dtype=torch.int32)
+    with pytest.raises(ValueError, match="device"):
+        K.kv4_append(c, x, x, torch.zeros(3, dtype=torch.int32), t, i, i, i, 3)
+    with pytest.raises(ValueError, match="device"):
+        K.attention_kv4(x, c, t, i, i, i, 3, 3, num_q_heads=2, scale=0.1)
+    with pytest.raises(ValueError, match="device"):
+        K.token_logprobs(x, torch.zeros(3, dtype=torch.int32))
