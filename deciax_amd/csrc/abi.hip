@@ -773,7 +773,7 @@ constexpr int32_t MOST_SLOTS = 1 << 30;  // of a sequence: spans of keys are cou
 
 int validate_cache(const dx_kv4_cache *c, Kv4Cache *out, const char *what) {
   REQUIRE(c && c->k && c->v && c->k_scale && c->v_scale && c->positions, "%s: null cache array", what);
-  REQUIRE(c->num_pages >= 0 && c->num_kv_heads > 0, "%s: %d pages of %d heads", what, c->num_pages, c->num_kv_heads);
+  REQUIRE(c->num_pages > 0 && c->num_kv_heads > 0, "%s: %d pages of %d heads", what, c->num_pages, c->num_kv_heads);
   SUPPORTED(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim %d not in {64, 128, 256}", what,
             c->head_dim);
   SUPPORTED(c->page_size >= 64 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0,

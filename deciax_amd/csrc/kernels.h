@@ -162,7 +162,7 @@ struct Kv4Attn {
   float *w_out;
   long wi_seq, wi_head, wo_seq, wo_head;
   float *partial, *stats, *lse;  // workspace, laid out by dx_kv4_attn_plan
-  int part_rows, max_rows, max_splits;
+  int part_rows, max_rows, max_splits, few_rows;
 };
 // Sizes that depend on the largest lengths alone: partial rows per (sequence, kv head), rows, splits.
 struct Kv4Plan {

@@ -38,7 +38,7 @@ struct Spans {
   int lo, keys, count;
 };
 
-constexpr int SPAN = 256, MAX_SPANS = 32, SPLIT_ROWS = 2048;
+constexpr int SPAN = 256, MAX_SPANS = 32, SPLIT_ROWS = 4096;
 
 __host__ __device__ inline int most_spans(int rows) {
   const int most = SPLIT_ROWS / (rows > 0 ? rows : 1);
@@ -55,18 +55,31 @@ __host__ __device__ inline Spans spans(int ctx, int n, int rows, int window) {
   return {lo, keys, count < 1 ? 1 : count};
 }
 
+// Rows of a KV head up to which waves share rows and split keys.
+constexpr int FEW_ROWS = 48;
+
 DX_DEVICE floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// The bf16 V tile of a wave: [32 keys][D], in 32-byte units (the 16 columns one transposed read takes of a row), unit u
-// of row r at u ^ (r & 7) (r >> 1 at D 64, where a row is half the banks): the rows that a read touches fall on
-// different banks.
-template <int D>
-DX_DEVICE int unit_at(int row, int unit) {
-  if constexpr (D == 64) return row * D + ((unit ^ ((row >> 1) & 3)) << 4);
-  else return row * D + ((unit ^ (row & 7)) << 4);
+// bf16 tiles in LDS: [keys][columns] in 16-byte chunks, chunk c of row r at c ^ swizzle(r), over banks of 16 chunks.
+// V tiles: 16 lanes write a chunk each, of four rows and four blocks (chunks 4 apart; 64 columns: eight rows, two blocks,
+// and two rows share the banks); 32 lanes read the halves of two neighbouring chunks of eight rows, transposed. So the low
+// two bits differ over the four rows, and the bits above the lowest over the eight. K tiles: 16 lanes read a chunk each of
+// 16 rows; their writes as V's.
+template <int W>
+DX_DEVICE int swizzle(int r) {
+  if constexpr (W == 64) {
+    const int t = r >> 1;
+    return (t & 3) | (t & 1) << 2;
+  } else {
+    return (r & 3) | (r & 1) << 2 | (r & 4) << 1;
+  }
 }
+template <int W>
+DX_DEVICE int v_chunk(int r, int c) { return r * W + ((c ^ swizzle<W>(r)) << 3); }
+template <int W>
+DX_DEVICE int k_chunk(int r, int c) { return r * W + ((c ^ (W == 64 ? (r >> 1) & 7 : r & 15)) << 3); }
 
 DX_DEVICE s16x4 read_transposed(const uint16_t *p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -111,41 +124,42 @@ DX_DEVICE void load_query(const void *base, long at, bf16x8 (&out)[NS]) {
   }
 }
 
-// 32 keys of a page as a wave holds them before use.
+// The keys of 32 slots as a wave holds them before use: lane l has key l % 16 of each 16-key half, 16 bytes a load.
 template <int D>
-struct Raw {
-  static constexpr int KJ = D == 256 ? 2 : 1;   // K loads a 16-key half: lane l has key l % 16
-  static constexpr int VJ = D / 64;             // V loads: lane l has 32 dimensions of one key, rows in order
-  u32x4 k[2][KJ], v[VJ];
-  uint32_t ks[2][KJ], vs[VJ];
+struct Keys {
+  static constexpr int N = D == 256 ? 2 : 1;
+  u32x4 k[2][N];
+  float scale[2][N];
 };
 
+// From memory; row0 is the same in all lanes.
 template <int D>
-DX_DEVICE void load_keys(Raw<D> &w, const Kv4Cache &c, long row0, int lane) {
+DX_DEVICE void load_keys(Keys<D> &w, const Kv4Cache &c, long row0, int lane) {
+  const uint8_t *codes = c.k + row0 * (D / 2), *scales = c.ks + row0 * (D / 32);
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const long row = row0 + t * 16 + (lane & 15);
+    const uint32_t row = t * 16 + (lane & 15), grp = lane >> 4;
     if constexpr (D == 64) {  // a lane group takes half a block
-      const u32x2 x = *reinterpret_cast<const u32x2 *>(c.k + row * 32 + (lane >> 4) * 8);
+      const u32x2 x = *reinterpret_cast<const u32x2 *>(codes + (row * 32 + grp * 8));
       w.k[t][0] = u32x4{x[0], x[1], 0, 0};
-      w.ks[t][0] = c.ks[row * 2 + (lane >> 5)];
+      w.scale[t][0] = scale_of(scales[row * 2 + (grp >> 1)]);
     } else {
 #pragma unroll
-      for (int j = 0; j < Raw<D>::KJ; ++j) {
-        w.k[t][j] = *reinterpret_cast<const u32x4 *>(c.k + row * (D / 2) + (j * 4 + (lane >> 4)) * 16);
-        w.ks[t][j] = c.ks[row * (D / 32) + j * 4 + (lane >> 4)];
+      for (int j = 0; j < Keys<D>::N; ++j) {
+        w.k[t][j] = *reinterpret_cast<const u32x4 *>(codes + (row * (D / 2) + (j * 4 + grp) * 16));
+        w.scale[t][j] = scale_of(scales[row * (D / 32) + j * 4 + grp]);
       }
     }
   }
 }
 
-template <int D>
-DX_DEVICE void load_values(Raw<D> &w, const Kv4Cache &c, long row0, int lane) {
+// The wait for these loads here and not at their first use: inside a loop it would be a wait for the loop's own loads.
+template <int N, int NS>
+DX_DEVICE void settle(bf16x8 (&q)[N][NS]) {
 #pragma unroll
-  for (int j = 0; j < Raw<D>::VJ; ++j) {
-    w.v[j] = *reinterpret_cast<const u32x4 *>(c.v + row0 * (D / 2) + (j * 64 + lane) * 16);
-    w.vs[j] = c.vs[row0 * (D / 32) + j * 64 + lane];
-  }
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int n = 0; n < NS; ++n) asm volatile("" : "+v"(q[i][n]));
 }
 
 // Dimension of element 0 of lane group `grp` in the i-th product of a 16-key half (eight consecutive ones follow).
@@ -154,66 +168,273 @@ DX_DEVICE int product_dim(int i, int grp) {
   return D == 64 ? grp * 16 + i * 8 : ((i >> 2) * 4 + grp) * 32 + (i & 3) * 8;
 }
 
-// Scores of one 16-key half, in base 2. The product is read in the block that issued it: where a uniform branch came
-// between the two, the compiler left out the wait states that a matrix result needs before it is read (a path of 6
-// instead of 8 was there, and the last two of the four values were stale).
-template <int D, int NS, bool CAP>
-DX_DEVICE void key_scores(const Raw<D> &w, int t, const bf16x8 (&q)[D / 32][NS], float scale, float softcap,
-                          float (&t2)[4]) {
-  floatx4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const int j = D == 64 ? 0 : i >> 2;
-    const bf16x8 a = as_bf16x8(decode8(w.k[t][j][i & 3], scale_of(w.ks[t][j])));
-#pragma unroll
-    for (int n = 0; n < NS; ++n) s = mfma16(a, q[i][n], s);
-  }
-  const float c = CAP ? scale / softcap : scale * LOG2E;
+// softcap log2(e) tanh(x) of four values. The continued fraction of tanh, cut after x^13, is x N(x^2) / M(x^2) with the
+// polynomials below, off by 1.2e-8 of the value at |x| <= 2 (scores up to twice the cap) and by fp32's rounding below
+// that: relative precision where scores are small, which 1 - 2 / (1 + e^2x) has not. That form serves beyond, in a
+// branch that real scores do not take.
+DX_DEVICE void capped(float (&x)[4], float cap2) {
+  float t[4];
+  bool far = false;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    t2[r] = s[r] * c;
-    asm volatile("" : "+v"(t2[r]));  // here, not where a later block uses it
+    const float y = x[r] * x[r];
+    const float n = __builtin_fmaf(__builtin_fmaf(y + 378.f, y, 17325.f), y, 135135.f);
+    const float m = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(28.f, y, 3150.f), y, 62370.f), y, 135135.f);
+    t[r] = x[r] * n * fast_rcp(m) * cap2;
+    far = far || !(y <= 4.f);
   }
-  if constexpr (CAP) {
+  if (__any(far)) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) t2[r] = softcap * LOG2E * tanhf(t2[r]);
+    for (int r = 0; r < 4; ++r) {
+      const float e = 1.f - 2.f * fast_rcp(1.f + fast_exp2(2.f * LOG2E * fabsf(x[r])));
+      t[r] = x[r] * x[r] <= 4.f ? t[r] : cap2 * copysignf(e, x[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = t[r];
+}
+
+// Products to what the soft-cap takes, or to scores in base 2. They are read in the block that issued them: where a
+// uniform branch came between, the compiler left out the wait states that a matrix result needs before it is read (a path
+// of 6 instead of 7 was there, and the last two of the four values were stale).
+template <int N, bool CAP>
+DX_DEVICE void products(const floatx4 (&s)[N], float scale, float softcap, float (&x)[N][4]) {
+  const float c = CAP ? scale / softcap : scale * LOG2E;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[n][r] = s[n][r] * c;
+      asm volatile("" : "+v"(x[n][r]));  // here, not where a later block uses it
+    }
+}
+
+// Scores of 32 keys: element 4 t + r is key 16 t + 4 (lane / 16) + r.
+template <int D, int NS, bool CAP>
+DX_DEVICE void key_scores(const Keys<D> &w, const bf16x8 (&q)[D / 32][NS], float scale, float softcap,
+                          float (&t2)[2][4]) {
+  floatx4 s[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int j = D == 64 ? 0 : i >> 2;
+      const bf16x8 a = as_bf16x8(decode8(w.k[t][j][i & 3], w.scale[t][j]));
+#pragma unroll
+      for (int n = 0; n < NS; ++n) s[t] = mfma16(a, q[i][n], s[t]);
+    }
+  products<2, CAP>(s, scale, softcap, t2);
+  if constexpr (CAP) {
+    capped(t2[0], softcap * LOG2E);
+    capped(t2[1], softcap * LOG2E);
   }
 }
 
-template <int D, int NS, bool CAP>
-__global__ void __launch_bounds__(THREADS) kv4_attn_kernel(Kv4Attn a) {
-  constexpr int LPK = D / 32;  // lanes (blocks) a key in a V load
-  __shared__ __attribute__((aligned(1024))) uint16_t tile[WAVES][STEP * D];
+// The pages of a span, a lane each (64 at a time), so that the loop over keys looks none up in memory.
+struct Pages {
+  const int32_t *table;
+  int width, first, page;  // `page`: of this lane, table[first + lane]
+
+  DX_DEVICE void load(int at, int lane) {
+    first = at;
+    page = at + lane < width ? table[at + lane] : -1;
+  }
+  // row_of(slot), for a slot that is the same in all lanes
+  DX_DEVICE long row(const Kv4Cache &c, int g, int slot, int lane) {
+    const int at = slot >> c.shift;
+    if (at - first >= 64 || at < first) {
+      load(at, lane);
+      // wait here: behind the branch the wait would be for all loads on their way, taken or not
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    }
+    const int p = __builtin_amdgcn_readlane(page, at - first);
+    if (p < 0 || p >= c.pages) return -1;
+    return (((long)p * c.hkv + g) << c.shift) + (slot & ((1 << c.shift) - 1));
+  }
+};
+
+// One query row as the mask and the addresses need it.
+struct Row {
+  bool real;    // a row of the packed q
+  int own;      // its own slot
+  int own_pos;  // and that slot's position, for a window
+  long at;      // its first element in q
+};
+
+DX_DEVICE Row query_row(const Kv4Attn &a, const Sequence &s, const int32_t *table, int g, int row, int rows, int group) {
+  Row r;
+  const int token = row / group;
+  r.real = row < rows && s.start + token >= 0 && s.start + token < a.q.rows;
+  r.own = s.ctx - s.n + token;
+  r.own_pos = 0;
+  if (a.window > 0 && r.real && r.own >= 0) {
+    const long at = row_of(a.c, table, g, r.own);
+    r.own_pos = at >= 0 ? a.c.pos[at] : 0;
+  }
+  // a row that is none reads the first one: its column of the products goes nowhere
+  r.at = r.real ? (s.start + token) * a.q_stride + (long)(g * group + row % group) * a.c.d : 0;
+  return r;
+}
+
+// Which of the four keys from `key` on (positions `pos`) a row sees; the scores of the others become -inf.
+template <bool WIN>
+DX_DEVICE uint32_t mask4(const Kv4Attn &a, const Row &row, int key, const int4 &pos, float (&t2)[4]) {
+  const int p[4] = {pos.x, pos.y, pos.z, pos.w};
+  uint32_t seen = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    bool see = key + r <= row.own;
+    if constexpr (WIN) see = see && key + r > row.own - a.slots && (long)p[r] > (long)row.own_pos - a.window;
+    if (!see) t2[r] = -INFINITY;
+    seen |= (uint32_t)see << r;
+  }
+  return seen;
+}
+
+// The softmax of eight more scores a lane (32 keys a row): raises the running maximum `m`, scales what was summed, and
+// gives P as the matrix operand. The lanes of a row keep partial sums `l`, joined at the end.
+template <int ND, int NS>
+DX_DEVICE void softmax_step(const float (&t2)[2][4], float &m, float &l, floatx4 (&o)[ND], bf16x8 (&pb)[NS]) {
+  float top = t2[0][0];
+#pragma unroll
+  for (int r = 1; r < 8; ++r) top = fmaxf(top, t2[r >> 2][r & 3]);
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  if (__any(top > m)) {
+    const float next = fmaxf(m, top);
+    const float f = next == -INFINITY ? 1.f : fast_exp2(m - next);
+    m = next;
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i] *= f;
+  }
+  const float base = m == -INFINITY ? 0.f : m;
+  float p[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    p[r] = fast_exp2(t2[r >> 2][r & 3] - base);
+    l += p[r];
+  }
+  split8<NS>(p, pb);
+}
+
+// How much a part with maximum m and sum l weighs beside a maximum `top`: 0 for one that saw nothing.
+DX_DEVICE float part_weight(float m, float l, float top) {
+  return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : fast_exp2(m - top);
+}
+
+// Four dimensions of one row: to the output where its keys are one span, else to the workspace.
+template <int D, int NS>
+DX_DEVICE void store_row(const Kv4Attn &a, const Sequence &s, const Spans &sp, long unit, int g, int group, int rows,
+                         int split, int row, int d, floatx4 acc, float m, float l) {
+  if (sp.count == 1) {
+    acc *= l == 0.f ? 0.f : 1.f / l;
+    const long out_row = s.start + row / group;
+    if (out_row >= 0 && out_row < a.q.rows) {
+      const long at = out_row * a.out_stride + (long)(g * group + row % group) * D + d;
+      if constexpr (NS == 1) {
+        const u32x2 y = {pack_bf2(acc[0], acc[1]), pack_bf2(acc[2], acc[3])};
+        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + at) = y;
+      } else {
+        *reinterpret_cast<floatx4 *>(static_cast<float *>(a.out) + at) = acc;
+      }
+    }
+    if (a.w_out && d == 0) a.lse[unit * a.max_rows + row] = m + log2f(l);
+  } else {
+    const long p = unit * a.part_rows + (long)split * rows + row;
+    *reinterpret_cast<floatx4 *>(a.partial + p * D + d) = acc;
+    if (d == 0) {
+      a.stats[p * 2] = m;
+      a.stats[p * 2 + 1] = l;
+    }
+  }
+}
+
+// Few rows: the four waves share 16 rows and take 32 keys in turn. What bounds this kernel is the time that a step's loads
+// take, so a step's registers are filled with the next one's as soon as they have been used: K's at the step's start, V's
+// once it is decoded. Loads are contiguous over the lanes (16 rows of one chunk, as the product wants K, made the vector
+// cache look at each lane by itself: 865 accesses a step where 140 do); K gets its order in LDS.
+template <int D>
+struct Stage {  // of a wave
+  static constexpr int VW = D < 128 ? D : 128;  // columns of V in bf16 at a time
+  alignas(1024) uint8_t k[STEP * D / 2];
+  uint16_t vt[STEP * VW];
+};
+
+template <int D, int NS, bool CAP, bool WIN>
+__global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_kernel(Kv4Attn a) {
+  constexpr int LPK = D / 32, VW = Stage<D>::VW, VB = VW / 32;  // blocks of a key, columns and blocks of V at a time
+  constexpr int KL = D / 64;                                    // loads of a step's K
+  constexpr int VK = 64 / VB, VJ = STEP / VK;                   // keys of one load of V, loads of VW columns
+  __shared__ union {
+    Stage<D> stage;
+    float part[16 * D];
+  } stages[WAVES];
   __shared__ float join_m[WAVES][16], join_l[WAVES][16];
   const int g = blockIdx.y, b = blockIdx.z;
-  const int split = blockIdx.x % a.max_splits, row_tile = blockIdx.x / a.max_splits;
+  const int tiles = gridDim.x / a.max_splits, row_tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
   const Sequence s = sequence(a.q, b, a.c.shift);
   const int group = a.hq / a.c.hkv, rows = s.n * group, r0 = row_tile * 16;
-  if (r0 >= rows) return;
+  if (r0 >= rows || rows > a.few_rows) return;
   const Spans sp = spans(s.ctx, s.n, rows, a.slots);
   if (split >= sp.count) return;
   const int32_t *table = a.q.table + (long)b * a.q.table_width;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int k0 = sp.lo + split * sp.keys, k1 = min(s.ctx, k0 + sp.keys);
+  Pages pages{table, a.q.table_width, 0, -1};
+  pages.load(k0 >> a.c.shift, lane);
+  Stage<D> &st = stages[wave].stage;
 
-  const int row = r0 + col, token = row / group;
-  const bool real = row < rows && s.start + token >= 0 && s.start + token < a.q.rows;
-  const int own = s.ctx - s.n + token;  // the row's own slot
+  // Where 16-byte chunk x of 32 rows of K stands in the stage: a row's chunks are exchanged so that 16 rows' reads of one
+  // chunk fall on all banks.
+  auto k_slot = [](int x) {
+    if constexpr (D == 256) return ((x & ~7) | ((x & 7) ^ ((x >> 4) & 7))) * 16;
+    else if constexpr (D == 128) return ((x & ~3) | ((x & 3) ^ ((x >> 4) & 3))) * 16;
+    else return x * 16;
+  };
+  u32x4 kr[KL], vr[D / VW][VJ];
+  uint32_t ks[2][Keys<D>::N], vs[D / VW][VJ];
+  int4 pos[2] = {};
+  // A step without a page, or past the span's end, reads the pool's first rows instead: nothing of them is seen. No branch
+  // goes round the loads, behind which the compiler could only wait for all of them.
+  auto fetch_keys = [&](int kb) {
+    const long row0 = kb < k1 ? pages.row(a.c, g, kb, lane) : -1, at = max(row0, 0L);
+    const uint8_t *codes = a.c.k + at * (D / 2), *scales = a.c.ks + at * LPK;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) kr[i] = *reinterpret_cast<const u32x4 *>(codes + (uint32_t)(i * 64 + lane) * 16);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < Keys<D>::N; ++j)
+        ks[t][j] = scales[(uint32_t)((t * 16 + col) * LPK + (D == 64 ? grp >> 1 : j * 4 + grp))];
+    if constexpr (WIN) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) pos[t] = *reinterpret_cast<const int4 *>(a.c.pos + at + t * 16 + grp * 4);
+    }
+    return row0;
+  };
+  auto fetch_values = [&](long row0) {
+    const long at = max(row0, 0L);
+    const uint8_t *codes = a.c.v + at * (D / 2), *scales = a.c.vs + at * LPK;
+#pragma unroll
+    for (int h = 0; h < D / VW; ++h)
+#pragma unroll
+      for (int j = 0; j < VJ; ++j) {
+        const uint32_t block = (j * VK + lane / VB) * LPK + h * VB + lane % VB;
+        vr[h][j] = *reinterpret_cast<const u32x4 *>(codes + block * 16);
+        vs[h][j] = scales[block];
+      }
+  };
+
+  const Row row = query_row(a, s, table, g, r0 + col, rows, group);
   bf16x8 q[D / 32][NS];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    if (real) load_query<NS>(a.query, (s.start + token) * a.q_stride + (long)(g * group + row % group) * D +
-                                          product_dim<D>(i, grp), q[i]);
-    else
-#pragma unroll
-      for (int n = 0; n < NS; ++n) q[i][n] = as_bf16x8(u32x4{0, 0, 0, 0});
-  }
-  int own_pos = 0;
-  if (a.window > 0 && real && own >= 0) {
-    const long r = row_of(a.c, table, g, own);
-    own_pos = r >= 0 ? a.c.pos[r] : 0;
-  }
+  for (int i = 0; i < D / 32; ++i) load_query<NS>(a.query, row.at + product_dim<D>(i, grp), q[i]);
+  int kb = k0 + wave * STEP;
+  long row0 = fetch_keys(kb);
+  fetch_values(row0);
+  settle(q);
   // keys below `open` are seen by every row of the tile, as far as the order of tokens goes
   const int open = s.ctx - s.n + r0 / group + 1;
 
@@ -221,100 +442,85 @@ __global__ void __launch_bounds__(THREADS) kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  uint16_t *mine = tile[wave];
 
-  for (int kb = k0 + wave * STEP; kb < k1; kb += WAVES * STEP) {
-    const long row0 = row_of(a.c, table, g, kb);
-    if (row0 < 0) continue;
-    Raw<D> w;
-    load_keys<D>(w, a.c, row0, lane);
-    load_values<D>(w, a.c, row0, lane);
-    float t2[8];
+  for (; kb < k1; kb += WAVES * STEP) {
+    const bool page = row0 >= 0;
+    Keys<D> w;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) *reinterpret_cast<u32x4 *>(st.k + k_slot(i * 64 + lane)) = kr[i];
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      float half[4];
-      key_scores<D, NS, CAP>(w, t, q, a.scale, a.softcap, half);
+      const int r = t * 16 + col;
+      if constexpr (D == 64) {
+        const u32x2 x = *reinterpret_cast<const u32x2 *>(st.k + r * 32 + grp * 8);
+        w.k[t][0] = u32x4{x[0], x[1], 0, 0};
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t2[t * 4 + r] = half[r];
+        for (int j = 0; j < Keys<D>::N; ++j) w.k[t][j] = *reinterpret_cast<const u32x4 *>(st.k + k_slot(r * LPK + j * 4 + grp));
+      }
+#pragma unroll
+      for (int j = 0; j < Keys<D>::N; ++j) {
+        w.scale[t][j] = scale_of(ks[t][j]);
+        asm volatile("" : "+v"(w.scale[t][j]));  // before the next ones are asked for, not with a copy of them
+      }
     }
-    const bool masked = a.window > 0 || kb + STEP > open;
+    int4 here[2] = {pos[0], pos[1]};
+    if constexpr (WIN) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(here[t].x), "+v"(here[t].y), "+v"(here[t].z), "+v"(here[t].w));
+    }
+    const long next = fetch_keys(kb + WAVES * STEP);
+
+    float t2[2][4];
+    key_scores<D, NS, CAP>(w, q, a.scale, a.softcap, t2);
+    const bool masked = WIN || kb + STEP > open || !page;
     uint32_t seen = 0xff;  // of this lane's eight keys
     if (masked) {
       seen = 0;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int key = kb + t * 16 + grp * 4;
-        int pos[4] = {0, 0, 0, 0};
-        if (a.window > 0) {
-          const int4 p = *reinterpret_cast<const int4 *>(a.c.pos + row0 + t * 16 + grp * 4);
-          pos[0] = p.x, pos[1] = p.y, pos[2] = p.z, pos[3] = p.w;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          bool see = key + r <= own;
-          if (a.window > 0)
-            see = see && key + r > own - a.slots && (long)pos[r] > (long)own_pos - a.window;
-          if (!see) t2[t * 4 + r] = -INFINITY;
-          seen |= (uint32_t)see << (t * 4 + r);
-        }
-      }
-    }
-    float top = t2[0];
-#pragma unroll
-    for (int r = 1; r < 8; ++r) top = fmaxf(top, t2[r]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m)) {
-      const float next = fmaxf(m, top);
-      const float f = next == -INFINITY ? 1.f : fast_exp2(m - next);
-      m = next;
-      l *= f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) o[i] *= f;
-    }
-    const float base = m == -INFINITY ? 0.f : m;
-    float p[8];
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      p[r] = fast_exp2(t2[r] - base);
-      l += p[r];
+      for (int t = 0; t < 2; ++t)
+        seen |= mask4<WIN>(a, row, page ? kb + t * 16 + grp * 4 : 0x7ffffff0, here[t], t2[t]) << (4 * t);
     }
     bf16x8 pb[NS];
-    split8<NS>(p, pb);
+    softmax_step<D / 16, NS>(t2, m, l, o, pb);
 
-    // V to LDS. Slots behind the sequence hold anything: zeros here. A block of NaN may stand behind a row's own token
-    // too, where 0 NaN would reach the row: such blocks are zero here and added below to the rows that see them.
-    uint64_t nan_blocks[Raw<D>::VJ];
+    // V to bf16, VW columns at a time. Slots behind the sequence hold anything: zeros here. A block of NaN may stand behind
+    // a row's own token too, where 0 NaN would reach the row: such blocks are zero here and added below to the rows that
+    // see them.
+    uint64_t nan_blocks[D / VW][VJ];
     bool any_nan = false;
 #pragma unroll
-    for (int j = 0; j < Raw<D>::VJ; ++j) {
-      const int key = j * (64 / LPK) + lane / LPK;
-      u32x4 x = w.v[j];
-      uint32_t byte = w.vs[j];
-      if (masked) {
-        const bool inside = kb + key < s.ctx, bad = byte == 255;
-        nan_blocks[j] = __ballot(inside && bad);
-        any_nan = any_nan || nan_blocks[j] != 0;
-        if (!inside || bad) {
-          x = u32x4{0, 0, 0, 0};
-          byte = 127;
+    for (int h = 0; h < D / VW; ++h) {
+#pragma unroll
+      for (int j = 0; j < VJ; ++j) {
+        const int key = j * VK + lane / VB;
+        u32x4 x = vr[h][j];
+        uint32_t byte = vs[h][j];
+        if (masked) {
+          const bool inside = page && kb + key < s.ctx, bad = byte == 255;
+          nan_blocks[h][j] = __ballot(inside && bad);
+          any_nan = any_nan || nan_blocks[h][j] != 0;
+          if (!inside || bad) {
+            x = u32x4{0, 0, 0, 0};
+            byte = 127;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<u32x4 *>(st.vt + v_chunk<VW>(key, lane % VB * 4 + i)) = decode8(x[i], scale_of(byte));
       }
-      const int unit = (lane % LPK) * 2;
+      if (h == D / VW - 1) fetch_values(next);
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<u32x4 *>(mine + unit_at<D>(key, unit + (i >> 1)) + (i & 1) * 8) =
-            decode8(x[i], scale_of(byte));
-    }
-    __builtin_amdgcn_wave_barrier();
+      for (int i = 0; i < VW / 16; ++i) {
+        const uint16_t *p0 = st.vt + v_chunk<VW>(grp * 4 + (col >> 2), 2 * i + ((col >> 1) & 1)) + (col & 1) * 4;
+        const s16x4 v0 = read_transposed(p0), v1 = read_transposed(p0 + 16 * VW);  // 16 rows on: the same place
+        const bf16x8 vt = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const uint16_t *p0 = mine + unit_at<D>(grp * 4 + (col >> 2), i) + (col & 3) * 4;
-      const uint16_t *p1 = mine + unit_at<D>(16 + grp * 4 + (col >> 2), i) + (col & 3) * 4;
-      const s16x4 v0 = read_transposed(p0), v1 = read_transposed(p1);
-      const bf16x8 vt = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int n = 0; n < NS; ++n) o[i] = mfma16(vt, pb[n], o[i]);
+        for (int n = 0; n < NS; ++n) o[h * (VW / 16) + i] = mfma16(vt, pb[n], o[h * (VW / 16) + i]);
+      }
+      __builtin_amdgcn_wave_barrier();
     }
     if (masked && any_nan) {
 #pragma unroll
@@ -323,10 +529,10 @@ __global__ void __launch_bounds__(THREADS) kv4_attn_kernel(Kv4Attn a) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const int key = (r >> 2) * 16 + grp * 4 + (r & 3);
-          uint64_t bits = nan_blocks[0];
+          uint64_t bits = nan_blocks[blk / VB][0];
 #pragma unroll
-          for (int j = 1; j < Raw<D>::VJ; ++j) bits = key / (64 / LPK) == j ? nan_blocks[j] : bits;
-          hit |= (int)((bits >> (key % (64 / LPK) * LPK + blk)) & 1) & (int)((seen >> r) & 1);
+          for (int j = 1; j < VJ; ++j) bits = key / VK == j ? nan_blocks[blk / VB][j] : bits;
+          hit |= (int)((bits >> (key % VK * VB + blk % VB)) & 1) & (int)((seen >> r) & 1);
         }
         hit |= __shfl_xor(hit, 16, 64);
         hit |= __shfl_xor(hit, 32, 64);
@@ -336,12 +542,12 @@ __global__ void __launch_bounds__(THREADS) kv4_attn_kernel(Kv4Attn a) {
         }
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    row0 = next;
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
-  // the four waves' parts, through LDS: [16 rows][D] fp32 a wave, where its V tile was
+  // the four waves' parts, through LDS: [16 rows][D] fp32 a wave, where its stage was
   if (grp == 0) {
     join_m[wave][col] = m;
     join_l[wave][col] = l;
@@ -350,9 +556,8 @@ __global__ void __launch_bounds__(THREADS) kv4_attn_kernel(Kv4Attn a) {
   float top = join_m[0][col];
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) top = fmaxf(top, join_m[w][col]);
-  const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : fast_exp2(m - top);
-  float *part = reinterpret_cast<float *>(mine);
-  static_assert(sizeof(tile[0]) >= 16 * D * sizeof(float), "a wave's rows fit its V tile");
+  const float f = part_weight(m, l, top);
+  float *part = stages[wave].part;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
     *reinterpret_cast<floatx4 *>(part + col * D + i * 16 + grp * 4) = o[i] * f;
@@ -367,34 +572,211 @@ __global__ void __launch_bounds__(THREADS) kv4_attn_kernel(Kv4Attn a) {
     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      const float lw = join_l[w][r], mw = join_m[w][r];
-      ll += lw * (mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw - mm));
-      acc += *reinterpret_cast<const floatx4 *>(reinterpret_cast<const float *>(tile[w]) + r * D + d);
+      ll += join_l[w][r] * part_weight(join_m[w][r], join_l[w][r], mm);
+      acc += *reinterpret_cast<const floatx4 *>(stages[w].part + r * D + d);
     }
-    const int tok = (r0 + r) / group, h = g * group + (r0 + r) % group;
-    const long unit = (long)b * a.c.hkv + g;
-    if (sp.count == 1) {
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;
-      acc *= inv;
-      const long out_row = s.start + tok;
-      if (out_row >= 0 && out_row < a.q.rows) {
-        const long at = out_row * a.out_stride + (long)h * D + d;
-        if constexpr (NS == 1) {
-          const u32x2 y = {pack_bf2(acc[0], acc[1]), pack_bf2(acc[2], acc[3])};
-          *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + at) = y;
-        } else {
-          *reinterpret_cast<floatx4 *>(static_cast<float *>(a.out) + at) = acc;
+    store_row<D, NS>(a, s, sp, (long)b * a.c.hkv + g, g, group, rows, split, r0 + r, d, acc, mm, ll);
+  }
+}
+
+// Many rows: TW waves of 16 NT rows each walk the same keys, decoded once a workgroup to bf16 in LDS, two tiles of TK
+// keys in turn: a tile's codes are on their way while the one before is used, and go to the other half of LDS after it.
+template <int D>
+constexpr int tile_keys() { return D == 256 ? 32 : 64; }
+
+template <int D, int NS, bool CAP, int NT, int TW>
+__global__ void __launch_bounds__(64 * TW, D == 256 && NS > 1 ? 1 : 2) kv4_attn_tile_kernel(Kv4Attn a) {
+  constexpr int TK = tile_keys<D>(), LPK = D / 32, T = 64 * TW;
+  constexpr int CHUNKS = TK * LPK;        // 16-byte chunks (blocks) of K, and of V, in a tile
+  constexpr int LOADS = 2 * CHUNKS / T;   // of a thread
+  static_assert(2 * CHUNKS % T == 0 && CHUNKS % 64 == 0, "whole waves load K or V");
+  __shared__ __attribute__((aligned(1024))) uint16_t kt[2][TK * D], vt[2][TK * D];
+  __shared__ uint8_t nan_block[2][CHUNKS];
+  __shared__ uint8_t nan_wave[2][TW];
+  const int g = blockIdx.y, b = blockIdx.z;
+  const int tiles = gridDim.x / a.max_splits, row_tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+  const Sequence s = sequence(a.q, b, a.c.shift);
+  const int group = a.hq / a.c.hkv, rows = s.n * group, r0 = row_tile * (16 * NT * TW);
+  if (r0 >= rows || rows <= a.few_rows) return;
+  const Spans sp = spans(s.ctx, s.n, rows, a.slots);
+  if (split >= sp.count) return;
+  const int32_t *table = a.q.table + (long)b * a.q.table_width;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  // the span's keys that some row of this workgroup sees
+  const int last_own = s.ctx - s.n + (min(r0 + 16 * NT * TW, rows) - 1) / group;
+  const int first_own = s.ctx - s.n + r0 / group;
+  int k0 = sp.lo + split * sp.keys;
+  const int k1 = min(min(s.ctx, k0 + sp.keys), last_own + 1);
+  if (a.window > 0) k0 = max(k0, (first_own - a.slots + 1) & ~63);
+  Pages pages{table, a.q.table_width, 0, -1};
+  pages.load(max(k0, 0) >> a.c.shift, lane);
+
+  const int w0 = r0 + wave * 16 * NT;  // this wave's first row
+  Row row[NT];
+  bf16x8 q[NT][D / 32][NS];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    row[n] = query_row(a, s, table, g, w0 + n * 16 + col, rows, group);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) load_query<NS>(a.query, row[n].at + i * 32 + grp * 8, q[n][i]);
+  }
+  const int open = s.ctx - s.n + w0 / group + 1;                               // as above, for the wave's rows
+  const int shut = s.ctx - s.n + (min(w0 + 16 * NT, rows) - 1) / group + 1;  // keys from here on no row sees
+  const bool idle = w0 >= rows;
+
+  floatx4 o[NT][D / 16];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  u32x4 raw[LOADS];
+  uint32_t byte[LOADS];
+  // Load c of a tile: block c % LPK of key c / LPK. A tile lies in one page.
+  auto fetch = [&](int kb) {
+    const long row0 = kb < k1 ? pages.row(a.c, g, kb, lane) : -1, from = max(row0, 0L);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int c = i * T + tid;
+      const uint32_t chunk = c % CHUNKS;
+      const bool keys = __builtin_amdgcn_readfirstlane(c) < CHUNKS;
+      raw[i] = *reinterpret_cast<const u32x4 *>((keys ? a.c.k : a.c.v) + from * (D / 2) + chunk * 16);
+      byte[i] = ((keys ? a.c.ks : a.c.vs) + from * LPK)[chunk];
+    }
+    return row0;
+  };
+  auto decode = [&](int half, int kb) {
+    bool bad_here = false;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int c = i * T + tid, chunk = c % CHUNKS, key = chunk / LPK, blk = chunk % LPK;
+      if (c < CHUNKS) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<u32x4 *>(kt[half] + k_chunk<D>(key, blk * 4 + x)) = decode8(raw[i][x], scale_of(byte[i]));
+      } else {
+        const bool inside = kb + key < k1, bad = inside && byte[i] == 255;
+        if (!inside || bad) {
+          raw[i] = u32x4{0, 0, 0, 0};
+          byte[i] = 127;
         }
-      }
-      if (a.w_out && d == 0) a.lse[unit * a.max_rows + r0 + r] = mm + log2f(ll);
-    } else {
-      const long p = unit * a.part_rows + (long)split * rows + r0 + r;
-      *reinterpret_cast<floatx4 *>(a.partial + p * D + d) = acc;
-      if (d == 0) {
-        a.stats[p * 2] = mm;
-        a.stats[p * 2 + 1] = ll;
+        nan_block[half][key * LPK + blk] = bad;
+        bad_here = bad_here || bad;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<u32x4 *>(vt[half] + v_chunk<D>(key, blk * 4 + x)) = decode8(raw[i][x], scale_of(byte[i]));
       }
     }
+    const bool any = __any(bad_here);
+    if (lane == 0) nan_wave[half][wave] = any;
+  };
+
+  // 32 keys of the tile in `half`, from row `at` of it, for this wave's rows
+  auto use = [&](int half, int at, int kb, long row0) {
+    if (idle || row0 < 0 || kb >= shut || kb >= k1) return;
+    const bool masked = a.window > 0 || kb + STEP > open;
+    float t2[NT][2][4];
+    uint32_t seen[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) seen[n] = 0xff;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int4 pos{0, 0, 0, 0};
+      if (a.window > 0) pos = *reinterpret_cast<const int4 *>(a.c.pos + row0 + t * 16 + grp * 4);
+      floatx4 sc[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const bf16x8 k = as_bf16x8(*reinterpret_cast<const u32x4 *>(kt[half] + k_chunk<D>(at + t * 16 + col, i * 4 + grp)));
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < NS; ++x) sc[n] = mfma16(k, q[n][i][x], sc[n]);
+      }
+      float part[NT][4];
+      products<NT, CAP>(sc, a.scale, a.softcap, part);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (CAP) capped(part[n], a.softcap * LOG2E);
+        if (masked) {
+          const uint32_t see = a.window > 0 ? mask4<true>(a, row[n], kb + t * 16 + grp * 4, pos, part[n])
+                                            : mask4<false>(a, row[n], kb + t * 16 + grp * 4, pos, part[n]);
+          seen[n] = t == 0 ? see : seen[n] | see << 4;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t2[n][t][r] = part[n][r];
+      }
+    }
+    bf16x8 pb[NT][NS];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) softmax_step<D / 16, NS>(t2[n], m[n], l[n], o[n], pb[n]);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const uint16_t *p0 = vt[half] + v_chunk<D>(at + grp * 4 + (col >> 2), 2 * i + ((col >> 1) & 1)) + (col & 1) * 4;
+      const uint16_t *p1 = p0 + 16 * D;
+      const s16x4 v0 = read_transposed(p0), v1 = read_transposed(p1);
+      const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < NS; ++x) o[n][i] = mfma16(v, pb[n][x], o[n][i]);
+    }
+    uint32_t flags = 0;
+#pragma unroll
+    for (int w = 0; w < TW; ++w) flags |= nan_wave[half][w];
+    if (flags) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int blk = 0; blk < LPK; ++blk) {
+          int hit = 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int key = at + (r >> 2) * 16 + grp * 4 + (r & 3);
+            hit |= (int)nan_block[half][key * LPK + blk] & (int)((seen[n] >> r) & 1);
+          }
+          hit |= __shfl_xor(hit, 16, 64);
+          hit |= __shfl_xor(hit, 32, 64);
+          if (hit) {
+            o[n][2 * blk] += NAN;
+            o[n][2 * blk + 1] += NAN;
+          }
+        }
+    }
+  };
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n) settle(q[n]);
+  if (k0 < k1) {
+    long here = fetch(k0);
+    decode(0, k0);
+    __syncthreads();
+    int half = 0;
+    for (int kb = k0; kb < k1; kb += TK) {
+      const long next = fetch(kb + TK);
+#pragma unroll
+      for (int at = 0; at < TK; at += STEP) use(half, at, kb + at, here < 0 ? -1 : here + at);
+      decode(half ^ 1, kb + TK);
+      here = next;
+      half ^= 1;
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    l[n] += __shfl_xor(l[n], 16, 64);
+    l[n] += __shfl_xor(l[n], 32, 64);
+    const int r = w0 + n * 16 + col;
+    if (r >= rows) continue;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      store_row<D, NS>(a, s, sp, (long)b * a.c.hkv + g, g, group, rows, split, r, i * 16 + grp * 4, o[n][i], m[n], l[n]);
   }
 }
 
@@ -418,13 +800,22 @@ __global__ void __launch_bounds__(THREADS) kv4_join_kernel(Kv4Attn a) {
     ls = a.stats[(first + (long)lane * rows) * 2 + 1];
   }
   m = wave_max(ms);
-  const float f = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : fast_exp2(ms - m);
+  const float f = lane < sp.count ? part_weight(ms, ls, m) : 0.f;
   l = wave_sum(ls * f);
-  for (int i = 0; i < sp.count; ++i) {
-    const float fi = __shfl(f, i, 64);
-    const float *p = a.partial + (first + (long)i * rows) * D + lane * E;
+  for (int i0 = 0; i0 < sp.count; i0 += 8) {  // eight spans' loads at a time
+    float x[8][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += p[e] * fi;
+    for (int i = 0; i < 8; ++i) {
+      const float *p = a.partial + (first + (long)min(i0 + i, sp.count - 1) * rows) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = p[e];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float fi = __shfl(f, i0 + i, 64);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = i0 + i < sp.count ? __builtin_fmaf(x[i][e], fi, acc[e]) : acc[e];
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const long out_row = s.start + r / group;
@@ -456,48 +847,30 @@ __global__ void __launch_bounds__(THREADS) kv4_weights_kernel(Kv4Attn a) {
   const int lo = a.window > 0 ? s.ctx - s.n - a.slots + 1 : 0;
   float sum[8] = {};
   if (row0 >= 0 && kb + STEP > lo) {
-    Raw<D> w;
+    Keys<D> w;
     load_keys<D>(w, a.c, row0, lane);
-    int pos[8] = {};
+    int4 pos[2] = {};
     if (a.window > 0) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int4 p = *reinterpret_cast<const int4 *>(a.c.pos + row0 + t * 16 + grp * 4);
-        pos[t * 4] = p.x, pos[t * 4 + 1] = p.y, pos[t * 4 + 2] = p.z, pos[t * 4 + 3] = p.w;
-      }
+      for (int t = 0; t < 2; ++t) pos[t] = *reinterpret_cast<const int4 *>(a.c.pos + row0 + t * 16 + grp * 4);
     }
     // the first row that can see a key here
     const int first = max(0, kb - (s.ctx - s.n)) * group;
-    for (int r0 = first & ~15; r0 < rows; r0 += 16) {
-      const int row = r0 + col, token = row / group, own = s.ctx - s.n + token;
-      const bool real = row < rows && s.start + token >= 0 && s.start + token < a.q.rows;
+    for (int r0 = first & ~15; a.q.rows > 0 && r0 < rows; r0 += 16) {
+      const Row row = query_row(a, s, table, g, r0 + col, rows, group);
       bf16x8 q[D / 32][NS];
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        if (real) load_query<NS>(a.query, (s.start + token) * a.q_stride + (long)(g * group + row % group) * D +
-                                              product_dim<D>(i, grp), q[i]);
-        else
-#pragma unroll
-          for (int n = 0; n < NS; ++n) q[i][n] = as_bf16x8(u32x4{0, 0, 0, 0});
-      }
-      const float lse = real ? a.lse[unit * a.max_rows + row] : 0.f;
-      int own_pos = 0;
-      if (a.window > 0 && real && own >= 0) {
-        const long r = row_of(a.c, table, g, own);
-        own_pos = r >= 0 ? a.c.pos[r] : 0;
-      }
+      for (int i = 0; i < D / 32; ++i) load_query<NS>(a.query, row.at + product_dim<D>(i, grp), q[i]);
+      const float lse = row.real ? a.lse[unit * a.max_rows + r0 + col] : 0.f;
+      float t2[2][4];
+      key_scores<D, NS, CAP>(w, q, a.scale, a.softcap, t2);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        float t2[4];
-        key_scores<D, NS, CAP>(w, t, q, a.scale, a.softcap, t2);
+        const int key = kb + t * 16 + grp * 4;
+        const uint32_t seen = a.window > 0 ? mask4<true>(a, row, key, pos[t], t2[t])
+                                           : mask4<false>(a, row, key, pos[t], t2[t]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = kb + t * 16 + grp * 4 + r;
-          bool see = real && key <= own;
-          if (a.window > 0)
-            see = see && key > own - a.slots && (long)pos[t * 4 + r] > (long)own_pos - a.window;
-          sum[t * 4 + r] += see ? fast_exp2(t2[r] - lse) : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) sum[t * 4 + r] += row.real && (seen >> r) & 1 ? fast_exp2(t2[t][r] - lse) : 0.f;
       }
     }
   }
@@ -517,15 +890,28 @@ __global__ void __launch_bounds__(THREADS) kv4_weights_kernel(Kv4Attn a) {
   }
 }
 
+// Workgroups are listed by row tile, then by span: a sequence of many rows has few spans, and the workgroups that have
+// work then follow each other over the XCDs (listed by span first they were every 32nd one, all on one XCD: 6 questions of
+// up to 611 tokens 10.6 ms instead of 1.4).
+// Sequences of few rows take kv4_attn_kernel, of more kv4_attn_tile_kernel; a batch of both launches both.
 template <int D, int NS, bool CAP>
 hipError_t launch(const Kv4Attn &a, hipStream_t s) {
-  const int tiles = (a.max_rows + 15) / 16;
+  constexpr int NT = NS == 1 && D < 256 ? 2 : 1, TW = NS == 1 && D == 256 ? 8 : 4;
+  const int few = a.q.rows > 0 ? (min(a.max_rows, a.few_rows) + 15) / 16 : 0;  // without rows: the weights alone
+  const int tiles = a.q.rows > 0 && a.max_rows > a.few_rows ? (a.max_rows + 16 * NT * TW - 1) / (16 * NT * TW) : 0;
   hipError_t e = hipSuccess;
-  if (tiles > 0) {
-    kv4_attn_kernel<D, NS, CAP><<<dim3(a.max_splits * tiles, a.c.hkv, a.q.num_seqs), dim3(THREADS), 0, s>>>(a);
+  if (few > 0) {
+    const dim3 grid(a.max_splits * few, a.c.hkv, a.q.num_seqs);
+    if (a.window > 0) kv4_attn_kernel<D, NS, CAP, true><<<grid, dim3(THREADS), 0, s>>>(a);
+    else kv4_attn_kernel<D, NS, CAP, false><<<grid, dim3(THREADS), 0, s>>>(a);
     e = hipGetLastError();
   }
-  if (e == hipSuccess && tiles > 0 && a.max_splits > 1) {
+  if (e == hipSuccess && tiles > 0) {
+    kv4_attn_tile_kernel<D, NS, CAP, NT, TW>
+        <<<dim3(a.max_splits * tiles, a.c.hkv, a.q.num_seqs), dim3(64 * TW), 0, s>>>(a);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && few > 0 && a.max_splits > 1) {
     const int split_rows = min(a.max_rows, SPLIT_ROWS / 2);  // rows with more than one span
     kv4_join_kernel<D, NS><<<dim3((split_rows + WAVES - 1) / WAVES, a.c.hkv, a.q.num_seqs), dim3(THREADS), 0, s>>>(a);
     e = hipGetLastError();
@@ -558,7 +944,9 @@ Kv4Plan dx_kv4_attn_plan(int max_seq_len, int max_ctx, int group, int window) {
   return p;
 }
 
-hipError_t dx_kv4_attn_launch(const Kv4Attn &a, bool f32, hipStream_t s) {
+hipError_t dx_kv4_attn_launch(const Kv4Attn &args, bool f32, hipStream_t s) {
+  Kv4Attn a = args;
+  a.few_rows = FEW_ROWS;
   if (a.c.d == 64) return by_type<64>(a, f32, s);
   if (a.c.d == 128) return by_type<128>(a, f32, s);
   return by_type<256>(a, f32, s);

@@ -21,7 +21,7 @@ def cache(k=0x10000, v=0x10000, ks=0x10000, vs=0x10000, pos=0x10000, pages=8, hk
 
 
 CACHES = [(dict(k=None), INVALID), (dict(v=None), INVALID), (dict(ks=None), INVALID), (dict(vs=None), INVALID),
-          (dict(pos=None), INVALID), (dict(pages=-1), INVALID), (dict(hkv=0), INVALID), (dict(d=96), UNSUPPORTED),
+          (dict(pos=None), INVALID), (dict(pages=-1), INVALID), (dict(pages=0), INVALID), (dict(hkv=0), INVALID), (dict(d=96), UNSUPPORTED),
           (dict(d=512), UNSUPPORTED), (dict(page=32), UNSUPPORTED), (dict(page=96), UNSUPPORTED),
           (dict(page=1 << 17), UNSUPPORTED), (dict(hkv=70000), UNSUPPORTED), (dict(k=0x10008), INVALID),
           (dict(ks=0x10004), INVALID), (dict(pos=0x10004), INVALID)]
