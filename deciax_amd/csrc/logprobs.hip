@@ -6,9 +6,9 @@
 //   parts_kernel: a wave takes 2048 neighbouring logits of a row in registers, its M (the shift is the cap itself with
 //     one: t - cap = -2 cap / (1 + e^{2x / cap}), which keeps its relative precision where the weight is), S and E, and
 //     the largest logit of each 32 neighbours.
-//   row_kernel: one workgroup a row joins the parts in their order and finds the alternatives from those largest ones:
-//     with k alternatives wanted, their k-th largest value L bounds what can be among the k best from below, so only the
-//     groups above L (fewer than k) and the first k groups that equal L are looked at again.
+//   row_kernel: one workgroup a row joins the parts in their order and finds the alternatives from those largest ones: the
+//     k-th largest of the threads' largest bounds the k best from below, so only the groups that reach it (a few more than
+//     k) are looked at again, each wave keeping a sorted list of its best, one a lane.
 // Chunks follow from the vocabulary alone, so a row's result does not depend on the others.
 #include "common.h"
 #include "kernels.h"
@@ -26,6 +26,11 @@ DX_DEVICE uint32_t order(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+
+template <bool B>
+struct Flag {
+  static constexpr bool value = B;
+};
 
 DX_DEVICE float to_float(uint16_t x) { return bf2f(x); }
 DX_DEVICE float to_float(float x) { return x; }
@@ -63,12 +68,14 @@ parts_kernel(const T *__restrict__ logits, int vocab, long ld, float cap, int ch
       for (int i = 0; i < V; ++i) x[j][i] = at + i < vocab ? to_float(p[at + i]) : -INFINITY;
     }
   }
-  float top = -INFINITY, mine[NV];
+  float top = -INFINITY, low = INFINITY, mine[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     float g = x[j][0];
 #pragma unroll
     for (int i = 1; i < V; ++i) g = fmaxf(g, x[j][i]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) low = fminf(low, x[j][i]);
     top = fmaxf(top, g);
 #pragma unroll
     for (int off = 1; off < QUAD; off *= 2) g = fmaxf(g, __shfl_xor(g, off, 64));
@@ -83,16 +90,23 @@ parts_kernel(const T *__restrict__ logits, int vocab, long ld, float cap, int ch
   }
   float shift = cap, s = 0.f, e = 0.f;
   if (cap > 0.f) {
+    // 1.5 of some 19 vector instructions' time a logit (three are transcendental, four each), 1500 x 256000 in bf16: a
+    // chunk without -inf, most are, does not look for it again
     const float c1 = 2.f * LOG2E / cap, c2 = -2.f * LOG2E * cap;
+    auto add = [&](auto banned) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float u = c2 * fast_rcp(1.f + fast_exp2(c1 * x[j][i]));
-        const float w = x[j][i] == -INFINITY ? 0.f : fast_exp2(u);
-        s += w;
-        e = __builtin_fmaf(w, u, e);
-      }
+        for (int i = 0; i < V; ++i) {
+          const float u = c2 * fast_rcp(1.f + fast_exp2(c1 * x[j][i]));
+          float w = fast_exp2(u);
+          if constexpr (decltype(banned)::value) w = x[j][i] == -INFINITY ? 0.f : w;
+          s += w;
+          e = __builtin_fmaf(w, u, e);
+        }
+    };
+    if (__any(low == -INFINITY)) add(Flag<true>{});
+    else add(Flag<false>{});
   } else {
     shift = wave_max(top);
     const float base = shift == -INFINITY ? 0.f : shift;
@@ -122,20 +136,8 @@ parts_kernel(const T *__restrict__ logits, int vocab, long ld, float cap, int ch
   }
 }
 
-DX_DEVICE float block_sum(float v, float *red) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
-}
-
-DX_DEVICE int block_count(int wave_count, int *red) {
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = wave_count;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
-}
+// The logit that order() made.
+DX_DEVICE float logit_of(uint32_t v) { return __uint_as_float(v & 0x80000000u ? v & 0x7fffffffu : ~v); }
 
 // t - shift of a logit, as accurate as parts_kernel's sum is.
 DX_DEVICE float shifted(float x, float cap, float shift) {
@@ -143,47 +145,121 @@ DX_DEVICE float shifted(float x, float cap, float shift) {
   return cap > 0.f ? -2.f * cap / (1.f + expf(2.f * x / cap)) : x - shift;
 }
 
+constexpr int ROW_WAVES = 8, ROW_THREADS = 64 * ROW_WAVES;
+constexpr int HELD = 16;  // groups that a thread keeps in registers: all of them up to a vocabulary of 262144
+
+// The workgroup's sums of a and of b, in the waves' order.
+DX_DEVICE void block_sums(float &a, float &b, float (&red)[2][ROW_WAVES]) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = a;
+    red[1][threadIdx.x >> 6] = b;
+  }
+  __syncthreads();
+  a = b = 0.f;
+#pragma unroll
+  for (int w = 0; w < ROW_WAVES; ++w) {
+    a += red[0][w];
+    b += red[1][w];
+  }
+}
+
+DX_DEVICE uint64_t from_lane(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// Each lane its lower neighbour's value (lane 0 anything).
+DX_DEVICE uint64_t from_below(uint64_t v) {
+  constexpr int SHIFT = 0x138;  // DPP: the whole wave by one lane
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, SHIFT, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), SHIFT, 0xf, 0xf, false);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// Insert v (the same in all lanes) into the wave's list, lane i its i-th largest; the last one falls off.
+DX_DEVICE void insert(uint64_t &list, uint64_t v, int lane) {
+  const uint64_t above = from_below(list);
+  const bool moves = list < v;
+  list = moves ? (lane == 0 || above >= v ? v : above) : list;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(ROW_THREADS)
 row_kernel(const T *__restrict__ logits, const int32_t *__restrict__ targets, int vocab, long ld, float cap, int top,
            int chunks, int groups, const float *__restrict__ parts, const float *__restrict__ largest,
            float *__restrict__ logprobs, float *__restrict__ entropy, int32_t *__restrict__ ids,
            float *__restrict__ top_logprobs) {
-  __shared__ float red[WAVES];
-  __shared__ int redi[WAVES];
-  __shared__ int found[2 * MOST_TOP];
-  __shared__ uint64_t best[WAVES][MOST_TOP];
+  __shared__ float red[2][ROW_WAVES], reds[ROW_WAVES];
+  __shared__ uint32_t lane_best[ROW_THREADS];
+  __shared__ uint64_t reach[ROW_WAVES][HELD];
+  __shared__ uint64_t best[ROW_WAVES][MOST_TOP];
   const long row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T *p = logits + row * ld;
-  const float *part = parts + row * chunks * 3;
+  const float *part = parts + row * chunks * 3, *big = largest + row * groups;
+
+  // What is known to be needed is asked for at once: a kernel's first loads come from memory, some 2 us each if one waits
+  // for the other (this row, its target's logit, its parts and groups in turn made a single row 14 us).
+  const int target = targets[row];
+  const float target_logit = to_float(p[min(max(target, 0), vocab - 1)]);
+  float first[3] = {-INFINITY, 0.f, 0.f};  // this thread's first part
+  if (tid < chunks) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) first[i] = part[tid * 3 + i];
+  }
+  // a thread's groups are tid, tid + 512, ...
+  constexpr int BLOCK = HELD * ROW_THREADS;
+  const int blocks = (groups + BLOCK - 1) / BLOCK;
+  uint32_t v[HELD];
+  auto hold = [&](int block) {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      const int i = block * BLOCK + j * ROW_THREADS + tid;
+      const uint32_t x = order(big[min(i, groups - 1)]);  // no branch: sixteen loads on their way at once
+      v[j] = i < groups ? x : 0;
+    }
+  };
+  if (top > 0) {
+    uint32_t mine = 0;
+    for (int block = 0; block < blocks; ++block) {
+      hold(block);
+#pragma unroll
+      for (int j = 0; j < HELD; ++j) mine = max(mine, v[j]);
+    }
+    lane_best[tid] = mine;
+  }
   // join: every thread the same largest shift, then sums in the threads' order
   float shift = cap;
   if (!(cap > 0.f)) {
-    float m = -INFINITY;
-    for (int i = tid; i < chunks; i += THREADS) m = fmaxf(m, part[i * 3]);
+    float m = first[0];
+    for (int i = tid + ROW_THREADS; i < chunks; i += ROW_THREADS) m = fmaxf(m, part[i * 3]);
     m = wave_max(m);
-    if (lane == 0) red[wave] = m;
+    if (lane == 0) reds[wave] = m;
     __syncthreads();
-    shift = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    shift = reds[0];
+#pragma unroll
+    for (int w = 1; w < ROW_WAVES; ++w) shift = fmaxf(shift, reds[w]);
   }
   float s = 0.f, e = 0.f;
-  for (int i = tid; i < chunks; i += THREADS) {
-    const float d = part[i * 3] == -INFINITY ? 0.f : (part[i * 3] - shift) * LOG2E;
-    const float f = fast_exp2(d), si = part[i * 3 + 1] * f;
+  auto add = [&](float top_i, float s_i, float e_i) {
+    const float d = top_i == -INFINITY ? 0.f : (top_i - shift) * LOG2E;
+    const float f = fast_exp2(d), si = s_i * f;
     s += si;
-    e += part[i * 3 + 2] * f + si * d;
-  }
-  s = block_sum(s, red);
-  e = block_sum(e, red) * LN2;
+    e += e_i * f + si * d;
+  };
+  add(first[0], first[1], first[2]);
+  for (int i = tid + ROW_THREADS; i < chunks; i += ROW_THREADS) add(part[i * 3], part[i * 3 + 1], part[i * 3 + 2]);
+  block_sums(s, e, red);
+  e *= LN2;
   // no finite logit at all: no token has any probability
   const bool empty = s == 0.f, lost = s != s;
   const float log_s = logf(s);
   if (tid == 0) {
-    const int target = targets[row];
     float lp = 0.f;
     if (target < -1 || target >= vocab) lp = NAN;
-    else if (target >= 0) lp = empty ? -INFINITY : shifted(to_float(p[target]), cap, shift) - log_s;
+    else if (target >= 0) lp = empty ? -INFINITY : shifted(target_logit, cap, shift) - log_s;
     logprobs[row] = lost && target != -1 ? NAN : lp;
     entropy[row] = lost ? NAN : empty ? 0.f : log_s - e / s;
   }
@@ -191,93 +267,83 @@ row_kernel(const T *__restrict__ logits, const int32_t *__restrict__ targets, in
   int32_t *out = ids + row * top;
   float *out_lp = top_logprobs + row * top;
   if (empty || lost) {
-    for (int i = tid; i < top; i += THREADS) {
+    for (int i = tid; i < top; i += ROW_THREADS) {
       out[i] = -1;
       out_lp[i] = lost ? NAN : -INFINITY;
     }
     return;
   }
-  // the k-th largest of the groups' largest, bit by bit
-  const float *big = largest + row * groups;
-  const int k = min(top, groups);
+  // The `top`-th largest of the threads' largest logits, bit by bit from the top: that many logits are as large, so the
+  // best ones are, and only groups that reach it are looked at. (Fewer threads with groups than `top`: all groups.) Half
+  // the bits, 0.1 us each, are near enough: 8 of a mantissa.
   uint32_t least = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = least | (1u << bit);
-    int c = 0;
-    for (int i = tid; i < groups; i += THREADS) c += order(big[i]) >= cand;
-    c = (int)wave_sum((float)c);
-    if (block_count(c, redi) >= k) least = cand;
-  }
-  // groups above it in any order, then the first k that equal it: thread t looks at groups t, t + 256, ...
-  int have = 0;  // entries of found
-  int equal = 0;
-  for (int i0 = 0; i0 < groups; i0 += THREADS) {
-    const int i = i0 + tid;
-    const uint32_t v = i < groups ? order(big[i]) : 0u;
-    const bool more = i < groups && v > least, same = i < groups && v == least;
-    const uint64_t bm = __ballot(more), bs = __ballot(same), lower = (1ull << lane) - 1;
-    __syncthreads();
-    if (lane == 0) {
-      redi[wave] = __popcll(bm) | (__popcll(bs) << 16);
+  {
+    uint32_t x[ROW_WAVES];
+#pragma unroll
+    for (int w = 0; w < ROW_WAVES; ++w) x[w] = lane_best[w * 64 + lane];
+    for (int bit = 31; bit >= 15; --bit) {
+      const uint32_t cand = least | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int w = 0; w < ROW_WAVES; ++w) c += __popcll(__ballot(x[w] >= cand));
+      if (c >= top) least = cand;
     }
-    __syncthreads();
-    int um = 0, us = 0, am = 0, as = 0;
-    for (int w = 0; w < WAVES; ++w) {
-      const int x = redi[w];
-      um += w < wave ? x & 0xffff : 0;
-      us += w < wave ? x >> 16 : 0;
-      am += x & 0xffff;
-      as += x >> 16;
-    }
-    if (more) found[have + um + __popcll(bm & lower)] = i;
-    const int rank = equal + us + __popcll(bs & lower);
-    if (same && rank < k) found[2 * MOST_TOP - 1 - rank] = i;
-    have += am;
-    equal += as;
   }
-  __syncthreads();
-  const int tied = min(equal, k), cands = have + tied;
-  // each wave the best of its share of the groups: lane i holds the i-th best as (logit, lower token first)
+  // a wave's own best, over its share of the groups, two groups of 32 at a time
   uint64_t list = 0;
-  const uint32_t floor = top <= groups ? least : 0;  // that many groups have a logit this large
-  for (int c = wave; c < (cands + 1) / 2; c += WAVES) {  // two groups of 32 at a time
-    const int which = c * 2 + (lane >> 5);
+  auto look = [&](int g0, int g1) {  // g1 = g0: one group
+    const int g = lane < 32 ? g0 : g1, token = g * GROUP + (lane & 31);
     uint64_t key = 0;
-    if (which < cands) {
-      const int g = which < have ? found[which] : found[2 * MOST_TOP - 1 - (which - have)];
-      const int token = g * GROUP + (lane & 31);
-      if (token < vocab) key = ((uint64_t)order(to_float(p[token])) << 32) | (uint32_t)~token;
-    }
-    uint64_t worst = __shfl(list, top - 1, 64);
-    uint64_t in = __ballot(key > worst && (uint32_t)(key >> 32) >= floor);
+    if (token < vocab && (lane < 32 || g1 != g0))
+      key = ((uint64_t)order(to_float(p[token])) << 32) | (uint32_t)~token;
+    uint64_t in = __ballot(key > from_lane(list, top - 1) && (uint32_t)(key >> 32) >= least);
     while (in) {
       const int src = __ffsll((unsigned long long)in) - 1;
       in &= in - 1;
-      const uint64_t v = __shfl(key, src, 64);
-      const uint64_t above = __shfl_up(list, 1, 64);
-      // lanes whose entry is below v move down by one
-      const bool below = list < v;
-      const bool first = below && (lane == 0 || above >= v);
-      list = first ? v : below ? above : list;
+      insert(list, from_lane(key, src), lane);
     }
+  };
+  int held = -1;  // a group that waits for a second one
+  for (int block = blocks - 1; block >= 0; --block) {
+    if (block < blocks - 1) hold(block);  // the last one still is
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      const uint64_t in = __ballot(v[j] >= least && v[j] != 0);
+      if (lane == 0) reach[wave][j] = in;
+    }
+    __builtin_amdgcn_wave_barrier();
+    for (int j = 0; j < HELD; ++j) {
+      uint64_t in = from_lane(reach[wave][j], 0);
+      while (in) {
+        const int g = block * BLOCK + j * ROW_THREADS + wave * 64 + __ffsll((unsigned long long)in) - 1;
+        in &= in - 1;
+        if (held < 0) {
+          held = g;
+        } else {
+          look(held, g);
+          held = -1;
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
   }
-  if (lane < MOST_TOP) best[wave][lane] = lane < top ? list : 0;
+  if (held >= 0) look(held, held);
+  best[wave][lane] = lane < top ? list : 0;
   __syncthreads();
   if (wave != 0) return;
-  for (int w = 1; w < WAVES; ++w)
+  for (int w = 1; w < ROW_WAVES; ++w) {
+    const uint64_t theirs = best[w][lane];
     for (int i = 0; i < top; ++i) {
-      const uint64_t v = best[w][i];
-      if (v == 0 || v <= __shfl(list, top - 1, 64)) break;
-      const uint64_t above = __shfl_up(list, 1, 64);
-      const bool below = list < v;
-      const bool first = below && (lane == 0 || above >= v);
-      list = first ? v : below ? above : list;
+      const uint64_t v = from_lane(theirs, i);
+      if (v <= from_lane(list, top - 1)) break;  // the rest is smaller still
+      insert(list, v, lane);
     }
+  }
   if (lane < top) {
     const int token = (int)~(uint32_t)list;
     const bool none = list == 0 || (uint32_t)(list >> 32) <= order(-INFINITY);
     out[lane] = none ? -1 : token;
-    out_lp[lane] = none ? -INFINITY : shifted(to_float(p[token]), cap, shift) - log_s;
+    out_lp[lane] = none ? -INFINITY : shifted(logit_of((uint32_t)(list >> 32)), cap, shift) - log_s;
   }
 }
 
@@ -301,11 +367,11 @@ hipError_t dx_token_logprobs_launch(const void *logits, const int32_t *targets, 
     if (e != hipSuccess) return e;
   }
   if (f32)
-    row_kernel<<<dim3((unsigned)rows), dim3(THREADS), 0, s>>>(static_cast<const float *>(logits), targets, vocab, ld,
+    row_kernel<<<dim3((unsigned)rows), dim3(ROW_THREADS), 0, s>>>(static_cast<const float *>(logits), targets, vocab, ld,
                                                               cap, top, chunks, ngroups, parts, groups, logprobs,
                                                               entropy, ids, top_logprobs);
   else
-    row_kernel<<<dim3((unsigned)rows), dim3(THREADS), 0, s>>>(static_cast<const uint16_t *>(logits), targets, vocab, ld,
+    row_kernel<<<dim3((unsigned)rows), dim3(ROW_THREADS), 0, s>>>(static_cast<const uint16_t *>(logits), targets, vocab, ld,
                                                               cap, top, chunks, ngroups, parts, groups, logprobs,
                                                               entropy, ids, top_logprobs);
   return hipGetLastError();
