@@ -806,7 +806,7 @@ int validate_kv_rows(const Kv4Cache &c, const Kv4Batch &q, const void *k, const 
   const int64_t width = (int64_t)c.hkv * c.d;
   REQUIRE(ks >= width && vs >= width && ks * bytes % 16 == 0 && vs * bytes % 16 == 0,
           "%s: row strides must cover heads * head_dim and be multiples of %d elements", what, 16 / bytes);
-  SUPPORTED((int64_t)q.max_seq_len * (width / 8) < (INT64_C(1) << 31), "%s: %d tokens of %ld values a sequence", what,
+  SUPPORTED(((int64_t)q.max_seq_len + 16) * (width / 8) < (INT64_C(1) << 31), "%s: %d tokens of %ld values a sequence", what,
             q.max_seq_len, (long)width);
   return DX_OK;
 }

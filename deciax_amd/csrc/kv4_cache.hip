@@ -39,58 +39,91 @@ DX_DEVICE void store_block(const float (&x)[8], uint8_t *codes, uint8_t *scales,
   if (at % 32 == 0) scales[at / 32] = (uint8_t)byte;
 }
 
-// Eight values of k and the same eight of v a thread. Rows of one sequence are consecutive items.
-template <typename T>
-__global__ void __launch_bounds__(THREADS)
-append_kernel(Kv4Cache c, Kv4Batch q, const T *__restrict__ k, const T *__restrict__ v,
-              const int32_t *__restrict__ positions, long k_stride, long v_stride, int per_block) {
+// An item is eight values of k and the same eight of v. Items go by blocks of BLOCK tokens, by head, by token: a head's
+// rows of neighbouring slots, its scales and positions, are then written together (token by token a line of 128 bytes of
+// scales was written 8 bytes at a time by 16 workgroups). A thread takes ITER items, all loads of one kind before the next,
+// since each waits for the one before: lengths, page, rows.
+struct Item {
+  int slot, col;
+  long row, at;  // the packed row (-1: none), the place in the cache (-1: none)
+};
+
+// False for a workgroup behind its sequence's last row.
+template <int ITER, int BLOCK>
+DX_DEVICE bool find_items(const Kv4Cache &c, const Kv4Batch &q, Item (&item)[ITER]) {
   const int b = blockIdx.y;
   const Sequence s = sequence(q, b, c.shift);
   const int32_t *table = q.table + (long)b * q.table_width;
-  const uint32_t row_items = c.hkv * c.d / 8, items = s.n * row_items;  // below 2^31 for the longest sequence
-  const uint32_t i0 = blockIdx.x * per_block;
-  for (uint32_t i = i0 + threadIdx.x; i < min(i0 + per_block, items); i += THREADS) {
-    const int t = (int)(i / row_items), col = (int)(i % row_items) * 8;
-    const long row = s.start + t;
-    const int slot = s.ctx - s.n + t, g = col / c.d, d = col % c.d;
-    float xk[8] = {}, xv[8] = {};
-    long at = -1;
-    if (slot >= 0 && row >= 0 && row < q.rows) {
-      load8(k + row * k_stride + col, xk);
-      load8(v + row * v_stride + col, xv);
-      const long r = row_of(c, table, g, slot);
-      if (r >= 0) {
-        at = r * c.d + d;
-        if (d == 0) c.pos[r] = positions[row];
-      }
-    }
-    store_block(xk, c.k, c.ks, at);
-    store_block(xv, c.v, c.vs, at);
+  const uint32_t head_items = c.d / 8, row_items = c.hkv * head_items;
+  if (blockIdx.x * ITER * THREADS >= (s.n + BLOCK - 1) / BLOCK * (BLOCK * row_items)) return false;
+  int page[ITER];
+#pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const uint32_t i = (blockIdx.x * ITER + k) * THREADS + threadIdx.x;
+    const uint32_t block = i / (BLOCK * row_items), r = i - block * (BLOCK * row_items);
+    const uint32_t g = r / (BLOCK * head_items), x = r - g * (BLOCK * head_items);
+    const int t = (int)(block * BLOCK + x / head_items);
+    item[k].col = (int)(g * c.d + x % head_items * 8);
+    item[k].slot = s.ctx - s.n + t;
+    item[k].row = s.start + t;
+    if (t >= s.n || item[k].row < 0 || item[k].row >= q.rows) item[k].row = -1;
+    const bool placed = item[k].row >= 0 && item[k].slot >= 0;
+    page[k] = placed ? table[item[k].slot >> c.shift] : -1;
+  }
+#pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int g = item[k].col / c.d, d = item[k].col % c.d;
+    const long row = (((long)page[k] * c.hkv + g) << c.shift) + (item[k].slot & ((1 << c.shift) - 1));
+    item[k].at = page[k] >= 0 && page[k] < c.pages ? row * c.d + d : -1;
+  }
+  return true;
+}
+
+template <typename T, int ITER, int BLOCK>
+__global__ void __launch_bounds__(THREADS)
+append_kernel(Kv4Cache c, Kv4Batch q, const T *__restrict__ k, const T *__restrict__ v,
+              const int32_t *__restrict__ positions, long k_stride, long v_stride) {
+  Item item[ITER];
+  if (!find_items<ITER, BLOCK>(c, q, item)) return;
+  float xk[ITER][8], xv[ITER][8];
+  int pos[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const long row = max(item[i].row, 0L);  // rows are there: a call without any is not launched
+    const int col = item[i].row >= 0 ? item[i].col : 0;
+    load8(k + row * k_stride + col, xk[i]);
+    load8(v + row * v_stride + col, xv[i]);
+    pos[i] = positions[row];
+  }
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    if (item[i].at >= 0 && item[i].at % c.d == 0) c.pos[item[i].at / c.d] = pos[i];
+    store_block(xk[i], c.k, c.ks, item[i].at);
+    store_block(xv[i], c.v, c.vs, item[i].at);
   }
 }
 
+template <int ITER, int BLOCK>
 __global__ void __launch_bounds__(THREADS)
-read_kernel(Kv4Cache c, Kv4Batch q, uint16_t *__restrict__ k, uint16_t *__restrict__ v, long k_stride, long v_stride,
-            int per_block) {
-  const int b = blockIdx.y;
-  const Sequence s = sequence(q, b, c.shift);
-  const int32_t *table = q.table + (long)b * q.table_width;
-  const uint32_t row_items = c.hkv * c.d / 8, items = s.n * row_items;  // below 2^31 for the longest sequence
-  const uint32_t i0 = blockIdx.x * per_block;
-  for (uint32_t i = i0 + threadIdx.x; i < min(i0 + per_block, items); i += THREADS) {
-    const int t = (int)(i / row_items), col = (int)(i % row_items) * 8;
-    const long row = s.start + t;
-    const int slot = s.ctx - s.n + t, g = col / c.d, d = col % c.d;
-    if (row < 0 || row >= q.rows) continue;
-    u32x4 wk = {0, 0, 0, 0}, wv = {0, 0, 0, 0};
-    const long r = slot >= 0 ? row_of(c, table, g, slot) : -1;
-    if (r >= 0) {
-      const long at = r * c.d + d;
-      wk = decode8(*reinterpret_cast<const uint32_t *>(c.k + at / 2), scale_of(c.ks[at / 32]));
-      wv = decode8(*reinterpret_cast<const uint32_t *>(c.v + at / 2), scale_of(c.vs[at / 32]));
-    }
-    *reinterpret_cast<u32x4 *>(k + row * k_stride + col) = wk;
-    *reinterpret_cast<u32x4 *>(v + row * v_stride + col) = wv;
+read_kernel(Kv4Cache c, Kv4Batch q, uint16_t *__restrict__ k, uint16_t *__restrict__ v, long k_stride, long v_stride) {
+  Item item[ITER];
+  if (!find_items<ITER, BLOCK>(c, q, item)) return;
+  uint32_t wk[ITER], wv[ITER], sk[ITER], sv[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const long at = max(item[i].at, 0L);
+    wk[i] = *reinterpret_cast<const uint32_t *>(c.k + at / 2);
+    wv[i] = *reinterpret_cast<const uint32_t *>(c.v + at / 2);
+    sk[i] = c.ks[at / 32];
+    sv[i] = c.vs[at / 32];
+  }
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    if (item[i].row < 0) continue;
+    const bool there = item[i].at >= 0;
+    const u32x4 none = {0, 0, 0, 0};
+    *reinterpret_cast<u32x4 *>(k + item[i].row * k_stride + item[i].col) = there ? decode8(wk[i], scale_of(sk[i])) : none;
+    *reinterpret_cast<u32x4 *>(v + item[i].row * v_stride + item[i].col) = there ? decode8(wv[i], scale_of(sv[i])) : none;
   }
 }
 
@@ -115,7 +148,7 @@ __global__ void __launch_bounds__(SEL_THREADS)
 select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const int32_t *__restrict__ ctx_len,
               int max_ctx, int keep, int recent, int32_t *__restrict__ list, int32_t *__restrict__ out_len) {
   __shared__ int counts[2][SEL_WAVES];
-  __shared__ int before[2][SEL_WAVES];
+  __shared__ uint32_t spread[ITEMS ? ITEMS : 16][SEL_WAVES];
   const int g = blockIdx.x, b = blockIdx.y, hkv = gridDim.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ctx = min(max(ctx_len[b], 0), max_ctx), kept = min(ctx, keep);
@@ -130,7 +163,8 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
   const int rounds = (ctx + SEL_THREADS - 1) / SEL_THREADS;
   auto fetch = [&](int i) -> uint32_t {  // 0: no slot; order() of a number is never 0
     const int slot = i * SEL_THREADS + tid;
-    return slot >= ctx ? 0u : slot >= guard ? PROTECTED : max(order(w[slot]), 1u);
+    const uint32_t x = max(order(w[min(slot, ctx - 1)]), 1u);  // no branch: a thread's loads are on their way at once
+    return slot >= ctx ? 0u : slot >= guard ? PROTECTED : x;
   };
   uint32_t key[ITEMS ? ITEMS : 1];
   if constexpr (ITEMS > 0) {
@@ -159,8 +193,13 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
     }
     c = total(c, bit & 1);
     if (c >= kept) least = cand;
+    if (c == kept) {  // these are they
+      least = cand - 1;
+      above = kept;
+      break;
+    }
   }
-  {
+  if (above == 0) {
     int c = 0;
     if constexpr (ITEMS > 0) {
 #pragma unroll
@@ -171,96 +210,135 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
     above = total(c, 1);
   }
   const int ties = kept - above;  // of the keys that equal `least`, the first in slot order
-  // 1024 slots at a time, in order
+  // Ranks: every wave its counts of both kinds for each 1024 slots, ITEMS (or 16) of those at a time, then sums over the
+  // waves before it and the slots before those. A wave of 64 neighbouring slots takes two ballots.
+  constexpr int SPREAD = ITEMS ? ITEMS : 16;
   int tied = 0, done = 0;
   const uint64_t lower = (1ull << lane) - 1;
-  auto place = [&](int i, uint32_t k) {
-    const uint64_t eq = __ballot(k == least && k != 0), gt = __ballot(k > least);
-    if (lane == 0) {
-      counts[i & 1][wave] = __popcll(eq);
-      before[i & 1][wave] = __popcll(gt);
+  for (int i0 = 0; i0 < rounds; i0 += SPREAD) {
+    uint32_t k[SPREAD];
+#pragma unroll
+    for (int i = 0; i < SPREAD; ++i) {
+      if constexpr (ITEMS > 0) k[i] = key[i];
+      else k[i] = fetch(i0 + i);
+      const uint64_t eq = __ballot(k[i] == least && k[i] != 0), gt = __ballot(k[i] > least);
+      if (lane == 0) spread[i][wave] = (uint32_t)__popcll(gt) << 16 | (uint32_t)__popcll(eq);
     }
     __syncthreads();
-    int eq_under = 0, gt_under = 0, eq_all = 0, gt_all = 0;
 #pragma unroll
-    for (int j = 0; j < SEL_WAVES; ++j) {
-      const int e = counts[i & 1][j], a = before[i & 1][j];
-      eq_under += j < wave ? e : 0;
-      gt_under += j < wave ? a : 0;
-      eq_all += e;
-      gt_all += a;
+    for (int i = 0; i < SPREAD; ++i) {
+      uint32_t sum = spread[i][lane & (SEL_WAVES - 1)];
+#pragma unroll
+      for (int off = 1; off < SEL_WAVES; off *= 2) {
+        const uint32_t under = __shfl_up(sum, off, SEL_WAVES);
+        sum += (lane & (SEL_WAVES - 1)) >= off ? under : 0;
+      }
+      const uint32_t all = __builtin_amdgcn_readlane(sum, SEL_WAVES - 1);
+      const uint32_t under = wave > 0 ? __builtin_amdgcn_readlane(sum, wave - 1) : 0;
+      const bool is_eq = k[i] == least && k[i] != 0, is_gt = k[i] > least;
+      const uint64_t eq = __ballot(is_eq), gt = __ballot(is_gt);
+      const int eq_rank = tied + (int)(under & 0xffff) + __popcll(eq & lower);
+      // ranks among the kept: greater ones before, and the tied ones before that are within the quota
+      const int rank = done + (int)(under >> 16) + __popcll(gt & lower) + min(eq_rank, ties);
+      if (is_gt || (is_eq && eq_rank < ties)) mine[rank] = (i0 + i) * SEL_THREADS + tid;
+      tied += (int)(all & 0xffff);
+      done += (int)(all >> 16);
     }
-    const int eq_rank = tied + eq_under + __popcll(eq & lower);
-    const bool is_eq = (eq >> lane) & 1, is_gt = (gt >> lane) & 1;
-    // ranks among the kept: greater ones before, and the tied ones before that are within the quota
-    const int at_rank = done + gt_under + __popcll(gt & lower) + min(eq_rank, ties);
-    if (is_gt || (is_eq && eq_rank < ties)) mine[at_rank] = i * SEL_THREADS + tid;
-    tied += eq_all;
-    done += gt_all;
-  };
-  if constexpr (ITEMS > 0) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if (i < rounds) place(i, key[i]);
-  } else {
-    for (int i = 0; i < rounds; ++i) place(i, fetch(i));
+    __syncthreads();
   }
 }
 
-// Kept rows to their new pages: 16 bytes a thread, then each row's scales, position and weight.
+// Kept rows to their new pages: 16 bytes of codes a thread, the row's scales, position and weight by one of its threads
+// each. Every step (slot, pages, rows) waits for the one before, so a thread takes four rows' steps together.
+template <int D>
 __global__ void __launch_bounds__(THREADS)
 move_kernel(Kv4Cache c, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ out_table,
             int out_width, const int32_t *__restrict__ ctx_len, int max_ctx, int keep,
             const int32_t *__restrict__ list, const float *__restrict__ weights, long w_seq, long w_head,
-            float *__restrict__ out_weights, long o_seq, long o_head, int per_block) {
+            float *__restrict__ out_weights, long o_seq, long o_head) {
+  constexpr int CHUNKS = D / 32, LANES = 2 * CHUNKS;  // 16-byte chunks of K's row, then of V's
+  constexpr int ROWS = THREADS / LANES, ITER = 4;
   const int g = blockIdx.y, b = blockIdx.z;
   const int kept = min(min(max(ctx_len[b], 0), max_ctx), keep);
   const int32_t *from = table + (long)b * width, *to = out_table + (long)b * out_width;
   const int32_t *mine = list + ((long)b * c.hkv + g) * keep;
-  const int chunks = c.d / 32, lanes = 2 * chunks;  // 16-byte chunks of K's row, then of V's
-  const int j0 = blockIdx.x * per_block, j1 = min(j0 + per_block, keep);
-  for (int i = threadIdx.x; i < (j1 - j0) * lanes; i += THREADS) {
-    const int j = j0 + i / lanes, l = i % lanes, chunk = l % chunks;
-    float w = 0.f;
-    if (j < kept) {
-      const int slot = mine[j];
-      const long src = row_of(c, from, g, slot), dst = row_of(c, to, g, j);
-      if (src >= 0 && dst >= 0) {
-        uint8_t *codes = l < chunks ? c.k : c.v, *scales = l < chunks ? c.ks : c.vs;
-        *reinterpret_cast<u32x4 *>(codes + dst * (c.d / 2) + chunk * 16) =
-            *reinterpret_cast<const u32x4 *>(codes + src * (c.d / 2) + chunk * 16);
-        scales[dst * chunks + chunk] = scales[src * chunks + chunk];
-        if (l == 0) c.pos[dst] = c.pos[src];
-      }
-      if (l == 0) w = weights[b * w_seq + g * w_head + slot];
+  const int l = threadIdx.x % LANES, chunk = l % CHUNKS;
+  const bool is_k = l < CHUNKS;
+  uint8_t *codes = is_k ? c.k : c.v, *scales = is_k ? c.ks : c.vs;
+  if (blockIdx.x * ITER * ROWS >= keep) return;
+  int j[ITER], slot[ITER];
+  long src[ITER], dst[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    j[i] = (blockIdx.x * ITER + i) * ROWS + threadIdx.x / LANES;
+    slot[i] = mine[max(min(j[i], kept - 1), 0)];
+  }
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const bool there = j[i] < kept;
+    src[i] = there ? row_of(c, from, g, slot[i]) : -1;
+    dst[i] = there ? row_of(c, to, g, j[i]) : -1;
+  }
+  u32x4 x[ITER];
+  uint64_t sc[ITER];
+  int pos[ITER];
+  float w[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const long at = max(src[i], 0L);
+    x[i] = *reinterpret_cast<const u32x4 *>(codes + at * (D / 2) + chunk * 16);
+    if constexpr (D == 256) sc[i] = *reinterpret_cast<const uint64_t *>(scales + at * CHUNKS);
+    else if constexpr (D == 128) sc[i] = *reinterpret_cast<const uint32_t *>(scales + at * CHUNKS);
+    else sc[i] = *reinterpret_cast<const uint16_t *>(scales + at * CHUNKS);
+    pos[i] = c.pos[at];
+    w[i] = j[i] < kept ? weights[b * w_seq + g * w_head + slot[i]] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    if (l == 0 && j[i] < keep) out_weights[b * o_seq + g * o_head + j[i]] = w[i];
+    if (src[i] < 0 || dst[i] < 0) continue;
+    *reinterpret_cast<u32x4 *>(codes + dst[i] * (D / 2) + chunk * 16) = x[i];
+    if (chunk == 0) {
+      if constexpr (D == 256) *reinterpret_cast<uint64_t *>(scales + dst[i] * CHUNKS) = sc[i];
+      else if constexpr (D == 128) *reinterpret_cast<uint32_t *>(scales + dst[i] * CHUNKS) = (uint32_t)sc[i];
+      else *reinterpret_cast<uint16_t *>(scales + dst[i] * CHUNKS) = (uint16_t)sc[i];
     }
-    if (l == 0) out_weights[b * o_seq + g * o_head + j] = w;
+    if (l == CHUNKS) c.pos[dst[i]] = pos[i];
   }
 }
 
 }  // namespace
 
+// Four items a thread and blocks of 16 tokens where a sequence has more than a few workgroups' worth of them.
+static bool few_items(const Kv4Cache &c, const Kv4Batch &q) { return (long)q.max_seq_len * (c.hkv * c.d / 8) <= 8 * THREADS; }
+static dim3 item_grid(const Kv4Cache &c, const Kv4Batch &q, int iter, int tokens) {
+  const long items = (long)(q.max_seq_len + tokens - 1) / tokens * tokens * (c.hkv * c.d / 8), block = (long)iter * THREADS;
+  return dim3((unsigned)((items + block - 1) / block), q.num_seqs);
+}
+
+template <typename T>
+static void append(const Kv4Cache &c, const Kv4Batch &q, const void *k, const void *v, const int32_t *positions,
+                   long k_stride, long v_stride, hipStream_t s) {
+  const T *kt = static_cast<const T *>(k), *vt = static_cast<const T *>(v);
+  if (few_items(c, q))
+    append_kernel<T, 1, 1><<<item_grid(c, q, 1, 1), dim3(THREADS), 0, s>>>(c, q, kt, vt, positions, k_stride, v_stride);
+  else
+    append_kernel<T, 4, 16><<<item_grid(c, q, 4, 16), dim3(THREADS), 0, s>>>(c, q, kt, vt, positions, k_stride, v_stride);
+}
+
 hipError_t dx_kv4_append_launch(const Kv4Cache &c, const Kv4Batch &q, const void *k, const void *v,
                                 const int32_t *positions, long k_stride, long v_stride, bool f32, hipStream_t s) {
-  const long items = (long)q.max_seq_len * (c.hkv * c.d / 8);
-  const int per_block = items <= 8 * THREADS ? THREADS : 4 * THREADS;
-  const dim3 grid((unsigned)((items + per_block - 1) / per_block), q.num_seqs);
-  if (f32)
-    append_kernel<<<grid, dim3(THREADS), 0, s>>>(c, q, static_cast<const float *>(k), static_cast<const float *>(v),
-                                                 positions, k_stride, v_stride, per_block);
-  else
-    append_kernel<<<grid, dim3(THREADS), 0, s>>>(c, q, static_cast<const uint16_t *>(k),
-                                                 static_cast<const uint16_t *>(v), positions, k_stride, v_stride,
-                                                 per_block);
+  if (f32) append<float>(c, q, k, v, positions, k_stride, v_stride, s);
+  else append<uint16_t>(c, q, k, v, positions, k_stride, v_stride, s);
   return hipGetLastError();
 }
 
 hipError_t dx_kv4_read_launch(const Kv4Cache &c, const Kv4Batch &q, uint16_t *k, uint16_t *v, long k_stride,
                               long v_stride, hipStream_t s) {
-  const long items = (long)q.max_seq_len * (c.hkv * c.d / 8);
-  const int per_block = items <= 8 * THREADS ? THREADS : 4 * THREADS;
-  const dim3 grid((unsigned)((items + per_block - 1) / per_block), q.num_seqs);
-  read_kernel<<<grid, dim3(THREADS), 0, s>>>(c, q, k, v, k_stride, v_stride, per_block);
+  if (few_items(c, q))
+    read_kernel<1, 1><<<item_grid(c, q, 1, 1), dim3(THREADS), 0, s>>>(c, q, k, v, k_stride, v_stride);
+  else
+    read_kernel<4, 16><<<item_grid(c, q, 4, 16), dim3(THREADS), 0, s>>>(c, q, k, v, k_stride, v_stride);
   return hipGetLastError();
 }
 
@@ -279,9 +357,13 @@ hipError_t dx_kv4_evict_launch(const Kv4Cache &c, const int32_t *table, int widt
 #undef SELECT
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int per_block = 64;
-  move_kernel<<<dim3((keep + per_block - 1) / per_block, c.hkv, num_seqs), dim3(THREADS), 0, s>>>(
-      c, table, width, out_table, out_width, ctx_len, max_ctx, keep, list, weights, w_seq, w_head, out_weights, o_seq,
-      o_head, per_block);
+#define MOVE(D)                                                                                                     \
+  move_kernel<D><<<dim3((keep + 4 * (THREADS * 16 / (D)) - 1) / (4 * (THREADS * 16 / (D))), c.hkv, num_seqs),       \
+                   dim3(THREADS), 0, s>>>(c, table, width, out_table, out_width, ctx_len, max_ctx, keep, list,      \
+                                          weights, w_seq, w_head, out_weights, o_seq, o_head)
+  if (c.d == 64) MOVE(64);
+  else if (c.d == 128) MOVE(128);
+  else MOVE(256);
+#undef MOVE
   return hipGetLastError();
 }
