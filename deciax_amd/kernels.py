@@ -12,7 +12,6 @@ from __future__ import annotations
 import weakref
 from collections.abc import Sequence
 from ctypes import byref
-from typing import NamedTuple
 
 import torch
 
@@ -664,16 +663,33 @@ def readout(hidden: torch.Tensor, norm_w: torch.Tensor, table: torch.Tensor, opt
 # ---------------------------------------------------------------------------- 4-bit cache, answers over it
 
 
-class KV4Cache(NamedTuple):
+class KV4Cache:
     """One layer's paged cache of keys and values in 4 bits (`dx_kv4_cache`, which states the format): `k`, `v` uint8
     [pages, kv heads, page size, head_dim / 2], their scales uint8 [.., head_dim / 32] and `positions` int32
-    [pages, kv heads, page size]. `kv4_cache` allocates one."""
+    [pages, kv heads, page size]. `kv4_cache` allocates one. The arrays are looked over once, here."""
 
-    k: torch.Tensor
-    v: torch.Tensor
-    k_scale: torch.Tensor
-    v_scale: torch.Tensor
-    positions: torch.Tensor
+    __slots__ = ("k", "v", "k_scale", "v_scale", "positions", "head_dim", "heads", "page_size", "index", "_c", "ref")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 positions: torch.Tensor) -> None:
+        if k.dim() != 4:
+            raise ValueError("KV4Cache: k must be [pages, kv heads, page size, head_dim / 2]")
+        shape, index = k.shape, k.get_device()
+        pages, heads, page, half = shape
+        scales = (pages, heads, page, half // 16)
+        if (v.shape != shape or k_scale.shape != scales or v_scale.shape != scales or positions.shape != scales[:3] or
+                half % 16):
+            raise ValueError("KV4Cache: the arrays' shapes do not belong together")
+        for t in (k, v, k_scale, v_scale):
+            if t.dtype != torch.uint8 or t.get_device() != index or not t.is_contiguous():
+                raise ValueError("KV4Cache: codes and scales must be contiguous uint8 on one device")
+        if positions.dtype != torch.int32 or positions.get_device() != index or not positions.is_contiguous():
+            raise ValueError("KV4Cache: positions must be contiguous int32 on the codes' device")
+        self.k, self.v, self.k_scale, self.v_scale, self.positions = k, v, k_scale, v_scale, positions
+        self.head_dim, self.heads, self.page_size, self.index = 2 * half, heads, page, index
+        self._c = _lib.Kv4Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                positions.data_ptr(), pages, heads, page, 2 * half)
+        self.ref = byref(self._c)
 
 
 def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, *, page_size: int = 64,
@@ -689,50 +705,40 @@ def kv4_cache(num_pages: int, num_kv_heads: int, head_dim: int, *, page_size: in
                     zeros(dtype=torch.int32))
 
 
-def _kv4(cache: KV4Cache, what: str) -> _lib.Kv4Cache:
-    k = cache.k
-    if k.dim() != 4 or not k.is_cuda:
-        raise ValueError(f"{what}: cache.k must be a device tensor [pages, kv heads, page size, head_dim / 2]")
-    pages, hkv, page, half = k.shape
-    for t, last, dtype in ((k, (half,), torch.uint8), (cache.v, (half,), torch.uint8),
-                           (cache.k_scale, (half // 16,), torch.uint8), (cache.v_scale, (half // 16,), torch.uint8),
-                           (cache.positions, (), torch.int32)):
-        if t.dtype != dtype or t.device != k.device or tuple(t.shape) != (pages, hkv, page, *last) or \
-                not t.is_contiguous():
-            raise ValueError(f"{what}: the cache's arrays must be contiguous, on one device and of one shape")
-    return _lib.Kv4Cache(k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-                         cache.positions.data_ptr(), pages, hkv, page, 2 * half)
-
-
-def _kv4_ints(what: str, device: torch.device, page_table: torch.Tensor, *lengths: torch.Tensor) -> None:
-    """A page table [seqs, pages] and arrays of one entry a sequence."""
+def _kv4_ints(what: str, cache: KV4Cache, page_table: torch.Tensor, *lengths: torch.Tensor) -> int:
+    """A page table [sequences, pages] and arrays of one entry a sequence, on the cache's device; the sequences."""
+    index = cache.index
+    if index < 0:
+        raise ValueError(f"{what}: the cache must be in device (HIP) memory")
     if page_table.dim() != 2:
         raise ValueError(f"{what}: page_table must be [sequences, pages]")
-    for t in (page_table, *lengths):
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.shape[0] != page_table.shape[0]:
-            raise ValueError(f"{what}: page tables and lengths must be contiguous int32 on {device}, one row a sequence")
-    if any(t.dim() != 1 for t in lengths):
-        raise ValueError(f"{what}: seq_start, seq_len and ctx_len must have one dimension")
+    seqs = page_table.shape[0]
+    if page_table.dtype != torch.int32 or page_table.get_device() != index or not page_table.is_contiguous():
+        raise ValueError(f"{what}: page_table must be contiguous int32 on the cache's device")
+    for t in lengths:
+        if t.dtype != torch.int32 or t.get_device() != index or t.shape != (seqs,) or not t.is_contiguous():
+            raise ValueError(f"{what}: starts and lengths must be contiguous int32 [{seqs}] on the cache's device")
+    return seqs
 
 
-def _call_on(device: torch.device, name: str, *args: object) -> None:
-    """`call` with `device` current and its current stream as the last argument."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+def _call_on(index: int, name: str, *args: object) -> None:
+    """`call` with device `index` current and its current stream as the last argument."""
+    if index == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _bytes(n: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
-def _rows_on(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype, width: int) -> int:
-    """Row stride of a [rows, >= width] tensor on `device`."""
-    _need(t, name, dtype, 2)
-    if t.device != device or t.shape[1] < width:
-        raise ValueError(f"{name} must be on {device} and hold {width} columns, got {tuple(t.shape)} on {t.device}")
+def _rows_on(t: torch.Tensor, name: str, index: int, dtype: torch.dtype, width: int) -> int:
+    """Row stride of a [rows, >= width] tensor on device `index`."""
+    if t.dim() != 2 or t.dtype != dtype or t.get_device() != index or t.shape[1] < width:
+        raise ValueError(f"{name} must be {dtype} on the cache's device and hold rows of {width}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return _rows(t, name)
 
 
@@ -742,21 +748,19 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, positions: tor
     into the last seq_len[b] of ctx_len[b] slots, in 4 bits, with one int32 position a row (see dx_kv4_append).
     Attention with a window expects positions that rise with the slots. A sequence's new slots must lie in pages that
     no other sequence of the call writes."""
-    c = _kv4(cache, "kv4_append")
-    dev = cache.k.device
-    if k.dtype not in (BF16, F32):
-        raise ValueError(f"kv4_append: k and v must be bf16 or fp32, got {k.dtype}")
-    width = c.num_kv_heads * c.head_dim
-    ks, vs = _rows_on(k, "k", dev, k.dtype, width), _rows_on(v, "v", dev, k.dtype, width)
-    _need(positions, "positions", torch.int32, 1)
-    if not k.shape[0] == v.shape[0] == positions.shape[0] or not positions.is_contiguous() or positions.device != dev:
-        raise ValueError("kv4_append: k, v and positions need one row a token, on the cache's device")
-    _kv4_ints("kv4_append", dev, page_table, seq_start, seq_len, ctx_len)
-    if k.shape[0] == 0 or page_table.shape[0] == 0:
+    seqs = _kv4_ints("kv4_append", cache, page_table, seq_start, seq_len, ctx_len)
+    index, dtype, rows, width = cache.index, k.dtype, k.shape[0], cache.heads * cache.head_dim
+    if dtype not in (BF16, F32):
+        raise ValueError(f"kv4_append: k and v must be bf16 or fp32, got {dtype}")
+    ks, vs = _rows_on(k, "k", index, dtype, width), _rows_on(v, "v", index, dtype, width)
+    if positions.dtype != torch.int32 or positions.shape != (rows,) or v.shape[0] != rows or \
+            positions.get_device() != index or not positions.is_contiguous():
+        raise ValueError("kv4_append: k, v and positions (contiguous int32) need one row a token, on the cache's device")
+    if rows == 0 or seqs == 0:
         return
-    _call_on(dev, "dx_kv4_append", byref(c), k.data_ptr(), v.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
-             page_table.shape[1], seq_start.data_ptr(), seq_len.data_ptr(), ctx_len.data_ptr(), page_table.shape[0],
-             max_seq_len, k.shape[0], ks, vs, DX_BF16 if k.dtype == BF16 else DX_F32)
+    _call_on(index, "dx_kv4_append", cache.ref, k.data_ptr(), v.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
+             page_table.shape[1], seq_start.data_ptr(), seq_len.data_ptr(), ctx_len.data_ptr(), seqs, max_seq_len, rows,
+             ks, vs, DX_BF16 if dtype == BF16 else DX_F32)
 
 
 def kv4_read(cache: KV4Cache, page_table: torch.Tensor, seq_start: torch.Tensor, seq_len: torch.Tensor,
@@ -764,32 +768,29 @@ def kv4_read(cache: KV4Cache, page_table: torch.Tensor, seq_start: torch.Tensor,
              out_v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [rows, Hkv * D] bf16: the last seq_len[b] slots of every sequence as the cache holds them, packed as
     `kv4_append` takes them (for `attention_varlen` over a cached state, say). Rows of no sequence are not written."""
-    c = _kv4(cache, "kv4_read")
-    dev = cache.k.device
-    width = c.num_kv_heads * c.head_dim
+    seqs = _kv4_ints("kv4_read", cache, page_table, seq_start, seq_len, ctx_len)
+    index, width = cache.index, cache.heads * cache.head_dim
     if rows < 0:
         raise ValueError("kv4_read: rows must be >= 0")
-    k = torch.empty((rows, width), dtype=BF16, device=dev) if out_k is None else out_k
-    v = torch.empty((rows, width), dtype=BF16, device=dev) if out_v is None else out_v
-    ks, vs = _rows_on(k, "out_k", dev, BF16, width), _rows_on(v, "out_v", dev, BF16, width)
+    k = torch.empty((rows, width), dtype=BF16, device=cache.k.device) if out_k is None else out_k
+    v = torch.empty((rows, width), dtype=BF16, device=cache.k.device) if out_v is None else out_v
+    ks, vs = _rows_on(k, "out_k", index, BF16, width), _rows_on(v, "out_v", index, BF16, width)
     if k.shape[0] < rows or v.shape[0] < rows:
         raise ValueError(f"kv4_read: out_k and out_v must hold {rows} rows")
-    _kv4_ints("kv4_read", dev, page_table, seq_start, seq_len, ctx_len)
-    if rows == 0 or page_table.shape[0] == 0:
+    if rows == 0 or seqs == 0:
         return k, v
-    _call_on(dev, "dx_kv4_read", byref(c), k.data_ptr(), v.data_ptr(), page_table.data_ptr(), page_table.shape[1],
-             seq_start.data_ptr(), seq_len.data_ptr(), ctx_len.data_ptr(), page_table.shape[0], max_seq_len, rows, ks, vs)
+    _call_on(index, "dx_kv4_read", cache.ref, k.data_ptr(), v.data_ptr(), page_table.data_ptr(), page_table.shape[1],
+             seq_start.data_ptr(), seq_len.data_ptr(), ctx_len.data_ptr(), seqs, max_seq_len, rows, ks, vs)
     return k, v
 
 
-def _weights(t: torch.Tensor, name: str, device: torch.device, seqs: int, heads: int, slots: int) -> tuple[int, int]:
+def _weights(t: torch.Tensor, name: str, index: int, seqs: int, heads: int, slots: int) -> tuple[int, int]:
     """Strides of accumulated weights [seqs, heads, >= slots]."""
-    _need(t, name, F32, 3)
-    if t.device != device or t.shape[0] != seqs or t.shape[1] != heads or t.shape[2] < slots or \
-            (t.stride(2) != 1 and t.shape[2] > 1):
-        raise ValueError(f"{name} must be [{seqs}, {heads}, >= {slots}] on {device} with neighbouring slots, "
-                         f"got {tuple(t.shape)}")
-    seq, head = t.stride(0), t.stride(1)
+    if t.dim() != 3 or t.dtype != F32 or t.get_device() != index or t.shape[:2] != (seqs, heads) or \
+            t.shape[2] < slots or (t.stride(2) != 1 and t.shape[2] > 1):
+        raise ValueError(f"{name} must be fp32 [{seqs}, {heads}, >= {slots}] on the cache's device with neighbouring "
+                         f"slots, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    seq, head, _ = t.stride()
     if (heads > 1 and head < t.shape[2]) or (seqs > 1 and seq < heads * head and seq < t.shape[2]):
         raise ValueError(f"{name}: rows must not overlap")
     return seq, max(head, t.shape[2])
@@ -806,33 +807,32 @@ def attention_kv4(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, se
     With `weights` (fp32 [sequences, Hkv, >= max_ctx_len]) every slot's accumulated attention weight goes to
     `weights_out` (default: `weights` itself): the old one, taken as 0 for the newest tokens' slots, plus the softmax
     weights of all rows and query heads that saw it. `kv4_evict` goes by them."""
-    c = _kv4(cache, "attention_kv4")
-    dev = cache.k.device
-    dtype = q.dtype
+    seqs = _kv4_ints("attention_kv4", cache, page_table, seq_start, seq_len, ctx_len)
+    index, heads, dtype, rows = cache.index, cache.heads, q.dtype, q.shape[0]
     if dtype not in (BF16, F32):
         raise ValueError(f"attention_kv4: q must be bf16 or fp32, got {dtype}")
-    width = num_q_heads * c.head_dim
-    qs = _rows_on(q, "q", dev, dtype, width)
+    width = num_q_heads * cache.head_dim
+    qs = _rows_on(q, "q", index, dtype, width)
     if out is None:
-        out = torch.empty((q.shape[0], width), dtype=dtype, device=dev)
-    os = _rows_on(out, "out", dev, dtype, width)
+        out = torch.empty((rows, width), dtype=dtype, device=q.device)
+    os = _rows_on(out, "out", index, dtype, width)
     _check_out(out, q, width)
-    _kv4_ints("attention_kv4", dev, page_table, seq_start, seq_len, ctx_len)
-    seqs = page_table.shape[0]
     if weights is None and weights_out is not None:
         raise ValueError("attention_kv4: weights_out needs weights")
+    w_in = w_out = None
     wi = wo = (0, 0)
     if weights is not None:
         weights_out = weights if weights_out is None else weights_out
-        wi = _weights(weights, "weights", dev, seqs, c.num_kv_heads, max_ctx_len)
-        wo = _weights(weights_out, "weights_out", dev, seqs, c.num_kv_heads, max_ctx_len)
+        wi = _weights(weights, "weights", index, seqs, heads, max_ctx_len)
+        wo = _weights(weights_out, "weights_out", index, seqs, heads, max_ctx_len)
+        w_in, w_out = weights.data_ptr(), weights_out.data_ptr()
     if seqs == 0:
         return out
-    ws = _bytes(_lib.lib().dx_attn_kv4_workspace(seqs, max_seq_len, max_ctx_len, num_q_heads, c.num_kv_heads,
-                                                 c.head_dim, window, weights is not None), dev)
-    _call_on(dev, "dx_attn_kv4", byref(c), q.data_ptr() or ws.data_ptr(), out.data_ptr() or ws.data_ptr(),
+    ws = _bytes(_lib.lib().dx_attn_kv4_workspace(seqs, max_seq_len, max_ctx_len, num_q_heads, heads, cache.head_dim,
+                                                 window, weights is not None), q.device)
+    _call_on(index, "dx_attn_kv4", cache.ref, q.data_ptr() or ws.data_ptr(), out.data_ptr() or ws.data_ptr(),
              page_table.data_ptr(), page_table.shape[1], seq_start.data_ptr(), seq_len.data_ptr(), ctx_len.data_ptr(),
-             seqs, max_seq_len, max_ctx_len, q.shape[0], num_q_heads, qs, os, float(scale), float(softcap), int(window), _ptr(weights), *wi, _ptr(weights_out), *wo,
+             seqs, max_seq_len, max_ctx_len, rows, num_q_heads, qs, os, scale, softcap, window, w_in, *wi, w_out, *wo,
              DX_BF16 if dtype == BF16 else DX_F32, ws.data_ptr(), ws.numel())
     return out
 
@@ -844,24 +844,24 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor, page_table: torch.Tensor, 
     call shares: each KV head keeps its last `recent` slots and the heaviest others by `weights`, in slot order (see
     dx_kv4_evict). Returns the kept slots' weights [sequences, Hkv, keep] (zeros behind them) and the new lengths; the
     old pages stay as they are."""
-    c = _kv4(cache, "kv4_evict")
-    dev = cache.k.device
-    _kv4_ints("kv4_evict", dev, page_table, ctx_len)
-    _kv4_ints("kv4_evict", dev, out_table, ctx_len)
-    seqs = page_table.shape[0]
+    seqs = _kv4_ints("kv4_evict", cache, page_table, ctx_len)
+    _kv4_ints("kv4_evict", cache, out_table, ctx_len)
+    index, heads, dev = cache.index, cache.heads, cache.k.device
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"kv4_evict: need keep >= 1 and 0 <= recent <= keep, got {keep} and {recent}")
-    wi = _weights(weights, "weights", dev, seqs, c.num_kv_heads, min(max_ctx_len, page_table.shape[1] * c.page_size))
+    wi = _weights(weights, "weights", index, seqs, heads, min(max_ctx_len, page_table.shape[1] * cache.page_size))
     if weights_out is None:
-        weights_out = torch.empty((seqs, c.num_kv_heads, keep), dtype=F32, device=dev)
-    wo = _weights(weights_out, "weights_out", dev, seqs, c.num_kv_heads, keep)
-    if weights_out.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
-        raise ValueError("kv4_evict: weights_out must have memory of its own")
+        weights_out = torch.empty((seqs, heads, keep), dtype=F32, device=dev)
+        wo = (heads * keep, keep)
+    else:
+        wo = _weights(weights_out, "weights_out", index, seqs, heads, keep)
+        if weights_out.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
+            raise ValueError("kv4_evict: weights_out must have memory of its own")
     out_len = torch.empty(seqs, dtype=torch.int32, device=dev)
     if seqs == 0:
         return weights_out, out_len
-    ws = _bytes(_lib.lib().dx_kv4_evict_workspace(seqs, c.num_kv_heads, keep), dev)
-    _call_on(dev, "dx_kv4_evict", byref(c), weights.data_ptr(), *wi, page_table.data_ptr(), page_table.shape[1],
+    ws = _bytes(_lib.lib().dx_kv4_evict_workspace(seqs, heads, keep), dev)
+    _call_on(index, "dx_kv4_evict", cache.ref, weights.data_ptr(), *wi, page_table.data_ptr(), page_table.shape[1],
              ctx_len.data_ptr(), seqs, max_ctx_len, out_table.data_ptr(), out_table.shape[1], keep, recent,
              weights_out.data_ptr(), *wo, out_len.data_ptr(), ws.data_ptr(), ws.numel())
     return weights_out, out_len
@@ -876,22 +876,24 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
     if dtype not in (BF16, F32):
         raise ValueError(f"token_logprobs: logits must be bf16 or fp32, got {dtype}")
     _need(logits, "logits", dtype, 2)
-    _need(targets, "targets", torch.int32, 1)
     rows, vocab = logits.shape
     dev = logits.device
-    if targets.shape[0] != rows or targets.device != dev or not targets.is_contiguous():
+    if targets.dtype != torch.int32 or targets.shape != (rows,) or targets.get_device() != dev.index or \
+            not targets.is_contiguous():
         raise ValueError("token_logprobs: targets must hold one contiguous int32 a row, on the logits' device")
     stride = _rows(logits, "logits")
     stride = stride if rows > 1 else max(stride, vocab)  # one row has no next one
-    logprobs = torch.empty(rows, dtype=F32, device=dev)
-    entropy = torch.empty(rows, dtype=F32, device=dev)
-    ids = torch.empty((rows, max(top, 0)), dtype=torch.int32, device=dev)
-    top_logprobs = torch.empty((rows, max(top, 0)), dtype=F32, device=dev)
+    n = max(top, 0)
+    scores = torch.empty(rows * (2 + n), dtype=F32, device=dev)  # log probabilities, entropies, the alternatives'
+    ids = torch.empty((rows, n), dtype=torch.int32, device=dev)
+    logprobs, entropy, top_logprobs = scores[:rows], scores[rows:2 * rows], scores[2 * rows:].view(rows, n)
+    if rows == 0:
+        return logprobs, entropy, ids, top_logprobs
     ws = _bytes(_lib.lib().dx_token_logprobs_workspace(rows, vocab, top), dev)
-    _call_on(dev, "dx_token_logprobs", logits.data_ptr() or ws.data_ptr(), targets.data_ptr() or ws.data_ptr(), rows,
-             vocab, stride, float(softcap), top,
-             logprobs.data_ptr() or ws.data_ptr(), entropy.data_ptr() or ws.data_ptr(), ids.data_ptr() or ws.data_ptr(),
-             top_logprobs.data_ptr() or ws.data_ptr(), DX_BF16 if dtype == BF16 else DX_F32, ws.data_ptr(), ws.numel())
+    at = scores.data_ptr()
+    _call_on(dev.index, "dx_token_logprobs", logits.data_ptr(), targets.data_ptr(), rows, vocab, stride, softcap, top, at,
+             at + 4 * rows, ids.data_ptr() or at, at + 8 * rows, DX_BF16 if dtype == BF16 else DX_F32, ws.data_ptr(),
+             ws.numel())
     return logprobs, entropy, ids, top_logprobs
 
 

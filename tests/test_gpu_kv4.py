@@ -17,6 +17,7 @@ from tests.conftest import i32, rng, say
 pytestmark = pytest.mark.gpu
 
 U32 = 2.0 ** -24
+FIELDS = ("k", "v", "k_scale", "v_scale", "positions")
 
 
 class Case:
@@ -445,7 +446,7 @@ def test_evict(ctx: list[int], keep: int, recent: int, d: int, hkv: int, page: i
     r = rng(keep)
     per = -(-keep // page)
     big = K.kv4_cache(c.pages + extra, hkv, d, page_size=page)
-    for n in c.cache._fields:
+    for n in FIELDS:
         getattr(big, n)[:c.pages] = getattr(c.cache, n)
     c.cache = big
     out_table = c.pages + r.permutation(extra).reshape(len(ctx), per)
@@ -497,7 +498,7 @@ def test_a_state_is_kept_cut_and_answered_over() -> None:
     keep = 100
     per = 3  # room for the answer behind what is kept
     big = K.kv4_cache(c.pages + 2 * per, hkv, d, page_size=page)
-    for n in c.cache._fields:
+    for n in FIELDS:
         getattr(big, n)[:c.pages] = getattr(c.cache, n)
     old_w = w[:, :, :].cpu().numpy()
     c.cache = big
