@@ -811,16 +811,18 @@ int validate_kv_rows(const Kv4Cache &c, const Kv4Batch &q, const void *k, const 
   return DX_OK;
 }
 
-// Where the parts of dx_attn_kv4's workspace start, in bytes: spans' outputs, their statistics, the rows' log sums.
+// Where the parts of dx_attn_kv4's workspace start, in bytes: spans' outputs, their statistics, the rows' log sums and
+// kept scores.
 struct Kv4Workspace {
-  int64_t stats, lse, total;
+  int64_t stats, lse, scores, total;
 };
 
 Kv4Workspace kv4_workspace(const Kv4Plan &p, int64_t units, int32_t d, bool weights) {
   Kv4Workspace w;
   w.stats = align_up(units * p.part_rows * d * 4, 256);
   w.lse = w.stats + align_up(units * p.part_rows * 8, 256);
-  w.total = w.lse + (weights ? units * p.max_rows * 4 : 0);
+  w.scores = w.lse + (weights ? align_up(units * p.max_rows * 4, 256) : 0);
+  w.total = w.scores + (weights ? units * p.score_rows * (int64_t)p.score_slots * 4 : 0);
   return w;
 }
 
@@ -913,6 +915,9 @@ int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32
   a.partial = reinterpret_cast<float *>(ws);
   a.stats = reinterpret_cast<float *>(ws + w.stats);
   a.lse = reinterpret_cast<float *>(ws + w.lse);
+  a.scores = weights_out && rows > 0 ? reinterpret_cast<float *>(ws + w.scores) : nullptr;
+  a.score_rows = p.score_rows;
+  a.score_slots = p.score_slots;
   a.part_rows = p.part_rows;
   a.max_rows = p.max_rows;
   a.max_splits = p.max_splits;

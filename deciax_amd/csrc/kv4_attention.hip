@@ -38,7 +38,7 @@ struct Spans {
   int lo, keys, count;
 };
 
-constexpr int SPAN = 256, MAX_SPANS = 32, SPLIT_ROWS = 4096;
+constexpr int SPAN = 512, MAX_SPANS = 32, SPLIT_ROWS = 4096;
 
 __host__ __device__ inline int most_spans(int rows) {
   const int most = SPLIT_ROWS / (rows > 0 ? rows : 1);
@@ -57,6 +57,8 @@ __host__ __device__ inline Spans spans(int ctx, int n, int rows, int window) {
 
 // Rows of a KV head up to which waves share rows and split keys.
 constexpr int FEW_ROWS = 48;
+// Rows of a KV head up to which their scores are kept for the accumulated weights, instead of computed again.
+constexpr int SCORE_ROWS = 16;
 
 DX_DEVICE floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -87,6 +89,14 @@ DX_DEVICE s16x4 read_transposed(const uint16_t *p) {
 #else
   return s16x4{};
 #endif
+}
+
+// A barrier for what went through LDS. __syncthreads() would wait for the loads and stores on their way as well: the next
+// keys' and this span's outputs'.
+DX_DEVICE void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // x = x0 + x1 + x2 in bf16 parts (24 bits and more), or its one rounding.
@@ -233,23 +243,26 @@ DX_DEVICE void key_scores(const Keys<D> &w, const bf16x8 (&q)[D / 32][NS], float
 // The pages of a span, a lane each (64 at a time), so that the loop over keys looks none up in memory.
 struct Pages {
   const int32_t *table;
-  int width, first, page;  // `page`: of this lane, table[first + lane]
+  int width, first;
+  long base;  // of this lane: the first row of page table[first + lane] for one head, -1 for none
 
-  DX_DEVICE void load(int at, int lane) {
+  DX_DEVICE void load(const Kv4Cache &c, int g, int at, int lane) {
     first = at;
-    page = at + lane < width ? table[at + lane] : -1;
+    const int page = at + lane < width ? table[at + lane] : -1;
+    base = page >= 0 && page < c.pages ? ((long)page * c.hkv + g) << c.shift : -1;
   }
   // row_of(slot), for a slot that is the same in all lanes
   DX_DEVICE long row(const Kv4Cache &c, int g, int slot, int lane) {
     const int at = slot >> c.shift;
-    if (at - first >= 64 || at < first) {
-      load(at, lane);
+    if (at - first >= 64) {  // slots only rise
+      load(c, g, at, lane);
       // wait here: behind the branch the wait would be for all loads on their way, taken or not
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     }
-    const int p = __builtin_amdgcn_readlane(page, at - first);
-    if (p < 0 || p >= c.pages) return -1;
-    return (((long)p * c.hkv + g) << c.shift) + (slot & ((1 << c.shift) - 1));
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)base, at - first);
+    const int hi = __builtin_amdgcn_readlane((int)(base >> 32), at - first);
+    const long row = (long)hi << 32 | lo;
+    return hi < 0 ? -1 : row + (slot & ((1 << c.shift) - 1));
   }
 };
 
@@ -291,6 +304,17 @@ DX_DEVICE uint32_t mask4(const Kv4Attn &a, const Row &row, int key, const int4 &
   return seen;
 }
 
+// The largest of the lanes l % 16 of all four lane groups: rows of 16 lanes, then of 32, exchanged in registers.
+DX_DEVICE float max_of_groups(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+#endif
+  return x;
+}
+
 // The softmax of eight more scores a lane (32 keys a row): raises the running maximum `m`, scales what was summed, and
 // gives P as the matrix operand. The lanes of a row keep partial sums `l`, joined at the end.
 template <int ND, int NS>
@@ -298,8 +322,7 @@ DX_DEVICE void softmax_step(const float (&t2)[2][4], float &m, float &l, floatx4
   float top = t2[0][0];
 #pragma unroll
   for (int r = 1; r < 8; ++r) top = fmaxf(top, t2[r >> 2][r & 3]);
-  top = fmaxf(top, __shfl_xor(top, 16, 64));
-  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  top = max_of_groups(top);
   if (__any(top > m)) {
     const float next = fmaxf(m, top);
     const float f = next == -INFINITY ? 1.f : fast_exp2(m - next);
@@ -372,18 +395,20 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
   } stages[WAVES];
   __shared__ float join_m[WAVES][16], join_l[WAVES][16];
   const int g = blockIdx.y, b = blockIdx.z;
-  const int tiles = gridDim.x / a.max_splits, row_tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+  const int tiles = a.few_tiles, row_tile = blockIdx.x % tiles;
   const Sequence s = sequence(a.q, b, a.c.shift);
   const int group = a.hq / a.c.hkv, rows = s.n * group, r0 = row_tile * 16;
   if (r0 >= rows || rows > a.few_rows) return;
   const Spans sp = spans(s.ctx, s.n, rows, a.slots);
-  if (split >= sp.count) return;
+  const int first_span = blockIdx.x / tiles * a.spans_each, end_span = min(first_span + a.spans_each, sp.count);
+  if (first_span >= sp.count) return;
   const int32_t *table = a.q.table + (long)b * a.q.table_width;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int k0 = sp.lo + split * sp.keys, k1 = min(s.ctx, k0 + sp.keys);
+  // this workgroup's spans: their keys follow each other, and so do its waves' steps
+  const int k0 = sp.lo + first_span * sp.keys, k1 = min(s.ctx, sp.lo + end_span * sp.keys);
   Pages pages{table, a.q.table_width, 0, -1};
-  pages.load(k0 >> a.c.shift, lane);
+  pages.load(a.c, g, k0 >> a.c.shift, lane);
   Stage<D> &st = stages[wave].stage;
 
   // Where 16-byte chunk x of 32 rows of K stands in the stage: a row's chunks are exchanged so that 16 rows' reads of one
@@ -396,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
   u32x4 kr[KL], vr[D / VW][VJ];
   uint32_t ks[2][Keys<D>::N], vs[D / VW][VJ];
   int4 pos[2] = {};
-  // A step without a page, or past the span's end, reads the pool's first rows instead: nothing of them is seen. No branch
+  // A step without a page, or past the last span's end, reads the pool's first rows instead: nothing of them is seen. No branch
   // goes round the loads, behind which the compiler could only wait for all of them.
   auto fetch_keys = [&](int kb) {
     const long row0 = kb < k1 ? pages.row(a.c, g, kb, lane) : -1, at = max(row0, 0L);
@@ -438,144 +463,157 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
   // keys below `open` are seen by every row of the tile, as far as the order of tokens goes
   const int open = s.ctx - s.n + r0 / group + 1;
 
-  floatx4 o[D / 16];
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int span = first_span; span < end_span; ++span) {
+    floatx4 o[D / 16];
+  #pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const int span_end = min(s.ctx, sp.lo + (span + 1) * sp.keys);
 
-  for (; kb < k1; kb += WAVES * STEP) {
-    const bool page = row0 >= 0;
-    Keys<D> w;
-#pragma unroll
-    for (int i = 0; i < KL; ++i) *reinterpret_cast<u32x4 *>(st.k + k_slot(i * 64 + lane)) = kr[i];
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int r = t * 16 + col;
-      if constexpr (D == 64) {
-        const u32x2 x = *reinterpret_cast<const u32x2 *>(st.k + r * 32 + grp * 8);
-        w.k[t][0] = u32x4{x[0], x[1], 0, 0};
-      } else {
-#pragma unroll
-        for (int j = 0; j < Keys<D>::N; ++j) w.k[t][j] = *reinterpret_cast<const u32x4 *>(st.k + k_slot(r * LPK + j * 4 + grp));
+    for (; kb < span_end; kb += WAVES * STEP) {
+      const bool page = row0 >= 0;
+      Keys<D> w;
+  #pragma unroll
+      for (int i = 0; i < KL; ++i) *reinterpret_cast<u32x4 *>(st.k + k_slot(i * 64 + lane)) = kr[i];
+      __builtin_amdgcn_wave_barrier();
+  #pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = t * 16 + col;
+        if constexpr (D == 64) {
+          const u32x2 x = *reinterpret_cast<const u32x2 *>(st.k + r * 32 + grp * 8);
+          w.k[t][0] = u32x4{x[0], x[1], 0, 0};
+        } else {
+  #pragma unroll
+          for (int j = 0; j < Keys<D>::N; ++j)
+            w.k[t][j] = *reinterpret_cast<const u32x4 *>(st.k + k_slot(r * LPK + j * 4 + grp));
+        }
+  #pragma unroll
+        for (int j = 0; j < Keys<D>::N; ++j) {
+          w.scale[t][j] = scale_of(ks[t][j]);
+          asm volatile("" : "+v"(w.scale[t][j]));  // before the next ones are asked for, not with a copy of them
+        }
       }
-#pragma unroll
-      for (int j = 0; j < Keys<D>::N; ++j) {
-        w.scale[t][j] = scale_of(ks[t][j]);
-        asm volatile("" : "+v"(w.scale[t][j]));  // before the next ones are asked for, not with a copy of them
+      int4 here[2] = {pos[0], pos[1]};
+      if constexpr (WIN) {
+  #pragma unroll
+        for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(here[t].x), "+v"(here[t].y), "+v"(here[t].z), "+v"(here[t].w));
       }
-    }
-    int4 here[2] = {pos[0], pos[1]};
-    if constexpr (WIN) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(here[t].x), "+v"(here[t].y), "+v"(here[t].z), "+v"(here[t].w));
-    }
-    const long next = fetch_keys(kb + WAVES * STEP);
+      const long next = fetch_keys(kb + WAVES * STEP);
 
-    float t2[2][4];
-    key_scores<D, NS, CAP>(w, q, a.scale, a.softcap, t2);
-    const bool masked = WIN || kb + STEP > open || !page;
-    uint32_t seen = 0xff;  // of this lane's eight keys
-    if (masked) {
-      seen = 0;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        seen |= mask4<WIN>(a, row, page ? kb + t * 16 + grp * 4 : 0x7ffffff0, here[t], t2[t]) << (4 * t);
-    }
-    bf16x8 pb[NS];
-    softmax_step<D / 16, NS>(t2, m, l, o, pb);
+      float t2[2][4];
+      key_scores<D, NS, CAP>(w, q, a.scale, a.softcap, t2);
+      const bool masked = WIN || kb + STEP > open || !page;
+      uint32_t seen = 0xff;  // of this lane's eight keys
+      if (masked) {
+        seen = 0;
+  #pragma unroll
+        for (int t = 0; t < 2; ++t)
+          seen |= mask4<WIN>(a, row, page ? kb + t * 16 + grp * 4 : 0x7ffffff0, here[t], t2[t]) << (4 * t);
+      }
+      if (a.scores && rows <= SCORE_ROWS && col < rows) {
+        float *to = a.scores + (((long)b * a.c.hkv + g) * a.score_rows + col) * a.score_slots + kb + grp * 4;
+  #pragma unroll
+        for (int t = 0; t < 2; ++t)
+          *reinterpret_cast<floatx4 *>(to + t * 16) = floatx4{t2[t][0], t2[t][1], t2[t][2], t2[t][3]};
+      }
+      bf16x8 pb[NS];
+      softmax_step<D / 16, NS>(t2, m, l, o, pb);
 
-    // V to bf16, VW columns at a time. Slots behind the sequence hold anything: zeros here. A block of NaN may stand behind
-    // a row's own token too, where 0 NaN would reach the row: such blocks are zero here and added below to the rows that
-    // see them.
-    uint64_t nan_blocks[D / VW][VJ];
-    bool any_nan = false;
-#pragma unroll
-    for (int h = 0; h < D / VW; ++h) {
-#pragma unroll
-      for (int j = 0; j < VJ; ++j) {
-        const int key = j * VK + lane / VB;
-        u32x4 x = vr[h][j];
-        uint32_t byte = vs[h][j];
-        if (masked) {
-          const bool inside = page && kb + key < s.ctx, bad = byte == 255;
-          nan_blocks[h][j] = __ballot(inside && bad);
-          any_nan = any_nan || nan_blocks[h][j] != 0;
-          if (!inside || bad) {
-            x = u32x4{0, 0, 0, 0};
-            byte = 127;
+      // V to bf16, VW columns at a time. Slots behind the sequence hold anything: zeros here. A block of NaN may stand behind
+      // a row's own token too, where 0 NaN would reach the row: such blocks are zero here and added below to the rows that
+      // see them.
+      uint64_t nan_blocks[D / VW][VJ];
+      bool any_nan = false;
+  #pragma unroll
+      for (int h = 0; h < D / VW; ++h) {
+  #pragma unroll
+        for (int j = 0; j < VJ; ++j) {
+          const int key = j * VK + lane / VB;
+          u32x4 x = vr[h][j];
+          uint32_t byte = vs[h][j];
+          if (masked) {
+            const bool inside = page && kb + key < s.ctx, bad = byte == 255;
+            nan_blocks[h][j] = __ballot(inside && bad);
+            any_nan = any_nan || nan_blocks[h][j] != 0;
+            if (!inside || bad) {
+              x = u32x4{0, 0, 0, 0};
+              byte = 127;
+            }
+          }
+  #pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<u32x4 *>(st.vt + v_chunk<VW>(key, lane % VB * 4 + i)) = decode8(x[i], scale_of(byte));
+        }
+        if (h == D / VW - 1) fetch_values(next);
+        __builtin_amdgcn_wave_barrier();
+  #pragma unroll
+        for (int i = 0; i < VW / 16; ++i) {
+          const uint16_t *p0 = st.vt + v_chunk<VW>(grp * 4 + (col >> 2), 2 * i + ((col >> 1) & 1)) + (col & 1) * 4;
+          const s16x4 v0 = read_transposed(p0), v1 = read_transposed(p0 + 16 * VW);  // 16 rows on: the same place
+          const bf16x8 vt = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+  #pragma unroll
+          for (int n = 0; n < NS; ++n) o[h * (VW / 16) + i] = mfma16(vt, pb[n], o[h * (VW / 16) + i]);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+      if (masked && any_nan) {
+  #pragma unroll
+        for (int blk = 0; blk < LPK; ++blk) {
+          int hit = 0;
+  #pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int key = (r >> 2) * 16 + grp * 4 + (r & 3);
+            uint64_t bits = nan_blocks[blk / VB][0];
+  #pragma unroll
+            for (int j = 1; j < VJ; ++j) bits = key / VK == j ? nan_blocks[blk / VB][j] : bits;
+            hit |= (int)((bits >> (key % VK * VB + blk % VB)) & 1) & (int)((seen >> r) & 1);
+          }
+          hit |= __shfl_xor(hit, 16, 64);
+          hit |= __shfl_xor(hit, 32, 64);
+          if (hit) {
+            o[2 * blk] += NAN;
+            o[2 * blk + 1] += NAN;
           }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<u32x4 *>(st.vt + v_chunk<VW>(key, lane % VB * 4 + i)) = decode8(x[i], scale_of(byte));
       }
-      if (h == D / VW - 1) fetch_values(next);
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int i = 0; i < VW / 16; ++i) {
-        const uint16_t *p0 = st.vt + v_chunk<VW>(grp * 4 + (col >> 2), 2 * i + ((col >> 1) & 1)) + (col & 1) * 4;
-        const s16x4 v0 = read_transposed(p0), v1 = read_transposed(p0 + 16 * VW);  // 16 rows on: the same place
-        const bf16x8 vt = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int n = 0; n < NS; ++n) o[h * (VW / 16) + i] = mfma16(vt, pb[n], o[h * (VW / 16) + i]);
-      }
-      __builtin_amdgcn_wave_barrier();
+      row0 = next;
     }
-    if (masked && any_nan) {
-#pragma unroll
-      for (int blk = 0; blk < LPK; ++blk) {
-        int hit = 0;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const int key = (r >> 2) * 16 + grp * 4 + (r & 3);
-          uint64_t bits = nan_blocks[blk / VB][0];
-#pragma unroll
-          for (int j = 1; j < VJ; ++j) bits = key / VK == j ? nan_blocks[blk / VB][j] : bits;
-          hit |= (int)((bits >> (key % VK * VB + blk % VB)) & 1) & (int)((seen >> r) & 1);
-        }
-        hit |= __shfl_xor(hit, 16, 64);
-        hit |= __shfl_xor(hit, 32, 64);
-        if (hit) {
-          o[2 * blk] += NAN;
-          o[2 * blk + 1] += NAN;
-        }
-      }
-    }
-    row0 = next;
-  }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
 
-  // the four waves' parts, through LDS: [16 rows][D] fp32 a wave, where its stage was
-  if (grp == 0) {
-    join_m[wave][col] = m;
-    join_l[wave][col] = l;
-  }
-  __syncthreads();
-  float top = join_m[0][col];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) top = fmaxf(top, join_m[w][col]);
-  const float f = part_weight(m, l, top);
-  float *part = stages[wave].part;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i)
-    *reinterpret_cast<floatx4 *>(part + col * D + i * 16 + grp * 4) = o[i] * f;
-  __syncthreads();
-
-  const int valid = min(16, rows - r0);
-  for (int i = tid; i < valid * (D / 4); i += THREADS) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float mm = join_m[0][r], ll = 0.f;
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, join_m[w][r]);
-    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      ll += join_l[w][r] * part_weight(join_m[w][r], join_l[w][r], mm);
-      acc += *reinterpret_cast<const floatx4 *>(stages[w].part + r * D + d);
+    // the four waves' parts, through LDS: [16 rows][D] fp32 a wave, where its stage was
+    if (grp == 0) {
+      join_m[wave][col] = m;
+      join_l[wave][col] = l;
     }
-    store_row<D, NS>(a, s, sp, (long)b * a.c.hkv + g, g, group, rows, split, r0 + r, d, acc, mm, ll);
+    lds_barrier();
+    float top = join_m[0][col];
+  #pragma unroll
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, join_m[w][col]);
+    const float f = part_weight(m, l, top);
+    float *part = stages[wave].part;
+    const int valid = min(16, rows - r0);
+    if (col < valid) {
+  #pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        *reinterpret_cast<floatx4 *>(part + col * D + i * 16 + grp * 4) = o[i] * f;
+    }
+    lds_barrier();
+
+    for (int i = tid; i < valid * (D / 4); i += THREADS) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float mm = join_m[0][r], ll = 0.f;
+  #pragma unroll
+      for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, join_m[w][r]);
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+  #pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        ll += join_l[w][r] * part_weight(join_m[w][r], join_l[w][r], mm);
+        acc += *reinterpret_cast<const floatx4 *>(stages[w].part + r * D + d);
+      }
+      store_row<D, NS>(a, s, sp, (long)b * a.c.hkv + g, g, group, rows, span, r0 + r, d, acc, mm, ll);
+    }
+    lds_barrier();
   }
 }
 
@@ -610,7 +648,7 @@ __global__ void __launch_bounds__(64 * TW, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
   const int k1 = min(min(s.ctx, k0 + sp.keys), last_own + 1);
   if (a.window > 0) k0 = max(k0, (first_own - a.slots + 1) & ~63);
   Pages pages{table, a.q.table_width, 0, -1};
-  pages.load(max(k0, 0) >> a.c.shift, lane);
+  pages.load(a.c, g, max(k0, 0) >> a.c.shift, lane);
 
   const int w0 = r0 + wave * 16 * NT;  // this wave's first row
   Row row[NT];
@@ -830,8 +868,42 @@ __global__ void __launch_bounds__(THREADS) kv4_join_kernel(Kv4Attn a) {
   if (a.w_out && lane == 0) a.lse[unit * a.max_rows + r] = m + log2f(l);
 }
 
-// weights_out_j = weights_in_j (0 for the newest slots) + sum over the rows that see j of e^{t_j} / sum e^t. A wave owns
-// 32 keys and walks all rows, so every sum has one owner and one order.
+// weights_out_j = weights_in_j (0 for the newest slots) + sum over the rows that see j of e^{t_j} / sum e^t, for sequences
+// of few rows, whose scores kv4_attn_kernel kept: 4 bytes a row and slot in the place of the key's 34, 68 or 136.
+__global__ void __launch_bounds__(THREADS) kv4_score_weights_kernel(Kv4Attn a) {
+  constexpr int ITER = 4;
+  const int g = blockIdx.y, b = blockIdx.z;
+  const Sequence s = sequence(a.q, b, a.c.shift);
+  const int group = a.hq / a.c.hkv, rows = s.n * group;
+  const int j0 = blockIdx.x * (ITER * THREADS) + threadIdx.x;
+  if (rows > SCORE_ROWS || j0 >= s.ctx) return;
+  const Spans sp = spans(s.ctx, s.n, rows, a.slots);
+  const long unit = (long)b * a.c.hkv + g;
+  const float *scores = a.scores + unit * a.score_rows * a.score_slots, *lse = a.lse + unit * a.max_rows;
+  const float *old = a.w_in + b * a.wi_seq + g * a.wi_head;
+  float sum[ITER] = {}, was[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) was[i] = old[min(j0 + i * THREADS, s.ctx - 1)];
+  for (int r = 0; r < rows; ++r) {
+    if (s.start + r / group < 0 || s.start + r / group >= a.q.rows) continue;  // no row of the packed q
+    const float base = lse[r];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int j = j0 + i * THREADS;
+      // no score below the window's first tile; a row that saw nothing has a base of -inf and scores of -inf
+      const float t = scores[(long)r * a.score_slots + min(max(j, sp.lo), s.ctx - 1)];
+      sum[i] += j >= sp.lo && t != -INFINITY ? fast_exp2(t - base) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int j = j0 + i * THREADS;
+    if (j < s.ctx) a.w_out[b * a.wo_seq + g * a.wo_head + j] = (j < s.ctx - s.n ? was[i] : 0.f) + sum[i];
+  }
+}
+
+// The same for sequences of more rows, from the keys. A wave owns 32 keys and walks all rows, so every sum has one owner and
+// one order.
 template <int D, int NS, bool CAP>
 __global__ void __launch_bounds__(THREADS) kv4_weights_kernel(Kv4Attn a) {
   const int g = blockIdx.y, b = blockIdx.z;
@@ -841,7 +913,7 @@ __global__ void __launch_bounds__(THREADS) kv4_weights_kernel(Kv4Attn a) {
   const int col = lane & 15, grp = lane >> 4;
   const int group = a.hq / a.c.hkv, rows = s.n * group;
   const int kb = (blockIdx.x * WAVES + wave) * STEP;
-  if (kb >= s.ctx) return;
+  if (kb >= s.ctx || (a.scores && rows <= SCORE_ROWS)) return;
   const long unit = (long)b * a.c.hkv + g;
   const long row0 = row_of(a.c, table, g, kb);
   const int lo = a.window > 0 ? s.ctx - s.n - a.slots + 1 : 0;
@@ -895,13 +967,19 @@ __global__ void __launch_bounds__(THREADS) kv4_weights_kernel(Kv4Attn a) {
 // up to 611 tokens 10.6 ms instead of 1.4).
 // Sequences of few rows take kv4_attn_kernel, of more kv4_attn_tile_kernel; a batch of both launches both.
 template <int D, int NS, bool CAP>
-hipError_t launch(const Kv4Attn &a, hipStream_t s) {
+hipError_t launch(Kv4Attn a, hipStream_t s) {
   constexpr int NT = NS == 1 && D < 256 ? 2 : 1, TW = NS == 1 && D == 256 ? 8 : 4;
   const int few = a.q.rows > 0 ? (min(a.max_rows, a.few_rows) + 15) / 16 : 0;  // without rows: the weights alone
   const int tiles = a.q.rows > 0 && a.max_rows > a.few_rows ? (a.max_rows + 16 * NT * TW - 1) / (16 * NT * TW) : 0;
+  a.few_tiles = few;
+  // Two spans a workgroup where there are many workgroups: a workgroup's start (lengths, page, query and first keys, each
+  // after the other) takes 3 us of some 13. 64 x 4000 137 -> 128 us, 32 x 14000 217 -> 206, 16 x 8000 64.3 -> 62.2;
+  // 4 x 16384 (1024 workgroups)
+  // 42.6 -> 44.3.
+  a.spans_each = (long)a.max_splits * few * a.c.hkv * a.q.num_seqs >= 2048 ? 2 : 1;
   hipError_t e = hipSuccess;
   if (few > 0) {
-    const dim3 grid(a.max_splits * few, a.c.hkv, a.q.num_seqs);
+    const dim3 grid((a.max_splits + a.spans_each - 1) / a.spans_each * few, a.c.hkv, a.q.num_seqs);
     if (a.window > 0) kv4_attn_kernel<D, NS, CAP, true><<<grid, dim3(THREADS), 0, s>>>(a);
     else kv4_attn_kernel<D, NS, CAP, false><<<grid, dim3(THREADS), 0, s>>>(a);
     e = hipGetLastError();
@@ -916,7 +994,12 @@ hipError_t launch(const Kv4Attn &a, hipStream_t s) {
     kv4_join_kernel<D, NS><<<dim3((split_rows + WAVES - 1) / WAVES, a.c.hkv, a.q.num_seqs), dim3(THREADS), 0, s>>>(a);
     e = hipGetLastError();
   }
-  if (e == hipSuccess && a.w_out && a.q.max_ctx > 0) {
+  if (e == hipSuccess && a.w_out && a.q.max_ctx > 0 && a.scores) {
+    kv4_score_weights_kernel<<<dim3((a.q.max_ctx + 4 * THREADS - 1) / (4 * THREADS), a.c.hkv, a.q.num_seqs),
+                               dim3(THREADS), 0, s>>>(a);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && a.w_out && a.q.max_ctx > 0 && (!a.scores || a.max_rows > SCORE_ROWS)) {
     kv4_weights_kernel<D, NS, CAP>
         <<<dim3((a.q.max_ctx + WAVES * STEP - 1) / (WAVES * STEP), a.c.hkv, a.q.num_seqs), dim3(THREADS), 0, s>>>(a);
     e = hipGetLastError();
@@ -941,6 +1024,8 @@ Kv4Plan dx_kv4_attn_plan(int max_seq_len, int max_ctx, int group, int window) {
   p.max_splits = most < 1 ? 1 : most > MAX_SPANS ? MAX_SPANS : (int)most;  // a shorter sequence may have more than a longer
   const long rows = (long)p.max_splits * p.max_rows;
   p.part_rows = p.max_splits == 1 ? 0 : (int)(rows < SPLIT_ROWS ? rows : SPLIT_ROWS);
+  p.score_rows = p.max_rows < SCORE_ROWS ? p.max_rows : SCORE_ROWS;
+  p.score_slots = (max_ctx + 63) & ~63;  // whole steps
   return p;
 }
 
