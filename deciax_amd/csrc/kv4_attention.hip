@@ -49,14 +49,21 @@ __host__ __device__ inline Spans spans(int ctx, int n, int rows, int window) {
   int lo = window > 0 && ctx - n - window + 1 > 0 ? ctx - n - window + 1 : 0;
   lo &= ~63;
   const int len = ctx - lo, most = most_spans(rows);
-  int keys = SPAN;
-  while ((long)keys * most < len) keys *= 2;
+  const int wanted = len / SPAN < most ? (len + SPAN - 1) / SPAN : most;
+  // whole turns of kv4_attn_kernel's waves
+  const int keys = wanted > 1 ? ((len + wanted - 1) / wanted + 127) & ~127 : SPAN;
   const int count = (len + keys - 1) / keys;
   return {lo, keys, count < 1 ? 1 : count};
 }
 
-// Rows of a KV head up to which waves share rows and split keys.
-constexpr int FEW_ROWS = 48;
+// Rows of a KV head up to which waves share rows and split keys (kv4_attn_kernel), by the row tiles a wave has beyond. A tile
+// of two wastes more when rows are few. 24 sequences of 24 rows over 3000 keys: D = 256, one tile, 92 us here and 87 there;
+// D = 128, two, 87 and 146. 8 of 40 rows over 4000: 66 and 54; 63 and 90.
+template <int NT>
+constexpr int few_rows() { return NT == 1 ? 32 : 48; }
+
+// Workgroups of kv4_attn_tile_kernel at most: 4 rounds of two a CU.
+constexpr int TILE_GROUPS = 2048;
 // Rows of a KV head up to which their scores are kept for the accumulated weights, instead of computed again.
 constexpr int SCORE_ROWS = 16;
 
@@ -178,26 +185,24 @@ DX_DEVICE int product_dim(int i, int grp) {
   return D == 64 ? grp * 16 + i * 8 : ((i >> 2) * 4 + grp) * 32 + (i & 3) * 8;
 }
 
-// softcap log2(e) tanh(x) of four values. The continued fraction of tanh, cut after x^13, is x N(x^2) / M(x^2) with the
-// polynomials below, off by 1.2e-8 of the value at |x| <= 2 (scores up to twice the cap) and by fp32's rounding below
-// that: relative precision where scores are small, which 1 - 2 / (1 + e^2x) has not. That form serves beyond, in a
+// cap2 tanh(x) of four values. The continued fraction of tanh, cut after x^9, is x (y^2 + 105 y + 945) / (15 (y^2 + 28 y +
+// 63)) with y = x^2, off by 2.4e-8 of the value at |x| <= 0.9 (scores up to 0.9 of the cap) and by fp32's rounding
+// below that: relative precision where scores are small, which 1 - 2 / (1 + e^2x) has not. That form serves beyond, in a
 // branch that real scores do not take.
 DX_DEVICE void capped(float (&x)[4], float cap2) {
   float t[4];
-  bool far = false;
+  const float far = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const float y = x[r] * x[r];
-    const float n = __builtin_fmaf(__builtin_fmaf(y + 378.f, y, 17325.f), y, 135135.f);
-    const float m = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(28.f, y, 3150.f), y, 62370.f), y, 135135.f);
-    t[r] = x[r] * n * fast_rcp(m) * cap2;
-    far = far || !(y <= 4.f);
+    const float n = __builtin_fmaf(y + 105.f, y, 945.f), m = __builtin_fmaf(y + 28.f, y, 63.f);
+    t[r] = x[r] * (cap2 * (1.f / 15.f)) * n * fast_rcp(m);
   }
-  if (__any(far)) {
+  if (__any(!(far <= 0.9f))) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float e = 1.f - 2.f * fast_rcp(1.f + fast_exp2(2.f * LOG2E * fabsf(x[r])));
-      t[r] = x[r] * x[r] <= 4.f ? t[r] : cap2 * copysignf(e, x[r]);
+      t[r] = fabsf(x[r]) <= 0.9f ? t[r] : cap2 * copysignf(e, x[r]);
     }
   }
 #pragma unroll
@@ -315,15 +320,18 @@ DX_DEVICE float max_of_groups(float x) {
   return x;
 }
 
-// The softmax of eight more scores a lane (32 keys a row): raises the running maximum `m`, scales what was summed, and
-// gives P as the matrix operand. The lanes of a row keep partial sums `l`, joined at the end.
+// The softmax of eight more scores a lane (32 keys a row): raises the running maximum `m` once it is SLACK behind in some
+// row, scales what was summed, and gives P as the matrix operand: 2^SLACK at most, as precise as below 1. The lanes of a
+// row keep partial sums `l`, joined at the end. (Raised at every new maximum, 16 rows did so in every second step of 90.)
+constexpr float SLACK = 8.f;
+
 template <int ND, int NS>
 DX_DEVICE void softmax_step(const float (&t2)[2][4], float &m, float &l, floatx4 (&o)[ND], bf16x8 (&pb)[NS]) {
   float top = t2[0][0];
 #pragma unroll
   for (int r = 1; r < 8; ++r) top = fmaxf(top, t2[r >> 2][r & 3]);
   top = max_of_groups(top);
-  if (__any(top > m)) {
+  if (__any(top > m + SLACK)) {
     const float next = fmaxf(m, top);
     const float f = next == -INFINITY ? 1.f : fast_exp2(m - next);
     m = next;
@@ -421,8 +429,8 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
   u32x4 kr[KL], vr[D / VW][VJ];
   uint32_t ks[2][Keys<D>::N], vs[D / VW][VJ];
   int4 pos[2] = {};
-  // A step without a page, or past the last span's end, reads the pool's first rows instead: nothing of them is seen. No branch
-  // goes round the loads, behind which the compiler could only wait for all of them.
+  // A step without a page, or past the last span's end, reads the pool's first rows instead: nothing of them is seen. No
+  // branch goes round the loads, behind which the compiler could only wait for all of them.
   auto fetch_keys = [&](int kb) {
     const long row0 = kb < k1 ? pages.row(a.c, g, kb, lane) : -1, at = max(row0, 0L);
     const uint8_t *codes = a.c.k + at * (D / 2), *scales = a.c.ks + at * LPK;
@@ -519,9 +527,9 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
       bf16x8 pb[NS];
       softmax_step<D / 16, NS>(t2, m, l, o, pb);
 
-      // V to bf16, VW columns at a time. Slots behind the sequence hold anything: zeros here. A block of NaN may stand behind
-      // a row's own token too, where 0 NaN would reach the row: such blocks are zero here and added below to the rows that
-      // see them.
+      // V to bf16, VW columns at a time. Slots behind the sequence hold anything: zeros here. A block of NaN may stand
+      // behind a row's own token too, where 0 NaN would reach the row: such blocks are zero here and added below to the
+      // rows that see them.
       uint64_t nan_blocks[D / VW][VJ];
       bool any_nan = false;
   #pragma unroll
@@ -617,204 +625,278 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
   }
 }
 
-// Many rows: TW waves of 16 NT rows each walk the same keys, decoded once a workgroup to bf16 in LDS, two tiles of TK
-// keys in turn: a tile's codes are on their way while the one before is used, and go to the other half of LDS after it.
+// Many rows: TW waves of 16 NT rows each walk the same keys, decoded once a workgroup to bf16 in LDS, TK keys at a time: a
+// tile's codes are on their way while the one before is used, and go over it afterwards. Two workgroups a CU, in step with
+// themselves alone, hide each other's waits; twice the rows a workgroup (half the decoding) or two tiles in turn (no wait
+// between use and decoding) were no faster: 6 questions of up to 611 tokens over up to 8803, D = 256, 358 us either way.
 template <int D>
 constexpr int tile_keys() { return D == 256 ? 32 : 64; }
 
 template <int D, int NS, bool CAP, int NT, int TW>
-__global__ void __launch_bounds__(64 * TW, D == 256 && NS > 1 ? 1 : 2) kv4_attn_tile_kernel(Kv4Attn a) {
+__global__ void __launch_bounds__(64 * TW, D == 256 ? (NS > 1 ? 1 : 2) : 2) kv4_attn_tile_kernel(Kv4Attn a) {
   constexpr int TK = tile_keys<D>(), LPK = D / 32, T = 64 * TW;
   constexpr int CHUNKS = TK * LPK;        // 16-byte chunks (blocks) of K, and of V, in a tile
   constexpr int LOADS = 2 * CHUNKS / T;   // of a thread
+  constexpr int KW = 64 / LPK;            // keys of a wave's load
   static_assert(2 * CHUNKS % T == 0 && CHUNKS % 64 == 0, "whole waves load K or V");
-  __shared__ __attribute__((aligned(1024))) uint16_t kt[2][TK * D], vt[2][TK * D];
-  __shared__ uint8_t nan_block[2][CHUNKS];
-  __shared__ uint8_t nan_wave[2][TW];
-  const int g = blockIdx.y, b = blockIdx.z;
-  const int tiles = gridDim.x / a.max_splits, row_tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
-  const Sequence s = sequence(a.q, b, a.c.shift);
-  const int group = a.hq / a.c.hkv, rows = s.n * group, r0 = row_tile * (16 * NT * TW);
-  if (r0 >= rows || rows <= a.few_rows) return;
-  const Spans sp = spans(s.ctx, s.n, rows, a.slots);
-  if (split >= sp.count) return;
-  const int32_t *table = a.q.table + (long)b * a.q.table_width;
+  __shared__ __attribute__((aligned(1024))) uint16_t kt[TK * D], vt[TK * D];
+  __shared__ uint8_t nan_block[CHUNKS];
+  __shared__ uint8_t nan_wave[TW];
+  constexpr int ROWS = 16 * NT * TW;
+  const int group = a.hq / a.c.hkv;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  // the span's keys that some row of this workgroup sees
-  const int last_own = s.ctx - s.n + (min(r0 + 16 * NT * TW, rows) - 1) / group;
-  const int first_own = s.ctx - s.n + r0 / group;
-  int k0 = sp.lo + split * sp.keys;
-  const int k1 = min(min(s.ctx, k0 + sp.keys), last_own + 1);
-  if (a.window > 0) k0 = max(k0, (first_own - a.slots + 1) & ~63);
-  Pages pages{table, a.q.table_width, 0, -1};
-  pages.load(a.c, g, max(k0, 0) >> a.c.shift, lane);
-
-  const int w0 = r0 + wave * 16 * NT;  // this wave's first row
-  Row row[NT];
-  bf16x8 q[NT][D / 32][NS];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    row[n] = query_row(a, s, table, g, w0 + n * 16 + col, rows, group);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) load_query<NS>(a.query, row[n].at + i * 32 + grp * 8, q[n][i]);
-  }
-  const int open = s.ctx - s.n + w0 / group + 1;                               // as above, for the wave's rows
-  const int shut = s.ctx - s.n + (min(w0 + 16 * NT, rows) - 1) / group + 1;  // keys from here on no row sees
-  const bool idle = w0 >= rows;
-
-  floatx4 o[NT][D / 16];
-  float m[NT], l[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  u32x4 raw[LOADS];
-  uint32_t byte[LOADS];
-  // Load c of a tile: block c % LPK of key c / LPK. A tile lies in one page.
-  auto fetch = [&](int kb) {
-    const long row0 = kb < k1 ? pages.row(a.c, g, kb, lane) : -1, from = max(row0, 0L);
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int c = i * T + tid;
-      const uint32_t chunk = c % CHUNKS;
-      const bool keys = __builtin_amdgcn_readfirstlane(c) < CHUNKS;
-      raw[i] = *reinterpret_cast<const u32x4 *>((keys ? a.c.k : a.c.v) + from * (D / 2) + chunk * 16);
-      byte[i] = ((keys ? a.c.ks : a.c.vs) + from * LPK)[chunk];
-    }
-    return row0;
-  };
-  auto decode = [&](int half, int kb) {
-    bool bad_here = false;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int c = i * T + tid, chunk = c % CHUNKS, key = chunk / LPK, blk = chunk % LPK;
-      if (c < CHUNKS) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<u32x4 *>(kt[half] + k_chunk<D>(key, blk * 4 + x)) = decode8(raw[i][x], scale_of(byte[i]));
-      } else {
-        const bool inside = kb + key < k1, bad = inside && byte[i] == 255;
-        if (!inside || bad) {
-          raw[i] = u32x4{0, 0, 0, 0};
-          byte[i] = 127;
-        }
-        nan_block[half][key * LPK + blk] = bad;
-        bad_here = bad_here || bad;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<u32x4 *>(vt[half] + v_chunk<D>(key, blk * 4 + x)) = decode8(raw[i][x], scale_of(byte[i]));
+  // Which row tile, span and head of which sequence: work items of all sequences, counted from their lengths.
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    int b = 0, before = 0;  // items of the sequences before
+    for (int b0 = 0;; b0 += 64) {
+      if (b0 >= a.q.num_seqs) return;
+      int mine = 0;
+      if (b0 + lane < a.q.num_seqs) {
+        const Sequence s = sequence(a.q, b0 + lane, a.c.shift);
+        const int rows = s.n * group;
+        if (rows > a.few_rows) mine = (rows + ROWS - 1) / ROWS * spans(s.ctx, s.n, rows, a.slots).count * a.c.hkv;
       }
+      int upto = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off *= 2) {
+        const int x = __shfl_up(upto, off, 64);
+        upto += lane >= off ? x : 0;
+      }
+      const uint64_t behind = __ballot(item - before < upto);
+      if (behind) {
+        const int at = __ffsll((unsigned long long)behind) - 1;
+        b = b0 + at;
+        before += __shfl(upto - mine, at, 64);
+        break;
+      }
+      before += __shfl(upto, 63, 64);
     }
-    const bool any = __any(bad_here);
-    if (lane == 0) nan_wave[half][wave] = any;
-  };
+    b = __builtin_amdgcn_readfirstlane(b);
+    const Sequence s = sequence(a.q, b, a.c.shift);
+    const int rows = s.n * group, tiles = (rows + ROWS - 1) / ROWS;
+    const Spans sp = spans(s.ctx, s.n, rows, a.slots);
+    const int place = __builtin_amdgcn_readfirstlane(item - before);
+    const int r0 = place % tiles * ROWS, split = place / tiles % sp.count, g = place / tiles / sp.count;
+    const int32_t *table = a.q.table + (long)b * a.q.table_width;
+    // the span's keys that some row of this workgroup sees
+    const int last_own = s.ctx - s.n + (min(r0 + ROWS, rows) - 1) / group;
+    const int first_own = s.ctx - s.n + r0 / group;
+    int k0 = sp.lo + split * sp.keys;
+    const int k1 = min(min(s.ctx, k0 + sp.keys), last_own + 1);
+    if (a.window > 0) k0 = max(k0, (first_own - a.slots + 1) & ~63);
+    Pages pages{table, a.q.table_width, 0, -1};
+    pages.load(a.c, g, max(k0, 0) >> a.c.shift, lane);
 
-  // 32 keys of the tile in `half`, from row `at` of it, for this wave's rows
-  auto use = [&](int half, int at, int kb, long row0) {
-    if (idle || row0 < 0 || kb >= shut || kb >= k1) return;
-    const bool masked = a.window > 0 || kb + STEP > open;
+    const int w0 = r0 + wave * 16 * NT;  // this wave's first row
+    Row row[NT];
+    bf16x8 q[NT][D / 32][NS];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      row[n] = query_row(a, s, table, g, w0 + n * 16 + col, rows, group);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) load_query<NS>(a.query, row[n].at + i * 32 + grp * 8, q[n][i]);
+    }
+    const int open = s.ctx - s.n + w0 / group + 1;                               // as above, for the wave's rows
+    const int shut = s.ctx - s.n + (min(w0 + 16 * NT, rows) - 1) / group + 1;  // keys from here on no row sees
+    const bool idle = w0 >= rows;
+
+    floatx4 o[NT][D / 16];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    u32x4 raw[LOADS];
+    uint32_t byte[LOADS];
+    // A wave's load has KW keys, a lane block lane / KW of key lane % KW: neighbours write the same columns of different
+    // rows of LDS, which the swizzle spreads over the banks (neighbouring blocks of one row: 4.9 conflict cycles where 0.8
+    // are left, and 9% of the kernel's time). A tile lies in one page.
+    const uint32_t in_wave = lane % KW * LPK + lane / KW;
+    auto fetch = [&](int kb) {
+      const long row0 = kb < k1 ? pages.row(a.c, g, kb, lane) : -1, from = max(row0, 0L);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int c = i * T + tid;
+        const uint32_t chunk = (c & ~63) % CHUNKS + in_wave;
+        const bool keys = __builtin_amdgcn_readfirstlane(c) < CHUNKS;
+        raw[i] = *reinterpret_cast<const u32x4 *>((keys ? a.c.k : a.c.v) + from * (D / 2) + chunk * 16);
+        byte[i] = ((keys ? a.c.ks : a.c.vs) + from * LPK)[chunk];
+      }
+      return row0;
+    };
+    auto decode = [&](int kb) {
+      bool bad_here = false;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int c = i * T + tid, chunk = (c & ~63) % CHUNKS + in_wave, key = chunk / LPK, blk = chunk % LPK;
+        if (c < CHUNKS) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<u32x4 *>(kt + k_chunk<D>(key, blk * 4 + x)) = decode8(raw[i][x], scale_of(byte[i]));
+        } else {
+          const bool inside = kb + key < k1, bad = inside && byte[i] == 255;
+          if (!inside || bad) {
+            raw[i] = u32x4{0, 0, 0, 0};
+            byte[i] = 127;
+          }
+          nan_block[key * LPK + blk] = bad;
+          bad_here = bad_here || bad;
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<u32x4 *>(vt + v_chunk<D>(key, blk * 4 + x)) = decode8(raw[i][x], scale_of(byte[i]));
+        }
+      }
+      const bool any = __any(bad_here);
+      if (lane == 0) nan_wave[wave] = any;
+    };
+
+    // 32 keys of the tile in `half`, from row `at` of it, for this wave's rows: their scores, then what they do to the rows
     float t2[NT][2][4];
     uint32_t seen[NT];
+    auto scores = [&](int at, int kb, long row0) {
+      if (idle || row0 < 0 || kb >= shut || kb >= k1) return;
+      const bool masked = a.window > 0 || kb + STEP > open;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) seen[n] = 0xff;
+      for (int n = 0; n < NT; ++n) seen[n] = 0xff;
+      // K's operands four at a time, the next four on their way while these are used: left to itself the compiler reads
+      // each one right before its product, and V's below likewise (6 questions of up to 611 tokens: 358 us, not 304)
+      constexpr int KG = D / 64;
+      bf16x8 kf[2][4];
+      auto load_k = [&](int x, bf16x8 (&f)[4]) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      int4 pos{0, 0, 0, 0};
-      if (a.window > 0) pos = *reinterpret_cast<const int4 *>(a.c.pos + row0 + t * 16 + grp * 4);
-      floatx4 sc[NT];
+        for (int y = 0; y < 4; ++y) {
+          const int i = 2 * x + y / 2, r = (y & 1) * 16 + col;
+          // column 16-byte chunk 4 i + grp; the swizzle is below 16, so chunks 16 on are at a constant distance
+          const uint16_t *p = kt + at * D + k_chunk<D>(r, (i & 3) * 4 + grp) + (i & ~3) * 32;
+          f[y] = as_bf16x8(*reinterpret_cast<const u32x4 *>(p));
+        }
+      };
+      floatx4 sc[2][NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) sc[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const bf16x8 k = as_bf16x8(*reinterpret_cast<const u32x4 *>(kt[half] + k_chunk<D>(at + t * 16 + col, i * 4 + grp)));
+        for (int n = 0; n < NT; ++n) sc[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+      load_k(0, kf[0]);
+#pragma unroll
+      for (int x = 0; x < KG; ++x) {
+        if (x + 1 < KG) load_k(x + 1, kf[(x + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int z = 0; z < NS; ++z) sc[y & 1][n] = mfma16(kf[x & 1][y], q[n][2 * x + y / 2][z], sc[y & 1][n]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      float part[2][NT][4];
+      products<NT, CAP>(sc[0], a.scale, a.softcap, part[0]);
+      products<NT, CAP>(sc[1], a.scale, a.softcap, part[1]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        int4 pos{0, 0, 0, 0};
+        if (a.window > 0) pos = *reinterpret_cast<const int4 *>(a.c.pos + row0 + t * 16 + grp * 4);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (CAP) capped(part[t][n], a.softcap * LOG2E);
+          if (masked) {
+            const uint32_t see = a.window > 0 ? mask4<true>(a, row[n], kb + t * 16 + grp * 4, pos, part[t][n])
+                                              : mask4<false>(a, row[n], kb + t * 16 + grp * 4, pos, part[t][n]);
+            seen[n] = t == 0 ? see : seen[n] | see << 4;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) t2[n][t][r] = part[t][n][r];
+        }
+      }
+    };
+    auto values = [&](int at, int kb, long row0) {
+      if (idle || row0 < 0 || kb >= shut || kb >= k1) return;
+      constexpr int VG = D / 64;
+      bf16x8 vf[2][4];
+      auto load_v = [&](int x, bf16x8 (&f)[4]) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int i = 4 * x + y;
+          const int chunk = 2 * (i & 7) + ((col >> 1) & 1);
+          const uint16_t *p0 = vt + at * D + v_chunk<D>(grp * 4 + (col >> 2), chunk) + (col & 1) * 4 + (i & ~7) * 16;
+          const s16x4 v0 = read_transposed(p0), v1 = read_transposed(p0 + 16 * D);
+          f[y] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+      };
+      load_v(0, vf[0]);
+      bf16x8 pb[NT][NS];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) softmax_step<D / 16, NS>(t2[n], m[n], l[n], o[n], pb[n]);
+#pragma unroll
+      for (int x = 0; x < VG; ++x) {
+        if (x + 1 < VG) load_v(x + 1, vf[(x + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int z = 0; z < NS; ++z) o[n][4 * x + y] = mfma16(vf[x & 1][y], pb[n][z], o[n][4 * x + y]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      uint32_t flags = 0;
+#pragma unroll
+      for (int w = 0; w < TW; ++w) flags |= nan_wave[w];
+      if (flags) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int x = 0; x < NS; ++x) sc[n] = mfma16(k, q[n][i][x], sc[n]);
-      }
-      float part[NT][4];
-      products<NT, CAP>(sc, a.scale, a.softcap, part);
+          for (int blk = 0; blk < LPK; ++blk) {
+            int hit = 0;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if constexpr (CAP) capped(part[n], a.softcap * LOG2E);
-        if (masked) {
-          const uint32_t see = a.window > 0 ? mask4<true>(a, row[n], kb + t * 16 + grp * 4, pos, part[n])
-                                            : mask4<false>(a, row[n], kb + t * 16 + grp * 4, pos, part[n]);
-          seen[n] = t == 0 ? see : seen[n] | see << 4;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) t2[n][t][r] = part[n][r];
-      }
-    }
-    bf16x8 pb[NT][NS];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) softmax_step<D / 16, NS>(t2[n], m[n], l[n], o[n], pb[n]);
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const uint16_t *p0 = vt[half] + v_chunk<D>(at + grp * 4 + (col >> 2), 2 * i + ((col >> 1) & 1)) + (col & 1) * 4;
-      const uint16_t *p1 = p0 + 16 * D;
-      const s16x4 v0 = read_transposed(p0), v1 = read_transposed(p1);
-      const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < NS; ++x) o[n][i] = mfma16(v, pb[n][x], o[n][i]);
-    }
-    uint32_t flags = 0;
-#pragma unroll
-    for (int w = 0; w < TW; ++w) flags |= nan_wave[half][w];
-    if (flags) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int blk = 0; blk < LPK; ++blk) {
-          int hit = 0;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const int key = at + (r >> 2) * 16 + grp * 4 + (r & 3);
-            hit |= (int)nan_block[half][key * LPK + blk] & (int)((seen[n] >> r) & 1);
+            for (int r = 0; r < 8; ++r) {
+              const int key = at + (r >> 2) * 16 + grp * 4 + (r & 3);
+              hit |= (int)nan_block[key * LPK + blk] & (int)((seen[n] >> r) & 1);
+            }
+            hit |= __shfl_xor(hit, 16, 64);
+            hit |= __shfl_xor(hit, 32, 64);
+            if (hit) {
+              o[n][2 * blk] += NAN;
+              o[n][2 * blk + 1] += NAN;
+            }
           }
-          hit |= __shfl_xor(hit, 16, 64);
-          hit |= __shfl_xor(hit, 32, 64);
-          if (hit) {
-            o[n][2 * blk] += NAN;
-            o[n][2 * blk + 1] += NAN;
-          }
-        }
-    }
-  };
+      }
+    };
 
 #pragma unroll
-  for (int n = 0; n < NT; ++n) settle(q[n]);
-  if (k0 < k1) {
-    long here = fetch(k0);
-    decode(0, k0);
-    __syncthreads();
-    int half = 0;
-    for (int kb = k0; kb < k1; kb += TK) {
-      const long next = fetch(kb + TK);
+    for (int n = 0; n < NT; ++n) settle(q[n]);
+    if (k0 < k1) {
+      long here = fetch(k0);
+      decode(k0);
+      lds_barrier();
+      for (int kb = k0; kb < k1; kb += TK) {
+        const long next = fetch(kb + TK);
 #pragma unroll
-      for (int at = 0; at < TK; at += STEP) use(half, at, kb + at, here < 0 ? -1 : here + at);
-      decode(half ^ 1, kb + TK);
-      here = next;
-      half ^= 1;
-      __syncthreads();
+        for (int at = 0; at < TK; at += STEP) {
+          scores(at, kb + at, here < 0 ? -1 : here + at);
+          values(at, kb + at, here < 0 ? -1 : here + at);
+        }
+        lds_barrier();
+        decode(kb + TK);
+        here = next;
+        lds_barrier();
+      }
     }
-  }
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    l[n] += __shfl_xor(l[n], 16, 64);
-    l[n] += __shfl_xor(l[n], 32, 64);
-    const int r = w0 + n * 16 + col;
-    if (r >= rows) continue;
+    for (int n = 0; n < NT; ++n) {
+      l[n] += __shfl_xor(l[n], 16, 64);
+      l[n] += __shfl_xor(l[n], 32, 64);
+      const int r = w0 + n * 16 + col;
+      if (r >= rows) continue;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-      store_row<D, NS>(a, s, sp, (long)b * a.c.hkv + g, g, group, rows, split, r, i * 16 + grp * 4, o[n][i], m[n], l[n]);
+      for (int i = 0; i < D / 16; ++i)
+        store_row<D, NS>(a, s, sp, (long)b * a.c.hkv + g, g, group, rows, split, r, i * 16 + grp * 4, o[n][i], m[n], l[n]);
+    }
   }
 }
 
@@ -902,50 +984,144 @@ __global__ void __launch_bounds__(THREADS) kv4_score_weights_kernel(Kv4Attn a) {
   }
 }
 
-// The same for sequences of more rows, from the keys. A wave owns 32 keys and walks all rows, so every sum has one owner and
-// one order.
+// The same for sequences of more rows, from the keys. A wave owns 32 keys, decoded once, and walks all rows, so every sum
+// has one owner and one order. Its workgroup brings the rows through LDS, 32 at a time and the next 32 on their way: read
+// by each wave as its products want them (16 rows of one chunk) they cost the vector cache a look at every lane: 261 us
+// where this takes 176, for 6 questions of up to 611 tokens over up to 8803.
 template <int D, int NS, bool CAP>
-__global__ void __launch_bounds__(THREADS) kv4_weights_kernel(Kv4Attn a) {
+__global__ void __launch_bounds__(THREADS, NS == 1 ? 3 : 1) kv4_weights_kernel(Kv4Attn a) {
+  constexpr int ROWS = 32, BYTES = NS == 1 ? 2 : 4, CHUNKS = D * BYTES / 16;  // 16-byte chunks of a row
+  constexpr int LOADS = ROWS * CHUNKS / THREADS;                               // of a thread
+  __shared__ u32x4 qs[2][ROWS * CHUNKS];  // chunk c of row r at c ^ (r % 8)
+  __shared__ float lses[2][ROWS];
   const int g = blockIdx.y, b = blockIdx.z;
   const Sequence s = sequence(a.q, b, a.c.shift);
   const int32_t *table = a.q.table + (long)b * a.q.table_width;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int group = a.hq / a.c.hkv, rows = s.n * group;
-  const int kb = (blockIdx.x * WAVES + wave) * STEP;
-  if (kb >= s.ctx || (a.scores && rows <= SCORE_ROWS)) return;
+  const int kb0 = blockIdx.x * (WAVES * STEP), kb = kb0 + wave * STEP;
+  if (kb0 >= s.ctx || (a.scores && rows <= SCORE_ROWS)) return;
   const long unit = (long)b * a.c.hkv + g;
-  const long row0 = row_of(a.c, table, g, kb);
+  const long row0 = kb < s.ctx ? row_of(a.c, table, g, kb) : -1;
   const int lo = a.window > 0 ? s.ctx - s.n - a.slots + 1 : 0;
+  const bool live = row0 >= 0 && kb + STEP > lo;
   float sum[8] = {};
-  if (row0 >= 0 && kb + STEP > lo) {
-    Keys<D> w;
-    load_keys<D>(w, a.c, row0, lane);
+  if (a.q.rows > 0 && kb0 + WAVES * STEP > lo) {
+    bf16x8 k[2][D / 32];
     int4 pos[2] = {};
-    if (a.window > 0) {
+    {
+      const long at = max(row0, 0L);
+      Keys<D> w;
+      load_keys<D>(w, a.c, at, lane);
+      if (a.window > 0) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) pos[t] = *reinterpret_cast<const int4 *>(a.c.pos + row0 + t * 16 + grp * 4);
+        for (int t = 0; t < 2; ++t) pos[t] = *reinterpret_cast<const int4 *>(a.c.pos + at + t * 16 + grp * 4);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const int j = D == 64 ? 0 : i >> 2;
+          k[t][i] = as_bf16x8(decode8(w.k[t][j][i & 3], w.scale[t][j]));
+        }
     }
-    // the first row that can see a key here
-    const int first = max(0, kb - (s.ctx - s.n)) * group;
-    for (int r0 = first & ~15; a.q.rows > 0 && r0 < rows; r0 += 16) {
-      const Row row = query_row(a, s, table, g, r0 + col, rows, group);
-      bf16x8 q[D / 32][NS];
+    const bool packed = s.start >= 0 && (long)s.start + s.n <= a.q.rows;
+    u32x4 raw[LOADS];
+    float raw_lse = 0.f;
+    auto fetch = [&](int r0) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) load_query<NS>(a.query, row.at + product_dim<D>(i, grp), q[i]);
-      const float lse = row.real ? a.lse[unit * a.max_rows + r0 + col] : 0.f;
+      for (int i = 0; i < LOADS; ++i) {
+        const int x = i * THREADS + tid, r = r0 + x / CHUNKS, token = r / group;
+        const bool real = r < rows && s.start + token >= 0 && s.start + token < a.q.rows;
+        const long at = real ? (s.start + token) * a.q_stride + (long)(g * group + r - token * group) * D : 0;
+        raw[i] = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.query) + at * BYTES + x % CHUNKS * 16);
+      }
+      raw_lse = a.lse[unit * a.max_rows + min(r0 + (tid & (ROWS - 1)), rows - 1)];
+    };
+    auto keep = [&](int half) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int x = i * THREADS + tid, r = x / CHUNKS, c = x % CHUNKS;
+        qs[half][r * CHUNKS + (c ^ (r & 7))] = raw[i];
+      }
+      if (tid < ROWS) lses[half][tid] = raw_lse;
+    };
+    auto add = [&](int half, int sub, int r0) {
+      const int r = sub + col;
+      auto load_q = [&](int i, bf16x8 (&q)[NS]) {
+        const u32x4 *p = qs[half] + r * CHUNKS;
+        const int c = product_dim<D>(i, grp) * BYTES / 16;
+        if constexpr (NS == 1) {
+          q[0] = as_bf16x8(p[c ^ (r & 7)]);
+        } else {
+          const floatx4 x = __builtin_bit_cast(floatx4, p[c ^ (r & 7)]);
+          const floatx4 y = __builtin_bit_cast(floatx4, p[(c + 1) ^ (r & 7)]);
+          const float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+          split8<NS>(z, q);
+        }
+      };
+      bf16x8 q[2][2][NS];  // two products' rows at a time, the next two on their way
+      floatx4 sc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+      load_q(0, q[0][0]);
+      load_q(1, q[0][1]);
+      const float lse = lses[half][r];
+#pragma unroll
+      for (int i = 0; i < D / 32; i += 2) {
+        if (i + 2 < D / 32) {
+          load_q(i + 2, q[(i / 2 + 1) & 1][0]);
+          load_q(i + 3, q[(i / 2 + 1) & 1][1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) sc[t] = mfma16(k[t][i + x], q[i / 2 & 1][x][n], sc[t]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       float t2[2][4];
-      key_scores<D, NS, CAP>(w, q, a.scale, a.softcap, t2);
+      products<2, CAP>(sc, a.scale, a.softcap, t2);
+      // whether some row of these does not see some key of these
+      const bool masked = a.window > 0 || !packed || r0 + 16 > rows || kb + STEP > s.ctx - s.n + r0 / group + 1;
+      Row row;
+      if (masked) row = query_row(a, s, table, g, r0 + col, rows, group);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int key = kb + t * 16 + grp * 4;
-        const uint32_t seen = a.window > 0 ? mask4<true>(a, row, key, pos[t], t2[t])
-                                           : mask4<false>(a, row, key, pos[t], t2[t]);
+        if constexpr (CAP) capped(t2[t], a.softcap * LOG2E);
+        if (masked) {
+          const int key = kb + t * 16 + grp * 4;
+          const uint32_t seen = a.window > 0 ? mask4<true>(a, row, key, pos[t], t2[t])
+                                             : mask4<false>(a, row, key, pos[t], t2[t]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum[t * 4 + r] += row.real && (seen >> r) & 1 ? fast_exp2(t2[t][r] - lse) : 0.f;
+          for (int r = 0; r < 4; ++r) sum[t * 4 + r] += row.real && (seen >> r) & 1 ? fast_exp2(t2[t][r] - lse) : 0.f;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[t * 4 + r] += fast_exp2(t2[t][r] - lse);
+        }
+      }
+    };
+    // the first row that can see a key of the workgroup's
+    const int first = min(max(0, kb0 - (s.ctx - s.n)), s.n) * group & ~(ROWS - 1);
+    if (first < rows) {
+      fetch(first);
+      keep(0);
+      lds_barrier();
+      int half = 0;
+      for (int r0 = first; r0 < rows; r0 += ROWS) {
+        fetch(r0 + ROWS);
+        if (live) {
+          add(half, 0, r0);
+          if (r0 + 16 < rows) add(half, 16, r0 + 16);
+        }
+        half ^= 1;
+        keep(half);
+        lds_barrier();
       }
     }
   }
+  if (kb >= s.ctx) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -962,20 +1138,20 @@ __global__ void __launch_bounds__(THREADS) kv4_weights_kernel(Kv4Attn a) {
   }
 }
 
-// Workgroups are listed by row tile, then by span: a sequence of many rows has few spans, and the workgroups that have
-// work then follow each other over the XCDs (listed by span first they were every 32nd one, all on one XCD: 6 questions of
-// up to 611 tokens 10.6 ms instead of 1.4).
+// kv4_attn_kernel's workgroups are listed by row tile, then by span: a sequence of many rows has few spans, and the
+// workgroups that have work then follow each other over the XCDs (listed by span first they were every 32nd one, all on one
+// XCD).
 // Sequences of few rows take kv4_attn_kernel, of more kv4_attn_tile_kernel; a batch of both launches both.
 template <int D, int NS, bool CAP>
 hipError_t launch(Kv4Attn a, hipStream_t s) {
-  constexpr int NT = NS == 1 && D < 256 ? 2 : 1, TW = NS == 1 && D == 256 ? 8 : 4;
+  constexpr int NT = NS == 1 && D < 256 ? 2 : 1, TW = 4;
+  a.few_rows = few_rows<NT>();
   const int few = a.q.rows > 0 ? (min(a.max_rows, a.few_rows) + 15) / 16 : 0;  // without rows: the weights alone
   const int tiles = a.q.rows > 0 && a.max_rows > a.few_rows ? (a.max_rows + 16 * NT * TW - 1) / (16 * NT * TW) : 0;
   a.few_tiles = few;
   // Two spans a workgroup where there are many workgroups: a workgroup's start (lengths, page, query and first keys, each
   // after the other) takes 3 us of some 13. 64 x 4000 137 -> 128 us, 32 x 14000 217 -> 206, 16 x 8000 64.3 -> 62.2;
-  // 4 x 16384 (1024 workgroups)
-  // 42.6 -> 44.3.
+  // 4 x 16384 (1024 workgroups) 42.6 -> 44.3.
   a.spans_each = (long)a.max_splits * few * a.c.hkv * a.q.num_seqs >= 2048 ? 2 : 1;
   hipError_t e = hipSuccess;
   if (few > 0) {
@@ -985,8 +1161,9 @@ hipError_t launch(Kv4Attn a, hipStream_t s) {
     e = hipGetLastError();
   }
   if (e == hipSuccess && tiles > 0) {
+    const long items = (long)a.max_splits * tiles * a.c.hkv * a.q.num_seqs;
     kv4_attn_tile_kernel<D, NS, CAP, NT, TW>
-        <<<dim3(a.max_splits * tiles, a.c.hkv, a.q.num_seqs), dim3(64 * TW), 0, s>>>(a);
+        <<<dim3((int)min(items, (long)TILE_GROUPS)), dim3(64 * TW), 0, s>>>(a);
     e = hipGetLastError();
   }
   if (e == hipSuccess && few > 0 && a.max_splits > 1) {
@@ -1029,9 +1206,7 @@ Kv4Plan dx_kv4_attn_plan(int max_seq_len, int max_ctx, int group, int window) {
   return p;
 }
 
-hipError_t dx_kv4_attn_launch(const Kv4Attn &args, bool f32, hipStream_t s) {
-  Kv4Attn a = args;
-  a.few_rows = FEW_ROWS;
+hipError_t dx_kv4_attn_launch(const Kv4Attn &a, bool f32, hipStream_t s) {
   if (a.c.d == 64) return by_type<64>(a, f32, s);
   if (a.c.d == 128) return by_type<128>(a, f32, s);
   return by_type<256>(a, f32, s);
