@@ -666,9 +666,14 @@ def readout(hidden: torch.Tensor, norm_w: torch.Tensor, table: torch.Tensor, opt
 class KV4Cache:
     """One layer's paged cache of keys and values in 4 bits (`dx_kv4_cache`, which states the format): `k`, `v` uint8
     [pages, kv heads, page size, head_dim / 2], their scales uint8 [.., head_dim / 32] and `positions` int32
-    [pages, kv heads, page size]. `kv4_cache` allocates one. The arrays are looked over once, here."""
+    [pages, kv heads, page size]. `kv4_cache` allocates one. The arrays are looked over once, here, and stay."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "positions", "head_dim", "heads", "page_size", "index", "_c", "ref")
+    __slots__ = ("_arrays", "head_dim", "heads", "page_size", "index", "_c", "ref")
+    k = property(lambda self: self._arrays[0])
+    v = property(lambda self: self._arrays[1])
+    k_scale = property(lambda self: self._arrays[2])
+    v_scale = property(lambda self: self._arrays[3])
+    positions = property(lambda self: self._arrays[4])
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                  positions: torch.Tensor) -> None:
@@ -685,7 +690,7 @@ class KV4Cache:
                 raise ValueError("KV4Cache: codes and scales must be contiguous uint8 on one device")
         if positions.dtype != torch.int32 or positions.get_device() != index or not positions.is_contiguous():
             raise ValueError("KV4Cache: positions must be contiguous int32 on the codes' device")
-        self.k, self.v, self.k_scale, self.v_scale, self.positions = k, v, k_scale, v_scale, positions
+        self._arrays = k, v, k_scale, v_scale, positions
         self.head_dim, self.heads, self.page_size, self.index = 2 * half, heads, page, index
         self._c = _lib.Kv4Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                 positions.data_ptr(), pages, heads, page, 2 * half)
@@ -791,9 +796,20 @@ def _weights(t: torch.Tensor, name: str, index: int, seqs: int, heads: int, slot
         raise ValueError(f"{name} must be fp32 [{seqs}, {heads}, >= {slots}] on the cache's device with neighbouring "
                          f"slots, got {t.dtype} {tuple(t.shape)} on {t.device}")
     seq, head, _ = t.stride()
-    if (heads > 1 and head < t.shape[2]) or (seqs > 1 and seq < heads * head and seq < t.shape[2]):
+    wide = t.shape[2]
+    head = max(head, wide) if heads == 1 else head  # one row has no next one
+    apart = seqs <= 1 or seq >= (heads - 1) * head + wide or (seq >= wide and head >= (seqs - 1) * seq + wide)
+    if head < wide or not apart:
         raise ValueError(f"{name}: rows must not overlap")
-    return seq, max(head, t.shape[2])
+    return seq, head
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from the first to the last element of one reaches into the other's."""
+    def end(t: torch.Tensor) -> int:
+        return t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def attention_kv4(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, seq_start: torch.Tensor,
@@ -824,7 +840,11 @@ def attention_kv4(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, se
     if weights is not None:
         weights_out = weights if weights_out is None else weights_out
         wi = _weights(weights, "weights", index, seqs, heads, max_ctx_len)
-        wo = _weights(weights_out, "weights_out", index, seqs, heads, max_ctx_len)
+        wo = wi
+        if weights_out is not weights:
+            wo = _weights(weights_out, "weights_out", index, seqs, heads, max_ctx_len)
+            if (weights_out.data_ptr(), wo) != (weights.data_ptr(), wi) and _meet(weights, weights_out):
+                raise ValueError("attention_kv4: weights_out must be weights itself or have memory of its own")
         w_in, w_out = weights.data_ptr(), weights_out.data_ptr()
     if seqs == 0:
         return out
@@ -855,7 +875,7 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor, page_table: torch.Tensor, 
         wo = (heads * keep, keep)
     else:
         wo = _weights(weights_out, "weights_out", index, seqs, heads, keep)
-        if weights_out.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
+        if _meet(weights, weights_out):
             raise ValueError("kv4_evict: weights_out must have memory of its own")
     out_len = torch.empty(seqs, dtype=torch.int32, device=dev)
     if seqs == 0:

@@ -334,6 +334,96 @@ def test_a_sequence_does_not_depend_on_its_batch(dtype: str) -> None:
             assert torch.equal(w_one[0], w_all[b, :, :m])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("new,ctx,hq,hkv,d", [([2, 1], [700, 90], 4, 2, 64), ([70, 3], [300, 100], 2, 1, 256)])
+def test_scores_beyond_the_soft_cap(new: list[int], ctx: list[int], hq: int, hkv: int, d: int, dtype: str) -> None:
+    """A cap that scores of 1.6 on average pass by far: both forms of the hyperbolic tangent, and the border of them."""
+    import torch
+
+    say(f"attention_kv4 beyond the soft-cap new={new} ctx={ctx} d={d} {dtype}")
+    c = Case(12, new, ctx, hq, hkv, d, 64, dtype)
+    c.fill(7)
+    c.append()
+    kw = dict(scale=1.6 / d ** 0.5, softcap=1.5, window=0)
+    w_in = np.zeros((2, hkv, max(ctx)), np.float32)
+    w = torch.zeros(w_in.shape, device="cuda")
+    out = c.attend(weights=w, **kw)
+    torch.cuda.synchronize()
+    c.check(out, w, w_in, **kw)
+
+
+def alone(c: Case, b: int, w, **kw):
+    """Output and weights of sequence b of a case in a call of its own."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    n, m = c.new[b], c.ctx[b]
+    rows = slice(c.starts[b], c.starts[b] + n)
+    w_one = torch.empty((1, c.hkv, m), device="cuda")
+    one = K.attention_kv4(c.q[rows], c.cache, c.d_table[b:b + 1].contiguous(), i32([0]), i32([n]), i32([m]), n, m,
+                          num_q_heads=c.hq, weights=w[b:b + 1], weights_out=w_one, **kw)
+    return one, w_one[0]
+
+
+# 2048 and more spans of few rows (two a workgroup); more sequences of many rows than a wave has lanes, among others of few
+# rows and none; more work items than workgroups
+LARGE = [([1] * 96, [1100 + 7 * i for i in range(96)], 8, 8, 64),
+         ([60 if i % 3 else i % 2 * 5 for i in range(70)], [64 + 9 * i for i in range(70)], 2, 2, 64),
+         ([65] * 34, [4000 + 100 * i for i in range(34)], 8, 8, 64)]
+
+
+@pytest.mark.parametrize("large", range(len(LARGE)))
+def test_large_batches_are_their_sequences(large: int) -> None:
+    import torch
+
+    new, ctx, hq, hkv, d = LARGE[large]
+    say(f"attention_kv4 of {len(new)} sequences, up to {max(new)} tokens over {max(ctx)} slots")
+    c = Case(20 + large, new, ctx, hq, hkv, d, 64, garbage=False)
+    codes = rng(large).integers(0, 256, c.raw["k"].shape).astype(np.uint8)
+    c.cache.k.copy_(torch.from_numpy(codes))
+    c.cache.v.copy_(torch.from_numpy(codes[::-1].copy()))
+    for t in (c.cache.k_scale, c.cache.v_scale):
+        t.fill_(126)
+    c.append()
+    kw = dict(scale=0.1, softcap=50.0, window=0)
+    w = torch.rand((len(new), hkv, max(ctx)), device="cuda")
+    w_all = torch.empty_like(w)
+    whole = c.attend(weights=w, weights_out=w_all, **kw)
+    torch.cuda.synchronize()
+    for b in range(len(new)):
+        if new[b] == 0:
+            assert torch.equal(w_all[b, :, :ctx[b]], w[b, :, :ctx[b]])
+            continue
+        one, w_one = alone(c, b, w, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(one, whole[c.starts[b]:c.starts[b] + new[b]]), f"sequence {b}"
+        assert torch.equal(w_one, w_all[b, :, :ctx[b]]), f"sequence {b}"
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_rows_outside_the_packed_ones_add_no_weight(n: int) -> None:
+    """The last token of a sequence lies behind the packed rows: the weights are those of the tokens before it. Both sums
+    of at most R weights of the same scores are off by R 2^-24 of the sum."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"attention_kv4 with a token outside the packed rows, {n} new")
+    c = Case(15, [2, n], [64, 300], 4, 2, 64)
+    c.fill(9)
+    c.append()
+    kw = dict(num_q_heads=4, scale=0.2)
+    w = torch.rand((2, 2, 300), device="cuda")
+    got, want = torch.empty_like(w), torch.empty((1, 2, 299), device="cuda")
+    K.attention_kv4(c.q[:-1], c.cache, c.d_table, c.d_starts, c.d_new, c.d_ctx, n, 300, weights=w, weights_out=got, **kw)
+    K.attention_kv4(c.q[2:-1], c.cache, c.d_table[1:].contiguous(), i32([0]), i32([n - 1]), i32([299]), n - 1, 299,
+                    weights=w[1:], weights_out=want, **kw)
+    torch.cuda.synchronize()
+    assert (got[1, :, 299] == 0).all()
+    assert ((got[1, :, :299] - want[0]).abs() <= 2 * 2 * n * U32 * want[0]).all()
+
+
 def test_window_goes_by_positions_after_eviction_left_gaps() -> None:
     """Positions with gaps: fewer slots than the window spans are seen."""
     import torch
@@ -399,6 +489,67 @@ def test_other_streams_and_graph_replays() -> None:
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(wg, w_want), f"replay {i} differs"
+
+
+def test_two_graphs_replayed_in_turn() -> None:
+    """Graphs of two batches, each with workspace of its own, replayed in turn on one stream and on two."""
+    import torch
+
+    say("kv4 two graphs")
+    kw = dict(scale=1 / 16, softcap=50.0)
+    cases = [Case(8, [1, 20], [1700, 65], 8, 2, 128), Case(9, [1], [2500], 8, 2, 128)]
+    graphs, outs, wants = [], [], []
+    for i, c in enumerate(cases):
+        c.fill(5 + i)
+        c.append()
+        wants.append(c.attend(**kw))
+        outs.append(torch.empty_like(wants[i]))
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            c.attend(out=outs[i], **kw)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(4):
+        for o in outs:
+            o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for s, g in zip(streams if i % 2 else streams[:1] * 2, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], wants[0]) and torch.equal(outs[1], wants[1]), f"replay {i} differs"
+
+
+def test_refused_tensors() -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("kv4 refusals of tensors")
+    c = Case(30, [1, 1], [70, 20], 4, 2, 64)
+    kw = dict(num_q_heads=4, scale=0.1)
+    w = torch.zeros((2, 2, 200), device="cuda")
+
+    def attend(q=c.q, table=c.d_table, new=c.d_new, max_ctx=70, **more):
+        K.attention_kv4(q, c.cache, table, c.d_starts, new, c.d_ctx, 1, max_ctx, **{**kw, **more})
+
+    for bad in (lambda: attend(q=c.q.half()), lambda: attend(q=c.q.cpu()), lambda: attend(q=c.q[:, :128]),
+                lambda: attend(table=c.d_table.long()), lambda: attend(table=c.d_table.cpu()),
+                lambda: attend(table=c.d_table.t()), lambda: attend(new=c.d_new[:1]),
+                lambda: attend(weights=w[..., :60]), lambda: attend(weights=w.double()), lambda: attend(weights=w[:1]),
+                lambda: attend(weights=w[..., ::2]), lambda: attend(weights=w.expand(2, 2, 200)[:, :1].expand(2, 2, 200)),
+                lambda: attend(weights=w[..., :100], weights_out=w[..., 50:150]), lambda: attend(weights_out=w),
+                lambda: attend(weights=w.as_strided((2, 2, 70), (105, 70, 1))),
+                lambda: attend(out=torch.empty_like(c.q, dtype=torch.float32)), lambda: attend(num_q_heads=3),
+                lambda: K.kv4_evict(c.cache, w, c.d_table, c.d_ctx, 70, c.d_table, keep=10, weights_out=w[..., 100:110]),
+                lambda: K.kv4_read(c.cache, c.d_table, c.d_starts, c.d_new, c.d_ctx, 1, rows=2, out_k=c.k.float()),
+                lambda: K.kv4_append(c.cache, c.k, c.v, c.positions.long(), c.d_table, c.d_starts, c.d_new, c.d_ctx, 1),
+                lambda: K.kv4_append(c.cache, c.k, c.v.float(), c.positions, c.d_table, c.d_starts, c.d_new, c.d_ctx, 1)):
+        with pytest.raises(ValueError):
+            bad()
+    both = torch.zeros((2, 2, 2, 70), device="cuda")
+    attend(weights=both[0], weights_out=both[1])  # one buffer's halves do not meet
+    torch.cuda.synchronize()
 
 
 def test_pages_beyond_32_bit_offsets() -> None:

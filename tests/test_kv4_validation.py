@@ -152,3 +152,25 @@ def test_tensors_in_host_memory_are_refused() -> None:
         K.attention_kv4(x, c, t, i, i, i, 3, 3, num_q_heads=2, scale=0.1)
     with pytest.raises(ValueError, match="device"):
         K.token_logprobs(x, torch.zeros(3, dtype=torch.int32))
+
+
+def test_a_cache_keeps_its_arrays() -> None:
+    """The library is given the arrays' addresses once: no other array can take the place of one."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    cache = K.kv4_cache(2, 1, 64, device="cpu")
+    for name in ("k", "v", "k_scale", "v_scale", "positions"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.zeros(1))
+    codes, scales = torch.zeros((2, 1, 64, 32), dtype=torch.uint8), torch.zeros((2, 1, 64, 2), dtype=torch.uint8)
+    at = torch.zeros((2, 1, 64), dtype=torch.int32)
+    for bad in ((codes[0], codes, scales, scales, at), (codes, codes[:1], scales, scales, at),
+                (codes, codes, scales, scales[..., :1], at), (codes, codes, scales, scales, at.long()),
+                (codes.int(), codes, scales, scales, at), (codes, codes, scales, scales, at[:, :, :32]),
+                (codes.transpose(0, 1).expand(2, 2, 64, 32)[:, :1], codes, scales, scales, at)):
+        with pytest.raises(ValueError):
+            K.KV4Cache(*bad)
+    with pytest.raises(ValueError, match="device"):
+        K.kv4_read(cache, torch.zeros((1, 1), dtype=torch.int32), *[torch.zeros(1, dtype=torch.int32)] * 3, 1, rows=1)
