@@ -275,7 +275,8 @@ struct Pages {
 struct Row {
   bool real;    // a row of the packed q
   int own;      // its own slot
-  int own_pos;  // and that slot's position, for a window
+  int first;     // with a window: the first slot in it
+  int first_pos;  // and the lowest position
   long at;      // its first element in q
 };
 
@@ -284,10 +285,11 @@ DX_DEVICE Row query_row(const Kv4Attn &a, const Sequence &s, const int32_t *tabl
   const int token = row / group;
   r.real = row < rows && s.start + token >= 0 && s.start + token < a.q.rows;
   r.own = s.ctx - s.n + token;
-  r.own_pos = 0;
+  r.first = r.first_pos = 0;
   if (a.window > 0 && r.real && r.own >= 0) {
     const long at = row_of(a.c, table, g, r.own);
-    r.own_pos = at >= 0 ? a.c.pos[at] : 0;
+    r.first = a.slots > 0 ? r.own - a.slots + 1 : 0;
+    r.first_pos = (int)max((long)(at >= 0 ? a.c.pos[at] : 0) - a.window + 1, -0x80000000L);
   }
   // a row that is none reads the first one: its column of the products goes nowhere
   r.at = r.real ? (s.start + token) * a.q_stride + (long)(g * group + row % group) * a.c.d : 0;
@@ -302,7 +304,7 @@ DX_DEVICE uint32_t mask4(const Kv4Attn &a, const Row &row, int key, const int4 &
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     bool see = key + r <= row.own;
-    if constexpr (WIN) see = see && key + r > row.own - a.slots && (long)p[r] > (long)row.own_pos - a.window;
+    if constexpr (WIN) see = see && key + r >= row.first && p[r] >= row.first_pos;
     if (!see) t2[r] = -INFINITY;
     seen |= (uint32_t)see << r;
   }
