@@ -5,10 +5,10 @@
 //   window and position_j > position_a - window); out = sum_j e^{t_j} v_j / sum_j e^{t_j}; a row that sees nothing is 0.
 // All query heads of a KV head and all new tokens are rows of one product: row r is token r / G, head g G + r % G.
 //
-// kv4_attn_kernel: a workgroup owns 16 rows and one span of the keys, its four waves take 32 keys in turn, each with a
-// softmax of its own (running maximum and sum in base 2), joined through LDS at the end; spans are joined by
-// kv4_join_kernel. How keys are split follows from the sequence alone (`spans`), so a row's result does not depend on
-// its batch.
+// kv4_attn_kernel: a workgroup owns 16 rows and one span of the keys (or two, one after the other), its four waves take 32
+// keys in turn, each with a softmax of its own (running maximum and sum in base 2), joined through LDS at the end; spans
+// are joined by kv4_join_kernel. kv4_attn_tile_kernel: a workgroup owns 64 or 128 rows and decodes keys once for all. How
+// keys are split follows from the sequence alone (`spans`), so a row's result does not depend on its batch.
 //
 // Per 32 keys, with 16x16x32 MFMAs (A: 16 rows, lane l row l % 16 and eight k of group l / 16; C: lane l column l % 16,
 // rows 4 (l / 16) + r):
@@ -38,6 +38,9 @@ struct Spans {
   int lo, keys, count;
 };
 
+// Keys of a span at least; spans of a sequence, and rows of all its spans together, at most (a row's part of a span is
+// written and read in 8 D bytes, where 512 keys have 544 D). With spans of 256 keys one sequence of 2111 takes 13.6 us
+// instead of 16.2, but 16 of 8000 72 instead of 61 and 64 of 4000 146 instead of 127.
 constexpr int SPAN = 512, MAX_SPANS = 32, SPLIT_ROWS = 4096;
 
 __host__ __device__ inline int most_spans(int rows) {
@@ -56,15 +59,17 @@ __host__ __device__ inline Spans spans(int ctx, int n, int rows, int window) {
   return {lo, keys, count < 1 ? 1 : count};
 }
 
-// Rows of a KV head up to which waves share rows and split keys (kv4_attn_kernel), by the row tiles a wave has beyond. A tile
-// of two wastes more when rows are few. 24 sequences of 24 rows over 3000 keys: D = 256, one tile, 92 us here and 87 there;
+// Rows of a KV head up to which waves share rows and split keys (kv4_attn_kernel), by the row tiles that a wave has
+// beyond. Two waste more when rows are few. 24 sequences of 24 rows over 3000 keys: D = 256, one tile, 92 us here and 87 there;
 // D = 128, two, 87 and 146. 8 of 40 rows over 4000: 66 and 54; 63 and 90.
 template <int NT>
 constexpr int few_rows() { return NT == 1 ? 32 : 48; }
 
 // Workgroups of kv4_attn_tile_kernel at most: 4 rounds of two a CU.
 constexpr int TILE_GROUPS = 2048;
-// Rows of a KV head up to which their scores are kept for the accumulated weights, instead of computed again.
+// Rows of a KV head up to which their scores are kept for the accumulated weights (4 bytes a row and slot of workspace),
+// instead of computed again. 24 sequences over 3000 slots, 8 heads of 256, attention with weights: 2 rows 48 and 80 us, 16
+// rows 70 and 91; 28 rows would gain 133 -> 114 for 112 bytes a slot, near the 136 of the key itself.
 constexpr int SCORE_ROWS = 16;
 
 DX_DEVICE floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) {
@@ -72,10 +77,10 @@ DX_DEVICE floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) {
 }
 
 // bf16 tiles in LDS: [keys][columns] in 16-byte chunks, chunk c of row r at c ^ swizzle(r), over banks of 16 chunks.
-// V tiles: 16 lanes write a chunk each, of four rows and four blocks (chunks 4 apart; 64 columns: eight rows, two blocks,
-// and two rows share the banks); 32 lanes read the halves of two neighbouring chunks of eight rows, transposed. So the low
-// two bits differ over the four rows, and the bits above the lowest over the eight. K tiles: 16 lanes read a chunk each of
-// 16 rows; their writes as V's.
+// V in kv4_attn_kernel: 16 lanes write a chunk each, of four rows and four blocks (chunks 4 apart; 64 columns: eight rows,
+// two blocks, and two rows share the banks); 32 lanes read the halves of two neighbouring chunks of eight rows, transposed.
+// So the low two bits differ over the four rows, and the bits above the lowest over the eight. In the tile kernel's tiles
+// 16 lanes write, and of K read, one chunk each of 16 rows.
 template <int W>
 DX_DEVICE int swizzle(int r) {
   if constexpr (W == 64) {
@@ -385,8 +390,10 @@ DX_DEVICE void store_row(const Kv4Attn &a, const Sequence &s, const Spans &sp, l
 
 // Few rows: the four waves share 16 rows and take 32 keys in turn. What bounds this kernel is the time that a step's loads
 // take, so a step's registers are filled with the next one's as soon as they have been used: K's at the step's start, V's
-// once it is decoded. Loads are contiguous over the lanes (16 rows of one chunk, as the product wants K, made the vector
-// cache look at each lane by itself: 865 accesses a step where 140 do); K gets its order in LDS.
+// once it is decoded. 32 sequences of up to 16384 slots, 8 heads of 256: 222 us (3.9 TB/s, where a copy reaches 5.0); 24
+// with a window of 4096, 16 heads of 128: 52 us; one of 2111: 12 us, of which 3 pass before the first keys are there. Loads
+// are contiguous over the lanes (16 rows of one chunk, as the product wants K, made the vector cache look at each lane by
+// itself: 865 accesses a step where 140 do); K gets its order in LDS.
 template <int D>
 struct Stage {  // of a wave
   static constexpr int VW = D < 128 ? D : 128;  // columns of V in bf16 at a time
@@ -631,6 +638,9 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
 // tile's codes are on their way while the one before is used, and go over it afterwards. Two workgroups a CU, in step with
 // themselves alone, hide each other's waits; twice the rows a workgroup (half the decoding) or two tiles in turn (no wait
 // between use and decoding) were no faster: 6 questions of up to 611 tokens over up to 8803, D = 256, 358 us either way.
+// Now 294 us: 4 sequences of 400 tokens over 6000 slots reach 410 TFLOP/s. Of its time the vector units work 47% (277
+// instructions a wave and 32 keys: soft-cap 100, softmax 75, decoding 60), LDS 38%, the matrix units 20%; two waves a SIMD
+// (236 registers) leave the rest to waits.
 template <int D>
 constexpr int tile_keys() { return D == 256 ? 32 : 64; }
 

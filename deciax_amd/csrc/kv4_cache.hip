@@ -43,6 +43,8 @@ DX_DEVICE void store_block(const float (&x)[8], uint8_t *codes, uint8_t *scales,
 // rows of neighbouring slots, its scales and positions, are then written together (token by token a line of 128 bytes of
 // scales was written 8 bytes at a time by 16 workgroups). A thread takes ITER items, all loads of one kind before the next,
 // since each waits for the one before: lengths, page, rows.
+// Bound: memory. 12 states, 50545 tokens of 8 heads of 256, bf16: written in 134 us (524 MB, 3.9 TB/s, where a copy reaches
+// 5.0), read back in 83 us (6.3 TB/s: what was just written). 48 tokens: 3.7 and 3.2 us, a launch and four loads in turn.
 struct Item {
   int slot, col;
   long row, at;  // the packed row (-1: none), the place in the cache (-1: none)
@@ -143,6 +145,7 @@ DX_DEVICE uint32_t order(float w) {
 // i 1024 + t. The kept-th largest key is found bit by bit from the top: a round counts the keys at or above a
 // candidate with one compare an item and the wave's population counts, no memory but one number a wave. ITEMS = 0
 // reads the weights again every round, for spans beyond the registers.
+// Bound: the 32 rounds, one after the other, of one workgroup: 9.8 us for 2900 slots, 31 us for up to 16384.
 template <int ITEMS>
 __global__ void __launch_bounds__(SEL_THREADS)
 select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const int32_t *__restrict__ ctx_len,
@@ -250,6 +253,7 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
 
 // Kept rows to their new pages: 16 bytes of codes a thread, the row's scales, position and weight by one of its threads
 // each. Every step (slot, pages, rows) waits for the one before, so a thread takes four rows' steps together.
+// 12 sequences cut to 4096 slots, 8 heads of 256: 47 to 62 us for 210 MB, rows of 128 bytes from anywhere.
 template <int D>
 __global__ void __launch_bounds__(THREADS)
 move_kernel(Kv4Cache c, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ out_table,

@@ -10,6 +10,8 @@
 //     k-th largest of the threads' largest bounds the k best from below, so only the groups that reach it (a few more than
 //     k) are looked at again, each wave keeping a sorted list of its best, one a lane.
 // Chunks follow from the vocabulary alone, so a row's result does not depend on the others.
+// Bound: 1500 rows of 256000 bf16 logits, soft-capped: parts 200 us (3.9 TB/s; two exponentials and a reciprocal a logit
+// keep the vector units as busy as the memory), rows 22 us. One row: 4.3 and 7.6 us, loads that wait for each other.
 #include "common.h"
 #include "kernels.h"
 
