@@ -60,8 +60,8 @@ __host__ __device__ inline Spans spans(int ctx, int n, int rows, int window) {
 }
 
 // Rows of a KV head up to which waves share rows and split keys (kv4_attn_kernel), by the row tiles that a wave has
-// beyond. Two waste more when rows are few. 24 sequences of 24 rows over 3000 keys: D = 256, one tile, 92 us here and 87 there;
-// D = 128, two, 87 and 146. 8 of 40 rows over 4000: 66 and 54; 63 and 90.
+// beyond. Two waste more when rows are few. 24 sequences of 24 rows over 3000 keys: D = 256, one tile, 92 us here and 87
+// there; D = 128, two, 87 and 146. 8 of 40 rows over 4000: 66 and 54; 63 and 90.
 template <int NT>
 constexpr int few_rows() { return NT == 1 ? 32 : 48; }
 

@@ -43,7 +43,7 @@ DX_DEVICE void store_block(const float (&x)[8], uint8_t *codes, uint8_t *scales,
 // rows of neighbouring slots, its scales and positions, are then written together (token by token a line of 128 bytes of
 // scales was written 8 bytes at a time by 16 workgroups). A thread takes ITER items, all loads of one kind before the next,
 // since each waits for the one before: lengths, page, rows.
-// Bound: memory. 12 states, 50545 tokens of 8 heads of 256, bf16: written in 134 us (524 MB, 3.9 TB/s, where a copy reaches
+// Bound: memory. 12 states, 50545 tokens of 8 heads of 256, bf16: written in 128 us (524 MB, 4.1 TB/s, where a copy reaches
 // 5.0), read back in 83 us (6.3 TB/s: what was just written). 48 tokens: 3.7 and 3.2 us, a launch and four loads in turn.
 struct Item {
   int slot, col;
@@ -313,8 +313,12 @@ move_kernel(Kv4Cache c, const int32_t *__restrict__ table, int width, const int3
 
 }  // namespace
 
-// Four items a thread and blocks of 16 tokens where a sequence has more than a few workgroups' worth of them.
-static bool few_items(const Kv4Cache &c, const Kv4Batch &q) { return (long)q.max_seq_len * (c.hkv * c.d / 8) <= 8 * THREADS; }
+// One item a thread up to 2^19 items (twice what the card holds at once), two and blocks of 16 tokens beyond. Append and
+// read of 8 heads of 256, us: 48 sequences of a token 7.2 and 7.8, 4 of 300 10.4 and 11.0, 2 of 1000 14.1 and 14.4; 4 of
+// 1000 22.1 and 21.4, 12 of 517 to 16384 261 and 222 (four items 225, two without blocks 229).
+static bool few_items(const Kv4Cache &c, const Kv4Batch &q) {
+  return (long)q.num_seqs * q.max_seq_len * (c.hkv * c.d / 8) <= 1L << 19;
+}
 static dim3 item_grid(const Kv4Cache &c, const Kv4Batch &q, int iter, int tokens) {
   const long items = (long)(q.max_seq_len + tokens - 1) / tokens * tokens * (c.hkv * c.d / 8), block = (long)iter * THREADS;
   return dim3((unsigned)((items + block - 1) / block), q.num_seqs);
@@ -327,7 +331,7 @@ static void append(const Kv4Cache &c, const Kv4Batch &q, const void *k, const vo
   if (few_items(c, q))
     append_kernel<T, 1, 1><<<item_grid(c, q, 1, 1), dim3(THREADS), 0, s>>>(c, q, kt, vt, positions, k_stride, v_stride);
   else
-    append_kernel<T, 4, 16><<<item_grid(c, q, 4, 16), dim3(THREADS), 0, s>>>(c, q, kt, vt, positions, k_stride, v_stride);
+    append_kernel<T, 2, 16><<<item_grid(c, q, 2, 16), dim3(THREADS), 0, s>>>(c, q, kt, vt, positions, k_stride, v_stride);
 }
 
 hipError_t dx_kv4_append_launch(const Kv4Cache &c, const Kv4Batch &q, const void *k, const void *v,
@@ -342,7 +346,7 @@ hipError_t dx_kv4_read_launch(const Kv4Cache &c, const Kv4Batch &q, uint16_t *k,
   if (few_items(c, q))
     read_kernel<1, 1><<<item_grid(c, q, 1, 1), dim3(THREADS), 0, s>>>(c, q, k, v, k_stride, v_stride);
   else
-    read_kernel<4, 16><<<item_grid(c, q, 4, 16), dim3(THREADS), 0, s>>>(c, q, k, v, k_stride, v_stride);
+    read_kernel<2, 16><<<item_grid(c, q, 2, 16), dim3(THREADS), 0, s>>>(c, q, k, v, k_stride, v_stride);
   return hipGetLastError();
 }
 
@@ -352,6 +356,8 @@ hipError_t dx_kv4_evict_launch(const Kv4Cache &c, const int32_t *table, int widt
                                long o_head, int32_t *out_len, int32_t *list, hipStream_t s) {
   const dim3 grid(c.hkv, num_seqs), block(SEL_THREADS);
   const int rounds = (max_ctx + SEL_THREADS - 1) / SEL_THREADS;
+// By the slots that a thread holds. us of an eviction to 1000: 2900 slots 20.5 with 4 a thread and 32.7 with 16, 14000
+// 44 with 16 and 93 with 64, 60000 101 with 64 and 327 when read again every round.
 #define SELECT(N) \
   select_kernel<N><<<grid, block, 0, s>>>(weights, w_seq, w_head, ctx_len, max_ctx, keep, recent, list, out_len)
   if (rounds <= 4) SELECT(4);
