@@ -552,9 +552,11 @@ int dx_kv4_read(const dx_kv4_cache *cache, void *k, void *v,
  * weight: weights_in (0 for the newest tokens' slots, whatever it holds there)
  * plus the softmax weights of all rows and query heads of the KV head that saw
  * it. weights are fp32 at b * seq_stride + g * head_stride + slot; weights_in may
- * be weights_out; slots from ctx_len on are not written. Sums have one order:
- * the same call gives the same bits, alone or in a batch. Workspace size from
- * dx_attn_kv4_workspace with the same sizes. */
+ * be weights_out with the same strides, and must not meet it otherwise; slots
+ * from ctx_len on are not written. Sums have one order: the same call gives the
+ * same bits, alone or in a batch. Workspace size from dx_attn_kv4_workspace with
+ * the same sizes (with weights, most of it 4 bytes a slot and row of a KV head,
+ * 16 rows at most). */
 int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out,
                 const int32_t *page_table, int32_t table_width,
                 const int32_t *seq_start, const int32_t *seq_len,
