@@ -120,7 +120,9 @@ class Case:
             qb = q[rows].reshape(n, self.hq, self.d)
             want, wsum, mass = oracle.attention(qb, k, v, pos, scale=scale, softcap=softcap, window=window)
             finite = np.nan_to_num(k)
-            biggest = max((np.abs(qb) @ np.abs(finite).reshape(-1, self.d).T).max(initial=0.0) * scale, 1.0)
+            # the largest score of the rows that have one: a query that is NaN has none, and is compared as NaN below
+            asked = np.where(np.isnan(qb), 0.0, np.abs(qb))
+            biggest = max((asked @ np.abs(finite).reshape(-1, self.d).T).max(initial=0.0) * scale, 1.0)
             seen = min(biggest, softcap) if softcap else biggest
             score_error = self.d * U32 * biggest + 8 * U32 * max(seen, softcap)
             moved = 2 * score_error + 8 * U32
@@ -290,6 +292,34 @@ def test_values_and_keys_that_are_nan_reach_only_rows_that_see_them(d: int, dtyp
     assert np.isfinite(got[:7]).all() and np.isfinite(got[20]).all()
     assert np.isnan(got[7, 0, 32:64]).all() and np.isfinite(got[7, 0, :32]).all() and np.isfinite(got[7, 2:]).all()
     c.check(out, scale=0.2, softcap=50.0, window=0)
+
+
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (50.0, 0), (0.0, 70), (50.0, 700)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,hkv,group", [(64, 2, 3), (128, 1, 8), (256, 2, 1)])
+def test_many_rows(d: int, hkv: int, group: int, dtype: str, softcap: float, window: int) -> None:
+    """Questions of many rows over states of a few spans, the last tiles of rows and keys half full, with NaN values in
+    the middle and in the newest slots and with a query that is NaN, which its KV head's weights show."""
+    import torch
+
+    new, ctx, hq = [129, 70, 66], [1300, 70, 97], hkv * group
+    say(f"attention_kv4 many rows d={d} hq={hq} hkv={hkv} {dtype} cap={softcap} window={window}")
+    c = Case(40 + d, new, ctx, hq, hkv, d, 64, dtype)
+    c.fill(3)
+    for token, col in ((0, 5), (63, d - 1), (128, 40), (129 + 69, 0)):
+        c.v[token, col] = float("nan")
+    c.q[129 + 69, 3] = float("nan")
+    c.append()
+    r = rng(d)
+    w = np.abs(r.normal(size=(3, hkv, 1303))).astype(np.float32)
+    w_in = torch.from_numpy(w.copy()).cuda()
+    w_out = torch.full_like(w_in, -7.0)
+    kw = dict(scale=d ** -0.5 * 2, softcap=softcap, window=window)
+    out = c.attend(weights=w_in, weights_out=w_out, **kw)
+    torch.cuda.synchronize()
+    c.check(out, w_out, w, **kw)
+    for b, m in enumerate(ctx):
+        assert (w_out[b, :, m:] == -7).all()
 
 
 def test_infinite_and_nan_queries_stay_in_their_rows() -> None:
