@@ -889,8 +889,9 @@ int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32
   REQUIRE(num_q_heads > 0 && num_q_heads % a.c.hkv == 0,
           "attn_kv4: num_q_heads %d must be a positive multiple of num_kv_heads %d", num_q_heads, a.c.hkv);
   REQUIRE(window >= 0, "attn_kv4: window must be >= 0, got %d", window);
-  REQUIRE(softcap >= 0.f && softcap < INFINITY && scale > 0.f && scale < INFINITY,
-          "attn_kv4: need a finite scale > 0 and softcap >= 0");
+  REQUIRE(softcap >= 0.f && softcap < INFINITY && scale > 0.f && scale < INFINITY &&
+              (softcap == 0.f || scale / softcap < INFINITY),
+          "attn_kv4: need a finite scale > 0 and softcap >= 0, and a finite scale / softcap");
   const int64_t vec = dtype == DX_BF16 ? 8 : 4, width = (int64_t)num_q_heads * a.c.d;
   REQUIRE(q_row_stride >= width && out_row_stride >= width && q_row_stride % vec == 0 && out_row_stride % vec == 0,
           "attn_kv4: row strides must cover heads * head_dim and be multiples of %ld elements", (long)vec);
@@ -986,7 +987,8 @@ int dx_token_logprobs(const void *logits, const int32_t *targets, int64_t rows, 
   REQUIRE(rows >= 0 && rows <= INT32_MAX && vocab > 0 && row_stride >= vocab,
           "token_logprobs: %ld rows of %d (stride %ld)", (long)rows, vocab, (long)row_stride);
   SUPPORTED(vocab <= MOST_SLOTS, "token_logprobs: vocabulary of %d", vocab);
-  REQUIRE(softcap >= 0.f && softcap < INFINITY, "token_logprobs: softcap must be >= 0 and finite");
+  REQUIRE(softcap >= 0.f && softcap < INFINITY && (softcap == 0.f || 4.f / softcap < INFINITY),
+          "token_logprobs: softcap must be >= 0 and finite, with a finite reciprocal");
   REQUIRE(top >= 0 && top <= vocab, "token_logprobs: %d alternatives of %d", top, vocab);
   SUPPORTED(top <= 64, "token_logprobs: %d alternatives, 64 at most", top);
   REQUIRE(top == 0 || (top_ids && top_logprobs), "token_logprobs: null output of the alternatives");

@@ -92,7 +92,7 @@ def test_read(bad, want) -> None:
 @pytest.mark.parametrize("bad,want", [
     (dict(q=None), INVALID), (dict(out=ODD), INVALID), (dict(table=None), INVALID), (dict(hq=3), INVALID),
     (dict(hq=0), INVALID), (dict(qs=256), INVALID), (dict(os=516), INVALID), (dict(scale=0.0), INVALID),
-    (dict(scale=float("nan")), INVALID), (dict(cap=-1.0), INVALID), (dict(window=-1), INVALID), (dict(dtype=3), INVALID),
+    (dict(scale=float("nan")), INVALID), (dict(cap=-1.0), INVALID), (dict(cap=1e-40), INVALID), (dict(window=-1), INVALID), (dict(dtype=3), INVALID),
     (dict(max_ctx=-1), INVALID), (dict(max_ctx=(1 << 30) + 1), UNSUPPORTED), (dict(max_new=1 << 26), UNSUPPORTED),
     (dict(w_out=P), INVALID), (dict(w_in=P, w_out=P, wi=(512, 255)), INVALID),
     (dict(w_in=P, w_out=P, wo=(512, 100)), INVALID), (dict(ws=None, max_ctx=256, w_in=P, w_out=P), INVALID),
@@ -115,7 +115,7 @@ def test_evict(bad, want) -> None:
 @pytest.mark.parametrize("bad,want", [
     (dict(x=None), INVALID), (dict(t=None), INVALID), (dict(lp=None), INVALID), (dict(ent=None), INVALID),
     (dict(ids=None), INVALID), (dict(tops=None), INVALID), (dict(rows=-1), INVALID), (dict(rows=1 << 31), INVALID),
-    (dict(vocab=0), INVALID), (dict(ld=99), INVALID), (dict(cap=-1.0), INVALID), (dict(top=-1), INVALID),
+    (dict(vocab=0), INVALID), (dict(ld=99), INVALID), (dict(cap=-1.0), INVALID), (dict(cap=1e-39), INVALID), (dict(top=-1), INVALID),
     (dict(top=101), INVALID), (dict(top=65), UNSUPPORTED), (dict(dtype=9), INVALID),
     (dict(x=ctypes.c_void_p(0x10001)), INVALID), (dict(x=ctypes.c_void_p(0x10002), dtype=_lib.DX_F32), INVALID),
     (dict(ws=None), INVALID), (dict(ws_bytes=10), INVALID), (dict(vocab=(1 << 30) + 1, ld=1 << 31), UNSUPPORTED),
