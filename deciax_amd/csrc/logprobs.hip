@@ -3,9 +3,9 @@
 // t = x, or cap tanh(x / cap) with a soft-cap (-inf stays -inf: no alternative); with M >= max t,
 //   S = sum e^{t - M}, E = sum (t - M) e^{t - M}:   log p_j = (t_j - M) - log S,   H = log S - E / S.
 // The logits are read once. Two launches:
-//   parts_kernel: a wave takes 2048 neighbouring logits of a row in registers, its M (the shift is the cap itself with
-//     one: t - cap = -2 cap / (1 + e^{2x / cap}), which keeps its relative precision where the weight is), S and E, and
-//     the largest logit of each 32 neighbours.
+//   parts_kernel: a wave takes 2048 neighbouring logits of a row in registers, its M (with a cap of up to 40, where e^{-2
+//     cap} is well above the smallest numbers, the cap itself: t - cap = -2 cap / (1 + e^{2x / cap}); else its largest t),
+//     S and E, and the largest logit of each 32 neighbours.
 //   row_kernel: one workgroup a row joins the parts in their order and finds the alternatives from those largest ones: the
 //     k-th largest of the threads' largest bounds the k best from below, so only the groups that reach it (a few more than
 //     k) are looked at again, each wave keeping a sorted list of its best, one a lane.
@@ -27,6 +27,18 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 DX_DEVICE uint32_t order(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+DX_DEVICE bool by_cap(float cap) { return cap > 0.f && cap <= 40.f; }  // whether M is the cap
+
+// cap tanh(x / cap), -inf staying -inf, to a few roundings of itself: with y = x / cap the continued fraction of tanh cut
+// after y^9, y (y^4 + 105 y^2 + 945) / (15 (y^4 + 28 y^2 + 63)), off by 2.4e-8 of the value at |y| <= 0.9, and the
+// exponential's form beyond.
+DX_DEVICE float capped(float x, float cap) {
+  const float y = x * (1.f / cap), z = y * y;
+  const float n = __builtin_fmaf(z + 105.f, z, 945.f), m = __builtin_fmaf(z + 28.f, z, 63.f);
+  const float far = cap * copysignf(1.f - 2.f * fast_rcp(1.f + fast_exp2(2.f * LOG2E * fabsf(y))), x);
+  return x == -INFINITY ? x : fabsf(y) > 0.9f ? far : x * (1.f / 15.f) * n * fast_rcp(m);
 }
 
 template <bool B>
@@ -91,7 +103,7 @@ parts_kernel(const T *__restrict__ logits, int vocab, long ld, float cap, int ch
     }
   }
   float shift = cap, s = 0.f, e = 0.f;
-  if (cap > 0.f) {
+  if (by_cap(cap)) {
     // 1.5 of some 19 vector instructions' time a logit (three are transcendental, four each), 1500 x 256000 in bf16: a
     // chunk without -inf, most are, does not look for it again
     const float c1 = 2.f * LOG2E / cap, c2 = -2.f * LOG2E * cap;
@@ -110,6 +122,16 @@ parts_kernel(const T *__restrict__ logits, int vocab, long ld, float cap, int ch
     if (__any(low == -INFINITY)) add(Flag<true>{});
     else add(Flag<false>{});
   } else {
+    if (cap > 0.f) {
+      top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          x[j][i] = capped(x[j][i], cap);
+          top = fmaxf(top, x[j][i]);
+        }
+    }
     shift = wave_max(top);
     const float base = shift == -INFINITY ? 0.f : shift;
 #pragma unroll
@@ -144,7 +166,8 @@ DX_DEVICE float logit_of(uint32_t v) { return __uint_as_float(v & 0x80000000u ? 
 // t - shift of a logit, as accurate as parts_kernel's sum is.
 DX_DEVICE float shifted(float x, float cap, float shift) {
   if (x == -INFINITY) return -INFINITY;
-  return cap > 0.f ? -2.f * cap / (1.f + expf(2.f * x / cap)) : x - shift;
+  if (by_cap(cap)) return -2.f * cap / (1.f + expf(2.f * x / cap));
+  return (cap > 0.f ? capped(x, cap) : x) - shift;
 }
 
 constexpr int ROW_WAVES = 8, ROW_THREADS = 64 * ROW_WAVES;
@@ -234,7 +257,7 @@ row_kernel(const T *__restrict__ logits, const int32_t *__restrict__ targets, in
   }
   // join: every thread the same largest shift, then sums in the threads' order
   float shift = cap;
-  if (!(cap > 0.f)) {
+  if (!by_cap(cap)) {
     float m = first[0];
     for (int i = tid + ROW_THREADS; i < chunks; i += ROW_THREADS) m = fmaxf(m, part[i * 3]);
     m = wave_max(m);

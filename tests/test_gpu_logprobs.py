@@ -17,13 +17,12 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
-def check(x: np.ndarray, targets: np.ndarray, top: int, cap: float, got) -> None:
+def check(x: np.ndarray, targets: np.ndarray, top: int, cap: float, got, size: float | None = None) -> None:
     lp, ent, ids, tops = (t.cpu().numpy().astype(np.float64) for t in got)
     for i in range(len(x)):
         want = oracle.token_logprobs(x[i], int(targets[i]), top, cap)
         finite = np.abs(x[i][np.isfinite(x[i])])
-        size = cap if cap else finite.max(initial=1.0)
-        tol = 2 * (12 * size + 96 + 8) * U
+        tol = 2 * (12 * (size or cap or finite.max(initial=1.0)) + 96 + 8) * U
         for g, w, what in ((lp[i], want[0], "log probability"), (ent[i], want[1], "entropy")):
             assert np.isnan(g) == np.isnan(w) and np.isinf(g) == np.isinf(w), (i, what, g, w)
             if np.isfinite(w):
@@ -142,3 +141,35 @@ def test_many_rows() -> None:
     want = torch.log_softmax(x.double().cpu(), 1)
     assert (lp.cpu().double() - want.gather(1, targets.cpu().long()[:, None])[:, 0]).abs().max() < 1e-5
     assert (ids[:, 0].cpu() == x.cpu().argmax(1)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cap", [41.0, 50.0, 120.0, 1000.0, 1e7, 1e38])
+def test_large_soft_caps(cap: float, dtype: str) -> None:
+    """Caps far above the logits and logits far below minus the cap: e^{t - cap} is no number there. A capped logit is off
+    by 8 u of itself (a fraction cut at 0.4 u and seven roundings; the form beyond 0.9 of the cap likewise), so by 8 u of
+    the smaller of the cap and the largest logit; its difference to the largest and its conversion by 4 u more."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"token_logprobs cap={cap} {dtype}")
+    r = rng(int(min(cap, 9999)))
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    x = (r.normal(size=(6, 5000)) * 4).astype(np.float32)
+    x[1] -= min(3 * cap, 1000.0)
+    x[2] *= 20
+    x[3, ::2] = -np.inf
+    x[4, :] = -np.inf
+    x[4, 77] = -5.0
+    x[5, 9] = np.inf
+    logits = torch.from_numpy(x).cuda().to(t)
+    host = logits.float().cpu().numpy()
+    targets = r.integers(0, 5000, 6)
+    targets[4] = 77
+    got = K.token_logprobs(logits, i32(targets), top=6, softcap=cap)
+    torch.cuda.synchronize()
+    for i in range(6):
+        finite = np.abs(host[i][np.isfinite(host[i])])
+        size = min(cap, max(finite.max(), cap if i == 5 else 0.0))
+        check(host[i:i + 1], targets[i:i + 1], 6, cap, [g[i:i + 1] for g in got], size)
