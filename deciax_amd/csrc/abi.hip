@@ -889,9 +889,9 @@ int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32
   REQUIRE(num_q_heads > 0 && num_q_heads % a.c.hkv == 0,
           "attn_kv4: num_q_heads %d must be a positive multiple of num_kv_heads %d", num_q_heads, a.c.hkv);
   REQUIRE(window >= 0, "attn_kv4: window must be >= 0, got %d", window);
-  REQUIRE(softcap >= 0.f && softcap < INFINITY && scale > 0.f && scale < INFINITY &&
+  REQUIRE(softcap >= 0.f && softcap <= 1e30f && scale > 0.f && scale < INFINITY &&
               (softcap == 0.f || scale / softcap < INFINITY),
-          "attn_kv4: need a finite scale > 0 and softcap >= 0, and a finite scale / softcap");
+          "attn_kv4: need a finite scale > 0, softcap in [0, 1e30] and a finite scale / softcap");
   const int64_t vec = dtype == DX_BF16 ? 8 : 4, width = (int64_t)num_q_heads * a.c.d;
   REQUIRE(q_row_stride >= width && out_row_stride >= width && q_row_stride % vec == 0 && out_row_stride % vec == 0,
           "attn_kv4: row strides must cover heads * head_dim and be multiples of %ld elements", (long)vec);

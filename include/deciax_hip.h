@@ -546,7 +546,7 @@ int dx_kv4_read(const dx_kv4_cache *cache, void *k, void *v,
  * and position[j] > position[own] - window. q and out: bf16, or fp32 with three
  * bf16 products for each fp32 one. A row that sees nothing is written as zeros;
  * rows that belong to no sequence are not written. num_q_heads is any multiple
- * of the cache's heads.
+ * of the cache's heads; softcap (0: none) at most 1e30 and not below scale / FLT_MAX.
  *
  * With weights_out, every slot below ctx_len gets its accumulated attention
  * weight: weights_in (0 for the newest tokens' slots, whatever it holds there)

@@ -382,6 +382,21 @@ def test_scores_beyond_the_soft_cap(new: list[int], ctx: list[int], hq: int, hkv
     c.check(out, w, w_in, **kw)
 
 
+@pytest.mark.parametrize("n", [1, 70])
+def test_a_large_soft_cap_is_none(n: int) -> None:
+    """A cap of 1e6 moves scores of at most some 20 by 1e-9 of themselves, and the arithmetic by 8 u of them: weights by
+    2 * 8 * 20 u = 2e-5 of themselves each, averages of values of at most 6 by twice that."""
+    import torch
+
+    say(f"attention_kv4 with a soft-cap of 1e6, {n} tokens")
+    c = Case(17, [n], [700], 4, 2, 128, 64, "f32")
+    c.fill(8)
+    c.append()
+    capped, plain = (c.attend(scale=0.1, softcap=cap) for cap in (1e6, 0.0))
+    torch.cuda.synchronize()
+    assert (capped - plain).abs().max().item() <= 2 * 2e-5 * 6
+
+
 def alone(c: Case, b: int, w, **kw):
     """Output and weights of sequence b of a case in a call of its own."""
     import torch

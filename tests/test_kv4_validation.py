@@ -92,7 +92,7 @@ def test_read(bad, want) -> None:
 @pytest.mark.parametrize("bad,want", [
     (dict(q=None), INVALID), (dict(out=ODD), INVALID), (dict(table=None), INVALID), (dict(hq=3), INVALID),
     (dict(hq=0), INVALID), (dict(qs=256), INVALID), (dict(os=516), INVALID), (dict(scale=0.0), INVALID),
-    (dict(scale=float("nan")), INVALID), (dict(cap=-1.0), INVALID), (dict(cap=1e-40), INVALID), (dict(window=-1), INVALID), (dict(dtype=3), INVALID),
+    (dict(scale=float("nan")), INVALID), (dict(cap=-1.0), INVALID), (dict(cap=1e-40), INVALID), (dict(cap=1e31), INVALID), (dict(window=-1), INVALID), (dict(dtype=3), INVALID),
     (dict(max_ctx=-1), INVALID), (dict(max_ctx=(1 << 30) + 1), UNSUPPORTED), (dict(max_new=1 << 26), UNSUPPORTED),
     (dict(w_out=P), INVALID), (dict(w_in=P, w_out=P, wi=(512, 255)), INVALID),
     (dict(w_in=P, w_out=P, wo=(512, 100)), INVALID), (dict(ws=None, max_ctx=256, w_in=P, w_out=P), INVALID),
