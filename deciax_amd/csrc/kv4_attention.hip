@@ -303,7 +303,7 @@ DX_DEVICE Row query_row(const Kv4Attn &a, const Sequence &s, const int32_t *tabl
 
 // Which of the four keys from `key` on (positions `pos`) a row sees; the scores of the others become -inf.
 template <bool WIN>
-DX_DEVICE uint32_t mask4(const Kv4Attn &a, const Row &row, int key, const int4 &pos, float (&t2)[4]) {
+DX_DEVICE uint32_t mask4(const Row &row, int key, const int4 &pos, float (&t2)[4]) {
   const int p[4] = {pos.x, pos.y, pos.z, pos.w};
   uint32_t seen = 0;
 #pragma unroll
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
         seen = 0;
   #pragma unroll
         for (int t = 0; t < 2; ++t)
-          seen |= mask4<WIN>(a, row, page ? kb + t * 16 + grp * 4 : 0x7ffffff0, here[t], t2[t]) << (4 * t);
+          seen |= mask4<WIN>(row, page ? kb + t * 16 + grp * 4 : 0x7ffffff0, here[t], t2[t]) << (4 * t);
       }
       if (a.scores && rows <= SCORE_ROWS && col < rows) {
         float *to = a.scores + (((long)b * a.c.hkv + g) * a.score_rows + col) * a.score_slots + kb + grp * 4;
@@ -817,8 +817,8 @@ __global__ void __launch_bounds__(64 * TW, D == 256 ? (NS > 1 ? 1 : 2) : 2) kv4_
         for (int n = 0; n < NT; ++n) {
           if constexpr (CAP) capped(part[t][n], a.softcap * LOG2E);
           if (masked) {
-            const uint32_t see = a.window > 0 ? mask4<true>(a, row[n], kb + t * 16 + grp * 4, pos, part[t][n])
-                                              : mask4<false>(a, row[n], kb + t * 16 + grp * 4, pos, part[t][n]);
+            const uint32_t see = a.window > 0 ? mask4<true>(row[n], kb + t * 16 + grp * 4, pos, part[t][n])
+                                              : mask4<false>(row[n], kb + t * 16 + grp * 4, pos, part[t][n]);
             seen[n] = t == 0 ? see : seen[n] | see << 4;
           }
 #pragma unroll
@@ -1104,8 +1104,8 @@ __global__ void __launch_bounds__(THREADS, NS == 1 ? 3 : 1) kv4_weights_kernel(K
         if constexpr (CAP) capped(t2[t], a.softcap * LOG2E);
         if (masked) {
           const int key = kb + t * 16 + grp * 4;
-          const uint32_t seen = a.window > 0 ? mask4<true>(a, row, key, pos[t], t2[t])
-                                             : mask4<false>(a, row, key, pos[t], t2[t]);
+          const uint32_t seen = a.window > 0 ? mask4<true>(row, key, pos[t], t2[t])
+                                             : mask4<false>(row, key, pos[t], t2[t]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum[t * 4 + r] += row.real && (seen >> r) & 1 ? fast_exp2(t2[t][r] - lse) : 0.f;
         } else {
