@@ -9,6 +9,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "kv4_plan.h"
 
 namespace {
 
@@ -817,7 +818,7 @@ struct Kv4Workspace {
   int64_t stats, lse, scores, total;
 };
 
-Kv4Workspace kv4_workspace(const Kv4Plan &p, int64_t units, int32_t d, bool weights) {
+Kv4Workspace kv4_workspace(const kv4::Plan &p, int64_t units, int32_t d, bool weights) {
   Kv4Workspace w;
   w.stats = align_up(units * p.part_rows * d * 4, 256);
   w.lse = w.stats + align_up(units * p.part_rows * 8, 256);
@@ -867,8 +868,8 @@ int64_t dx_attn_kv4_workspace(int32_t num_seqs, int32_t max_seq_len, int32_t max
   if (num_seqs <= 0 || max_seq_len < 0 || max_ctx_len < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || window < 0 ||
       max_ctx_len > MOST_SLOTS || (int64_t)max_seq_len * (num_q_heads / num_kv_heads) > MOST_SLOTS / 32)
     return 0;
-  const Kv4Plan p =
-      dx_kv4_attn_plan(max_seq_len, max_ctx_len, num_q_heads / num_kv_heads, in_range(window, max_ctx_len));
+  const kv4::Plan p =
+      kv4::attn_plan(max_seq_len, max_ctx_len, num_q_heads / num_kv_heads, in_range(window, max_ctx_len));
   return kv4_workspace(p, (int64_t)num_seqs * num_kv_heads, head_dim, with_weights != 0).total;
 }
 
@@ -907,7 +908,7 @@ int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32
   if (num_seqs == 0 || ((rows == 0 || max_seq_len == 0) && !weights_out)) return DX_OK;
   a.window = window;
   a.slots = in_range(window, max_ctx_len);
-  const Kv4Plan p = dx_kv4_attn_plan(max_seq_len, max_ctx_len, group, a.slots);
+  const kv4::Plan p = kv4::attn_plan(max_seq_len, max_ctx_len, group, a.slots);
   const Kv4Workspace w = kv4_workspace(p, (int64_t)num_seqs * a.c.hkv, a.c.d, weights_out != nullptr);
   REQUIRE(workspace_bytes >= w.total, "attn_kv4: workspace of %ld bytes, need %ld", (long)workspace_bytes,
           (long)w.total);

@@ -161,17 +161,11 @@ struct Kv4Attn {
   const float *w_in;  // accumulated weights [seqs][hkv][slots], strides below; null without them
   float *w_out;
   long wi_seq, wi_head, wo_seq, wo_head;
-  float *partial, *stats, *lse, *scores;  // workspace, sizes by dx_kv4_attn_plan; scores null without rows to score
+  float *partial, *stats, *lse, *scores;  // workspace, sizes by kv4::attn_plan; scores null without rows to score
   int score_rows;
   long score_slots;
   int part_rows, max_rows, max_splits, few_rows, few_tiles, spans_each;  // the last three by the launcher
 };
-// Sizes that depend on the largest lengths alone: partial rows per (sequence, kv head), rows, splits; rows and slots of
-// kept scores.
-struct Kv4Plan {
-  int part_rows, max_rows, max_splits, score_rows, score_slots;
-};
-Kv4Plan dx_kv4_attn_plan(int max_seq_len, int max_ctx, int group, int window);
 hipError_t dx_kv4_attn_launch(const Kv4Attn &a, bool f32, hipStream_t s);
 
 // Log probabilities (logprobs.hip). groups: largest logit of each 32 of the vocabulary; parts: per 2048, see there.

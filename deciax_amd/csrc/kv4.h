@@ -13,6 +13,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "kv4_plan.h"
 
 namespace kv4 {
 

@@ -33,32 +33,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// How a sequence's keys are split: [lo, ctx) in `count` spans of `keys`.
-struct Spans {
-  int lo, keys, count;
-};
-
-// Keys of a span at least; spans of a sequence, and rows of all its spans together, at most (a row's part of a span is
-// written and read in 8 D bytes, where 512 keys have 544 D). With spans of 256 keys one sequence of 2111 takes 13.6 us
-// instead of 16.2, but 16 of 8000 72 instead of 61 and 64 of 4000 146 instead of 127.
-constexpr int SPAN = 512, MAX_SPANS = 32, SPLIT_ROWS = 4096;
-
-__host__ __device__ inline int most_spans(int rows) {
-  const int most = SPLIT_ROWS / (rows > 0 ? rows : 1);
-  return most < 1 ? 1 : most > MAX_SPANS ? MAX_SPANS : most;
-}
-
-__host__ __device__ inline Spans spans(int ctx, int n, int rows, int window) {
-  int lo = window > 0 && ctx - n - window + 1 > 0 ? ctx - n - window + 1 : 0;
-  lo &= ~63;
-  const int len = ctx - lo, most = most_spans(rows);
-  const int wanted = len / SPAN < most ? (len + SPAN - 1) / SPAN : most;
-  // whole turns of kv4_attn_kernel's waves
-  const int keys = wanted > 1 ? ((len + wanted - 1) / wanted + 127) & ~127 : SPAN;
-  const int count = (len + keys - 1) / keys;
-  return {lo, keys, count < 1 ? 1 : count};
-}
-
 // Rows of a KV head up to which waves share rows and split keys (kv4_attn_kernel), by the row tiles that a wave has
 // beyond. Two waste more when rows are few. 24 sequences of 24 rows over 3000 keys: D = 256, one tile, 92 us here and 87
 // there; D = 128, two, 87 and 146. 8 of 40 rows over 4000: 66 and 54; 63 and 90.
@@ -67,11 +41,6 @@ constexpr int few_rows() { return NT == 1 ? 32 : 48; }
 
 // Workgroups of kv4_attn_tile_kernel at most: 4 rounds of two a CU.
 constexpr int TILE_GROUPS = 2048;
-// Rows of a KV head up to which their scores are kept for the accumulated weights (4 bytes a row and slot of workspace),
-// instead of computed again. 24 sequences over 3000 slots, 8 heads of 256, attention with weights: 2 rows 48 and 80 us, 16
-// rows 70 and 91; 28 rows would gain 133 -> 114 for 112 bytes a slot, near the 136 of the key itself.
-constexpr int SCORE_ROWS = 16;
-
 DX_DEVICE floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -1179,7 +1148,7 @@ hipError_t launch(Kv4Attn a, hipStream_t s) {
     e = hipGetLastError();
   }
   if (e == hipSuccess && few > 0 && a.max_splits > 1) {
-    const int split_rows = min(a.max_rows, SPLIT_ROWS / 2);  // rows with more than one span
+    const int split_rows = min(a.max_rows, MOST_SPLIT_ROWS);
     kv4_join_kernel<D, NS><<<dim3((split_rows + WAVES - 1) / WAVES, a.c.hkv, a.q.num_seqs), dim3(THREADS), 0, s>>>(a);
     e = hipGetLastError();
   }
@@ -1203,20 +1172,6 @@ hipError_t by_type(const Kv4Attn &a, bool f32, hipStream_t s) {
 }
 
 }  // namespace
-
-Kv4Plan dx_kv4_attn_plan(int max_seq_len, int max_ctx, int group, int window) {
-  Kv4Plan p;
-  p.max_rows = max_seq_len * group;
-  // a window's span starts at a multiple of 64 below it and ends with the newest tokens
-  const long seen = window > 0 ? (long)window + 64 + max_seq_len : max_ctx;
-  const long len = seen < max_ctx ? seen : max_ctx, most = (len + SPAN - 1) / SPAN;
-  p.max_splits = most < 1 ? 1 : most > MAX_SPANS ? MAX_SPANS : (int)most;  // a shorter sequence may have more than a longer
-  const long rows = (long)p.max_splits * p.max_rows;
-  p.part_rows = p.max_splits == 1 ? 0 : (int)(rows < SPLIT_ROWS ? rows : SPLIT_ROWS);
-  p.score_rows = p.max_rows < SCORE_ROWS ? p.max_rows : SCORE_ROWS;
-  p.score_slots = (max_ctx + 63) & ~63;  // whole steps
-  return p;
-}
 
 hipError_t dx_kv4_attn_launch(const Kv4Attn &a, bool f32, hipStream_t s) {
   if (a.c.d == 64) return by_type<64>(a, f32, s);

@@ -729,3 +729,36 @@ def test_a_state_is_kept_cut_and_answered_over() -> None:
         want = oracle.token_logprobs(x[i], int(t[i]), 5, 30.0)
         assert abs(lp[i].item() - want[0]) < 1e-4 and abs(ent[i].item() - want[1]) < 1e-4
         assert ids[i].cpu().tolist() == want[2].tolist()
+
+
+# ------------------------------------------------------------------------------------------ prompts
+
+PROMPTS = [  # new, ctx, hq, hkv, d: more than 2048 rows of a KV head, whose keys are one span, beside sequences of several
+    ([1100, 3, 400], [2111, 1300, 1000], 4, 2, 64),
+    ([300], [700], 8, 1, 128),
+    ([2, 1030], [600, 1100], 2, 1, 256),
+]
+
+
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (50.0, 700)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("prompt", range(len(PROMPTS)))
+def test_prompts(prompt: int, dtype: str, softcap: float, window: int) -> None:
+    import torch
+
+    new, ctx, hq, hkv, d = PROMPTS[prompt]
+    say(f"attention_kv4 prompts new={new} ctx={ctx} hq={hq} hkv={hkv} d={d} {dtype} cap={softcap} window={window}")
+    c = Case(60 + prompt, new, ctx, hq, hkv, d, 64, dtype)
+    c.fill(prompt)
+    c.append()
+    w = np.abs(rng(prompt).normal(size=(len(new), hkv, max(ctx)))).astype(np.float32)
+    w_in = torch.from_numpy(w.copy()).cuda()
+    w_out = torch.full_like(w_in, -7.0)
+    kw = dict(scale=d ** -0.5 * 2, softcap=softcap, window=window)
+    plain = c.attend(**kw)
+    out = c.attend(weights=w_in, weights_out=w_out, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(plain, out), "weights change no output"
+    c.check(out, w_out, w, **kw)
+    for b, m in enumerate(ctx):
+        assert (w_out[b, :, m:] == -7.0).all(), "slots behind the sequence were written"
