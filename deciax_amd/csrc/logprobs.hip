@@ -269,7 +269,8 @@ row_kernel(const T *__restrict__ logits, const int32_t *__restrict__ targets, in
   }
   float s = 0.f, e = 0.f;
   auto add = [&](float top_i, float s_i, float e_i) {
-    const float d = top_i == -INFINITY ? 0.f : (top_i - shift) * LOG2E;
+    // a part of masked logits may lie as far below as numbers go: the same bound as a logit's there
+    const float d = top_i == -INFINITY ? 0.f : top_i - shift < -1e30f ? -1e30f : (top_i - shift) * LOG2E;
     const float f = fast_exp2(d), si = s_i * f;
     s += si;
     e += e_i * f + si * d;

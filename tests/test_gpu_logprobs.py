@@ -173,3 +173,31 @@ def test_large_soft_caps(cap: float, dtype: str) -> None:
         finite = np.abs(host[i][np.isfinite(host[i])])
         size = min(cap, max(finite.max(), cap if i == 5 else 0.0))
         check(host[i:i + 1], targets[i:i + 1], 6, cap, [g[i:i + 1] for g in got], size)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_chunks_masked_with_the_lowest_value(dtype: str) -> None:
+    """The type's lowest value as a mask, over whole chunks of 2048 logits or the short last one: their weight is 0, and
+    the entropy that of the others."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"token_logprobs with chunks of the lowest value {dtype}")
+    vocab = 5000
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    lowest = torch.finfo(t).min
+    logits = torch.from_numpy((rng(3).normal(size=(6, vocab)) * 4).astype(np.float32)).cuda().to(t)
+    logits[0, 2048:4096] = lowest
+    logits[1, 4096:] = lowest
+    logits[2, :4096] = lowest
+    logits[3, 1:] = lowest
+    logits[4, 100:] = lowest
+    logits[4, 2048:4000] = -float("inf")
+    logits[5, :4090] = -float("inf")
+    logits[5, 4096:] = lowest
+    host = logits.float().cpu().numpy()
+    targets = np.array([5, 4999, 4200, 0, 99, 4095])
+    got = K.token_logprobs(logits, i32(targets), top=6)
+    torch.cuda.synchronize()
+    check(host, targets, 6, 0.0, got, float(np.abs(host[host > lowest]).max(where=np.isfinite(host[host > lowest]), initial=1.0)))
