@@ -38,7 +38,7 @@ DX_DEVICE float capped(float x, float cap) {
   const float y = x * (1.f / cap), z = y * y;
   const float n = __builtin_fmaf(z + 105.f, z, 945.f), m = __builtin_fmaf(z + 28.f, z, 63.f);
   const float far = cap * copysignf(1.f - 2.f * fast_rcp(1.f + fast_exp2(2.f * LOG2E * fabsf(y))), x);
-  return x == -INFINITY ? x : fabsf(y) > 0.9f ? far : x * (1.f / 15.f) * n * fast_rcp(m);
+  return x == -INFINITY ? x : fabsf(y) > 0.9f ? far : x * ((1.f / 15.f) * n * fast_rcp(m));
 }
 
 template <bool B>

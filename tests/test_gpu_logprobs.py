@@ -201,3 +201,28 @@ def test_chunks_masked_with_the_lowest_value(dtype: str) -> None:
     got = K.token_logprobs(logits, i32(targets), top=6)
     torch.cuda.synchronize()
     check(host, targets, 6, 0.0, got, float(np.abs(host[host > lowest]).max(where=np.isfinite(host[host > lowest]), initial=1.0)))
+
+
+@pytest.mark.parametrize("cap", [1e37, 1e38, 3e38])
+def test_logits_near_a_cap_near_the_largest_number(cap: float) -> None:
+    """Logits of up to such a cap beside ordinary ones: t is at most the cap, a number, whatever its factors are. Ordinary
+    logits weigh nothing beside those."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"token_logprobs of huge logits, cap={cap}")
+    x = (rng(8).normal(size=(4, 3000)) * 4).astype(np.float32)
+    for i, y in enumerate((0.3, 0.6, 0.85, 1.0)):
+        x[i, 2500] = np.float32(cap * y)
+    x[1, :2000] = -np.inf
+    x[2, 7] = x[2, 2500]
+    low = x.copy()
+    low[:, :2000] = -np.float32(cap)  # weighs nothing either
+    # one logit far above all others, or (row 2 of x) two equal ones: a few roundings of 1
+    for logits, targets, want in ((x, [2500, 2500, 7, 2500], [0.0, 0.0, -np.log(2), 0.0]), (low, [2500] * 4, [0.0] * 4)):
+        lp, ent, ids, tops = (t.cpu().numpy().astype(np.float64) for t in
+                              K.token_logprobs(torch.from_numpy(logits).cuda(), i32(targets), top=1, softcap=cap))
+        for got in (lp, -ent, tops[:, 0]):
+            assert (np.abs(got - want) <= 16 * U).all(), (cap, got, want)
+        assert ids[:, 0].tolist() == targets
