@@ -1,17 +1,20 @@
 // Log probabilities of given tokens, entropy and the best alternatives, from rows of logits.
 //
-// t = x, or cap tanh(x / cap) with a soft-cap (-inf stays -inf: no alternative); with M >= max t,
-//   S = sum e^{t - M}, E = sum (t - M) e^{t - M}:   log p_j = (t_j - M) - log S,   H = log S - E / S.
+// t = x, or cap tanh(x / cap) with a soft-cap (-inf stays -inf: no alternative); with M = max t,
+//   S = sum e^{t - M} = 1 + R, E = sum (t - M) e^{t - M}:   log p_j = (t_j - M) - log(1 + R), H = log(1 + R) - E / (1 + R).
+// R, the weights beside the largest one's own, is kept instead of S: where one token is all but certain, its log probability
+// and the entropy are as small as R, which 1 + R has lost. All terms have one sign, so log p <= 0 and H >= 0.
+// With a cap of up to 40, t = cap - 2 cap r with r = 1 / (1 + e^{2x / cap}), and t - M = 2 cap (r_M - r): off by a few
+// roundings of the cap. Beyond, t by `capped`, off by a few of itself.
 // The logits are read once. Two launches:
-//   parts_kernel: a wave takes 2048 neighbouring logits of a row in registers, its M (with a cap of up to 40, where e^{-2
-//     cap} is well above the smallest numbers, the cap itself: t - cap = -2 cap / (1 + e^{2x / cap}); else its largest t),
-//     S and E, and the largest logit of each 32 neighbours.
+//   parts_kernel: a wave takes 2048 neighbouring logits of a row in registers, its M, R and E, and the largest logit of each
+//     32 neighbours.
 //   row_kernel: one workgroup a row joins the parts in their order and finds the alternatives from those largest ones: the
 //     k-th largest of the threads' largest bounds the k best from below, so only the groups that reach it (a few more than
 //     k) are looked at again, each wave keeping a sorted list of its best, one a lane.
 // Chunks follow from the vocabulary alone, so a row's result does not depend on the others.
-// Bound: 1500 rows of 256000 bf16 logits, soft-capped: parts 200 us (3.9 TB/s; two exponentials and a reciprocal a logit
-// keep the vector units as busy as the memory), rows 22 us. One row: 4.3 and 7.6 us, loads that wait for each other.
+// Bound: 1500 rows of 256000 bf16 logits, soft-capped: parts 215 us (3.6 TB/s; two exponentials and a reciprocal a logit
+// keep the vector units as busy as the memory), rows 23 us. One row: 4.6 and 8.2 us, loads that wait for each other.
 #include "common.h"
 #include "kernels.h"
 
@@ -29,22 +32,61 @@ DX_DEVICE uint32_t order(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-DX_DEVICE bool by_cap(float cap) { return cap > 0.f && cap <= 40.f; }  // whether M is the cap
+DX_DEVICE bool by_cap(float cap) { return cap > 0.f && cap <= 40.f; }  // whether t is taken by its distance to the cap
 
 // cap tanh(x / cap), -inf staying -inf, to a few roundings of itself: with y = x / cap the continued fraction of tanh cut
 // after y^9, y (y^4 + 105 y^2 + 945) / (15 (y^4 + 28 y^2 + 63)), off by 2.4e-8 of the value at |y| <= 0.9, and the
-// exponential's form beyond.
+// exponential's form beyond. One value for one x wherever it is computed: the difference of a row's largest logit to
+// itself is 0 in both kernels, so no product here may join a later difference.
 DX_DEVICE float capped(float x, float cap) {
+#pragma clang fp contract(off)
   const float y = x * (1.f / cap), z = y * y;
   const float n = __builtin_fmaf(z + 105.f, z, 945.f), m = __builtin_fmaf(z + 28.f, z, 63.f);
   const float far = cap * copysignf(1.f - 2.f * fast_rcp(1.f + fast_exp2(2.f * LOG2E * fabsf(y))), x);
   return x == -INFINITY ? x : fabsf(y) > 0.9f ? far : x * ((1.f / 15.f) * n * fast_rcp(m));
 }
 
-template <bool B>
-struct Flag {
-  static constexpr bool value = B;
+// Where a logit stands: t = constant + unit level, whose differences are as accurate as said above. -inf for -inf.
+DX_DEVICE float unit_of(float cap) { return by_cap(cap) ? 2.f * cap : 1.f; }
+DX_DEVICE float fall(float x, float c1) { return fast_rcp(1.f + fast_exp2(c1 * x)); }  // r, with c1 = 2 log2(e) / cap
+DX_DEVICE float level(float x, float cap) {
+  if (cap == 0.f || x == -INFINITY) return x;
+  return by_cap(cap) ? -fall(x, 2.f * LOG2E / cap) : capped(x, cap);
+}
+
+// A difference of levels, bounded below so that a weight of 0 times it is 0; NaN stays.
+DX_DEVICE float below(float v, float top) {
+  const float d = v - top;
+  return d < -1e30f ? -1e30f : d;
+}
+
+template <int N>
+struct Number {
+  static constexpr int value = N;
 };
+
+// Reductions over a wave in registers, all lanes the same result: pairs, quads, eights and rows of 16 by DPP, then rows and
+// halves exchanged. The largest logit is needed before the sums start: with shuffles through LDS 1500 x 256000 in bf16 take
+// 225 us instead of 215, one row 13.6 instead of 12.8.
+template <typename F>
+DX_DEVICE float over_wave(float x, F f) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  auto moved = [&](auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  x = f(x, moved(Number<0xb1>{}));   // quad_perm 1 0 3 2
+  x = f(x, moved(Number<0x4e>{}));   // quad_perm 2 3 0 1
+  x = f(x, moved(Number<0x141>{}));  // row_half_mirror
+  x = f(x, moved(Number<0x140>{}));  // row_mirror
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+#endif
+  return x;
+}
+DX_DEVICE float max_of_wave(float x) { return over_wave(x, [](float a, float b) { return fmaxf(a, b); }); }
+DX_DEVICE float sum_of_wave(float x) { return over_wave(x, [](float a, float b) { return a + b; }); }
 
 DX_DEVICE float to_float(uint16_t x) { return bf2f(x); }
 DX_DEVICE float to_float(float x) { return x; }
@@ -102,60 +144,63 @@ parts_kernel(const T *__restrict__ logits, int vocab, long ld, float cap, int ch
       if (lane % QUAD == 0 && g < groups) largest[row * groups + g] = mine[j];
     }
   }
-  float shift = cap, s = 0.f, e = 0.f;
+  float s = 0.f, e = 0.f;
+  top = max_of_wave(top);
+  if (cap > 0.f) top = level(top, cap);
+  const float base = top == -INFINITY ? 0.f : top, unit = unit_of(cap) * LOG2E;
   if (by_cap(cap)) {
-    // 1.5 of some 19 vector instructions' time a logit (three are transcendental, four each), 1500 x 256000 in bf16: a
-    // chunk without -inf, most are, does not look for it again
-    const float c1 = 2.f * LOG2E / cap, c2 = -2.f * LOG2E * cap;
+    // u = unit (r_M - r) in one instruction, the rounding of its constant taken out of the sums afterwards
+    const float c1 = 2.f * LOG2E / cap, shift = -unit * base, off = __builtin_fmaf(unit, base, shift);
+    // most chunks have no -inf, and do not look for it again
     auto add = [&](auto banned) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float u = c2 * fast_rcp(1.f + fast_exp2(c1 * x[j][i]));
+          const float u = __builtin_fmaf(-unit, fall(x[j][i], c1), shift);
           float w = fast_exp2(u);
           if constexpr (decltype(banned)::value) w = x[j][i] == -INFINITY ? 0.f : w;
           s += w;
           e = __builtin_fmaf(w, u, e);
         }
     };
-    if (__any(low == -INFINITY)) add(Flag<true>{});
-    else add(Flag<false>{});
+    if (__any(low == -INFINITY)) add(Number<1>{});
+    else add(Number<0>{});
+    const float f = fast_exp2(-off);
+    e = (e - off * s) * f;
+    s *= f;
   } else {
-    if (cap > 0.f) {
-      top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[j][i] = capped(x[j][i], cap);
-          top = fmaxf(top, x[j][i]);
-        }
-    }
-    shift = wave_max(top);
-    const float base = shift == -INFINITY ? 0.f : shift;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float u = fmaxf(x[j][i] - base, -1e30f) * LOG2E;
-        const float w = fast_exp2(u);
+        if (cap > 0.f) x[j][i] = capped(x[j][i], cap);
+        const float u = below(x[j][i], base) * LOG2E, w = fast_exp2(u);
         s += w;
         e = __builtin_fmaf(w, u, e);
       }
-    // fmaxf passes over a NaN: keep it (and inf - inf)
+  }
+  s = sum_of_wave(s);
+  e = sum_of_wave(e);
+  float rest = top == -INFINITY ? s : s - 1.f;  // no logit at all: 0, or NaN
+  if (s < 1.0625f && top != -INFINITY) {        // the sums' roundings are too much of these: all but the largest again
+    rest = e = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) s = x[j][i] != x[j][i] ? NAN : s;
-    if (base == INFINITY) s = NAN;
+      for (int i = 0; i < V; ++i) {
+        const float u = below(by_cap(cap) ? level(x[j][i], cap) : x[j][i], base) * unit;
+        const float w = u < 0.f ? fast_exp2(u) : 0.f;
+        rest += w;
+        e = __builtin_fmaf(w, u, e);
+      }
+    rest = sum_of_wave(rest);
+    e = sum_of_wave(e);
   }
-  s = wave_sum(s);
-  e = wave_sum(e);
   if (lane == 0) {
     float *out = parts + (row * chunks + chunk) * 3;
-    out[0] = shift;
-    out[1] = s;
+    out[0] = top;
+    out[1] = rest;
     out[2] = e;  // in base 2
   }
 }
@@ -163,30 +208,22 @@ parts_kernel(const T *__restrict__ logits, int vocab, long ld, float cap, int ch
 // The logit that order() made.
 DX_DEVICE float logit_of(uint32_t v) { return __uint_as_float(v & 0x80000000u ? v & 0x7fffffffu : ~v); }
 
-// t - shift of a logit, as accurate as parts_kernel's sum is.
-DX_DEVICE float shifted(float x, float cap, float shift) {
-  if (x == -INFINITY) return -INFINITY;
-  if (by_cap(cap)) return -2.f * cap / (1.f + expf(2.f * x / cap));
-  return (cap > 0.f ? capped(x, cap) : x) - shift;
-}
-
 constexpr int ROW_WAVES = 8, ROW_THREADS = 64 * ROW_WAVES;
 constexpr int HELD = 16;  // groups that a thread keeps in registers: all of them up to a vocabulary of 262144
 
-// The workgroup's sums of a and of b, in the waves' order.
-DX_DEVICE void block_sums(float &a, float &b, float (&red)[2][ROW_WAVES]) {
-  a = wave_sum(a);
-  b = wave_sum(b);
-  if ((threadIdx.x & 63) == 0) {
-    red[0][threadIdx.x >> 6] = a;
-    red[1][threadIdx.x >> 6] = b;
+// The workgroup's sums of three numbers a thread, in the waves' order.
+DX_DEVICE void block_sums(float (&x)[3], float (&red)[3][ROW_WAVES]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    x[i] = sum_of_wave(x[i]);
+    if ((threadIdx.x & 63) == 0) red[i][threadIdx.x >> 6] = x[i];
   }
   __syncthreads();
-  a = b = 0.f;
 #pragma unroll
-  for (int w = 0; w < ROW_WAVES; ++w) {
-    a += red[0][w];
-    b += red[1][w];
+  for (int i = 0; i < 3; ++i) {
+    x[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < ROW_WAVES; ++w) x[i] += red[i][w];
   }
 }
 
@@ -216,7 +253,7 @@ row_kernel(const T *__restrict__ logits, const int32_t *__restrict__ targets, in
            int chunks, int groups, const float *__restrict__ parts, const float *__restrict__ largest,
            float *__restrict__ logprobs, float *__restrict__ entropy, int32_t *__restrict__ ids,
            float *__restrict__ top_logprobs) {
-  __shared__ float red[2][ROW_WAVES], reds[ROW_WAVES];
+  __shared__ float red[3][ROW_WAVES], reds[ROW_WAVES];
   __shared__ uint32_t lane_best[ROW_THREADS];
   __shared__ uint64_t reach[ROW_WAVES][HELD];
   __shared__ uint64_t best[ROW_WAVES][MOST_TOP];
@@ -255,39 +292,41 @@ row_kernel(const T *__restrict__ logits, const int32_t *__restrict__ targets, in
     }
     lane_best[tid] = mine;
   }
-  // join: every thread the same largest shift, then sums in the threads' order
-  float shift = cap;
-  if (!by_cap(cap)) {
-    float m = first[0];
-    for (int i = tid + ROW_THREADS; i < chunks; i += ROW_THREADS) m = fmaxf(m, part[i * 3]);
-    m = wave_max(m);
-    if (lane == 0) reds[wave] = m;
-    __syncthreads();
-    shift = reds[0];
+  // join: every thread the same highest level, then sums in the threads' order
+  float most = first[0];
+  for (int i = tid + ROW_THREADS; i < chunks; i += ROW_THREADS) most = fmaxf(most, part[i * 3]);
+  most = max_of_wave(most);
+  if (lane == 0) reds[wave] = most;
+  __syncthreads();
+  most = reds[0];
 #pragma unroll
-    for (int w = 1; w < ROW_WAVES; ++w) shift = fmaxf(shift, reds[w]);
-  }
-  float s = 0.f, e = 0.f;
-  auto add = [&](float top_i, float s_i, float e_i) {
-    // a part of masked logits may lie as far below as numbers go: the same bound as a logit's there
-    const float d = top_i == -INFINITY ? 0.f : top_i - shift < -1e30f ? -1e30f : (top_i - shift) * LOG2E;
-    const float f = fast_exp2(d), si = s_i * f;
-    s += si;
-    e += e_i * f + si * d;
+  for (int w = 1; w < ROW_WAVES; ++w) most = fmaxf(most, reds[w]);
+  const float unit = unit_of(cap);
+  float sums[3] = {0.f, 0.f, 0.f};  // of R, of E, and of the parts that hold the largest t: one 1 of theirs is 1 + R's
+  auto add = [&](float top_i, float rest_i, float e_i) {
+    if (top_i == -INFINITY) {
+      sums[0] += rest_i;  // 0, or NaN
+      return;
+    }
+    // a part of masked logits may lie as far below as numbers go
+    const bool holds = top_i == most;
+    const float d = below(top_i, most) * unit * LOG2E, f = fast_exp2(d);
+    sums[0] += holds ? rest_i : (1.f + rest_i) * f;
+    sums[1] += f * (e_i + (1.f + rest_i) * d);
+    sums[2] += holds ? 1.f : 0.f;
   };
   add(first[0], first[1], first[2]);
   for (int i = tid + ROW_THREADS; i < chunks; i += ROW_THREADS) add(part[i * 3], part[i * 3 + 1], part[i * 3 + 2]);
-  block_sums(s, e, red);
-  e *= LN2;
+  block_sums(sums, red);
   // no finite logit at all: no token has any probability
-  const bool empty = s == 0.f, lost = s != s;
-  const float log_s = logf(s);
+  const bool empty = most == -INFINITY && sums[0] == 0.f, lost = sums[0] != sums[0];
+  const float rest = sums[0] + (sums[2] - 1.f), log_s = log1pf(rest), e = sums[1] * LN2;
   if (tid == 0) {
     float lp = 0.f;
     if (target < -1 || target >= vocab) lp = NAN;
-    else if (target >= 0) lp = empty ? -INFINITY : shifted(target_logit, cap, shift) - log_s;
+    else if (target >= 0) lp = empty ? -INFINITY : (level(target_logit, cap) - most) * unit - log_s;
     logprobs[row] = lost && target != -1 ? NAN : lp;
-    entropy[row] = lost ? NAN : empty ? 0.f : log_s - e / s;
+    entropy[row] = lost ? NAN : empty ? 0.f : log_s - e / (1.f + rest);
   }
   if (top == 0) return;
   int32_t *out = ids + row * top;
@@ -369,7 +408,7 @@ row_kernel(const T *__restrict__ logits, const int32_t *__restrict__ targets, in
     const int token = (int)~(uint32_t)list;
     const bool none = list == 0 || (uint32_t)(list >> 32) <= order(-INFINITY);
     out[lane] = none ? -1 : token;
-    out_lp[lane] = none ? -INFINITY : shifted(logit_of((uint32_t)(list >> 32)), cap, shift) - log_s;
+    out_lp[lane] = none ? -INFINITY : (level(logit_of((uint32_t)(list >> 32)), cap) - most) * unit - log_s;
   }
 }
 

@@ -226,3 +226,39 @@ def test_logits_near_a_cap_near_the_largest_number(cap: float) -> None:
         for got in (lp, -ent, tops[:, 0]):
             assert (np.abs(got - want) <= 16 * U).all(), (cap, got, want)
         assert ids[:, 0].tolist() == targets
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cap,vocab", [(0.0, 3000), (30.0, 3000), (30.0, 50257), (40.0, 3000), (50.0, 3000), (30.0, 90)])
+def test_tokens_of_a_probability_near_one(cap: float, vocab: int, dtype: str) -> None:
+    """One logit far above the others: its log probability is -log(1 + R), R the others' weights beside its own, and keeps
+    the precision of R, however small. With s the larger of the capped logits, each weight's exponent is off by 2 * 8 u s
+    (see above) and 3 u times its size of at most 2 s, itself by 2 u, their sum by 96 u, the logarithm by 2: 22 s + 100
+    roundings relative to R, below the bound of `check` relative to the value. The entropy, log(1 + R) - E / (1 + R) with
+    both terms positive, takes the exponents' error once more. No log probability is above 0 and no entropy below."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"token_logprobs of near certain tokens vocab={vocab} cap={cap} {dtype}")
+    r = rng(vocab)
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    sizes = np.array([22.0, 23.0, 26.0, 30.0, 40.0, 55.0, 70.0, 130.0])
+    x = r.normal(size=(len(sizes), vocab)).astype(np.float32)
+    targets = r.integers(0, vocab, len(sizes))
+    x[np.arange(len(sizes)), targets] = sizes
+    logits = torch.from_numpy(x).cuda().to(t)
+    host = logits.float().cpu().numpy()
+    lp, ent, ids, tops = (g.cpu().numpy().astype(np.float64) for g in K.token_logprobs(logits, i32(targets), top=2, softcap=cap))
+    for i in range(len(sizes)):
+        row = host[i].astype(np.float64)
+        c = cap * np.tanh(row / cap) if cap else row
+        d = np.delete(c, targets[i]) - c[targets[i]]
+        others = np.exp(d).sum()  # by themselves: of 1 + R, 64 bits too lose what is below 1e-16
+        want, want_ent = -np.log1p(others), np.log1p(others) - (np.exp(d) * d).sum() / (1 + others)
+        assert want > -1e-3
+        tol = 2 * (12 * min(cap or 1e9, sizes[i]) + 96 + 8) * U
+        assert lp[i] <= 0 and ent[i] >= 0, (i, lp[i], ent[i])
+        assert abs(lp[i] - want) <= tol * abs(want) + 1e-37, (i, lp[i], want)
+        assert abs(ent[i] - want_ent) <= 2 * tol * want_ent + 1e-36, (i, ent[i], want_ent)
+        assert tops[i, 0] == lp[i] and ids[i].tolist() == oracle.token_logprobs(host[i], int(targets[i]), 2, cap)[2].tolist()
