@@ -431,13 +431,21 @@ hipError_t dx_token_logprobs_launch(const void *logits, const int32_t *targets, 
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (f32)
-    row_kernel<<<dim3((unsigned)rows), dim3(ROW_THREADS), 0, s>>>(static_cast<const float *>(logits), targets, vocab, ld,
-                                                              cap, top, chunks, ngroups, parts, groups, logprobs,
-                                                              entropy, ids, top_logprobs);
-  else
-    row_kernel<<<dim3((unsigned)rows), dim3(ROW_THREADS), 0, s>>>(static_cast<const uint16_t *>(logits), targets, vocab, ld,
-                                                              cap, top, chunks, ngroups, parts, groups, logprobs,
-                                                              entropy, ids, top_logprobs);
-  return hipGetLastError();
+  // a launch's threads are counted in 32 bits
+  constexpr long MOST_ROWS = (1L << 32) / ROW_THREADS / 2;
+  for (long r0 = 0; r0 < rows; r0 += MOST_ROWS) {
+    const dim3 grid((unsigned)min(rows - r0, MOST_ROWS)), block(ROW_THREADS);
+    const float *pr = parts + r0 * chunks * 3, *gr = groups + (top > 0 ? r0 * ngroups : 0);
+    int32_t *id = top > 0 ? ids + r0 * top : nullptr;
+    float *tl = top > 0 ? top_logprobs + r0 * top : nullptr;
+    if (f32)
+      row_kernel<<<grid, block, 0, s>>>(static_cast<const float *>(logits) + r0 * ld, targets + r0, vocab, ld, cap, top, chunks,
+                                        ngroups, pr, gr, logprobs + r0, entropy + r0, id, tl);
+    else
+      row_kernel<<<grid, block, 0, s>>>(static_cast<const uint16_t *>(logits) + r0 * ld, targets + r0, vocab, ld, cap, top,
+                                        chunks, ngroups, pr, gr, logprobs + r0, entropy + r0, id, tl);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }

@@ -262,3 +262,25 @@ def test_tokens_of_a_probability_near_one(cap: float, vocab: int, dtype: str) ->
         assert abs(lp[i] - want) <= tol * abs(want) + 1e-37, (i, lp[i], want)
         assert abs(ent[i] - want_ent) <= 2 * tol * want_ent + 1e-36, (i, ent[i], want_ent)
         assert tops[i, 0] == lp[i] and ids[i].tolist() == oracle.token_logprobs(host[i], int(targets[i]), 2, cap)[2].tolist()
+
+
+def test_more_rows_than_one_launch_holds() -> None:
+    """2^23 workgroups of 512 threads are as many threads as 32 bits count. Two logits a row: log p = -log(1 + e^d) with
+    d = x_other - x_target exact in fp32 (both are bf16 near each other): a few roundings of it."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    rows = (1 << 23) + 77
+    say(f"token_logprobs {rows} rows")
+    x = torch.randn((rows, 2), device="cuda", dtype=torch.bfloat16)
+    targets = torch.arange(rows, device="cuda", dtype=torch.int32) % 3 - 1
+    lp, ent, ids, tops = K.token_logprobs(x, targets, top=1)
+    torch.cuda.synchronize()
+    want = torch.log_softmax(x.double(), 1)
+    at = want.gather(1, targets.clamp(min=0).long()[:, None])[:, 0]
+    at = torch.where(targets < 0, 0.0, at)
+    assert ((lp - at).abs() <= 16 * U * (1 + at.abs())).all()
+    assert ((ent + (want.exp() * want).sum(1)).abs() <= 16 * U * 2).all()
+    assert (ids[:, 0] == (x[:, 1] > x[:, 0]).int()).all()
+    assert ((tops[:, 0] - want.amax(1)).abs() <= 16 * U).all()
