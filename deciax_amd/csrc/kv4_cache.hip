@@ -144,35 +144,49 @@ DX_DEVICE uint32_t order(float w) {
 // The slots one (sequence, kv head) keeps, ascending, into list[0, kept). One workgroup; thread t holds slots
 // i 1024 + t. The kept-th largest key is found bit by bit from the top: a round counts the keys at or above a
 // candidate with one compare an item and the wave's population counts, no memory but one number a wave. ITEMS = 0
-// reads the weights again every round, for spans beyond the registers.
+// reads the weights again every round, for spans beyond the registers. A slot without a page has the key of no slot.
 // Bound: the 32 rounds, one after the other, of one workgroup: 9.8 us for 2900 slots, 31 us for up to 16384.
 template <int ITEMS>
 __global__ void __launch_bounds__(SEL_THREADS)
-select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const int32_t *__restrict__ ctx_len,
-              int max_ctx, int keep, int recent, int32_t *__restrict__ list, int32_t *__restrict__ out_len) {
+select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const int32_t *__restrict__ table, int width,
+              int pages, int shift, const int32_t *__restrict__ ctx_len, int max_ctx, int keep, int recent,
+              int32_t *__restrict__ list, int32_t *__restrict__ out_len) {
   __shared__ int counts[2][SEL_WAVES];
   __shared__ uint32_t spread[ITEMS ? ITEMS : 16][SEL_WAVES];
   const int g = blockIdx.x, b = blockIdx.y, hkv = gridDim.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ctx = min(max(ctx_len[b], 0), max_ctx), kept = min(ctx, keep);
-  if (g == 0 && tid == 0) out_len[b] = kept;
+  const int ctx = min(max(ctx_len[b], 0), max_ctx);
   int32_t *mine = list + ((long)b * hkv + g) * keep;
-  if (kept == ctx) {
-    for (int i = tid; i < kept; i += SEL_THREADS) mine[i] = i;
-    return;
-  }
   const float *w = weights + b * w_seq + g * w_head;
+  const int32_t *page_of = table + (long)b * width;
+  auto no_page = [&](int page) { return page < 0 || page >= pages; };
+  int gone = 0;  // whether some slot has no page
   const int guard = ctx - recent;  // slots from here on are kept
   const int rounds = (ctx + SEL_THREADS - 1) / SEL_THREADS;
   auto fetch = [&](int i) -> uint32_t {  // 0: no slot; order() of a number is never 0
-    const int slot = i * SEL_THREADS + tid;
-    const uint32_t x = max(order(w[min(slot, ctx - 1)]), 1u);  // no branch: a thread's loads are on their way at once
+    const int slot = i * SEL_THREADS + tid, at = min(slot, ctx - 1);
+    const uint32_t x = max(order(w[at]), 1u);  // no branch: a thread's loads are on their way at once
     return slot >= ctx ? 0u : slot >= guard ? PROTECTED : x;
   };
+  auto fetch_there = [&](int i) -> uint32_t {
+    const uint32_t x = fetch(i);
+    return gone && no_page(page_of[min(i * SEL_THREADS + tid, ctx - 1) >> shift]) ? 0u : x;
+  };
   uint32_t key[ITEMS ? ITEMS : 1];
+  if (ctx == 0) {
+    if (g == 0 && tid == 0) out_len[b] = 0;
+    return;
+  }
   if constexpr (ITEMS > 0) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) key[i] = fetch(i);
+  }
+  for (int p = tid; p << shift < ctx; p += SEL_THREADS) gone |= no_page(page_of[p]);
+  gone = __syncthreads_or(gone);
+  if (!gone && ctx <= keep) {
+    if (g == 0 && tid == 0) out_len[b] = ctx;
+    for (int i = tid; i < ctx; i += SEL_THREADS) mine[i] = i;
+    return;
   }
   // waves' numbers to every wave; `turn` alternates, so one barrier a sum is enough
   auto total = [&](int c, int turn) {
@@ -183,32 +197,50 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
     for (int j = 0; j < SEL_WAVES; ++j) sum += counts[turn][j];
     return sum;
   };
-  uint32_t least = 0;  // the kept-th largest key
-  int above = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  int present = ctx;
+  if (gone) {
+    int c = 0;
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int at = min(i * SEL_THREADS + tid, ctx - 1);
+        key[i] = no_page(page_of[at >> shift]) ? 0u : key[i];
+        c += __popcll(__ballot(key[i] != 0));
+      }
+    } else {
+      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch_there(i) != 0));
+    }
+    present = total(c, 0);
+  }
+  const int kept = min(present, keep);
+  if (g == 0 && tid == 0) out_len[b] = kept;
+  uint32_t least = 0;  // the kept-th largest key, or that of no slot where all are kept
+  bool found = present == kept;
+  int above = found ? kept : 0;
+  for (int bit = 31; bit >= 0 && !found; --bit) {
     const uint32_t cand = least | (1u << bit);
     int c = 0;
     if constexpr (ITEMS > 0) {
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) c += __popcll(__ballot(key[i] >= cand));
     } else {
-      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch(i) >= cand));
+      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch_there(i) >= cand));
     }
     c = total(c, bit & 1);
     if (c >= kept) least = cand;
     if (c == kept) {  // these are they
       least = cand - 1;
       above = kept;
-      break;
+      found = true;
     }
   }
-  if (above == 0) {
+  if (!found) {
     int c = 0;
     if constexpr (ITEMS > 0) {
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) c += __popcll(__ballot(key[i] > least));
     } else {
-      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch(i) > least));
+      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch_there(i) > least));
     }
     above = total(c, 1);
   }
@@ -223,7 +255,7 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
 #pragma unroll
     for (int i = 0; i < SPREAD; ++i) {
       if constexpr (ITEMS > 0) k[i] = key[i];
-      else k[i] = fetch(i0 + i);
+      else k[i] = fetch_there(i0 + i);
       const uint64_t eq = __ballot(k[i] == least && k[i] != 0), gt = __ballot(k[i] > least);
       if (lane == 0) spread[i][wave] = (uint32_t)__popcll(gt) << 16 | (uint32_t)__popcll(eq);
     }
@@ -257,13 +289,13 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
 template <int D>
 __global__ void __launch_bounds__(THREADS)
 move_kernel(Kv4Cache c, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ out_table,
-            int out_width, const int32_t *__restrict__ ctx_len, int max_ctx, int keep,
-            const int32_t *__restrict__ list, const float *__restrict__ weights, long w_seq, long w_head,
-            float *__restrict__ out_weights, long o_seq, long o_head) {
+            int out_width, const int32_t *__restrict__ out_len, int keep, const int32_t *__restrict__ list,
+            const float *__restrict__ weights, long w_seq, long w_head, float *__restrict__ out_weights, long o_seq,
+            long o_head) {
   constexpr int CHUNKS = D / 32, LANES = 2 * CHUNKS;  // 16-byte chunks of K's row, then of V's
   constexpr int ROWS = THREADS / LANES, ITER = 4;
   const int g = blockIdx.y, b = blockIdx.z;
-  const int kept = min(min(max(ctx_len[b], 0), max_ctx), keep);
+  const int kept = out_len[b];
   const int32_t *from = table + (long)b * width, *to = out_table + (long)b * out_width;
   const int32_t *mine = list + ((long)b * c.hkv + g) * keep;
   const int l = threadIdx.x % LANES, chunk = l % CHUNKS;
@@ -359,7 +391,8 @@ hipError_t dx_kv4_evict_launch(const Kv4Cache &c, const int32_t *table, int widt
 // By the slots that a thread holds. us of an eviction to 1000: 2900 slots 20.5 with 4 a thread and 32.7 with 16, 14000
 // 44 with 16 and 93 with 64, 60000 101 with 64 and 327 when read again every round.
 #define SELECT(N) \
-  select_kernel<N><<<grid, block, 0, s>>>(weights, w_seq, w_head, ctx_len, max_ctx, keep, recent, list, out_len)
+  select_kernel<N><<<grid, block, 0, s>>>(weights, w_seq, w_head, table, width, c.pages, c.shift, ctx_len, max_ctx,      \
+                                          keep, recent, list, out_len)
   if (rounds <= 4) SELECT(4);
   else if (rounds <= 16) SELECT(16);
   else if (rounds <= 64) SELECT(64);
@@ -369,7 +402,7 @@ hipError_t dx_kv4_evict_launch(const Kv4Cache &c, const int32_t *table, int widt
   if (e != hipSuccess) return e;
 #define MOVE(D)                                                                                                     \
   move_kernel<D><<<dim3((keep + 4 * (THREADS * 16 / (D)) - 1) / (4 * (THREADS * 16 / (D))), c.hkv, num_seqs),       \
-                   dim3(THREADS), 0, s>>>(c, table, width, out_table, out_width, ctx_len, max_ctx, keep, list,      \
+                   dim3(THREADS), 0, s>>>(c, table, width, out_table, out_width, out_len, keep, list,               \
                                           weights, w_seq, w_head, out_weights, o_seq, o_head)
   if (c.d == 64) MOVE(64);
   else if (c.d == 128) MOVE(128);

@@ -861,9 +861,9 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor, page_table: torch.Tensor, 
               out_table: torch.Tensor, *, keep: int, recent: int = 0,
               weights_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Cut every sequence to `keep` slots, in pages of the same cache listed by `out_table` that no page table of the
-    call shares: each KV head keeps its last `recent` slots and the heaviest others by `weights`, in slot order (see
-    dx_kv4_evict). Returns the kept slots' weights [sequences, Hkv, keep] (zeros behind them) and the new lengths; the
-    old pages stay as they are."""
+    call shares: each KV head keeps its last `recent` slots and the heaviest others by `weights`, in slot order, but none
+    whose page is outside the pool (see dx_kv4_evict). Returns the kept slots' weights [sequences, Hkv, keep] (zeros
+    behind them) and the new lengths; the old pages stay as they are."""
     seqs = _kv4_ints("kv4_evict", cache, page_table, ctx_len)
     _kv4_ints("kv4_evict", cache, out_table, ctx_len)
     index, heads, dev = cache.index, cache.heads, cache.k.device

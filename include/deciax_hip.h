@@ -579,10 +579,11 @@ int64_t dx_attn_kv4_workspace(int32_t num_seqs, int32_t max_seq_len,
  * page_table: the old pages stay as they are, for sequences that share them). A
  * KV head keeps the last `recent` slots and, of the others, the heaviest by
  * `weights`, the lower slot first where weights are equal (a NaN is above all);
- * what is kept stays in slot order, with its position. weights_out[b, g, 0..keep)
- * gets the kept slots' weights and zeros behind them, out_len[b] = min(ctx_len,
- * keep). 0 <= recent <= keep, 1 <= keep. No counterpart in the reference.
- * Workspace size from dx_kv4_evict_workspace. */
+ * what is kept stays in slot order, with its position. Slots below ctx_len whose
+ * page is outside the pool are not kept. weights_out[b, g, 0..keep) gets the kept
+ * slots' weights and zeros behind them, out_len[b] = min(slots with a page, keep).
+ * 0 <= recent <= keep, 1 <= keep. No counterpart in the reference. Workspace size
+ * from dx_kv4_evict_workspace. */
 int dx_kv4_evict(const dx_kv4_cache *cache, const float *weights,
                  int64_t weights_seq_stride, int64_t weights_head_stride,
                  const int32_t *page_table, int32_t table_width,

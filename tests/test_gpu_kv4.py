@@ -762,3 +762,58 @@ def test_prompts(prompt: int, dtype: str, softcap: float, window: int) -> None:
     c.check(out, w_out, w, **kw)
     for b, m in enumerate(ctx):
         assert (w_out[b, :, m:] == -7.0).all(), "slots behind the sequence were written"
+
+
+# ------------------------------------------------------------------------------------------ slots without a page
+
+
+@pytest.mark.parametrize("ctx,keep,recent,page,gone", [
+    ([1000, 300, 640, 100], 200, 64, 64, [(0, 3), (0, 14), (1, 0), (2, 8), (2, 9), (3, 1)]),  # old and recent slots
+    ([300, 100, 64], 250, 250, 64, [(0, 2), (0, 3), (1, 0), (2, 0)]),  # no more than `keep` are left; none are
+    ([20000], 4097, 100, 256, [(0, 7), (0, 78)]),
+    ([70001, 500], 60000, 500, 1024, [(0, 0), (0, 68), (1, 0)]),
+    ([40, 2000], 2000, 0, 64, [(1, 5)]),  # nothing is cut
+])
+def test_eviction_drops_slots_without_a_page(ctx: list[int], keep: int, recent: int, page: int, gone: list[tuple[int, int]]) -> None:
+    """Slots whose page is outside the pool are not seen before an eviction and do not come back by it: they are not kept,
+    however heavy or recent, where a used page would stand in for them."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    hkv, d = 2, 64
+    say(f"kv4_evict with missing pages ctx={ctx} keep={keep} recent={recent} page={page} gone={gone}")
+    per = -(-keep // page)
+    c = Case(keep + 1, [0] * len(ctx), [*ctx], hkv, hkv, d, page)
+    r = rng(keep)
+    extra = per * len(ctx)
+    big = K.kv4_cache(c.pages + extra, hkv, d, page_size=page)
+    for n in FIELDS:
+        getattr(big, n)[:c.pages] = getattr(c.cache, n)
+        getattr(big, n)[c.pages:] = 77  # what a used page holds
+    c.cache = big
+    out_table = c.pages + r.permutation(extra).reshape(len(ctx), per)
+    for i, (b, p) in enumerate(gone):
+        c.table[b, p] = (-1, c.pages + extra, -(1 << 31), (1 << 31) - 1)[i % 4]
+    w = np.exp(r.normal(size=(len(ctx), hkv, max(ctx)))).astype(np.float32)
+    for b, p in gone:
+        w[b, :, p * page:(p + 1) * page] += 100.0  # heavier than all others
+    w_out, length = K.kv4_evict(big, torch.from_numpy(w).cuda(), i32(c.table), c.d_ctx, max(ctx), i32(out_table), keep=keep,
+                                recent=recent)
+    torch.cuda.synchronize()
+    for b, m in enumerate(ctx):
+        slot = np.arange(m)
+        there = slot[~np.isin(slot // page, [p for s, p in gone if s == b])]
+        n = min(len(there), keep)
+        assert length[b].item() == n
+        for g in range(hkv):
+            slots = there[oracle.evict(w[b, g, there], keep, int((there >= m - recent).sum()))]
+            assert len(slots) == n
+            np.testing.assert_array_equal(w_out[b, g, :n].cpu().numpy(), w[b, g, slots])
+            assert (w_out[b, g, n:] == 0).all()
+            j = np.arange(per * page)
+            for name in FIELDS:
+                a = c.host(name)
+                new = a[out_table[b, j // page], g, j % page]
+                np.testing.assert_array_equal(new[:n], a[c.table[b, slots // page], g, slots % page])
+                assert (new[n:] == 77).all()
