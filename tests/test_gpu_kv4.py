@@ -817,3 +817,75 @@ def test_eviction_drops_slots_without_a_page(ctx: list[int], keep: int, recent: 
                 new = a[out_table[b, j // page], g, j % page]
                 np.testing.assert_array_equal(new[:n], a[c.table[b, slots // page], g, slots % page])
                 assert (new[n:] == 77).all()
+
+
+MISSING = [  # new, ctx, hq, hkv, d, pages that are not there: kept scores, few rows and many rows, spans that start or end in one
+    ([2, 1], [1500, 300], 4, 2, 128, [(0, 3), (0, 8), (0, 9), (0, 20), (1, 0), (1, 1)]),
+    ([20, 3], [1500, 64], 2, 1, 64, [(0, 0), (0, 11), (0, 22)]),
+    ([20], [1100], 1, 1, 256, [(0, 0), (0, 8), (0, 9), (0, 15)]),
+    ([150, 60], [1300, 200], 4, 2, 64, [(0, 1), (0, 10), (0, 17), (1, 0)]),
+    ([100], [700], 2, 1, 256, [(0, 0), (0, 4), (0, 8)]),
+    ([1200], [2000], 2, 1, 128, [(0, 0), (0, 7), (0, 11)]),
+]
+
+
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (50.0, 400)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("missing", range(len(MISSING)))
+def test_slots_without_a_page_are_not_seen(missing: int, dtype: str, softcap: float, window: int,
+                                           monkeypatch: pytest.MonkeyPatch) -> None:
+    """Outputs and weights are those of the slots that have a page; weights of the others stay. The pool's first rows, which
+    hold anything, NaN among it, never stand in for them. Without a window the newest tokens' last page is missing too."""
+    import torch
+
+    new, ctx, hq, hkv, d, gone = MISSING[missing]
+    if window == 0:
+        gone = [*gone, (0, (ctx[0] - 1) // 64)]
+    say(f"attention_kv4 with missing pages new={new} ctx={ctx} hq={hq} hkv={hkv} d={d} gone={gone} {dtype} window={window}")
+    c = Case(80 + missing, new, ctx, hq, hkv, d, 64, dtype)
+    c.fill(missing)
+    c.append()
+    table = c.table.copy()
+    for i, (b, p) in enumerate(gone):
+        table[b, p] = (-1, c.pages, (1 << 31) - 1, -(1 << 31))[i % 4]
+    c.d_table = i32(table)
+    w = np.abs(rng(missing).normal(size=(len(new), hkv, max(ctx)))).astype(np.float32)
+    w_in = torch.from_numpy(w.copy()).cuda()
+    w_out = torch.full_like(w_in, -7.0)
+    kw = dict(scale=d ** -0.5 * 2, softcap=softcap, window=window)
+    plain = c.attend(**kw)
+    out = c.attend(weights=w_in, weights_out=w_out, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(plain, out), "weights change no output"
+
+    sequences = iter(range(len(new)))
+
+    def seen_only(q, k, v, positions, *, scale, softcap, window):
+        b = next(sequences)
+        n, slot = len(q), np.arange(ctx[b])
+        there = ~np.isin(slot // 64, [p for s, p in gone if s == b])
+        o, mass, weights = np.zeros(q.shape), np.zeros(q.shape), np.zeros((hkv, ctx[b]))
+        for i in range(n):
+            own = ctx[b] - n + i
+            for h in range(hq):
+                g = h // (hq // hkv)
+                see = there & (slot <= own)
+                if window > 0:
+                    see &= (slot > own - window) & (positions[g] > positions[g][own] - window)
+                if not see.any():
+                    continue
+                t = k[g][see] @ q[i, h] * scale
+                t = softcap * np.tanh(t / softcap) if softcap else t
+                p = np.exp(t - t.max())
+                p /= p.sum()
+                o[i, h], mass[i, h] = p @ v[g][see], p @ np.abs(v[g][see])
+                weights[g][see] += p
+        return o, weights, mass
+
+    monkeypatch.setattr(oracle, "attention", seen_only)
+    c.check(out, w_out, w, **kw)
+    for b, m in enumerate(ctx):
+        assert (w_out[b, :, m:] == -7.0).all(), "slots behind the sequence were written"
+        for s, p in gone:
+            if s == b and (p + 1) * 64 <= m - new[b]:
+                assert torch.equal(w_out[b, :, p * 64:p * 64 + 64], w_in[b, :, p * 64:p * 64 + 64])
