@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 
 from oracle import kv4 as oracle
-from tests.conftest import i32, rng, say
+from tests.conftest import ROOT, i32, rng, say
 
 pytestmark = pytest.mark.gpu
 
@@ -889,3 +889,48 @@ def test_slots_without_a_page_are_not_seen(missing: int, dtype: str, softcap: fl
         for s, p in gone:
             if s == b and (p + 1) * 64 <= m - new[b]:
                 assert torch.equal(w_out[b, :, p * 64:p * 64 + 64], w_in[b, :, p * 64:p * 64 + 64])
+
+
+# the documents' examples of a kept state
+STEPS = [pytest.param(block[len("python\n"):], id=doc.stem) for doc in sorted(ROOT.glob("*.md"))
+         for block in doc.read_text().split("```") if block.startswith("python\n") and "kv4_evict(" in block]
+
+
+@pytest.mark.parametrize("steps", STEPS)
+def test_the_documented_steps_go_on_after_an_eviction(steps: str) -> None:
+    """The documents' own lines on states of two lengths, then a further token over what they leave: the slots that it sees,
+    their weights and their positions are those that were kept."""
+    import torch
+
+    say("kv4: documented steps")
+    hq, hkv, d, keep, lengths = 4, 2, 64, 100, [400, 130]
+    c = Case(50, lengths, [*lengths], hq, hkv, d)
+    new_table = c.pages + np.arange(6).reshape(2, 3)  # a page of room
+    x = torch.from_numpy(rng(1).normal(size=(c.rows, 128)).astype(np.float32)).cuda().bfloat16()
+    w_qkv = torch.from_numpy(rng(2).normal(size=((hq + 2 * hkv) * d, 128)).astype(np.float32) / 12).cuda().bfloat16()
+    angle = np.arange(500)[:, None] * 1e4 ** (-np.arange(d // 2) / (d // 2))
+    logits = torch.from_numpy(rng(3).normal(size=(5, 1000)).astype(np.float32)).cuda()
+    ns = dict(num_pages=c.pages + 6, num_q_heads=hq, num_kv_heads=hkv, head_dim=d, num_seqs=2, max_ctx_len=400, k=c.k, v=c.v,
+              q=c.q, positions=c.positions, page_table=c.d_table, seq_start=c.d_starts, seq_len=c.d_new, ctx_len=c.d_ctx,
+              max_seq_len=400, new_table=i32(new_table), keep=keep, recent=16, logits=logits, answers=i32([1, 2, 3, 4, 5]),
+              x=x, w_qkv=w_qkv, cos=torch.from_numpy(np.cos(angle)).cuda().bfloat16(),
+              sin=torch.from_numpy(np.sin(angle)).cuda().bfloat16(), kept_start=i32([0, keep]))
+    exec(steps, ns)
+    torch.cuda.synchronize()
+    assert ns["kept_len"].cpu().tolist() == [keep, keep]
+
+    # a further token
+    a = Case(51, [1, 1], [keep + 1, keep + 1], hq, hkv, d)
+    a.cache, a.table, a.d_table = ns["cache"], new_table, ns["page_table"]
+    a.positions = i32(lengths)
+    a.append()
+    before = ns["weights"].cpu().numpy().copy()
+    kw = dict(scale=1 / 16, softcap=50.0, window=200)
+    out = a.attend(weights=ns["weights"], **kw)
+    torch.cuda.synchronize()
+    a.check(out, ns["weights"], before, **kw)
+    assert (before[:, :, :keep] > 0).any() and (before[:, :, keep:] == 0).all()
+    for b, n in enumerate(lengths):
+        held = a.held_positions(b)
+        assert (held[:, keep] == n).all() and (np.diff(held, axis=1) > 0).all()
+        assert (held[:, keep - 16:keep] == np.arange(n - 16, n)).all()
