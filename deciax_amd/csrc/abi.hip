@@ -1,6 +1,7 @@
 // extern "C" entry points declared in include/deciax_hip.h: argument
 // validation, then dispatch to the kernel launchers. Nothing here allocates
 // or synchronises.
+#include <float.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -891,8 +892,8 @@ int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32
           "attn_kv4: num_q_heads %d must be a positive multiple of num_kv_heads %d", num_q_heads, a.c.hkv);
   REQUIRE(window >= 0, "attn_kv4: window must be >= 0, got %d", window);
   REQUIRE(softcap >= 0.f && softcap <= 1e30f && scale > 0.f && scale < INFINITY &&
-              (softcap == 0.f || scale / softcap < INFINITY),
-          "attn_kv4: need a finite scale > 0, softcap in [0, 1e30] and a finite scale / softcap");
+              (softcap == 0.f || (scale / softcap < INFINITY && scale / softcap >= FLT_MIN)),
+          "attn_kv4: need a finite scale > 0, softcap in [0, 1e30] and scale / softcap a normal number");
   const int64_t vec = dtype == DX_BF16 ? 8 : 4, width = (int64_t)num_q_heads * a.c.d;
   REQUIRE(q_row_stride >= width && out_row_stride >= width && q_row_stride % vec == 0 && out_row_stride % vec == 0,
           "attn_kv4: row strides must cover heads * head_dim and be multiples of %ld elements", (long)vec);
@@ -906,6 +907,7 @@ int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32
   SUPPORTED((int64_t)max_seq_len * group <= MOST_SLOTS / 32, "attn_kv4: %d tokens of %d heads beyond the launch grid",
             max_seq_len, group);
   if (num_seqs == 0 || ((rows == 0 || max_seq_len == 0) && !weights_out)) return DX_OK;
+  REQUIRE(!weights_out || out != q, "attn_kv4: with weights, out must not be q");
   a.window = window;
   a.slots = in_range(window, max_ctx_len);
   const kv4::Plan p = kv4::attn_plan(max_seq_len, max_ctx_len, group, a.slots);
@@ -967,6 +969,8 @@ int dx_kv4_evict(const dx_kv4_cache *cache, const float *weights, int64_t weight
   REQUIRE(workspace_bytes >= need, "kv4_evict: workspace of %ld bytes, need %ld", (long)workspace_bytes, (long)need);
   if (num_seqs == 0) return DX_OK;
   REQUIRE(workspace && aligned16(workspace), "kv4_evict: needs a 16-byte aligned workspace");
+  REQUIRE(weights_out != weights && out_len != ctx_len && out_table != page_table,
+          "kv4_evict: weights_out, out_len and out_table must not be weights, ctx_len and page_table");
   return check_launch(dx_kv4_evict_launch(c, page_table, table_width, out_table, out_table_width, ctx_len, num_seqs, ctx,
                                           keep, recent, weights, weights_seq_stride, weights_head_stride, weights_out,
                                           weights_out_seq_stride, weights_out_head_stride, out_len,

@@ -822,7 +822,7 @@ def attention_kv4(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, se
 
     With `weights` (fp32 [sequences, Hkv, >= max_ctx_len]) every slot's accumulated attention weight goes to
     `weights_out` (default: `weights` itself): the old one, taken as 0 for the newest tokens' slots, plus the softmax
-    weights of all rows and query heads that saw it. `kv4_evict` goes by them."""
+    weights of all rows and query heads that saw it; `out` must not meet q then. `kv4_evict` goes by them."""
     seqs = _kv4_ints("attention_kv4", cache, page_table, seq_start, seq_len, ctx_len)
     index, heads, dtype, rows = cache.index, cache.heads, q.dtype, q.shape[0]
     if dtype not in (BF16, F32):

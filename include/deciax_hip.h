@@ -546,17 +546,18 @@ int dx_kv4_read(const dx_kv4_cache *cache, void *k, void *v,
  * and position[j] > position[own] - window. q and out: bf16, or fp32 with three
  * bf16 products for each fp32 one. A row that sees nothing is written as zeros;
  * rows that belong to no sequence are not written. num_q_heads is any multiple
- * of the cache's heads; softcap (0: none) at most 1e30 and not below scale / FLT_MAX.
+ * of the cache's heads; softcap (0: none) at most 1e30, scale / softcap a normal
+ * number.
  *
  * With weights_out, every slot below ctx_len gets its accumulated attention
  * weight: weights_in (0 for the newest tokens' slots, whatever it holds there)
  * plus the softmax weights of all rows and query heads of the KV head that saw
  * it. weights are fp32 at b * seq_stride + g * head_stride + slot; weights_in may
- * be weights_out with the same strides, and must not meet it otherwise; slots
- * from ctx_len on are not written. Sums have one order: the same call gives the
- * same bits, alone or in a batch. Workspace size from dx_attn_kv4_workspace with
- * the same sizes (with weights, most of it 4 bytes a slot and row of a KV head,
- * 16 rows at most). */
+ * be weights_out with the same strides, and must not meet it otherwise; out must
+ * not meet q then; slots from ctx_len on are not written. Sums have one order: the
+ * same call gives the same bits, alone or in a batch. Workspace size from
+ * dx_attn_kv4_workspace with the same sizes (with weights, most of it 4 bytes a
+ * slot and row of a KV head, 16 rows at most). */
 int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out,
                 const int32_t *page_table, int32_t table_width,
                 const int32_t *seq_start, const int32_t *seq_len,
@@ -582,8 +583,8 @@ int64_t dx_attn_kv4_workspace(int32_t num_seqs, int32_t max_seq_len,
  * what is kept stays in slot order, with its position. Slots below ctx_len whose
  * page is outside the pool are not kept. weights_out[b, g, 0..keep) gets the kept
  * slots' weights and zeros behind them, out_len[b] = min(slots with a page, keep).
- * 0 <= recent <= keep, 1 <= keep. No counterpart in the reference. Workspace size
- * from dx_kv4_evict_workspace. */
+ * What is written must not meet what is read. 0 <= recent <= keep, 1 <= keep. No
+ * counterpart in the reference. Workspace size from dx_kv4_evict_workspace. */
 int dx_kv4_evict(const dx_kv4_cache *cache, const float *weights,
                  int64_t weights_seq_stride, int64_t weights_head_stride,
                  const int32_t *page_table, int32_t table_width,

@@ -174,3 +174,20 @@ def test_a_cache_keeps_its_arrays() -> None:
             K.KV4Cache(*bad)
     with pytest.raises(ValueError, match="device"):
         K.kv4_read(cache, torch.zeros((1, 1), dtype=torch.int32), *[torch.zeros(1, dtype=torch.int32)] * 3, 1, rows=1)
+
+
+@pytest.mark.parametrize("call,what", [
+    (lambda: attend(w_in=P, w_out=P), b"out must not be q"),      # the weights read q after out is written
+    (lambda: evict(w_out=P, ctx=ODD, table=ODD), b"weights_out"),  # kept weights over those that are still to be read
+    (lambda: evict(w_out=ODD, table=ODD), b"out_len"),             # lengths that other heads still read
+    (lambda: evict(w_out=ODD, ctx=ODD), b"out_table"),             # the old pages
+])
+def test_arrays_that_a_call_reads_and_writes_must_differ(call, what: bytes) -> None:
+    check(call(), INVALID)
+    assert what in _lib.lib().dx_last_error()
+
+
+def test_a_scale_that_vanishes_beside_the_soft_cap_is_refused() -> None:
+    """Scores are taken over the soft-cap: scale / softcap has to be a normal number."""
+    check(attend(scale=1e-9, cap=1e30), INVALID)
+    check(attend(scale=1e-9, cap=1e28, rows=0), OK)
