@@ -934,3 +934,24 @@ def test_the_documented_steps_go_on_after_an_eviction(steps: str) -> None:
         held = a.held_positions(b)
         assert (held[:, keep] == n).all() and (np.diff(held, axis=1) > 0).all()
         assert (held[:, keep - 16:keep] == np.arange(n - 16, n)).all()
+
+
+@pytest.mark.parametrize("dtype,softcap,window", [("bf16", 50.0, 0), ("f32", 0.0, 0), ("bf16", 0.0, 120000)])
+@pytest.mark.parametrize("new,ctx,hq,page", [([2, 1], [150000, 700], 2, 64), ([40], [140001], 1, 64), ([1030], [5000], 2, 64),
+                                             ([1, 70], [70000, 300], 2, 65536)])
+def test_spans_of_more_pages_than_a_wave_has_lanes(new: list[int], ctx: list[int], hq: int, page: int, dtype: str,
+                                                   softcap: float, window: int) -> None:
+    """A span's pages are looked up 64 at a time: spans of 65 and more, and pages of 65536 slots."""
+    import torch
+
+    say(f"attention_kv4 of long spans new={new} ctx={ctx} page={page} {dtype} cap={softcap} window={window}")
+    c = Case(90 + hq, new, ctx, hq, 1, 64, page, dtype)
+    c.fill(5)
+    c.append()
+    w = np.abs(rng(4).normal(size=(len(new), 1, max(ctx)))).astype(np.float32)
+    w_in = torch.from_numpy(w.copy()).cuda()
+    w_out = torch.empty_like(w_in)
+    kw = dict(scale=1 / 8, softcap=softcap, window=window)
+    out = c.attend(weights=w_in, weights_out=w_out, **kw)
+    torch.cuda.synchronize()
+    c.check(out, w_out, w, **kw)

@@ -284,3 +284,22 @@ def test_more_rows_than_one_launch_holds() -> None:
     assert ((ent + (want.exp() * want).sum(1)).abs() <= 16 * U * 2).all()
     assert (ids[:, 0] == (x[:, 1] > x[:, 0]).int()).all()
     assert ((tops[:, 0] - want.amax(1)).abs() <= 16 * U).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("vocab,top", [(262145, 64), (600001, 7), (1100003, 64), (5000000, 1)])
+def test_vocabularies_beyond_a_workgroups_registers(vocab: int, top: int, cap: float, dtype: str) -> None:
+    """More groups than the threads hold at once, and more chunks than threads, with ties among the best."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"token_logprobs vocab={vocab} top={top} cap={cap} {dtype}")
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    x = torch.from_numpy((rng(vocab).normal(size=(2, vocab)) * 3).astype(np.float32)).cuda().to(t)
+    x[1, vocab - 1] = x[1, 5] = x[1, vocab // 2] = x[1].max() + 1
+    targets = np.array([vocab // 3, vocab - 1])
+    got = K.token_logprobs(x, i32(targets), top=top, softcap=cap)
+    torch.cuda.synchronize()
+    check(x.float().cpu().numpy(), targets, top, cap, got)
