@@ -145,7 +145,7 @@ DX_DEVICE uint32_t order(float w) {
 // i 1024 + t. The kept-th largest key is found bit by bit from the top: a round counts the keys at or above a
 // candidate with one compare an item and the wave's population counts, no memory but one number a wave. ITEMS = 0
 // reads the weights again every round, for spans beyond the registers. A slot without a page has the key of no slot.
-// Bound: the 32 rounds, one after the other, of one workgroup: 9.8 us for 2900 slots, 31 us for up to 16384.
+// Bound: the 32 rounds, one after the other, of one workgroup: 11 us for 2900 slots, 30 us for up to 16384.
 template <int ITEMS>
 __global__ void __launch_bounds__(SEL_THREADS)
 select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const int32_t *__restrict__ table, int width,
@@ -170,7 +170,7 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
   };
   auto fetch_there = [&](int i) -> uint32_t {
     const uint32_t x = fetch(i);
-    return gone && no_page(page_of[min(i * SEL_THREADS + tid, ctx - 1) >> shift]) ? 0u : x;
+    return no_page(page_of[min(i * SEL_THREADS + tid, ctx - 1) >> shift]) ? 0u : x;
   };
   uint32_t key[ITEMS ? ITEMS : 1];
   if (ctx == 0) {
@@ -212,6 +212,18 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
     }
     present = total(c, 0);
   }
+  auto count = [&](uint32_t least) {  // a wave's keys from `least` on
+    int c = 0;
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) c += __popcll(__ballot(key[i] >= least));
+    } else if (gone) {
+      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch_there(i) >= least));
+    } else {
+      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch(i) >= least));
+    }
+    return c;
+  };
   const int kept = min(present, keep);
   if (g == 0 && tid == 0) out_len[b] = kept;
   uint32_t least = 0;  // the kept-th largest key, or that of no slot where all are kept
@@ -219,14 +231,7 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
   int above = found ? kept : 0;
   for (int bit = 31; bit >= 0 && !found; --bit) {
     const uint32_t cand = least | (1u << bit);
-    int c = 0;
-    if constexpr (ITEMS > 0) {
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) c += __popcll(__ballot(key[i] >= cand));
-    } else {
-      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch_there(i) >= cand));
-    }
-    c = total(c, bit & 1);
+    const int c = total(count(cand), bit & 1);
     if (c >= kept) least = cand;
     if (c == kept) {  // these are they
       least = cand - 1;
@@ -234,16 +239,8 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
       found = true;
     }
   }
-  if (!found) {
-    int c = 0;
-    if constexpr (ITEMS > 0) {
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) c += __popcll(__ballot(key[i] > least));
-    } else {
-      for (int i = 0; i < rounds; ++i) c += __popcll(__ballot(fetch_there(i) > least));
-    }
-    above = total(c, 1);
-  }
+  // least + 1 is a number: as many keys as are kept and no more are PROTECTED, and with so many the search has ended
+  if (!found) above = total(count(least + 1), 1);
   const int ties = kept - above;  // of the keys that equal `least`, the first in slot order
   // Ranks: every wave its counts of both kinds for each 1024 slots, ITEMS (or 16) of those at a time, then sums over the
   // waves before it and the slots before those. A wave of 64 neighbouring slots takes two ballots.
@@ -255,7 +252,7 @@ select_kernel(const float *__restrict__ weights, long w_seq, long w_head, const 
 #pragma unroll
     for (int i = 0; i < SPREAD; ++i) {
       if constexpr (ITEMS > 0) k[i] = key[i];
-      else k[i] = fetch_there(i0 + i);
+      else k[i] = gone ? fetch_there(i0 + i) : fetch(i0 + i);
       const uint64_t eq = __ballot(k[i] == least && k[i] != 0), gt = __ballot(k[i] > least);
       if (lane == 0) spread[i][wave] = (uint32_t)__popcll(gt) << 16 | (uint32_t)__popcll(eq);
     }
@@ -388,8 +385,8 @@ hipError_t dx_kv4_evict_launch(const Kv4Cache &c, const int32_t *table, int widt
                                long o_head, int32_t *out_len, int32_t *list, hipStream_t s) {
   const dim3 grid(c.hkv, num_seqs), block(SEL_THREADS);
   const int rounds = (max_ctx + SEL_THREADS - 1) / SEL_THREADS;
-// By the slots that a thread holds. us of an eviction to 1000: 2900 slots 20.5 with 4 a thread and 32.7 with 16, 14000
-// 44 with 16 and 93 with 64, 60000 101 with 64 and 327 when read again every round.
+// By the slots that a thread holds. us of an eviction to 1000, in a graph: 2900 slots 15.3 with 4 a thread and 23.4 with
+// 16, 14000 27 with 16 and 74 with 64, 60000 88 with 64 and 326 when read again every round.
 #define SELECT(N) \
   select_kernel<N><<<grid, block, 0, s>>>(weights, w_seq, w_head, table, width, c.pages, c.shift, ctx_len, max_ctx,      \
                                           keep, recent, list, out_len)
