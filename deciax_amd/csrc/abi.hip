@@ -824,7 +824,9 @@ Kv4Workspace kv4_workspace(const kv4::Plan &p, int64_t units, int32_t d, bool we
   w.stats = align_up(units * p.part_rows * d * 4, 256);
   w.lse = w.stats + align_up(units * p.part_rows * 8, 256);
   w.scores = w.lse + (weights ? align_up(units * p.max_rows * 4, 256) : 0);
-  w.total = w.scores + (weights ? units * p.score_rows * (int64_t)p.score_slots * 4 : 0);
+  // this alone can pass 64 bits: then no workspace is large enough
+  const bool fits = (double)units * p.score_rows * p.score_slots * 4 < 4e18;
+  w.total = !weights ? w.scores : fits ? w.scores + units * p.score_rows * (int64_t)p.score_slots * 4 : INT64_MAX;
   return w;
 }
 
@@ -942,7 +944,9 @@ int dx_attn_kv4(const dx_kv4_cache *cache, const void *q, void *out, const int32
 }
 
 int64_t dx_kv4_evict_workspace(int32_t num_seqs, int32_t num_kv_heads, int32_t keep) {
-  return num_seqs > 0 && num_kv_heads > 0 && keep > 0 ? (int64_t)num_seqs * num_kv_heads * keep * 4 : 0;
+  if (num_seqs <= 0 || num_kv_heads <= 0 || keep <= 0) return 0;
+  const int64_t heads = (int64_t)num_seqs * num_kv_heads;
+  return heads <= INT64_MAX / 4 / keep ? heads * keep * 4 : INT64_MAX;
 }
 
 int dx_kv4_evict(const dx_kv4_cache *cache, const float *weights, int64_t weights_seq_stride,
