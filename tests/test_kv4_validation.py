@@ -200,8 +200,8 @@ def test_workspaces_beyond_64_bits_are_refused() -> None:
     assert lib.dx_attn_kv4_workspace(65535, 1, 1 << 30, 65535, 65535, 64, 0, 1) == most
     assert lib.dx_kv4_evict_workspace(65535, 65535, 1 << 30) == most
     many = cache(hkv=65535, d=64)
-    check(attend(c=many, hq=65535, qs=65535 * 64, os=65535 * 64, seqs=65535, max_new=1, max_ctx=1 << 30, w_in=P, w_out=ODD,
-                 wi=(1 << 47, 1 << 30), wo=(1 << 47, 1 << 30)), INVALID)
+    check(attend(c=many, out=ctypes.c_void_p(0x20000), hq=65535, qs=65535 * 64, os=65535 * 64, seqs=65535, max_new=1,
+                 max_ctx=1 << 30, w_in=P, w_out=ODD, wi=(1 << 47, 1 << 30), wo=(1 << 47, 1 << 30)), INVALID)
     assert b"workspace" in lib.dx_last_error()
     check(evict(c=many, seqs=65535, keep=1 << 30, out_width=1 << 24, wo=(1 << 47, 1 << 30)), INVALID)
     assert b"workspace" in lib.dx_last_error()
