@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, D == 256 && NS > 1 ? 1 : 2) kv4_attn_
 // tile's codes are on their way while the one before is used, and go over it afterwards. Two workgroups a CU, in step with
 // themselves alone, hide each other's waits; twice the rows a workgroup (half the decoding) or two tiles in turn (no wait
 // between use and decoding) were no faster: 6 questions of up to 611 tokens over up to 8803, D = 256, 358 us either way.
-// Now 294 us: 4 sequences of 400 tokens over 6000 slots reach 410 TFLOP/s. Of its time the vector units work 47% (277
+// Now 295 to 302 us: 4 sequences of 400 tokens over 6000 slots reach 410 TFLOP/s. Of its time the vector units work 47% (277
 // instructions a wave and 32 keys: soft-cap 100, softmax 75, decoding 60), LDS 38%, the matrix units 20%; two waves a SIMD
 // (236 registers) leave the rest to waits.
 template <int D>
@@ -968,7 +968,7 @@ __global__ void __launch_bounds__(THREADS) kv4_score_weights_kernel(Kv4Attn a) {
 // The same for sequences of more rows, from the keys. A wave owns 32 keys, decoded once, and walks all rows, so every sum
 // has one owner and one order. Its workgroup brings the rows through LDS, 32 at a time and the next 32 on their way: read
 // by each wave as its products want them (16 rows of one chunk) they cost the vector cache a look at every lane: 261 us
-// where this takes 176, for 6 questions of up to 611 tokens over up to 8803.
+// where this takes 176, for 6 questions of up to 611 tokens over up to 8803; with three waves a SIMD 147.
 template <int D, int NS, bool CAP>
 __global__ void __launch_bounds__(THREADS, NS == 1 ? 3 : 1) kv4_weights_kernel(Kv4Attn a) {
   constexpr int ROWS = 32, BYTES = NS == 1 ? 2 : 4, CHUNKS = D * BYTES / 16;  // 16-byte chunks of a row
