@@ -101,7 +101,7 @@ def token_logprobs(x: np.ndarray, target: int, top: int, softcap: float) -> tupl
         logp = t
     else:
         m = t.max()
-        logp = t - (m + np.log(np.exp(t - m).sum()))
+        logp = (t - m) - np.log(np.exp(t - m).sum())
         p = np.exp(logp)
         ent = float(-(p[p > 0] * logp[p > 0]).sum())
         lp = logp[target] if 0 <= target < len(x) else np.nan

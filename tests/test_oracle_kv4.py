@@ -48,3 +48,13 @@ def test_evict_keeps_recent_then_heavy_then_low_slots() -> None:
     assert kv4.evict(w, 4, 1).tolist() == [0, 2, 4, 7]
     assert kv4.evict(w, 8, 1).tolist() == list(range(8))
     assert kv4.evict(w, 2, 2).tolist() == [6, 7]
+
+
+def test_log_probabilities_far_from_zero() -> None:
+    """A common shift changes nothing, however large it is beside the differences."""
+    for x in (np.full(35, -3.4e38), np.full(35, 1e300), np.arange(35.0) + 2.0 ** 50):
+        lp, ent, ids, tops = kv4.token_logprobs(x, 3, 2, 0.0)
+        want = kv4.token_logprobs(x - x[0], 3, 2, 0.0)
+        assert abs(lp - want[0]) < 1e-12 and abs(ent - want[1]) < 1e-12
+        assert ids.tolist() == want[2].tolist() and np.abs(tops - want[3]).max() < 1e-12
+    assert abs(kv4.token_logprobs(np.full(35, -3.4e38), 3, 2, 0.0)[0] + np.log(35)) < 1e-12
