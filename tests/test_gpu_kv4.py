@@ -955,3 +955,22 @@ def test_spans_of_more_pages_than_a_wave_has_lanes(new: list[int], ctx: list[int
     out = c.attend(weights=w_in, weights_out=w_out, **kw)
     torch.cuda.synchronize()
     c.check(out, w_out, w, **kw)
+
+
+@pytest.mark.parametrize("large", [0, 1])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_large_batches_against_the_oracle(large: int, dtype: str) -> None:
+    import torch
+
+    new, ctx, hq, hkv, d = LARGE[large]
+    say(f"attention_kv4 of {len(new)} sequences against the oracle, {dtype}")
+    c = Case(70 + large, new, ctx, hq, hkv, d, 64, dtype)
+    c.fill(large)
+    c.append()
+    w = np.abs(rng(large).normal(size=(len(new), hkv, max(ctx)))).astype(np.float32)
+    w_in = torch.from_numpy(w.copy()).cuda()
+    w_out = torch.empty_like(w_in)
+    kw = dict(scale=1 / 8, softcap=50.0, window=0)
+    out = c.attend(weights=w_in, weights_out=w_out, **kw)
+    torch.cuda.synchronize()
+    c.check(out, w_out, w, **kw)
