@@ -147,6 +147,22 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [_p, _p, c_int64, c_int32, c_int64, c_float, c_int32, _p, _p, _p, _p, c_int32, _p, c_int64, _p],
     ),
     "dx_token_logprobs_workspace": (c_int64, [c_int64, c_int32, c_int32]),
+    "dx_q4_quantize": (c_int, [_p, c_int64, _p, _p, c_int32, c_int32, c_int32, _p]),
+    "dx_q4_pack": (c_int, [_p, _p, c_int32, _p, _p, _p, c_int32, c_int32, c_int32, _p]),
+    "dx_q4_values": (c_int, [_p, _p, _p, c_int64, c_int32, c_int32, c_int32, _p]),
+    "dx_linear_q4": (
+        c_int, [_p, _p, _p, _p, c_int64, c_int32, c_int32, c_int32, c_int64, c_int64, c_int32, _p]),
+    "dx_qk_norm_rope": (
+        c_int,
+        [_p, _p, _p, _p, _p, _p, c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_float, c_float,
+         c_int32, c_int32, _p],
+    ),
+    "dx_linear_attn": (
+        c_int,
+        [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
+         c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int32, _p, c_int64, _p],
+    ),
+    "dx_linear_attn_workspace": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -20,7 +20,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libdeciax_hip.so"
 SOURCES = ("abi.hip", "gemm.hip", "attention.hip", "rowwise.hip", "head.hip", "kv4_cache.hip",
-           "kv4_attention.hip", "logprobs.hip")
+           "kv4_attention.hip", "logprobs.hip", "q4.hip", "head_rope.hip", "linear_attention.hip")
 ARCH = "gfx950"
 
 # Packed-fp32 VALU forms stay disabled in every device compile.

@@ -11,6 +11,7 @@
 #include "common.h"
 #include "kernels.h"
 #include "kv4_plan.h"
+#include "linear_attention_plan.h"
 
 namespace {
 
@@ -1014,4 +1015,167 @@ int dx_token_logprobs(const void *logits, const int32_t *targets, int64_t rows, 
                                                parts + rows * dx_ceil_div(vocab, 2048) * 3, dtype == DX_F32,
                                                as_stream(stream)),
                       "token_logprobs launch");
+}
+
+// ---------------------------------------------------------------------------- a token layer: 4-bit weights, rotation, state
+
+namespace {
+
+int validate_q4(const void *codes, const void *groups, int32_t n, int32_t k, int32_t group, Q4Weight *out,
+                const char *what) {
+  REQUIRE(codes && groups, "%s: null codes or groups", what);
+  REQUIRE(n > 0 && k > 0, "%s: a weight of %d x %d", what, n, k);
+  SUPPORTED(group == 32 || group == 64 || group == 128, "%s: groups of %d, not 32, 64 or 128", what, group);
+  SUPPORTED(k % group == 0, "%s: k = %d must be a multiple of the group %d", what, k, group);
+  SUPPORTED(n <= 1 << 24 && k <= 1 << 24 && (int64_t)n * k <= INT64_C(1) << 40, "%s: a weight of %d x %d", what, n, k);
+  REQUIRE(aligned16(codes) && aligned16(groups), "%s: codes and groups must be 16-byte aligned", what);
+  *out = Q4Weight{const_cast<void *>(codes), static_cast<uint32_t *>(const_cast<void *>(groups)), n, k, group};
+  return DX_OK;
+}
+
+}  // namespace
+
+int dx_q4_quantize(const void *w, int64_t w_row_stride, void *codes, void *groups, int32_t n, int32_t k, int32_t group,
+                   void *stream) {
+  Q4Weight q;
+  const int st = validate_q4(codes, groups, n, k, group, &q, "q4_quantize");
+  if (st) return st;
+  REQUIRE(w && aligned16(w), "q4_quantize: w must be 16-byte aligned");
+  REQUIRE(w_row_stride >= k && w_row_stride % 8 == 0, "q4_quantize: row stride %ld must cover k and be a multiple of 8",
+          (long)w_row_stride);
+  return check_launch(dx_quantize_q4_launch(q, static_cast<const uint16_t *>(w), w_row_stride, as_stream(stream)),
+                      "q4_quantize launch");
+}
+
+int dx_q4_pack(const uint8_t *code, const void *scales, int32_t scales_fp16, const uint8_t *zeros, void *codes,
+               void *groups, int32_t n, int32_t k, int32_t group, void *stream) {
+  Q4Weight q;
+  const int st = validate_q4(codes, groups, n, k, group, &q, "q4_pack");
+  if (st) return st;
+  REQUIRE(code && scales, "q4_pack: null code or scales");
+  REQUIRE(reinterpret_cast<uintptr_t>(scales) % 2 == 0, "q4_pack: scales not aligned to their type");
+  return check_launch(dx_pack_q4_launch(q, code, static_cast<const uint16_t *>(scales), scales_fp16 != 0, zeros,
+                                        as_stream(stream)),
+                      "q4_pack launch");
+}
+
+int dx_q4_values(const void *codes, const void *groups, float *w, int64_t w_row_stride, int32_t n, int32_t k,
+                 int32_t group, void *stream) {
+  Q4Weight q;
+  const int st = validate_q4(codes, groups, n, k, group, &q, "q4_values");
+  if (st) return st;
+  REQUIRE(w && reinterpret_cast<uintptr_t>(w) % 4 == 0, "q4_values: null or misaligned w");
+  REQUIRE(w_row_stride >= k, "q4_values: row stride %ld smaller than k = %d", (long)w_row_stride, k);
+  return check_launch(dx_q4_values_launch(q, w, w_row_stride, as_stream(stream)), "q4_values launch");
+}
+
+int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y, int64_t m, int32_t n, int32_t k,
+                 int32_t group, int64_t x_row_stride, int64_t y_row_stride, int32_t out_dtype, void *stream) {
+  Q4Weight q;
+  const int st = validate_q4(codes, groups, n, k, group, &q, "linear_q4");
+  if (st) return st;
+  REQUIRE(x && y, "linear_q4: null x or y");
+  REQUIRE(m >= 0, "linear_q4: %ld rows", (long)m);
+  SUPPORTED(m <= 1 << 20, "linear_q4: %ld rows beyond the launch grid", (long)m);
+  REQUIRE(out_dtype == DX_BF16 || out_dtype == DX_F32, "linear_q4: unknown out dtype %d", out_dtype);
+  REQUIRE(x_row_stride >= k && x_row_stride % 8 == 0 && y_row_stride >= n,
+          "linear_q4: row strides must cover the rows, x's be a multiple of 8");
+  REQUIRE(aligned16(x) && reinterpret_cast<uintptr_t>(y) % (out_dtype == DX_BF16 ? 2 : 4) == 0,
+          "linear_q4: x must be 16-byte aligned, y to its type");
+  if (m == 0) return DX_OK;
+  return check_launch(dx_linear_q4_launch(q, static_cast<const uint16_t *>(x), y, m, x_row_stride, y_row_stride,
+                                          out_dtype == DX_F32, as_stream(stream)),
+                      "linear_q4 launch");
+}
+
+int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions, const double *inv_freq, const void *q_norm,
+                    const void *k_norm, int64_t rows, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                    int32_t rotary_dim, int64_t x_row_stride, int64_t out_row_stride, float eps, float attention_factor,
+                    int32_t interleaved, int32_t dtype, void *stream) {
+  REQUIRE(x && out && positions && (inv_freq || rotary_dim == 0), "qk_norm_rope: null pointer argument");
+  REQUIRE((q_norm == nullptr) == (k_norm == nullptr), "qk_norm_rope: q_norm and k_norm go together");
+  REQUIRE(rows >= 0 && num_q_heads >= 0 && num_kv_heads >= 0 && num_q_heads <= 1 << 20 && num_kv_heads <= 1 << 20,
+          "qk_norm_rope: bad rows or heads");
+  REQUIRE(dtype == DX_BF16 || dtype == DX_F32, "qk_norm_rope: unknown dtype %d", dtype);
+  SUPPORTED(head_dim == 64 || head_dim == 128 || head_dim == 256, "qk_norm_rope: head_dim %d not in {64, 128, 256}",
+            head_dim);
+  SUPPORTED(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0,
+            "qk_norm_rope: rotary_dim %d must be a multiple of 16 up to head_dim %d", rotary_dim, head_dim);
+  const int64_t vec = dtype == DX_BF16 ? 8 : 4, width = ((int64_t)num_q_heads + num_kv_heads) * head_dim;
+  REQUIRE(x_row_stride >= width && out_row_stride >= width && x_row_stride % vec == 0 && out_row_stride % vec == 0,
+          "qk_norm_rope: row strides must cover heads * head_dim and be multiples of %ld elements", (long)vec);
+  REQUIRE(aligned16(x) && aligned16(out) && aligned16(q_norm) && aligned16(k_norm),
+          "qk_norm_rope: x, out and norms must be 16-byte aligned");
+  REQUIRE(reinterpret_cast<uintptr_t>(inv_freq) % 8 == 0, "qk_norm_rope: inv_freq not aligned to its type");
+  REQUIRE(!q_norm || eps >= 0.f, "qk_norm_rope: eps must be >= 0");
+  SUPPORTED(rows <= INT64_C(1) << 31, "qk_norm_rope: %ld rows beyond the launch grid", (long)rows);
+  if (rows == 0 || width == 0) return DX_OK;
+  const HeadRope a{x, q_norm, k_norm, out, positions, inv_freq, rows, x_row_stride, out_row_stride,
+                   num_q_heads, num_kv_heads, head_dim, rotary_dim / 2, eps, attention_factor, interleaved != 0};
+  return check_launch(dx_qk_norm_rope_launch(a, dtype == DX_F32, as_stream(stream)), "qk_norm_rope launch");
+}
+
+namespace {
+
+struct LinearAttnWorkspace {
+  int64_t sums, total;  // where the sums start, in bytes
+};
+
+// INT64_MAX: no workspace is large enough.
+LinearAttnWorkspace linear_attn_workspace(int64_t seqs, int32_t max_len, int64_t heads, int64_t dk, int64_t dv) {
+  const int64_t most = la::most_segments(max_len);
+  if (most <= 1 || seqs <= 0) return {0, 0};
+  if ((double)seqs * most * heads * dk * dv * 4 > 4e18) return {INT64_MAX, INT64_MAX};
+  const int64_t units = seqs * most * heads;
+  const int64_t sums = align_up(units * dk * dv * 4, 256);
+  return {sums, sums + units * 8};
+}
+
+bool state_dim(int32_t d) { return d == 64 || d == 128 || d == 256; }
+
+}  // namespace
+
+int64_t dx_linear_attn_workspace(int32_t num_seqs, int32_t max_seq_len, int32_t num_heads, int32_t k_dim, int32_t v_dim) {
+  if (num_seqs <= 0 || max_seq_len <= 0 || num_heads <= 0 || k_dim <= 0 || v_dim <= 0) return 0;
+  return linear_attn_workspace(num_seqs, max_seq_len, num_heads, k_dim, v_dim).total;
+}
+
+int dx_linear_attn(const void *q, const void *k, const void *v, const float *decay, void *out, const float *state_in,
+                   float *state_out, const int32_t *seq_start, const int32_t *seq_len, const int32_t *state_index,
+                   int32_t num_seqs, int32_t max_seq_len, int32_t num_states, int64_t rows, int32_t num_k_heads,
+                   int32_t num_heads, int32_t k_dim, int32_t v_dim, int64_t q_row_stride, int64_t k_row_stride,
+                   int64_t v_row_stride, int64_t decay_row_stride, int64_t out_row_stride, float scale, int32_t dtype,
+                   void *workspace, int64_t workspace_bytes, void *stream) {
+  REQUIRE(q && k && v && decay && out && state_in && state_out && seq_start && seq_len,
+          "linear_attn: null pointer argument");
+  REQUIRE(num_seqs >= 0 && max_seq_len >= 0 && num_states >= 0 && rows >= 0,
+          "linear_attn: negative sequence count, length, states or rows");
+  REQUIRE(num_k_heads > 0 && num_heads > 0 && num_heads % num_k_heads == 0,
+          "linear_attn: num_heads %d must be a positive multiple of num_k_heads %d", num_heads, num_k_heads);
+  REQUIRE(dtype == DX_BF16 || dtype == DX_F32, "linear_attn: unknown dtype %d", dtype);
+  SUPPORTED(state_dim(k_dim) && state_dim(v_dim), "linear_attn: k_dim %d, v_dim %d not in {64, 128, 256}", k_dim, v_dim);
+  SUPPORTED(num_seqs <= 65535 && num_heads <= 65535, "linear_attn: %d sequences or %d heads beyond the launch grid",
+            num_seqs, num_heads);
+  SUPPORTED(max_seq_len <= MOST_SLOTS, "linear_attn: sequences of more than 2^30 tokens");
+  REQUIRE(scale > 0.f && scale < INFINITY, "linear_attn: need a finite scale > 0");
+  REQUIRE(state_index || num_states >= num_seqs, "linear_attn: %d states for %d sequences", num_states, num_seqs);
+  const int64_t vec = dtype == DX_BF16 ? 8 : 4, kw = (int64_t)num_k_heads * k_dim, vw = (int64_t)num_heads * v_dim;
+  REQUIRE(q_row_stride >= kw && k_row_stride >= kw && v_row_stride >= vw && out_row_stride >= vw &&
+              q_row_stride % vec == 0 && k_row_stride % vec == 0 && v_row_stride % vec == 0 && out_row_stride % vec == 0,
+          "linear_attn: row strides must cover heads * dim and be multiples of %ld elements", (long)vec);
+  REQUIRE(decay_row_stride == 0 || decay_row_stride >= num_heads, "linear_attn: decay rows of %ld for %d heads",
+          (long)decay_row_stride, num_heads);
+  REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(state_in) && aligned16(state_out),
+          "linear_attn: pointers must be 16-byte aligned");
+  REQUIRE(out != q && out != k && out != v, "linear_attn: out must not be q, k or v");
+  const LinearAttnWorkspace w = linear_attn_workspace(num_seqs, max_seq_len, num_heads, k_dim, v_dim);
+  REQUIRE(workspace_bytes >= w.total, "linear_attn: workspace of %ld bytes, need %ld", (long)workspace_bytes,
+          (long)w.total);
+  REQUIRE(w.total == 0 || (workspace && aligned16(workspace)), "linear_attn: needs a 16-byte aligned workspace");
+  if (num_seqs == 0) return DX_OK;
+  LinearAttn a{q, k, v, out, decay, state_in, state_out, seq_start, seq_len, state_index, rows, q_row_stride,
+               k_row_stride, v_row_stride, out_row_stride, decay_row_stride, num_seqs, max_seq_len, num_states,
+               num_k_heads, num_heads, k_dim, v_dim, scale, static_cast<float *>(workspace),
+               reinterpret_cast<double *>(static_cast<char *>(workspace) + w.sums)};
+  return check_launch(dx_linear_attn_launch(a, dtype == DX_F32, as_stream(stream)), "linear_attn launch");
 }

@@ -172,3 +172,44 @@ hipError_t dx_kv4_attn_launch(const Kv4Attn &a, bool f32, hipStream_t s);
 hipError_t dx_token_logprobs_launch(const void *logits, const int32_t *targets, long rows, int vocab, long ld, float cap,
                                     int top, float *logprobs, float *entropy, int32_t *ids, float *top_logprobs,
                                     float *parts, float *groups, bool f32, hipStream_t s);
+
+// A weight in 4 bits (q4.hip): codes in tiles, one word a group; group 32, 64 or 128.
+struct Q4Weight {
+  void *codes;
+  uint32_t *words;
+  int n, k, group;
+};
+hipError_t dx_linear_q4_launch(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32,
+                               hipStream_t s);
+hipError_t dx_quantize_q4_launch(const Q4Weight &w, const uint16_t *values, long ldw, hipStream_t s);
+hipError_t dx_pack_q4_launch(const Q4Weight &w, const uint8_t *code, const uint16_t *scales, bool half,
+                             const uint8_t *zeros, hipStream_t s);
+hipError_t dx_q4_values_launch(const Q4Weight &w, float *values, long ldw, hipStream_t s);
+
+// Norms of query and key heads with the rotation by position (head_rope.hip).
+struct HeadRope {
+  const void *x, *q_norm, *k_norm;  // norms null without them
+  void *out;
+  const int32_t *positions;
+  const double *inv_freq;  // pairs of them: the first 2 pairs dimensions turn
+  long rows, x_stride, out_stride;
+  int hq, hkv, d, pairs;
+  float eps, factor;
+  bool interleaved;
+};
+hipError_t dx_qk_norm_rope_launch(const HeadRope &a, bool f32, hipStream_t s);
+
+// Linear attention with decay over packed sequences (linear_attention.hip).
+struct LinearAttn {
+  const void *q, *k, *v;
+  void *out;
+  const float *decay, *state_in;
+  float *state_out;
+  const int32_t *seq_start, *seq_len, *index;  // index null: sequence b has state b
+  long rows, qs, ks, vs, os, ds;               // row strides
+  int num_seqs, max_len, slots, hk, h, dk, dv;
+  float scale;
+  float *parts;  // workspace: segments' states and the sums of their g, sizes by la::most_segments
+  double *sums;
+};
+hipError_t dx_linear_attn_launch(const LinearAttn &a, bool f32, hipStream_t s);

@@ -1,0 +1,343 @@
+// Linear attention with a decay for each token and head, over packed sequences with a kept state:
+//   S_t = e^g_t S_(t-1) + k_t v_t^T,   o_t = scale q_t S_t,   S [DK, DV] fp32.
+//
+// In chunks: with G_i the sum of g over the chunk's tokens up to i,
+//   o_i = scale (e^G_i q_i S + sum_(j <= i) e^(G_i - G_j) (q_i . k_j) v_j),   S' = e^G_C S + sum_j e^(G_C - G_j) k_j v_j^T.
+// Sums and differences of g are taken in 64 bits: behind a strong decay they are small differences of large numbers. The
+// state is multiplied by e^G_C as a sum of two floats: rounded to one, the same error in every chunk of a head of constant
+// decay adds up over all the chunks that the state remembers.
+//
+// A long sequence is cut into segments (linear_attention_plan.h): kernel 1 finds what each adds to the state, kernel 2
+// joins them to every segment's start, kernel 3 runs each from there. The cut follows from the sequence's own length, so a
+// result does not depend on the batch.
+#include "common.h"
+#include "kernels.h"
+#include "linear_attention_plan.h"
+
+namespace {
+
+constexpr int THREADS = 256, COLS = 64;  // columns of the state a workgroup has
+constexpr float NO_DECAY_BELOW = -1e4f;  // e^g is 0 from there on, and sums of g stay exact enough
+
+struct Sequence {
+  long start, slot;  // first packed row, state (-1: none)
+  int len;
+};
+
+// A sequence that reaches outside the packed rows has none.
+DX_DEVICE Sequence sequence(const LinearAttn &a, int b) {
+  Sequence s;
+  s.start = a.seq_start[b];
+  s.len = min(max(a.seq_len[b], 0), a.max_len);
+  if (s.start < 0 || s.start + s.len > a.rows) s.len = 0;
+  s.slot = a.index ? a.index[b] : b;
+  if (s.slot < 0 || s.slot >= a.slots) s.slot = -1;
+  return s;
+}
+
+DX_DEVICE float decay_of(float g) { return g < NO_DECAY_BELOW ? NO_DECAY_BELOW : g; }
+
+template <typename T>
+DX_DEVICE float value(const T *p) {
+  if constexpr (sizeof(T) == 2) return bf2f(*p);
+  else return *p;
+}
+template <typename T>
+DX_DEVICE void put(T *p, float x) {
+  if constexpr (sizeof(T) == 2) *p = f2bf(x);
+  else *p = x;
+}
+
+// x = e^g as the sum of two floats.
+struct Factor {
+  float hi, lo;
+};
+DX_DEVICE Factor factor_of(double g) {
+  const double e = exp(g);
+  const float hi = (float)e;
+  return Factor{hi, hi < INFINITY ? (float)(e - (double)hi) : 0.f};  // NaN and infinity as they are
+}
+DX_DEVICE float times(float x, Factor f) { return fmaf(x, f.hi, x * f.lo); }
+
+// Token by token: thread 16 r + c has four columns and the rows r, r + 16, ..
+template <typename T, int DK>
+DX_DEVICE void step_body(const LinearAttn &a, const Sequence &s, int head, int col0, float *lds) {
+  constexpr int R = DK / 16;
+  float *kq = lds;                    // [2][DK]
+  float *part = lds + 2 * DK;         // [4 waves][COLS]
+  const int tid = threadIdx.x, c = tid & 15, r = tid >> 4, wave = tid >> 6;
+  const int kh = head / (a.h / a.hk);
+  const long at = ((s.slot * a.h + head) * DK + r) * (long)a.dv + col0 + 4 * c;
+  floatx4 st[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    st[i] = s.slot < 0 ? floatx4{0, 0, 0, 0}
+                       : *reinterpret_cast<const floatx4 *>(a.state_in + at + 16L * i * a.dv);
+  for (int t = 0; t < s.len; ++t) {
+    const long row = s.start + t;
+    const T *q = static_cast<const T *>(a.q) + row * a.qs + kh * DK, *k = static_cast<const T *>(a.k) + row * a.ks + kh * DK;
+    if (t > 0) __syncthreads();
+    for (int i = tid; i < 2 * DK; i += THREADS) kq[i] = i < DK ? value(k + i) : value(q + i - DK);
+    const T *v = static_cast<const T *>(a.v) + row * a.vs + head * a.dv + col0 + 4 * c;
+    floatx4 vv;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vv[e] = value(v + e);
+    const Factor d = factor_of((double)decay_of(a.decay[row * a.ds + head]));
+    __syncthreads();
+    floatx4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float kk = kq[r + 16 * i], qq = kq[DK + r + 16 * i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        st[i][e] = fmaf(kk, vv[e], times(st[i][e], d));
+        o[e] = fmaf(qq, st[i][e], o[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] += __shfl_xor(o[e], 16, 64);
+      o[e] += __shfl_xor(o[e], 32, 64);
+    }
+    if ((tid & 63) < 16) *reinterpret_cast<floatx4 *>(part + wave * COLS + 4 * c) = o;
+    __syncthreads();
+    if (tid < COLS)
+      put(static_cast<T *>(a.out) + row * a.os + head * a.dv + col0 + tid,
+          a.scale * ((part[tid] + part[COLS + tid]) + (part[2 * COLS + tid] + part[3 * COLS + tid])));
+  }
+  if (s.slot >= 0)
+#pragma unroll
+    for (int i = 0; i < R; ++i) *reinterpret_cast<floatx4 *>(a.state_out + at + 16L * i * a.dv) = st[i];
+}
+
+template <typename T, int DK>
+__global__ void __launch_bounds__(THREADS) step_kernel(LinearAttn a) {
+  __shared__ __align__(16) float lds[2 * DK + 4 * COLS];
+  const int blocks = a.dv / COLS;
+  step_body<T, DK>(a, sequence(a, blockIdx.y), blockIdx.x / blocks, blockIdx.x % blocks * COLS, lds);
+}
+
+// Chunks of 32 tokens with fp32 products (v_mfma_f32_16x16x4_f32: lane l has row or column l % 16 of an operand and k
+// l / 16, and of the result column l % 16, rows 4 (l / 16) + r).
+DX_DEVICE floatx4 mfma_f32(float x, float y, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0); }
+
+template <int DK>
+struct Chunk {
+  static constexpr int TOKENS = 32, W = DK + 4, VW = COLS + 4, PW = TOKENS + 4;
+  float q[TOKENS][W], k[TOKENS][W], v[TOKENS][VW], p[TOKENS][PW], s[DK][VW];
+  double sum[TOKENS];
+  float from_start[TOKENS], to_end[TOKENS];  // e^G_i, e^(G_C - G_j)
+  Factor all;
+  int lost;  // whether a value is no finite number
+};
+
+// The wave's columns of the state: tile i has rows 16 i + 4 (l / 16) + r, column 16 wave + l % 16.
+template <int DK>
+DX_DEVICE long state_at(const LinearAttn &a, int i, int r, int col0) {
+  const int lane = threadIdx.x & 63;
+  return (long)(16 * i + 4 * (lane >> 4) + r) * a.dv + col0 + 16 * (threadIdx.x >> 6) + (lane & 15);
+}
+
+// Tokens [t0, t1) of a sequence from the state st on; OUT: with their outputs. Returns the sum of their g.
+template <typename T, int DK, bool OUT>
+DX_DEVICE double chunks(const LinearAttn &a, const Sequence &s, int head, int col0, int t0, int t1, floatx4 (&st)[DK / 16],
+                        Chunk<DK> &m) {
+  constexpr int N = Chunk<DK>::TOKENS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  const int kh = head / (a.h / a.hk);
+  double total = 0.0;
+  for (int t = t0; t < t1; t += N) {
+    const int n = min(N, t1 - t);
+    const long row = s.start + t;
+    __syncthreads();
+    if (tid == 0) m.lost = 0;
+    __syncthreads();
+    for (int i = tid; i < N * DK; i += THREADS) {
+      const int j = i / DK, d = i % DK;
+      if (OUT) m.q[j][d] = j < n ? value(static_cast<const T *>(a.q) + (row + j) * a.qs + kh * DK + d) : 0.f;
+      m.k[j][d] = j < n ? value(static_cast<const T *>(a.k) + (row + j) * a.ks + kh * DK + d) : 0.f;
+    }
+    for (int i = tid; i < N * COLS; i += THREADS) {
+      const int j = i / COLS, d = i % COLS;
+      const float x = j < n ? value(static_cast<const T *>(a.v) + (row + j) * a.vs + head * a.dv + col0 + d) : 0.f;
+      m.v[j][d] = x;
+      if (!(fabsf(x) < INFINITY)) m.lost = 1;
+    }
+    if (wave == 0) {
+      double x = lane < n ? (double)decay_of(a.decay[(row + lane) * a.ds + head]) : 0.0;
+#pragma unroll
+      for (int off = 1; off < N; off <<= 1) {
+        const double y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+      }
+      const double end = __shfl(x, N - 1, 64);
+      if (lane < N) {
+        m.sum[lane] = x;
+        m.from_start[lane] = expf((float)x);
+        m.to_end[lane] = expf((float)(end - x));
+      }
+      if (lane == 0) m.all = factor_of(end);
+    }
+    __syncthreads();
+    total += m.sum[N - 1];
+    if constexpr (OUT) {
+      {
+        const int i0 = 16 * (wave >> 1), j0 = 16 * (wave & 1);  // the wave's tile of the weights
+        floatx4 p = {0, 0, 0, 0};
+        if (i0 >= j0)
+          for (int d = 0; d < DK; d += 4) p = mfma_f32(m.q[i0 + c][d + g], m.k[j0 + c][d + g], p);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = i0 + 4 * g + r, j = j0 + c;
+          m.p[i][j] = j <= i ? p[r] * expf((float)(m.sum[i] - m.sum[j])) : 0.f;
+        }
+      }
+      // the state's columns of this wave are written and read by it alone
+#pragma unroll
+      for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m.s[16 * i + 4 * g + r][16 * wave + c] = st[i][r];
+      floatx4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      for (int d = 0; d < DK; d += 4) {
+        const float y = m.s[d + g][16 * wave + c];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) o[i] = mfma_f32(m.q[16 * i + c][d + g], y, o[i]);
+      }
+      __syncthreads();
+      const bool lost = m.lost;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[i][r] *= m.from_start[16 * i + 4 * g + r];
+        if (!lost) {
+          for (int j = 0; j < N; j += 4) o[i] = mfma_f32(m.p[16 * i + c][j + g], m.v[j + g][16 * wave + c], o[i]);
+        } else {  // a weight of 0 would carry a later token's infinity or NaN to this one
+          for (int r = 0; r < 4; ++r)
+            for (int j = 0; j <= 16 * i + 4 * g + r; ++j)
+              o[i][r] = fmaf(m.p[16 * i + 4 * g + r][j], m.v[j][16 * wave + c], o[i][r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = 16 * i + 4 * g + r;
+          if (j < n) put(static_cast<T *>(a.out) + (row + j) * a.os + head * a.dv + col0 + 16 * wave + c, a.scale * o[i][r]);
+        }
+      }
+    }
+    const Factor all = m.all;
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[i][r] = times(st[i][r], all);
+    for (int j = 0; j < N; j += 4) {
+      const float y = m.v[j + g][16 * wave + c] * m.to_end[j + g];
+#pragma unroll
+      for (int i = 0; i < DK / 16; ++i) st[i] = mfma_f32(m.k[j + g][16 * i + c], y, st[i]);
+    }
+  }
+  return total;
+}
+
+// What each segment but the last adds to the state, and the sum of its g.
+template <typename T, int DK>
+__global__ void __launch_bounds__(THREADS) segment_kernel(LinearAttn a, float *parts, double *sums, int most) {
+  __shared__ Chunk<DK> m;
+  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / COLS;
+  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * COLS;
+  const Sequence s = sequence(a, b);
+  const la::Segments seg = la::segments(s.len);
+  if (s.len <= la::STEP || i >= seg.count - 1) return;
+  floatx4 st[DK / 16];
+#pragma unroll
+  for (int x = 0; x < DK / 16; ++x) st[x] = floatx4{0, 0, 0, 0};
+  const double total = chunks<T, DK, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, m);
+  const long unit = ((long)b * most + i) * a.h + head;
+  float *to = parts + unit * DK * a.dv;
+#pragma unroll
+  for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) to[state_at<DK>(a, x, r, col0)] = st[x][r];
+  if (col0 == 0 && threadIdx.x == 0) sums[unit] = total;
+}
+
+// In the place of each segment's part the state that it starts from. Four values a thread.
+__global__ void __launch_bounds__(THREADS) join_kernel(LinearAttn a, float *parts, const double *sums, int most) {
+  const int b = blockIdx.z, head = blockIdx.y;
+  const Sequence s = sequence(a, b);
+  const la::Segments seg = la::segments(s.len);
+  const long size = (long)a.dk * a.dv, at = ((long)blockIdx.x * THREADS + threadIdx.x) * 4;
+  if (s.len <= la::STEP || seg.count == 1 || at >= size) return;
+  floatx4 st = {0, 0, 0, 0};
+  if (s.slot >= 0) st = *reinterpret_cast<const floatx4 *>(a.state_in + (s.slot * a.h + head) * size + at);
+  for (int i = 0; i < seg.count; ++i) {
+    const long unit = ((long)b * most + i) * a.h + head;
+    floatx4 *p = reinterpret_cast<floatx4 *>(parts + unit * size + at);
+    floatx4 next = st;
+    if (i < seg.count - 1) {
+      const Factor f = factor_of(sums[unit]);
+      next = *p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) next[e] += times(st[e], f);
+    }
+    *p = st;
+    st = next;
+  }
+}
+
+template <typename T, int DK>
+__global__ void __launch_bounds__(THREADS) chunk_kernel(LinearAttn a, const float *parts, int most) {
+  __shared__ Chunk<DK> m;
+  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / COLS;
+  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * COLS;
+  const Sequence s = sequence(a, b);
+  if (s.len <= la::STEP) {
+    if (i == 0) step_body<T, DK>(a, s, head, col0, &m.q[0][0]);
+    return;
+  }
+  const la::Segments seg = la::segments(s.len);
+  if (i >= seg.count) return;
+  const float *from = seg.count > 1 ? parts + (((long)b * most + i) * a.h + head) * DK * a.dv
+                      : s.slot >= 0 ? a.state_in + (s.slot * a.h + head) * DK * a.dv : nullptr;
+  floatx4 st[DK / 16];
+#pragma unroll
+  for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) st[x][r] = from ? from[state_at<DK>(a, x, r, col0)] : 0.f;
+  chunks<T, DK, true>(a, s, head, col0, i * seg.tokens, min((i + 1) * seg.tokens, s.len), st, m);
+  if (i == seg.count - 1 && s.slot >= 0) {
+    float *to = a.state_out + (s.slot * a.h + head) * DK * a.dv;
+#pragma unroll
+    for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to[state_at<DK>(a, x, r, col0)] = st[x][r];
+  }
+}
+
+template <typename T, int DK>
+hipError_t run(const LinearAttn &a, hipStream_t s) {
+  const unsigned x = (unsigned)(a.h * (a.dv / COLS));
+  if (a.max_len <= la::STEP) {
+    step_kernel<T, DK><<<dim3(x, a.num_seqs), dim3(THREADS), 0, s>>>(a);
+    return hipGetLastError();
+  }
+  const int most = la::most_segments(a.max_len);
+  if (most > 1) {
+    segment_kernel<T, DK><<<dim3(x, most - 1, a.num_seqs), dim3(THREADS), 0, s>>>(a, a.parts, a.sums, most);
+    const unsigned y = (unsigned)dx_ceil_div((long)a.dk * a.dv, 4 * THREADS);
+    join_kernel<<<dim3(y, a.h, a.num_seqs), dim3(THREADS), 0, s>>>(a, a.parts, a.sums, most);
+  }
+  chunk_kernel<T, DK><<<dim3(x, most, a.num_seqs), dim3(THREADS), 0, s>>>(a, a.parts, most);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t by_dim(const LinearAttn &a, hipStream_t s) {
+  if (a.dk == 64) return run<T, 64>(a, s);
+  if (a.dk == 128) return run<T, 128>(a, s);
+  return run<T, 256>(a, s);
+}
+
+}  // namespace
+
+hipError_t dx_linear_attn_launch(const LinearAttn &a, bool f32, hipStream_t s) {
+  return f32 ? by_dim<float>(a, s) : by_dim<uint16_t>(a, s);
+}

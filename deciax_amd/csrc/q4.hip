@@ -1,0 +1,351 @@
+// Weights in 4 bits with one scale and zero point a group, and products with them.
+//
+// Format: W[n, k] = scale (code - zero), code and zero 0..15; a group is 32, 64 or 128 neighbouring k of a row. Codes lie
+// in tiles of 16 rows and 128 columns, 1 KB each, [n / 16][k / 128][64 lanes][16 bytes]: lane 16 q + r holds row r, its
+// dword j the columns 32 j + 8 q + 0..7, which is the second operand of the j-th 16x16x32 product of the tile. Within a
+// dword the nibbles are the columns 0, 2, 4, 6, 1, 3, 5, 7, so that one shift, one mask and one or make two bf16 values.
+// A group's word [n / 16][k / group][16] is its scale (a bf16 or fp16 number) as fp32 with the zero in the lowest four
+// bits. Missing rows and columns of a tile have code 0; missing rows word 0.
+#include "common.h"
+#include "kernels.h"
+
+namespace {
+
+constexpr int WAVES = 8, THREADS = 64 * WAVES;
+
+DX_DEVICE floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+
+// Eight codes as bf16 numbers 8 + code / 2: a code's four bits are the highest of the mantissa of a number in [8, 16).
+DX_DEVICE u32x4 halves(uint32_t w) {
+  constexpr uint32_t MASK = 0x00780078u, EIGHT = 0x41004100u;
+  return u32x4{((w << 3) & MASK) | EIGHT, ((w >> 1) & MASK) | EIGHT, ((w >> 5) & MASK) | EIGHT,
+               ((w >> 9) & MASK) | EIGHT};
+}
+
+DX_DEVICE float scale_of(uint32_t word) { return __uint_as_float(word & ~15u); }
+DX_DEVICE float zero_of(uint32_t word) { return (float)(word & 15u); }
+
+// y = x W^T. A workgroup has 16 MT rows of x and 16 NT rows of W, wave w the tiles w, w + 8, .. of their columns; the
+// eight partial sums are added in their order. So the order of a sum goes by k alone, and a row of y depends on its row of
+// x alone, whatever MT and NT are.
+//
+// The products are of x and 8 + code / 2, both exact: with X the group's sum of x (one more product, by ones),
+// sum x (code - zero) = 2 (sum x (8 + code / 2) - (8 + zero / 2) X), the difference rounded once, and only then the scale.
+template <int MT, int NT, int SPG, int DEPTH, typename OUT>
+__global__ void __launch_bounds__(THREADS)
+linear_q4_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
+                 OUT *__restrict__ y, long m, int n, int k, long ldx, long ldy) {
+  constexpr int GROUPS = 4 / SPG;  // of a tile's columns
+  __shared__ float parts[WAVES][16][16 * NT + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = lane & 15, q = lane >> 4;
+  const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4, groups = k / (32 * SPG);
+  const int n0 = blockIdx.x * NT;
+  const long m0 = (long)blockIdx.y * (16 * MT);
+
+  const uint16_t *xr[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xr[i] = x + min(m0 + 16 * i + c, m - 1) * ldx + 8 * q;  // rows behind the last: not stored
+  const u32x4 *cp[NT];
+  const uint32_t *wp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const long tile = min(n0 + j, tiles_n - 1);
+    cp[j] = codes + tile * tiles_k * 64 + lane;
+    wp[j] = words + tile * groups * 16 + c;
+  }
+  const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  floatx4 sum[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sum[i][j] = floatx4{0, 0, 0, 0};
+
+  u32x4 raw[DEPTH][NT];
+  uint32_t word[DEPTH][NT][GROUPS];
+  auto load = [&](int t, int d) {
+    if (t >= tiles_k) return;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      raw[d][j] = cp[j][(long)t * 64];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) word[d][j][g] = wp[j][(long)min(t * GROUPS + g, groups - 1) * 16];
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) load(wave + d * WAVES, d);
+  for (int t0 = wave; t0 < tiles_k; t0 += DEPTH * WAVES) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int t = t0 + d * WAVES;
+      if (t >= tiles_k) break;
+      const int steps = min(4, (k - t * 128) >> 5);  // of 32 columns; whole groups
+      u32x4 xf[4][MT];
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s < steps)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) xf[s][i] = *reinterpret_cast<const u32x4 *>(xr[i] + t * 128 + 32 * s);
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        if (g * SPG >= steps) break;
+        floatx4 acc[MT][NT], xs[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          xs[i] = floatx4{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) xs[i] = mfma16(xf[s][i], ones, xs[i]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const u32x4 b = halves(raw[d][j][s]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(xf[s][i], b, acc[i][j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float s2 = 2.f * scale_of(word[d][j][g]), off = -8.f - 0.5f * zero_of(word[d][j][g]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[i][j][e] = fmaf(s2, fmaf(off, xs[i][e], acc[i][j][e]), sum[i][j][e]);
+        }
+      }
+      load(t + DEPTH * WAVES, d);
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    if (i > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) parts[wave][4 * q + e][16 * j + c] = sum[i][j][e];
+    __syncthreads();
+    for (int at = threadIdx.x; at < 256 * NT; at += THREADS) {
+      const int row = at / (16 * NT), col = at % (16 * NT);
+      const long r = m0 + 16 * i + row;
+      const int o = n0 * 16 + col;
+      if (r >= m || o >= n) continue;
+      float v = parts[0][row][col];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v += parts[w][row][col];
+      if constexpr (sizeof(OUT) == 2)
+        y[r * ldy + o] = f2bf(v);
+      else
+        y[r * ldy + o] = v;
+    }
+  }
+}
+
+// A wave lays out one tile: lane 16 q + r the codes of row r that linear_q4_kernel reads there. Once a weight, not tuned.
+struct Place {
+  int row, col;  // of the lane's first value of step 0
+  bool in;       // the row exists
+};
+
+DX_DEVICE Place place(long tile, int tiles_k, int n) {
+  const int lane = threadIdx.x & 63;
+  const int row = (int)(tile / tiles_k) * 16 + (lane & 15);
+  return Place{row, (int)(tile % tiles_k) * 128 + 8 * (lane >> 4), row < n};
+}
+
+DX_DEVICE uint32_t nibbles(const uint32_t (&code)[8]) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w |= code[e] << (4 * (e / 2) + 16 * (e % 2));
+  return w;
+}
+
+// Each group's range is widened to hold 0; scale = bf16((hi - lo) / 15), zero = round(-lo / scale), code = round(w / scale)
+// + zero, cut to 0..15 (the scale's own rounding can pass them by one). A group that holds an infinity or a NaN has a NaN
+// for its scale and reads as NaN; one whose scale rounds to 0 reads as 0.
+template <int SPG>
+__global__ void __launch_bounds__(256)
+quantize_q4_kernel(const uint16_t *__restrict__ w, long ldw, u32x4 *__restrict__ codes, uint32_t *__restrict__ words,
+                   int n, int k, long tiles) {
+  const long tile = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tile >= tiles) return;
+  const int tiles_k = (k + 127) >> 7, lane = threadIdx.x & 63, groups = k / (32 * SPG);
+  const Place p = place(tile, tiles_k, n);
+  float v[4][8];
+  float lo[4 / SPG], hi[4 / SPG];
+  bool fine[4 / SPG];
+#pragma unroll
+  for (int g = 0; g < 4 / SPG; ++g) {
+    lo[g] = hi[g] = 0.f;
+    fine[g] = true;
+#pragma unroll
+    for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
+      const int col = p.col + 32 * s;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[s][e] = 0.f;
+      if (p.in && col < k) {
+        const u32x4 r = *reinterpret_cast<const u32x4 *>(w + p.row * ldw + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[s][2 * e] = lo_bf(r[e]);
+          v[s][2 * e + 1] = hi_bf(r[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        lo[g] = fminf(lo[g], v[s][e]);
+        hi[g] = fmaxf(hi[g], v[s][e]);
+        fine[g] &= fabsf(v[s][e]) < INFINITY;
+      }
+    }
+#pragma unroll
+    for (int off = 16; off <= 32; off <<= 1) {  // the four lanes of a row
+      lo[g] = fminf(lo[g], __shfl_xor(lo[g], off, 64));
+      hi[g] = fmaxf(hi[g], __shfl_xor(hi[g], off, 64));
+      fine[g] &= __shfl_xor((int)fine[g], off, 64) != 0;
+    }
+  }
+  u32x4 out;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int g = s / SPG;
+    const float scale = round_bf(hi[g] / 15.f - lo[g] / 15.f);
+    const bool real = fine[g] && scale > 0.f;
+    const float zero = real ? fminf(rintf(-lo[g] / scale), 15.f) : 0.f;
+    uint32_t code[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      code[e] = real && p.in && p.col + 32 * s < k ? (uint32_t)fminf(fmaxf(rintf(v[s][e] / scale) + zero, 0.f), 15.f) : 0u;
+    out[s] = nibbles(code);
+    const int group = (p.col + 32 * s) / (32 * SPG);
+    if (s % SPG == 0 && lane < 16 && group < groups)
+      words[((tile / tiles_k) * groups + group) * 16 + lane] =
+          !p.in ? 0u : !fine[g] ? 0x7fc00000u : __float_as_uint(real ? scale : 0.f) | (uint32_t)zero;
+  }
+  codes[tile * 64 + lane] = out;
+}
+
+// Given codes (a byte each, its low four bits), scales (bf16, or fp16) and zeros (a byte a group; 8 without them).
+template <int SPG, bool HALF>
+__global__ void __launch_bounds__(256)
+pack_q4_kernel(const uint8_t *__restrict__ code, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros,
+               u32x4 *__restrict__ codes, uint32_t *__restrict__ words, int n, int k, long tiles) {
+  const long tile = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tile >= tiles) return;
+  const int tiles_k = (k + 127) >> 7, lane = threadIdx.x & 63, groups = k / (32 * SPG);
+  const Place p = place(tile, tiles_k, n);
+  u32x4 out;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int col = p.col + 32 * s;
+    uint32_t c[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = p.in && col < k ? code[(long)p.row * k + col + e] & 15u : 0u;
+    out[s] = nibbles(c);
+    const int group = col / (32 * SPG);
+    if (s % SPG == 0 && lane < 16 && group < groups) {
+      uint32_t word = 0;
+      if (p.in) {
+        const uint16_t b = scales[(long)p.row * groups + group];
+        const float scale = HALF ? (float)__builtin_bit_cast(_Float16, b) : bf2f(b);
+        word = (__float_as_uint(scale) & ~15u) | (zeros ? zeros[(long)p.row * groups + group] & 15u : 8u);
+      }
+      words[((tile / tiles_k) * groups + group) * 16 + lane] = word;
+    }
+  }
+  codes[tile * 64 + lane] = out;
+}
+
+template <int SPG>
+__global__ void __launch_bounds__(256)
+q4_values_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words, float *__restrict__ w, int n, int k,
+                 long ldw, long tiles) {
+  const long tile = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tile >= tiles) return;
+  const int tiles_k = (k + 127) >> 7, lane = threadIdx.x & 63, groups = k / (32 * SPG);
+  const Place p = place(tile, tiles_k, n);
+  const u32x4 raw = codes[tile * 64 + lane];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int col = p.col + 32 * s;
+    if (!p.in || col >= k) continue;
+    const uint32_t word = words[((tile / tiles_k) * groups + col / (32 * SPG)) * 16 + (lane & 15)];
+    const u32x4 h = halves(raw[s]);
+    const float off = 16.f + zero_of(word);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[p.row * ldw + col + 2 * e] = (2.f * lo_bf(h[e]) - off) * scale_of(word);
+      w[p.row * ldw + col + 2 * e + 1] = (2.f * hi_bf(h[e]) - off) * scale_of(word);
+    }
+  }
+}
+
+template <int MT, int NT, int SPG, int DEPTH>
+hipError_t run(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
+  const dim3 grid((unsigned)dx_ceil_div(w.n, 16 * NT), (unsigned)dx_ceil_div(m, 16 * MT));
+  const u32x4 *codes = static_cast<const u32x4 *>(w.codes);
+  if (f32)
+    linear_q4_kernel<MT, NT, SPG, DEPTH, float>
+        <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<float *>(y), m, w.n, w.k, ldx, ldy);
+  else
+    linear_q4_kernel<MT, NT, SPG, DEPTH, uint16_t>
+        <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<uint16_t *>(y), m, w.n, w.k, ldx, ldy);
+  return hipGetLastError();
+}
+
+template <int SPG>
+hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
+  if (m <= 16) return run<1, 1, SPG, 4>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 32) return run<2, 1, SPG, 2>(w, x, y, m, ldx, ldy, f32, s);
+  return run<4, 4, SPG, 1>(w, x, y, m, ldx, ldy, f32, s);
+}
+
+inline long tiles_of(const Q4Weight &w) { return (long)dx_ceil_div(w.n, 16) * dx_ceil_div(w.k, 128); }
+
+}  // namespace
+
+hipError_t dx_linear_q4_launch(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32,
+                               hipStream_t s) {
+  if (w.group == 32) return by_rows<1>(w, x, y, m, ldx, ldy, f32, s);
+  if (w.group == 64) return by_rows<2>(w, x, y, m, ldx, ldy, f32, s);
+  return by_rows<4>(w, x, y, m, ldx, ldy, f32, s);
+}
+
+hipError_t dx_quantize_q4_launch(const Q4Weight &w, const uint16_t *values, long ldw, hipStream_t s) {
+  const long tiles = tiles_of(w);
+  const dim3 grid((unsigned)dx_ceil_div(tiles, 4));
+  u32x4 *codes = static_cast<u32x4 *>(w.codes);
+  auto go = [&](auto kernel) { kernel<<<grid, dim3(256), 0, s>>>(values, ldw, codes, w.words, w.n, w.k, tiles); };
+  if (w.group == 32) go(quantize_q4_kernel<1>);
+  else if (w.group == 64) go(quantize_q4_kernel<2>);
+  else go(quantize_q4_kernel<4>);
+  return hipGetLastError();
+}
+
+hipError_t dx_pack_q4_launch(const Q4Weight &w, const uint8_t *code, const uint16_t *scales, bool half,
+                             const uint8_t *zeros, hipStream_t s) {
+  const long tiles = tiles_of(w);
+  const dim3 grid((unsigned)dx_ceil_div(tiles, 4));
+  u32x4 *codes = static_cast<u32x4 *>(w.codes);
+  auto go = [&](auto kernel) { kernel<<<grid, dim3(256), 0, s>>>(code, scales, zeros, codes, w.words, w.n, w.k, tiles); };
+  if (w.group == 32) half ? go(pack_q4_kernel<1, true>) : go(pack_q4_kernel<1, false>);
+  else if (w.group == 64) half ? go(pack_q4_kernel<2, true>) : go(pack_q4_kernel<2, false>);
+  else half ? go(pack_q4_kernel<4, true>) : go(pack_q4_kernel<4, false>);
+  return hipGetLastError();
+}
+
+hipError_t dx_q4_values_launch(const Q4Weight &w, float *values, long ldw, hipStream_t s) {
+  const long tiles = tiles_of(w);
+  const dim3 grid((unsigned)dx_ceil_div(tiles, 4));
+  const u32x4 *codes = static_cast<const u32x4 *>(w.codes);
+  auto go = [&](auto kernel) { kernel<<<grid, dim3(256), 0, s>>>(codes, w.words, values, w.n, w.k, ldw, tiles); };
+  if (w.group == 32) go(q4_values_kernel<1>);
+  else if (w.group == 64) go(q4_values_kernel<2>);
+  else go(q4_values_kernel<4>);
+  return hipGetLastError();
+}

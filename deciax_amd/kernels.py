@@ -9,9 +9,11 @@ asynchronously on `torch.cuda.current_stream()`.
 
 from __future__ import annotations
 
+import math
 import weakref
-from collections.abc import Sequence
+from collections.abc import Mapping, Sequence
 from ctypes import byref
+from typing import Any
 
 import torch
 
@@ -915,6 +917,287 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0,
              at + 4 * rows, ids.data_ptr() or at, at + 8 * rows, DX_BF16 if dtype == BF16 else DX_F32, ws.data_ptr(),
              ws.numel())
     return logprobs, entropy, ids, top_logprobs
+
+
+# ---------------------------------------------------------------------------- a token layer: 4-bit weights, rotation, state
+
+
+class Q4Weight:
+    """A weight [n, k] in 4 bits (`dx_linear_q4`, the header states the format): `codes` uint8 [ceil(n / 16),
+    ceil(k / 128), 64, 16] and `groups` int32 [ceil(n / 16), k / group, 16]. `quantize_q4` makes one from bf16, `pack_q4`
+    from given codes, scales and zeros. The arrays are looked over once, here, and stay."""
+
+    __slots__ = ("_arrays", "n", "k", "group", "index", "_at")
+    codes = property(lambda self: self._arrays[0])
+    groups = property(lambda self: self._arrays[1])
+
+    def __init__(self, codes: torch.Tensor, groups: torch.Tensor, n: int, k: int) -> None:
+        if n < 1 or k < 1 or groups.dim() != 3 or groups.shape[1] < 1 or k % groups.shape[1]:
+            raise ValueError("Q4Weight: groups must be [ceil(n / 16), k / group, 16]")
+        tiles = -(-n // 16)
+        if codes.shape != (tiles, -(-k // 128), 64, 16) or groups.shape != (tiles, groups.shape[1], 16):
+            raise ValueError(f"Q4Weight: codes {tuple(codes.shape)} and groups {tuple(groups.shape)} are not those of a "
+                             f"weight of {n} x {k}")
+        index = codes.get_device()
+        if codes.dtype != torch.uint8 or not codes.is_contiguous():
+            raise ValueError("Q4Weight: codes must be contiguous uint8")
+        if groups.dtype != torch.int32 or groups.get_device() != index or not groups.is_contiguous():
+            raise ValueError("Q4Weight: groups must be contiguous int32 on the codes' device")
+        self._arrays = codes, groups
+        self.n, self.k, self.group, self.index = n, k, k // groups.shape[1], index
+        if self.group not in (32, 64, 128):
+            raise ValueError(f"Q4Weight: groups of {self.group}, not 32, 64 or 128")
+        self._at = codes.data_ptr(), groups.data_ptr()
+
+
+def _q4_empty(n: int, k: int, group: int, device: torch.device) -> Q4Weight:
+    if group not in (32, 64, 128) or n < 1 or k < 1 or k % group:
+        raise ValueError(f"a weight of {n} x {k} has no groups of {group}: 32, 64 or 128, dividing k")
+    tiles = -(-n // 16)
+    return Q4Weight(torch.empty((tiles, -(-k // 128), 64, 16), dtype=torch.uint8, device=device),
+                    torch.empty((tiles, k // group, 16), dtype=torch.int32, device=device), n, k)
+
+
+def _stride(t: torch.Tensor, name: str, width: int) -> int:
+    """Row stride of a 2-D view; one row has no next one."""
+    stride = _rows(t, name) if t.shape[1] > 1 else t.stride(0)
+    return stride if t.shape[0] > 1 else -(-width // 8) * 8
+
+
+def quantize_q4(w: torch.Tensor, *, group: int = 128) -> Q4Weight:
+    """A bf16 weight [n, k] in 4 bits, one scale and zero for `group` (32, 64 or 128) neighbouring k (see
+    dx_q4_quantize)."""
+    _need(w, "w", BF16, 2)
+    q = _q4_empty(w.shape[0], w.shape[1], group, w.device)
+    _call_on(q.index, "dx_q4_quantize", w.data_ptr(), _stride(w, "w", q.k), *q._at, q.n, q.k, group)
+    return q
+
+
+def pack_q4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> Q4Weight:
+    """scales[n, g] (codes[n, k] - zeros[n, g]) as a weight in 4 bits: codes uint8 [n, k] of 0..15, scales bf16 or fp16
+    [n, k / group], zeros uint8 [n, k / group] of 0..15 (default: 8)."""
+    _need(codes, "codes", torch.uint8, 2)
+    n, k = codes.shape
+    if scales.dtype not in (BF16, torch.float16):
+        raise ValueError(f"pack_q4: scales must be bf16 or fp16, got {scales.dtype}")
+    _need(scales, "scales", scales.dtype, 2)
+    if scales.shape[0] != n or scales.shape[1] < 1 or k % scales.shape[1]:
+        raise ValueError(f"pack_q4: scales {tuple(scales.shape)} do not divide codes {tuple(codes.shape)}")
+    if zeros is not None:
+        _need(zeros, "zeros", torch.uint8, 2)
+        if zeros.shape != scales.shape:
+            raise ValueError("pack_q4: one zero a scale")
+    if any(t is not None and t.device != codes.device for t in (scales, zeros)):
+        raise ValueError("pack_q4: codes, scales and zeros must be on one device")
+    q = _q4_empty(n, k, k // scales.shape[1], codes.device)
+    codes, scales = codes.contiguous(), scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    _call_on(q.index, "dx_q4_pack", codes.data_ptr(), scales.data_ptr(), int(scales.dtype == torch.float16), _ptr(zeros),
+             *q._at, n, k, q.group)
+    return q
+
+
+def q4_values(weight: Q4Weight) -> torch.Tensor:
+    """The numbers that a weight in 4 bits stands for, fp32 [n, k]."""
+    if weight.index < 0:
+        raise ValueError("q4_values: the weight must be in device (HIP) memory")
+    out = torch.empty((weight.n, weight.k), dtype=F32, device=weight.codes.device)
+    _call_on(weight.index, "dx_q4_values", *weight._at, out.data_ptr(), weight.k, weight.n, weight.k, weight.group)
+    return out
+
+
+def linear_q4(x: torch.Tensor, weight: Q4Weight, *, out: torch.Tensor | None = None,
+              out_dtype: torch.dtype = BF16) -> torch.Tensor:
+    """`x @ w.T` for bf16 rows x [m, k] and a weight in 4 bits: `linear` of the numbers that it stands for, with exact
+    products and fp32 sums, rounded once to `out_dtype` (bf16 or fp32; see dx_linear_q4). A row of the result depends on
+    its row of x alone. `out` must not meet x."""
+    index, n, k = weight.index, weight.n, weight.k
+    if index < 0:
+        raise ValueError("linear_q4: the weight must be in device (HIP) memory")
+    if x.dim() != 2 or x.dtype != BF16 or x.get_device() != index or x.shape[1] != k:
+        raise ValueError(f"linear_q4: x must be bf16 [m, {k}] on the weight's device, got {x.dtype} {tuple(x.shape)} on "
+                         f"{x.device}")
+    if out_dtype not in (BF16, F32):
+        raise ValueError(f"linear_q4: out_dtype must be bf16 or fp32, got {out_dtype}")
+    m = x.shape[0]
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    elif out.dtype != out_dtype or out.get_device() != index or out.shape != (m, n):
+        raise ValueError(f"linear_q4: out must be {out_dtype} [{m}, {n}] on x's device, got {out.dtype} "
+                         f"{tuple(out.shape)} on {out.device}")
+    elif _meet(out, x):
+        raise ValueError("linear_q4: out must not meet x")
+    if m == 0:
+        return out
+    _call_on(index, "dx_linear_q4", x.data_ptr(), *weight._at, out.data_ptr(), m, n, k, weight.group, _stride(x, "x", k),
+             _stride(out, "out", n), DX_BF16 if out_dtype == BF16 else DX_F32)
+    return out
+
+
+def rope_frequencies(rotary_dim: int, *, theta: float = 10000.0, scaling: Mapping[str, Any] | None = None,
+                     device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq fp64 [rotary_dim / 2], attention factor) of `qk_norm_rope`: theta ** (-2 j / rotary_dim) radians a
+    position, scaled for long contexts as a configuration's `rope_scaling` says:
+
+    {"rope_type": "default"}   as they are
+    {"rope_type": "linear", "factor": f}   positions divided by f
+    {"rope_type": "yarn", "factor": f, "original_max_position_embeddings": n, "beta_fast": 32, "beta_slow": 1,
+     "attention_factor": 0.1 ln f + 1}   pairs that turn less than beta_slow times within n positions divided by f, those
+        that turn more than beta_fast times kept, a ramp over j between
+    {"rope_type": "llama3", "factor": f, "original_max_position_embeddings": n, "low_freq_factor": 1,
+     "high_freq_factor": 4}   the same, with a ramp over the number of turns"""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rope_frequencies: rotary_dim {rotary_dim} must be even and positive")
+    if not theta > 0:
+        raise ValueError(f"rope_frequencies: theta must be > 0, got {theta}")
+    pair = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    inv_freq = theta ** (-2.0 * pair / rotary_dim)
+    options = dict(scaling or {})
+    kind = options.get("rope_type", options.get("type", "default"))
+    factor, attention = float(options.get("factor", 1.0)), 1.0
+    if kind not in ("default", "linear", "yarn", "llama3"):
+        raise ValueError(f"rope_frequencies: unknown rope_type {kind!r}")
+    if not factor >= 1.0:
+        raise ValueError(f"rope_frequencies: factor must be >= 1, got {factor}")
+    if kind == "linear":
+        inv_freq = inv_freq / factor
+    elif kind in ("yarn", "llama3"):
+        if "original_max_position_embeddings" not in options:
+            raise ValueError(f"rope_frequencies: {kind} needs original_max_position_embeddings")
+        length = float(options["original_max_position_embeddings"])
+        turns = length * inv_freq / (2 * math.pi)
+        if kind == "yarn":
+            # pair j turns `beta` times within the length at j = rotary_dim ln(length / (2 pi beta)) / (2 ln theta)
+            def at(beta: float) -> float:
+                return rotary_dim * math.log(length / (2 * math.pi * beta)) / (2 * math.log(theta))
+
+            low = max(math.floor(at(float(options.get("beta_fast", 32.0)))), 0)
+            high = min(math.ceil(at(float(options.get("beta_slow", 1.0)))), rotary_dim - 1)
+            keep = 1.0 - ((pair - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+            given = options.get("attention_factor")
+            attention = 0.1 * math.log(factor) + 1.0 if given is None else float(given)
+        else:
+            least, most = float(options.get("low_freq_factor", 1.0)), float(options.get("high_freq_factor", 4.0))
+            if not most > least:
+                raise ValueError("rope_frequencies: high_freq_factor must be above low_freq_factor")
+            keep = ((turns - least) / (most - least)).clamp(0.0, 1.0)
+        inv_freq = inv_freq * (keep + (1.0 - keep) / factor)
+    return inv_freq.to(device), attention
+
+
+def qk_norm_rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, num_q_heads: int,
+                 num_kv_heads: int, head_dim: int, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, eps: float = 1e-6, layout: str = "half",
+                 attention_factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The q and k heads of rows x [rows, >= (Hq + Hkv) * D] (bf16 or fp32; a packed q | k | v projection, say): with
+    `q_norm` and `k_norm` ([D], x's type) each head's RMSNorm (1 + w) first, then its first 2 * len(inv_freq) dimensions
+    turned by positions[row] (int32) * inv_freq (fp64, `rope_frequencies`), as pairs (j, j + half) or, with
+    layout="interleaved", (2 j, 2 j + 1), cos and sin times `attention_factor` (see dx_qk_norm_rope). In place, as `rope`,
+    or into `out` [rows, >= (Hq + Hkv) * D], which must not meet x; columns behind the heads are left as they are."""
+    dtype = x.dtype
+    if dtype not in (BF16, F32):
+        raise ValueError(f"qk_norm_rope: x must be bf16 or fp32, got {dtype}")
+    index = x.get_device()
+    if x.dim() != 2 or index < 0:
+        raise ValueError("qk_norm_rope: x must be a 2-D device (HIP) tensor")
+    rows, width = x.shape[0], (num_q_heads + num_kv_heads) * head_dim
+    if num_q_heads < 0 or num_kv_heads < 0 or x.shape[1] < width:
+        raise ValueError(f"qk_norm_rope: rows of {x.shape[1]} do not hold {num_q_heads} + {num_kv_heads} heads of {head_dim}")
+    if positions.dtype != torch.int32 or positions.shape != (rows,) or positions.get_device() != index or \
+            not positions.is_contiguous():
+        raise ValueError(f"qk_norm_rope: positions must be contiguous int32 [{rows}] on x's device")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.get_device() != index or \
+            not inv_freq.is_contiguous():
+        raise ValueError("qk_norm_rope: inv_freq must be contiguous fp64 [rotary_dim / 2] on x's device")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"qk_norm_rope: layout must be 'half' or 'interleaved', got {layout!r}")
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("qk_norm_rope: q_norm and k_norm go together")
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is not None and (t.dtype != dtype or t.shape != (head_dim,) or t.get_device() != index or
+                              not t.is_contiguous()):
+            raise ValueError(f"qk_norm_rope: {name} must be contiguous {dtype} [{head_dim}] on x's device")
+    xs = _stride(x, "x", width)
+    if out is None:
+        out = x
+    if out is x:
+        os = xs
+    else:
+        if out.dim() != 2 or out.dtype != dtype or out.get_device() != index or out.shape[0] < rows or \
+                out.shape[1] < width:
+            raise ValueError(f"qk_norm_rope: out must be {dtype} [>= {rows}, >= {width}] on x's device, got {out.dtype} "
+                             f"{tuple(out.shape)} on {out.device}")
+        os = _stride(out, "out", width)
+        if (out.data_ptr(), os) != (x.data_ptr(), xs) and _meet(out, x):
+            raise ValueError("qk_norm_rope: out must be x itself or have memory of its own")
+    if rows == 0 or width == 0:
+        return out
+    _call_on(index, "dx_qk_norm_rope", x.data_ptr(), out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr() or None,
+             _ptr(q_norm), _ptr(k_norm), rows, num_q_heads, num_kv_heads, head_dim, 2 * inv_freq.shape[0], xs, os, eps,
+             attention_factor, int(layout == "interleaved"), DX_BF16 if dtype == BF16 else DX_F32)
+    return out
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
+                     seq_start: torch.Tensor, seq_len: torch.Tensor, max_seq_len: int, *, num_k_heads: int,
+                     num_heads: int, k_dim: int, v_dim: int, scale: float, state_index: torch.Tensor | None = None,
+                     state_out: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """S_t = e^g_t S_(t-1) + k_t v_t^T, o_t = scale q_t S_t over packed sequences (see dx_linear_attn): q, k
+    [rows, >= Hk * Dk] and v [rows, >= H * Dv], bf16 or fp32, g = decay [rows, H] fp32 (log decays, <= 0; rows may be one
+    row expanded), states fp32 [states, H, Dk, Dv]. Sequence b goes on from state[state_index[b]] (default: b) and leaves
+    its state in `state_out` (default: `state` itself). One token a sequence and whole prompts take the same call. Returns
+    [rows, H * Dv]; rows of no sequence are not written, `out` must not meet q, k or v."""
+    dtype, index = q.dtype, q.get_device()
+    if dtype not in (BF16, F32):
+        raise ValueError(f"linear_attention: q must be bf16 or fp32, got {dtype}")
+    if q.dim() != 2 or index < 0:
+        raise ValueError("linear_attention: q must be a 2-D device (HIP) tensor")
+    rows, kw, vw = q.shape[0], num_k_heads * k_dim, num_heads * v_dim
+    if num_k_heads < 1 or num_heads < 1 or num_heads % num_k_heads:
+        raise ValueError(f"linear_attention: num_heads {num_heads} must be a positive multiple of num_k_heads {num_k_heads}")
+    for t, name, width in ((q, "q", kw), (k, "k", kw), (v, "v", vw)):
+        if t.dim() != 2 or t.dtype != dtype or t.get_device() != index or t.shape[0] != rows or t.shape[1] < width:
+            raise ValueError(f"linear_attention: {name} must be {dtype} [{rows}, >= {width}] on q's device, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+    if decay.dtype != F32 or decay.get_device() != index or decay.shape != (rows, num_heads) or \
+            (num_heads > 1 and decay.stride(1) != 1):
+        raise ValueError(f"linear_attention: decay must be fp32 [{rows}, {num_heads}] on q's device, heads side by side")
+    shape = (num_heads, k_dim, v_dim)
+    for t, name in ((state, "state"), (state_out, "state_out")):
+        if t is not None and (t.dtype != F32 or t.get_device() != index or t.dim() != 4 or t.shape[1:] != shape or
+                              not t.is_contiguous() or t.shape != state.shape):
+            raise ValueError(f"linear_attention: {name} must be contiguous fp32 [states, {num_heads}, {k_dim}, {v_dim}] on "
+                             f"q's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    seqs = seq_start.shape[0] if seq_start.dim() == 1 else -1
+    for t, name in ((seq_start, "seq_start"), (seq_len, "seq_len"), (state_index, "state_index")):
+        if t is not None and (t.dtype != torch.int32 or t.get_device() != index or t.shape != (seqs,) or
+                              not t.is_contiguous()):
+            raise ValueError(f"linear_attention: {name} must be contiguous int32 [sequences] on q's device")
+    if state_index is None and state.shape[0] < seqs:
+        raise ValueError(f"linear_attention: {state.shape[0]} states for {seqs} sequences")
+    if out is None:
+        out = torch.empty((rows, vw), dtype=dtype, device=q.device)
+    elif out.dim() != 2 or out.dtype != dtype or out.get_device() != index or out.shape[0] < rows or out.shape[1] < vw:
+        raise ValueError(f"linear_attention: out must be {dtype} [>= {rows}, >= {vw}] on q's device, got {out.dtype} "
+                         f"{tuple(out.shape)} on {out.device}")
+    elif _meet(out, q) or _meet(out, k) or _meet(out, v):
+        raise ValueError("linear_attention: out must not meet q, k or v")
+    if state_out is None:
+        state_out = state
+    elif state_out.data_ptr() != state.data_ptr() and _meet(state, state_out):
+        raise ValueError("linear_attention: state_out must be state itself or have memory of its own")
+    if seqs == 0:
+        return out
+    ds = decay.stride(0) if rows > 1 else num_heads
+    ws = _bytes(_lib.lib().dx_linear_attn_workspace(seqs, max_seq_len, num_heads, k_dim, v_dim), q.device)
+    spare = ws.data_ptr()  # stands in for the arrays of no rows or no states, which have no address
+    _call_on(index, "dx_linear_attn", q.data_ptr() or spare, k.data_ptr() or spare, v.data_ptr() or spare,
+             decay.data_ptr() or spare, out.data_ptr() or spare + 16, state.data_ptr() or spare,
+             state_out.data_ptr() or spare, seq_start.data_ptr(), seq_len.data_ptr(), _ptr(state_index), seqs, max_seq_len,
+             state.shape[0], rows, num_k_heads, num_heads, k_dim, v_dim, _stride(q, "q", kw), _stride(k, "k", kw),
+             _stride(v, "v", vw), ds, _stride(out, "out", vw), scale, DX_BF16 if dtype == BF16 else DX_F32, spare,
+             ws.numel())
+    return out
 
 
 # ---------------------------------------------------------------------------- Clef joint head (fp32)

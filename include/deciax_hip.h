@@ -617,6 +617,105 @@ int dx_token_logprobs(const void *logits, const int32_t *targets, int64_t rows,
 
 int64_t dx_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top);
 
+/* ------------------------------------------------------------------------ */
+/* A token layer: weights in 4 bits, head norms with rotation, kept states    */
+/* ------------------------------------------------------------------------ */
+
+/* Weights in 4 bits: W[n, k] = scale (code - zero), code and zero 0..15, one
+ * scale and zero for `group` (32, 64 or 128) neighbouring k of a row; k a
+ * multiple of the group, n any.
+ * codes: bytes [ceil(n / 16)][ceil(k / 128)][64][16], a tile of 16 rows and 128
+ * columns in 1 KB: lane 16 q + r of its 64 has row r, its 32-bit word j the
+ * columns 32 j + 8 q + 0..7, as nibbles from the lowest up: columns 0, 2, 4, 6,
+ * 1, 3, 5, 7. Missing rows and columns have code 0.
+ * groups: 32-bit words [ceil(n / 16)][k / group][16], the scale (a bf16 or fp16
+ * number) as fp32 with the zero in its lowest four bits; missing rows 0.
+ * No counterpart in the reference, whose weights are bf16.
+ *
+ * dx_q4_quantize: from bf16 rows. A group's range, widened to hold 0, is cut
+ * into 15 steps: scale = bf16((hi - lo) / 15), zero = round(-lo / scale), code =
+ * round(w / scale) + zero, cut to 0..15. A group with an infinity or a NaN reads
+ * as NaN, one whose scale rounds to 0 as 0.
+ * dx_q4_pack: from given codes [n, k] (a byte each, low four bits), scales
+ * [n, k / group] (bf16, or fp16) and zeros [n, k / group] (bytes; null: 8).
+ * dx_q4_values: the numbers that the weight stands for, fp32 [n, k]. */
+int dx_q4_quantize(const void *w, int64_t w_row_stride, void *codes,
+                   void *groups, int32_t n, int32_t k, int32_t group,
+                   void *stream);
+
+int dx_q4_pack(const uint8_t *code, const void *scales, int32_t scales_fp16,
+               const uint8_t *zeros, void *codes, void *groups, int32_t n,
+               int32_t k, int32_t group, void *stream);
+
+int dx_q4_values(const void *codes, const void *groups, float *w,
+                 int64_t w_row_stride, int32_t n, int32_t k, int32_t group,
+                 void *stream);
+
+/* y[m, n] = x W^T for bf16 rows x and a weight in 4 bits, as dx_linear
+ * (src/deciax/nn.py:11-19): exact products, fp32 sums, one rounding to out_dtype
+ * (DX_BF16 or DX_F32). The order of a sum goes by k alone: a row of y depends on
+ * its row of x, whatever m is. n is any size, y rows need no alignment. A row of
+ * x with an infinity or a NaN, or whose sums of 16 x over a group pass fp32's
+ * range, gives infinities or NaN in its own row of y. */
+int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y,
+                 int64_t m, int32_t n, int32_t k, int32_t group,
+                 int64_t x_row_stride, int64_t y_row_stride, int32_t out_dtype,
+                 void *stream);
+
+/* Norms of query and key heads and the rotation by position in one pass, over
+ * rows of q | k heads (columns behind them are not touched). Per head
+ *   u = x / sqrt(mean(x^2) + eps) (1 + w), w = q_norm or k_norm [head_dim]
+ * of x's type (both null: u = x); then its first rotary_dim dimensions turn by
+ * the angle positions[row] * inv_freq[j] (fp64 [rotary_dim / 2], radians a
+ * position; the angle is taken in 64 bits), cos and sin times attention_factor:
+ * dimensions j and j + rotary_dim / 2, or 2 j and 2 j + 1 when `interleaved`.
+ * Replaces the q / k norms and the partial rotation of
+ * src/deciax/models/qwen3_5/text.py:75-91 and `apply_rope`
+ * (src/deciax/nn.py:35-44). rotary_dim is a multiple of 16 up to head_dim;
+ * fp32 throughout, rounded once to dtype. out is x itself (same row stride) or
+ * memory that does not meet it. */
+int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
+                    const double *inv_freq, const void *q_norm,
+                    const void *k_norm, int64_t rows, int32_t num_q_heads,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                    int64_t x_row_stride, int64_t out_row_stride, float eps,
+                    float attention_factor, int32_t interleaved, int32_t dtype,
+                    void *stream);
+
+/* Linear attention with a decay for each token and head, over packed sequences
+ * with a kept state of fixed size:
+ *   S_t = e^g_t S_(t-1) + k_t v_t^T,   o_t = scale q_t S_t
+ * per head, S fp32 [k_dim, v_dim], g = decay[row * decay_row_stride + head] (fp32;
+ * a row stride of 0: the same for every token; -inf, and anything below -1e4,
+ * forgets the state). q and k rows hold num_k_heads heads of k_dim, shared by
+ * num_heads / num_k_heads heads each; v and out rows num_heads of v_dim; k_dim and
+ * v_dim 64, 128 or 256. The token recurrence without the delta rule of
+ * src/deciax/kernels/gdn/reference.py:24-37, and its chunked form :40-92.
+ * Sequence b has rows seq_start[b] .. + seq_len[b] (one that reaches outside the
+ * `rows` has none) and the state state_index[b] of num_states (null: b) of
+ * state_in, state_out: [num_states][num_heads][k_dim][v_dim]; an index outside
+ * starts from zeros and is not kept, and no two sequences may share one.
+ * state_out is state_in itself or memory that does not meet it; a sequence of no
+ * tokens keeps its state. One token a sequence and whole prompts take the same
+ * call; results do not depend on the batch. A NaN or infinity in a token's row
+ * does not reach earlier tokens. max_seq_len bounds the grid: longer device
+ * lengths are cut to it. Workspace size from dx_linear_attn_workspace. */
+int dx_linear_attn(const void *q, const void *k, const void *v,
+                   const float *decay, void *out, const float *state_in,
+                   float *state_out, const int32_t *seq_start,
+                   const int32_t *seq_len, const int32_t *state_index,
+                   int32_t num_seqs, int32_t max_seq_len, int32_t num_states,
+                   int64_t rows, int32_t num_k_heads, int32_t num_heads,
+                   int32_t k_dim, int32_t v_dim, int64_t q_row_stride,
+                   int64_t k_row_stride, int64_t v_row_stride,
+                   int64_t decay_row_stride, int64_t out_row_stride,
+                   float scale, int32_t dtype, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+
+int64_t dx_linear_attn_workspace(int32_t num_seqs, int32_t max_seq_len,
+                                 int32_t num_heads, int32_t k_dim,
+                                 int32_t v_dim);
+
 #ifdef __cplusplus
 }
 #endif
