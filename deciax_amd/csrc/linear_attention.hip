@@ -237,6 +237,399 @@ DX_DEVICE double chunks(const LinearAttn &a, const Sequence &s, int head, int co
   return total;
 }
 
+// ------------------------------------------------------------------------------------------ bf16, chunks of 64 tokens
+//
+// bf16 products (16x16x32: lane l has row or column l % 16 of an operand and eight k of group g = l / 16; of the result
+// column l % 16, rows 4 g + r). Wave w has the columns 16 NC w .. of the state, in registers, as results S[DK rows, column].
+//   Weights P^T = K Q^T: wave w the queries 16 w .., all earlier keys. A lane holds keys 4 g + r of a query, which is what
+//     the product O^T = V^T P^T takes as eight k when V is read back transposed by the same rows; P goes through LDS as
+//     two bf16 parts, since every wave needs all of it.
+//   O^T += S^T Q^T: two tiles of S are eight k of a lane as they lie, again as two bf16 parts; Q is read by the same rows.
+//   S = K^T (w V): both read transposed; w V, w = e^(G_C - G_j), as three bf16 parts: the state keeps fp32's precision.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+DX_DEVICE floatx4 mfma16(bf16x8 x, bf16x8 y, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+
+// 16 lanes read four rows of 16 values, lane i gets column i.
+DX_DEVICE s16x4 read_transposed(const uint16_t *p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
+#else
+  return s16x4{};
+#endif
+}
+
+// A barrier for what went through LDS alone: loads of the next chunk stay on their way.
+DX_DEVICE void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Rows of W values in 16-byte chunks, chunk c of row r at c ^ f(r): 16 rows' reads of one chunk, and eight rows' transposed
+// reads of two neighbouring ones, fall on all banks (a line of them is 16 chunks).
+template <int W>
+DX_DEVICE int place(int r, int c) {
+  const int f = W == 64 ? ((r >> 1) & 3) << 1 | ((r >> 3) & 1) : (r & 7) << 1 | ((r >> 3) & 1);
+  return r * W + ((c ^ f) << 3);
+}
+
+DX_DEVICE bf16x8 both(s16x4 x, s16x4 y) {
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Columns 16 t .. of the rows 32 a + 4 g .. and 32 a + 16 + 4 g .. as eight k.
+template <int W>
+DX_DEVICE bf16x8 columns(const uint16_t *rows, int a, int t) {
+  const int lane = threadIdx.x & 63, c = lane & 15, r = 32 * a + 4 * (lane >> 4) + (c >> 2);
+  const uint16_t *p = rows + place<W>(r, 2 * t + ((c >> 1) & 1)) + (c & 1) * 4;
+  return both(read_transposed(p), read_transposed(p + 16 * W));  // 16 rows on: the same place
+}
+
+// x = the sum of N bf16 parts, nearly: what N parts cannot hold is below 2^(-8 N) of it.
+template <int N>
+DX_DEVICE void split(const float (&x)[8], bf16x8 (&out)[N]) {
+  float rest[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = x[e];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = pack_bf2(rest[2 * e], rest[2 * e + 1]);
+      if (n + 1 < N) {
+        rest[2 * e] -= lo_bf(w[e]);
+        rest[2 * e + 1] -= hi_bf(w[e]);
+      }
+    }
+    out[n] = as_bf16x8(w);
+  }
+}
+
+template <int DK, int NC>
+struct Tile {
+  static constexpr int TOKENS = 64, W = COLS * NC;
+  uint16_t q[TOKENS * DK], k[TOKENS * DK], v[TOKENS * W];
+  u32x4 p[4][2][2][64];  // [16 queries][32 keys][part][lane]
+  struct Decay {
+    double sum[TOKENS];  // of g, in powers of two
+    float from_start[TOKENS], to_end[TOKENS];
+    Factor all;
+    double total;
+  } decay[2];  // this chunk's and the next one's
+  int lost[2];
+};
+
+// A chunk's rows on their way from memory.
+template <int DK, int NC, bool OUT>
+struct Fetched {
+  static constexpr int KI = DK / 32, VI = 2 * NC;
+  u32x4 q[OUT ? KI : 1], k[KI], v[VI];
+  float g;
+
+  DX_DEVICE void load(const LinearAttn &a, long row, int n, int head, int kh, int col0) {
+    const int tid = threadIdx.x;
+    const u32x4 none = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
+      const bool in = r < n;
+      if (OUT)
+        q[i] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.q) + (row + r) * a.qs + kh * DK + 8 * c)
+                  : none;
+      k[i] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.k) + (row + r) * a.ks + kh * DK + 8 * c)
+                : none;
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
+      v[i] = r < n ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.v) + (row + r) * a.vs +
+                                                      head * a.dv + col0 + 8 * c)
+                   : none;
+    }
+    if (tid < 64) g = tid < n ? a.decay[(row + tid) * a.ds + head] : 0.f;
+  }
+
+  // The first wave's: what the chunk's decays come to.
+  DX_DEVICE void sums(typename Tile<DK, NC>::Decay &d) const {
+    const int lane = threadIdx.x;
+    double x = (double)decay_of(g) * 1.4426950408889634;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const double y = __shfl_up(x, off, 64);
+      if (lane >= off) x += y;
+    }
+    const double end = __shfl(x, 63, 64);
+    d.sum[lane] = x;
+    d.from_start[lane] = fast_exp2((float)x);
+    d.to_end[lane] = fast_exp2((float)(end - x));
+    if (lane == 0) {
+      d.all = factor_of(end * 0.6931471805599453);
+      d.total = end;
+    }
+  }
+
+  DX_DEVICE void store(Tile<DK, NC> &m, int par) const {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
+      if (OUT) *reinterpret_cast<u32x4 *>(m.q + place<DK>(r, c)) = q[i];
+      *reinterpret_cast<u32x4 *>(m.k + place<DK>(r, c)) = k[i];
+    }
+    bool lost = false;
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
+      *reinterpret_cast<u32x4 *>(m.v + place<COLS * NC>(r, c)) = v[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        lost |= (v[i][e] & 0x7f80u) == 0x7f80u || (v[i][e] & 0x7f800000u) == 0x7f800000u;
+    }
+    if (OUT && lost) m.lost[par] = 1;
+  }
+};
+
+// Tokens [t0, t1) of a sequence from the state st on; OUT: with their outputs. Returns the sum of their g, in powers of two.
+template <int DK, int NC, bool OUT>
+DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col0, int t0, int t1,
+                       floatx4 (&st)[DK / 16][NC], Tile<DK, NC> &m) {
+  constexpr int N = 64, W = COLS * NC;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int kh = head / (a.h / a.hk);
+  double total = 0.0;
+  Fetched<DK, NC, OUT> f;
+  f.load(a, s.start + t0, min(N, t1 - t0), head, kh, col0);
+  if (tid < 2) m.lost[tid] = 0;
+  if (wave == 0) f.sums(m.decay[0]);
+  lds_barrier();
+  int par = 0;
+  for (int t = t0; t < t1; t += N, par ^= 1) {
+    const int n = min(N, t1 - t);
+    const long row = s.start + t;
+    f.store(m, par);
+    lds_barrier();
+    if (t + N < t1) f.load(a, row + N, min(N, t1 - t - N), head, kh, col0);
+    const typename Tile<DK, NC>::Decay &d = m.decay[par];
+    total += d.total;
+    floatx4 o[4][NC];
+    if constexpr (OUT) {
+      bf16x8 qf[DK / 32];
+#pragma unroll
+      for (int x = 0; x < DK / 32; ++x)
+        qf[x] = as_bf16x8(*reinterpret_cast<const u32x4 *>(m.q + place<DK>(16 * wave + c, 4 * x + g)));
+      const double mine = d.sum[16 * wave + c];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if (2 * b > wave) break;
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = 32 * b + 16 * j;
+          floatx4 w = {0, 0, 0, 0};
+          if (2 * b + j <= wave)
+#pragma unroll
+            for (int x = 0; x < DK / 32; ++x)
+              w = mfma16(as_bf16x8(*reinterpret_cast<const u32x4 *>(m.k + place<DK>(key + c, 4 * x + g))), qf[x], w);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = key + 4 * g + r;
+            p[4 * j + r] = at <= 16 * wave + c ? w[r] * fast_exp2((float)(mine - d.sum[at])) : 0.f;
+          }
+        }
+        bf16x8 parts[2];
+        split(p, parts);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) m.p[wave][b][x][lane] = __builtin_bit_cast(u32x4, parts[x]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < NC; ++x) o[i][x] = floatx4{0, 0, 0, 0};
+#pragma unroll
+      for (int x = 0; x < DK / 32; ++x) {
+        bf16x8 sf[NC][2], qx[4];
+#pragma unroll
+        for (int y = 0; y < NC; ++y) {
+          float both_tiles[8];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            both_tiles[r] = st[2 * x][y][r];
+            both_tiles[4 + r] = st[2 * x + 1][y][r];
+          }
+          split(both_tiles, sf[y]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint16_t *p0 = m.q + place<DK>(16 * i + c, 4 * x + (g >> 1)) + (g & 1) * 4;
+          const uint16_t *p1 = m.q + place<DK>(16 * i + c, 4 * x + 2 + (g >> 1)) + (g & 1) * 4;
+          qx[i] = both(*reinterpret_cast<const s16x4 *>(p0), *reinterpret_cast<const s16x4 *>(p1));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int y = 0; y < NC; ++y)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) o[i][y] = mfma16(sf[y][z], qx[i], o[i][y]);
+      }
+    }
+    if (wave == 0 && t + N < t1) f.sums(m.decay[par ^ 1]);
+    lds_barrier();
+    bf16x8 vf[2][NC];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int y = 0; y < NC; ++y) vf[b][y] = columns<W>(m.v, b, NC * wave + y);
+    if constexpr (OUT) {
+      const bool lost = m.lost[par];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float from = d.from_start[16 * i + c];
+#pragma unroll
+        for (int y = 0; y < NC; ++y)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[i][y][r] *= from;
+        if (!lost) {
+#pragma unroll
+          for (int b = 0; b <= i / 2; ++b)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const bf16x8 p = as_bf16x8(m.p[i][b][x][lane]);
+#pragma unroll
+              for (int y = 0; y < NC; ++y) o[i][y] = mfma16(vf[b][y], p, o[i][y]);
+            }
+        } else {  // a weight of 0 would carry a later token's infinity or NaN to this one
+          for (int j = 0; j <= 16 * i + c; ++j) {
+            const int other = c + 16 * ((j & 15) >> 2), e = (j & 3) + 4 * ((j >> 4) & 1);
+            float p = 0.f;
+            for (int x = 0; x < 2; ++x) p += bf2f(reinterpret_cast<const uint16_t *>(&m.p[i][j >> 5][x][other])[e]);
+            for (int y = 0; y < NC; ++y)
+              for (int r = 0; r < 4; ++r) {
+                const int col = 16 * (NC * wave + y) + 4 * g + r;
+                o[i][y][r] = fmaf(p, bf2f(m.v[place<W>(j, col >> 3) + (col & 7)]), o[i][y][r]);
+              }
+          }
+        }
+        if (16 * i + c < n) {
+          uint16_t *out = static_cast<uint16_t *>(a.out) + (row + 16 * i + c) * a.os + head * a.dv + col0 + 4 * g;
+#pragma unroll
+          for (int y = 0; y < NC; ++y)
+            *reinterpret_cast<u32x2 *>(out + 16 * (NC * wave + y)) =
+                u32x2{pack_bf2(a.scale * o[i][y][0], a.scale * o[i][y][1]), pack_bf2(a.scale * o[i][y][2], a.scale * o[i][y][3])};
+        }
+      }
+      if (tid == 0) m.lost[par ^ 1] = 0;
+    }
+    const Factor all = d.all;
+#pragma unroll
+    for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+      for (int y = 0; y < NC; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[x][y][r] = times(st[x][y][r], all);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      bf16x8 wv[NC][3];
+      const floatx4 w0 = *reinterpret_cast<const floatx4 *>(d.to_end + 32 * b + 4 * g);
+      const floatx4 w1 = *reinterpret_cast<const floatx4 *>(d.to_end + 32 * b + 16 + 4 * g);
+#pragma unroll
+      for (int y = 0; y < NC; ++y) {
+        const u32x4 raw = __builtin_bit_cast(u32x4, vf[b][y]);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = lo_bf(raw[e]) * (e < 2 ? w0[2 * e] : w1[2 * e - 4]);
+          x[2 * e + 1] = hi_bf(raw[e]) * (e < 2 ? w0[2 * e + 1] : w1[2 * e - 3]);
+        }
+        split(x, wv[y]);
+      }
+#pragma unroll
+      for (int x = 0; x < DK / 16; ++x) {
+        const bf16x8 kt = columns<DK>(m.k, b, x);
+#pragma unroll
+        for (int y = 0; y < NC; ++y)
+#pragma unroll
+          for (int z = 2; z >= 0; --z) st[x][y] = mfma16(kt, wv[y][z], st[x][y]);
+      }
+    }
+    lds_barrier();
+  }
+  return total;
+}
+
+// Element r of the wave's result tile (x, y) in a state.
+template <int NC>
+DX_DEVICE long tile_at(const LinearAttn &a, int x, int y, int r, int col0) {
+  const int lane = threadIdx.x & 63;
+  return (long)(16 * x + 4 * (lane >> 4) + r) * a.dv + col0 + 16 * (NC * (threadIdx.x >> 6) + y) + (lane & 15);
+}
+
+template <int DK, int NC>
+__global__ void __launch_bounds__(THREADS) segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
+  __shared__ __align__(16) Tile<DK, NC> m;
+  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / (COLS * NC);
+  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * (COLS * NC);
+  const Sequence s = sequence(a, b);
+  const la::Segments seg = la::segments(s.len);
+  if (s.len <= la::STEP || i >= seg.count - 1) return;
+  floatx4 st[DK / 16][NC];
+#pragma unroll
+  for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+    for (int y = 0; y < NC; ++y) st[x][y] = floatx4{0, 0, 0, 0};
+  const double total = tiles<DK, NC, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, m);
+  const long unit = ((long)b * most + i) * a.h + head;
+  float *to = parts + unit * DK * a.dv;
+#pragma unroll
+  for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+    for (int y = 0; y < NC; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to[tile_at<NC>(a, x, y, r, col0)] = st[x][y][r];
+  if (col0 == 0 && threadIdx.x == 0) sums[unit] = total * 0.6931471805599453;
+}
+
+template <int DK, int NC>
+__global__ void __launch_bounds__(THREADS) chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
+  __shared__ __align__(16) Tile<DK, NC> m;
+  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / (COLS * NC);
+  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * (COLS * NC);
+  const Sequence s = sequence(a, b);
+  if (s.len <= la::STEP) {
+    if (i > 0) return;
+    for (int y = 0; y < NC; ++y) {
+      if (y > 0) __syncthreads();
+      step_body<uint16_t, DK>(a, s, head, col0 + COLS * y, reinterpret_cast<float *>(&m));
+    }
+    return;
+  }
+  const la::Segments seg = la::segments(s.len);
+  if (i >= seg.count) return;
+  const float *from = seg.count > 1 ? parts + (((long)b * most + i) * a.h + head) * DK * a.dv
+                      : s.slot >= 0 ? a.state_in + (s.slot * a.h + head) * DK * a.dv : nullptr;
+  floatx4 st[DK / 16][NC];
+#pragma unroll
+  for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+    for (int y = 0; y < NC; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[x][y][r] = from ? from[tile_at<NC>(a, x, y, r, col0)] : 0.f;
+  tiles<DK, NC, true>(a, s, head, col0, i * seg.tokens, min((i + 1) * seg.tokens, s.len), st, m);
+  if (i == seg.count - 1 && s.slot >= 0) {
+    float *to = a.state_out + (s.slot * a.h + head) * DK * a.dv;
+#pragma unroll
+    for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+      for (int y = 0; y < NC; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[tile_at<NC>(a, x, y, r, col0)] = st[x][y][r];
+  }
+}
+
+// ------------------------------------------------------------------------------------------ segments
+
 // What each segment but the last adds to the state, and the sum of its g.
 template <typename T, int DK>
 __global__ void __launch_bounds__(THREADS) segment_kernel(LinearAttn a, float *parts, double *sums, int most) {
@@ -314,18 +707,31 @@ __global__ void __launch_bounds__(THREADS) chunk_kernel(LinearAttn a, const floa
 
 template <typename T, int DK>
 hipError_t run(const LinearAttn &a, hipStream_t s) {
-  const unsigned x = (unsigned)(a.h * (a.dv / COLS));
+  unsigned x = (unsigned)(a.h * (a.dv / COLS));
   if (a.max_len <= la::STEP) {
     step_kernel<T, DK><<<dim3(x, a.num_seqs), dim3(THREADS), 0, s>>>(a);
     return hipGetLastError();
   }
   const int most = la::most_segments(a.max_len);
+  const bool two = sizeof(T) == 2 && a.dv > COLS;  // columns of a workgroup: 2 COLS, which read each row of q and k once
+  if (two) x /= 2;
+  const dim3 grid(x, most, a.num_seqs), before(x, most - 1, a.num_seqs), block(THREADS);
   if (most > 1) {
-    segment_kernel<T, DK><<<dim3(x, most - 1, a.num_seqs), dim3(THREADS), 0, s>>>(a, a.parts, a.sums, most);
+    if constexpr (sizeof(T) == 2) {
+      if (two) segment_bf16_kernel<DK, 2><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
+      else segment_bf16_kernel<DK, 1><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
+    } else {
+      segment_kernel<T, DK><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
+    }
     const unsigned y = (unsigned)dx_ceil_div((long)a.dk * a.dv, 4 * THREADS);
-    join_kernel<<<dim3(y, a.h, a.num_seqs), dim3(THREADS), 0, s>>>(a, a.parts, a.sums, most);
+    join_kernel<<<dim3(y, a.h, a.num_seqs), block, 0, s>>>(a, a.parts, a.sums, most);
   }
-  chunk_kernel<T, DK><<<dim3(x, most, a.num_seqs), dim3(THREADS), 0, s>>>(a, a.parts, most);
+  if constexpr (sizeof(T) == 2) {
+    if (two) chunk_bf16_kernel<DK, 2><<<grid, block, 0, s>>>(a, a.parts, most);
+    else chunk_bf16_kernel<DK, 1><<<grid, block, 0, s>>>(a, a.parts, most);
+  } else {
+    chunk_kernel<T, DK><<<grid, block, 0, s>>>(a, a.parts, most);
+  }
   return hipGetLastError();
 }
 
