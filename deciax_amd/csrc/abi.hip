@@ -1163,6 +1163,10 @@ int dx_linear_attn(const void *q, const void *k, const void *v, const float *dec
   REQUIRE(q_row_stride >= kw && k_row_stride >= kw && v_row_stride >= vw && out_row_stride >= vw &&
               q_row_stride % vec == 0 && k_row_stride % vec == 0 && v_row_stride % vec == 0 && out_row_stride % vec == 0,
           "linear_attn: row strides must cover heads * dim and be multiples of %ld elements", (long)vec);
+  const int64_t most_stride = INT64_C(1) << 24;
+  SUPPORTED(q_row_stride < most_stride && k_row_stride < most_stride && v_row_stride < most_stride &&
+                out_row_stride < most_stride,
+            "linear_attn: row strides of 2^24 elements or more");
   REQUIRE(decay_row_stride == 0 || decay_row_stride >= num_heads, "linear_attn: decay rows of %ld for %d heads",
           (long)decay_row_stride, num_heads);
   REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(state_in) && aligned16(state_out),

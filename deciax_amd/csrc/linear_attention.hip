@@ -70,9 +70,10 @@ DX_DEVICE void step_body(const LinearAttn &a, const Sequence &s, int head, int c
   const long at = ((s.slot * a.h + head) * DK + r) * (long)a.dv + col0 + 4 * c;
   floatx4 st[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-    st[i] = s.slot < 0 ? floatx4{0, 0, 0, 0}
-                       : *reinterpret_cast<const floatx4 *>(a.state_in + at + 16L * i * a.dv);
+  for (int i = 0; i < R; ++i) st[i] = floatx4{0, 0, 0, 0};
+  if (s.slot >= 0)  // one branch around all loads
+#pragma unroll
+    for (int i = 0; i < R; ++i) st[i] = *reinterpret_cast<const floatx4 *>(a.state_in + at + 16L * i * a.dv);
   for (int t = 0; t < s.len; ++t) {
     const long row = s.start + t;
     const T *q = static_cast<const T *>(a.q) + row * a.qs + kh * DK, *k = static_cast<const T *>(a.k) + row * a.ks + kh * DK;
@@ -281,8 +282,8 @@ DX_DEVICE bf16x8 both(s16x4 x, s16x4 y) {
 
 // Columns 16 t .. of the rows 32 a + 4 g .. and 32 a + 16 + 4 g .. as eight k.
 template <int W>
-DX_DEVICE bf16x8 columns(const uint16_t *rows, int a, int t) {
-  const int lane = threadIdx.x & 63, c = lane & 15, r = 32 * a + 4 * (lane >> 4) + (c >> 2);
+DX_DEVICE bf16x8 columns(const uint16_t *rows, int a, int t, int lane) {
+  const int c = lane & 15, r = 32 * a + 4 * (lane >> 4) + (c >> 2);
   const uint16_t *p = rows + place<W>(r, 2 * t + ((c >> 1) & 1)) + (c & 1) * 4;
   return both(read_transposed(p), read_transposed(p + 16 * W));  // 16 rows on: the same place
 }
@@ -316,79 +317,78 @@ struct Tile {
   struct Decay {
     double sum[TOKENS];  // of g, in powers of two
     float from_start[TOKENS], to_end[TOKENS];
-    Factor all;
-    double total;
+    int shift;
+    double total, rest;  // of g; of the state's scale behind the chunk
   } decay[2];  // this chunk's and the next one's
-  int lost[2];
 };
 
-// A chunk's rows on their way from memory.
+// A chunk's rows on their way from memory. A row's place is a uniform address and 32 bits a lane (strides are below 2^24).
 template <int DK, int NC, bool OUT>
 struct Fetched {
-  static constexpr int KI = DK / 32, VI = 2 * NC;
+  static constexpr int KI = DK / 32, VI = 2 * NC, KR = THREADS / (DK / 8), VR = THREADS / (8 * NC);  // loads, rows a load
   u32x4 q[OUT ? KI : 1], k[KI], v[VI];
   float g;
 
-  DX_DEVICE void load(const LinearAttn &a, long row, int n, int head, int kh, int col0) {
-    const int tid = threadIdx.x;
+  DX_DEVICE static u32x4 at(const uint16_t *base, uint32_t bytes) {
+    return *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(base) + bytes);
+  }
+
+  DX_DEVICE void load(const LinearAttn &a, long row, int n, int head, int kh, int col0, int tid) {
     const u32x4 none = {0, 0, 0, 0};
+    const uint32_t kr = tid / (DK / 8), kc = 16 * (tid % (DK / 8)), vr = tid / (8 * NC), vc = 16 * (tid % (8 * NC));
+    const uint32_t qo = 2 * kr * (uint32_t)a.qs + kc, ko = 2 * kr * (uint32_t)a.ks + kc, vo = 2 * vr * (uint32_t)a.vs + vc;
+    const uint16_t *qp = static_cast<const uint16_t *>(a.q) + row * a.qs + kh * DK;
+    const uint16_t *kp = static_cast<const uint16_t *>(a.k) + row * a.ks + kh * DK;
+    const uint16_t *vp = static_cast<const uint16_t *>(a.v) + row * a.vs + head * a.dv + col0;
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
-      const int at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
-      const bool in = r < n;
-      if (OUT)
-        q[i] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.q) + (row + r) * a.qs + kh * DK + 8 * c)
-                  : none;
-      k[i] = in ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.k) + (row + r) * a.ks + kh * DK + 8 * c)
-                : none;
+      const bool in = (int)kr + KR * i < n;
+      if (OUT) q[i] = in ? at(qp + (long)(KR * i) * a.qs, qo) : none;
+      k[i] = in ? at(kp + (long)(KR * i) * a.ks, ko) : none;
     }
 #pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
-      v[i] = r < n ? *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.v) + (row + r) * a.vs +
-                                                      head * a.dv + col0 + 8 * c)
-                   : none;
-    }
+    for (int i = 0; i < VI; ++i) v[i] = (int)vr + VR * i < n ? at(vp + (long)(VR * i) * a.vs, vo) : none;
     if (tid < 64) g = tid < n ? a.decay[(row + tid) * a.ds + head] : 0.f;
   }
 
-  // The first wave's: what the chunk's decays come to.
-  DX_DEVICE void sums(typename Tile<DK, NC>::Decay &d) const {
+  // The first wave's: what the chunk's decays come to. The state is 2^x times what the registers hold: a chunk moves x, and
+  // the registers are shifted by whole powers of two when x leaves [-8, 8]. So no rounding of a decay is ever multiplied
+  // in, and a head that forgets slowly has nothing to multiply.
+  DX_DEVICE double sums(typename Tile<DK, NC>::Decay &d, double x, float log2_scale) const {
     const int lane = threadIdx.x;
-    double x = (double)decay_of(g) * 1.4426950408889634;
+    double sum = (double)decay_of(g) * 1.4426950408889634;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const double y = __shfl_up(x, off, 64);
-      if (lane >= off) x += y;
+      const double y = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += y;
     }
-    const double end = __shfl(x, 63, 64);
-    d.sum[lane] = x;
-    d.from_start[lane] = fast_exp2((float)x);
-    d.to_end[lane] = fast_exp2((float)(end - x));
+    const double end = __shfl(sum, 63, 64);
+    d.sum[lane] = sum;
+    d.from_start[lane] = fast_exp2((float)(sum + x + log2_scale));
+    x += end;
+    const double whole = x < -8.0 || x > 8.0 ? rint(x) : 0.0;
+    x -= whole;
+    d.to_end[lane] = fast_exp2((float)(end - sum - x));
     if (lane == 0) {
-      d.all = factor_of(end * 0.6931471805599453);
+      d.shift = (int)fmin(fmax(whole, -4096.0), 4096.0);
       d.total = end;
+      d.rest = x;
     }
+    return x;
   }
 
-  DX_DEVICE void store(Tile<DK, NC> &m, int par) const {
-    const int tid = threadIdx.x;
+  DX_DEVICE void store(Tile<DK, NC> &m, int tid) const {
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       const int at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
       if (OUT) *reinterpret_cast<u32x4 *>(m.q + place<DK>(r, c)) = q[i];
       *reinterpret_cast<u32x4 *>(m.k + place<DK>(r, c)) = k[i];
     }
-    bool lost = false;
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
       const int at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
       *reinterpret_cast<u32x4 *>(m.v + place<COLS * NC>(r, c)) = v[i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        lost |= (v[i][e] & 0x7f80u) == 0x7f80u || (v[i][e] & 0x7f800000u) == 0x7f800000u;
     }
-    if (OUT && lost) m.lost[par] = 1;
   }
 };
 
@@ -397,93 +397,100 @@ template <int DK, int NC, bool OUT>
 DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col0, int t0, int t1,
                        floatx4 (&st)[DK / 16][NC], Tile<DK, NC> &m) {
   constexpr int N = 64, W = COLS * NC;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kh = head / (a.h / a.hk);
-  double total = 0.0;
+  const float log2_scale = log2f(a.scale);
+  double total = 0.0, next = 0.0, rest = 0.0;  // next: the first wave's, behind the chunk that it has summed last
   Fetched<DK, NC, OUT> f;
-  f.load(a, s.start + t0, min(N, t1 - t0), head, kh, col0);
-  if (tid < 2) m.lost[tid] = 0;
-  if (wave == 0) f.sums(m.decay[0]);
-  lds_barrier();
+  f.load(a, s.start + t0, min(N, t1 - t0), head, kh, col0, threadIdx.x);
+  if (wave == 0) next = f.sums(m.decay[0], 0.0, log2_scale);
   int par = 0;
   for (int t = t0; t < t1; t += N, par ^= 1) {
     const int n = min(N, t1 - t);
     const long row = s.start + t;
-    f.store(m, par);
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // places in LDS are found again for every chunk: held over all of them they take registers
+    const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+    f.store(m, tid);
     lds_barrier();
-    if (t + N < t1) f.load(a, row + N, min(N, t1 - t - N), head, kh, col0);
+    if (t + N < t1) f.load(a, row + N, min(N, t1 - t - N), head, kh, col0, tid);
     const typename Tile<DK, NC>::Decay &d = m.decay[par];
     total += d.total;
     floatx4 o[4][NC];
     if constexpr (OUT) {
       bf16x8 qf[DK / 32];
 #pragma unroll
-      for (int x = 0; x < DK / 32; ++x)
-        qf[x] = as_bf16x8(*reinterpret_cast<const u32x4 *>(m.q + place<DK>(16 * wave + c, 4 * x + g)));
-      const double mine = d.sum[16 * wave + c];
+      for (int u = 0; u < DK / 32; ++u)
+        qf[u] = as_bf16x8(*reinterpret_cast<const u32x4 *>(m.q + place<DK>(16 * wave + c, 4 * u + g)));
+      const double mine = d.sum[16 * wave + c] + log2_scale;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         if (2 * b > wave) break;
+        floatx4 w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int u = 0; u < DK / 32; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)  // the second is hidden for the even waves' last: 0 by the mask below
+            w[j] = mfma16(as_bf16x8(*reinterpret_cast<const u32x4 *>(m.k + place<DK>(32 * b + 16 * j + c, 4 * u + g))), qf[u], w[j]);
         float p[8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = 32 * b + 16 * j;
-          floatx4 w = {0, 0, 0, 0};
-          if (2 * b + j <= wave)
-#pragma unroll
-            for (int x = 0; x < DK / 32; ++x)
-              w = mfma16(as_bf16x8(*reinterpret_cast<const u32x4 *>(m.k + place<DK>(key + c, 4 * x + g))), qf[x], w);
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int at = key + 4 * g + r;
-            p[4 * j + r] = at <= 16 * wave + c ? w[r] * fast_exp2((float)(mine - d.sum[at])) : 0.f;
+            const int at = 32 * b + 16 * j + 4 * g + r;
+            p[4 * j + r] = at <= 16 * wave + c ? w[j][r] * fast_exp2((float)(mine - d.sum[at])) : 0.f;
           }
-        }
         bf16x8 parts[2];
         split(p, parts);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) m.p[wave][b][x][lane] = __builtin_bit_cast(u32x4, parts[x]);
+        for (int z = 0; z < 2; ++z) m.p[wave][b][z][lane] = __builtin_bit_cast(u32x4, parts[z]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int x = 0; x < NC; ++x) o[i][x] = floatx4{0, 0, 0, 0};
+        for (int y = 0; y < NC; ++y) o[i][y] = floatx4{0, 0, 0, 0};
 #pragma unroll
-      for (int x = 0; x < DK / 32; ++x) {
+      for (int u = 0; u < DK / 32; ++u) {
+        __builtin_amdgcn_sched_barrier(0);  // what is read ahead has to fit the registers
         bf16x8 sf[NC][2], qx[4];
 #pragma unroll
         for (int y = 0; y < NC; ++y) {
-          float both_tiles[8];
+          float pair[8];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            both_tiles[r] = st[2 * x][y][r];
-            both_tiles[4 + r] = st[2 * x + 1][y][r];
+            pair[r] = st[2 * u][y][r];
+            pair[4 + r] = st[2 * u + 1][y][r];
           }
-          split(both_tiles, sf[y]);
+          split(pair, sf[y]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint16_t *p0 = m.q + place<DK>(16 * i + c, 4 * x + (g >> 1)) + (g & 1) * 4;
-          const uint16_t *p1 = m.q + place<DK>(16 * i + c, 4 * x + 2 + (g >> 1)) + (g & 1) * 4;
+          const uint16_t *p0 = m.q + place<DK>(16 * i + c, 4 * u + (g >> 1)) + (g & 1) * 4;
+          const uint16_t *p1 = m.q + place<DK>(16 * i + c, 4 * u + 2 + (g >> 1)) + (g & 1) * 4;
           qx[i] = both(*reinterpret_cast<const s16x4 *>(p0), *reinterpret_cast<const s16x4 *>(p1));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int z = 0; z < 2; ++z)
 #pragma unroll
-          for (int y = 0; y < NC; ++y)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int z = 0; z < 2; ++z) o[i][y] = mfma16(sf[y][z], qx[i], o[i][y]);
+            for (int y = 0; y < NC; ++y) o[i][y] = mfma16(sf[y][z], qx[i], o[i][y]);
       }
     }
-    if (wave == 0 && t + N < t1) f.sums(m.decay[par ^ 1]);
+    if (wave == 0 && t + N < t1) next = f.sums(m.decay[par ^ 1], next, log2_scale);
     lds_barrier();
     bf16x8 vf[2][NC];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int y = 0; y < NC; ++y) vf[b][y] = columns<W>(m.v, b, NC * wave + y);
+      for (int y = 0; y < NC; ++y) vf[b][y] = columns<W>(m.v, b, NC * wave + y, lane);
     if constexpr (OUT) {
-      const bool lost = m.lost[par];
+      const bf16x8 nothing = as_bf16x8(u32x4{0, 0, 0, 0});
+      floatx4 sum = {0, 0, 0, 0};  // 0 times each value: NaN where one is no finite number
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int y = 0; y < NC; ++y) sum = mfma16(nothing, vf[b][y], sum);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float from = d.from_start[16 * i + c];
@@ -491,44 +498,52 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
         for (int y = 0; y < NC; ++y)
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[i][y][r] *= from;
-        if (!lost) {
+      }
+      if (!__any(sum[0] != 0.f)) {
 #pragma unroll
-          for (int b = 0; b <= i / 2; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const bf16x8 p = as_bf16x8(m.p[i][b][x][lane]);
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int i = 2 * b; i < 4; ++i) {
+              const bf16x8 p = as_bf16x8(m.p[i][b][z][lane]);
 #pragma unroll
               for (int y = 0; y < NC; ++y) o[i][y] = mfma16(vf[b][y], p, o[i][y]);
             }
-        } else {  // a weight of 0 would carry a later token's infinity or NaN to this one
+      } else {  // a weight of 0 would carry a later token's infinity or NaN to this one
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
           for (int j = 0; j <= 16 * i + c; ++j) {
             const int other = c + 16 * ((j & 15) >> 2), e = (j & 3) + 4 * ((j >> 4) & 1);
             float p = 0.f;
-            for (int x = 0; x < 2; ++x) p += bf2f(reinterpret_cast<const uint16_t *>(&m.p[i][j >> 5][x][other])[e]);
+            for (int z = 0; z < 2; ++z) p += bf2f(reinterpret_cast<const uint16_t *>(&m.p[i][j >> 5][z][other])[e]);
+#pragma unroll
             for (int y = 0; y < NC; ++y)
+#pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const int col = 16 * (NC * wave + y) + 4 * g + r;
                 o[i][y][r] = fmaf(p, bf2f(m.v[place<W>(j, col >> 3) + (col & 7)]), o[i][y][r]);
               }
           }
-        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
         if (16 * i + c < n) {
-          uint16_t *out = static_cast<uint16_t *>(a.out) + (row + 16 * i + c) * a.os + head * a.dv + col0 + 4 * g;
+          uint16_t *base = static_cast<uint16_t *>(a.out) + (row + 16 * i) * a.os + head * a.dv + col0 + 16 * NC * wave;
+          char *out = reinterpret_cast<char *>(base) + 2 * ((uint32_t)c * (uint32_t)a.os + 4 * g);
 #pragma unroll
           for (int y = 0; y < NC; ++y)
-            *reinterpret_cast<u32x2 *>(out + 16 * (NC * wave + y)) =
-                u32x2{pack_bf2(a.scale * o[i][y][0], a.scale * o[i][y][1]), pack_bf2(a.scale * o[i][y][2], a.scale * o[i][y][3])};
+            *reinterpret_cast<u32x2 *>(out + 32 * y) = u32x2{pack_bf2(o[i][y][0], o[i][y][1]), pack_bf2(o[i][y][2], o[i][y][3])};
         }
-      }
-      if (tid == 0) m.lost[par ^ 1] = 0;
     }
-    const Factor all = d.all;
+    const int shift = __builtin_amdgcn_readfirstlane(d.shift);
+    if (shift != 0)
 #pragma unroll
-    for (int x = 0; x < DK / 16; ++x)
+      for (int u = 0; u < DK / 16; ++u)
 #pragma unroll
-      for (int y = 0; y < NC; ++y)
+        for (int y = 0; y < NC; ++y)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st[x][y][r] = times(st[x][y][r], all);
+          for (int r = 0; r < 4; ++r) st[u][y][r] = ldexpf(st[u][y][r], shift);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       bf16x8 wv[NC][3];
@@ -537,25 +552,39 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #pragma unroll
       for (int y = 0; y < NC; ++y) {
         const u32x4 raw = __builtin_bit_cast(u32x4, vf[b][y]);
-        float x[8];
+        float p[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[2 * e] = lo_bf(raw[e]) * (e < 2 ? w0[2 * e] : w1[2 * e - 4]);
-          x[2 * e + 1] = hi_bf(raw[e]) * (e < 2 ? w0[2 * e + 1] : w1[2 * e - 3]);
+          p[2 * e] = lo_bf(raw[e]) * (e < 2 ? w0[2 * e] : w1[2 * e - 4]);
+          p[2 * e + 1] = hi_bf(raw[e]) * (e < 2 ? w0[2 * e + 1] : w1[2 * e - 3]);
         }
-        split(x, wv[y]);
+        split(p, wv[y]);
       }
+      constexpr int AT_ONCE = 2;
 #pragma unroll
-      for (int x = 0; x < DK / 16; ++x) {
-        const bf16x8 kt = columns<DK>(m.k, b, x);
+      for (int u0 = 0; u0 < DK / 16; u0 += AT_ONCE) {
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 kt[AT_ONCE];
 #pragma unroll
-        for (int y = 0; y < NC; ++y)
+        for (int u = 0; u < AT_ONCE; ++u) kt[u] = columns<DK>(m.k, b, u0 + u, lane);
 #pragma unroll
-          for (int z = 2; z >= 0; --z) st[x][y] = mfma16(kt, wv[y][z], st[x][y]);
+        for (int z = 2; z >= 0; --z)
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int y = 0; y < NC; ++y) st[u0 + u][y] = mfma16(kt[u], wv[y][z], st[u0 + u][y]);
       }
     }
+    rest = d.rest;
     lds_barrier();
   }
+  const Factor scale = factor_of(rest * 0.6931471805599453);
+#pragma unroll
+  for (int u = 0; u < DK / 16; ++u)
+#pragma unroll
+    for (int y = 0; y < NC; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[u][y][r] = times(st[u][y][r], scale);
   return total;
 }
 
@@ -567,7 +596,7 @@ DX_DEVICE long tile_at(const LinearAttn &a, int x, int y, int r, int col0) {
 }
 
 template <int DK, int NC>
-__global__ void __launch_bounds__(THREADS) segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
+__global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
   __shared__ __align__(16) Tile<DK, NC> m;
   const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / (COLS * NC);
   const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * (COLS * NC);
@@ -592,7 +621,7 @@ __global__ void __launch_bounds__(THREADS) segment_bf16_kernel(LinearAttn a, flo
 }
 
 template <int DK, int NC>
-__global__ void __launch_bounds__(THREADS) chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
+__global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
   __shared__ __align__(16) Tile<DK, NC> m;
   const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / (COLS * NC);
   const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * (COLS * NC);
@@ -613,9 +642,14 @@ __global__ void __launch_bounds__(THREADS) chunk_bf16_kernel(LinearAttn a, const
 #pragma unroll
   for (int x = 0; x < DK / 16; ++x)
 #pragma unroll
-    for (int y = 0; y < NC; ++y)
+    for (int y = 0; y < NC; ++y) st[x][y] = floatx4{0, 0, 0, 0};
+  if (from)  // one branch around all loads
 #pragma unroll
-      for (int r = 0; r < 4; ++r) st[x][y][r] = from ? from[tile_at<NC>(a, x, y, r, col0)] : 0.f;
+    for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+      for (int y = 0; y < NC; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[x][y][r] = from[tile_at<NC>(a, x, y, r, col0)];
   tiles<DK, NC, true>(a, s, head, col0, i * seg.tokens, min((i + 1) * seg.tokens, s.len), st, m);
   if (i == seg.count - 1 && s.slot >= 0) {
     float *to = a.state_out + (s.slot * a.h + head) * DK * a.dv;
@@ -692,9 +726,12 @@ __global__ void __launch_bounds__(THREADS) chunk_kernel(LinearAttn a, const floa
                       : s.slot >= 0 ? a.state_in + (s.slot * a.h + head) * DK * a.dv : nullptr;
   floatx4 st[DK / 16];
 #pragma unroll
-  for (int x = 0; x < DK / 16; ++x)
+  for (int x = 0; x < DK / 16; ++x) st[x] = floatx4{0, 0, 0, 0};
+  if (from)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) st[x][r] = from ? from[state_at<DK>(a, x, r, col0)] : 0.f;
+    for (int x = 0; x < DK / 16; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[x][r] = from[state_at<DK>(a, x, r, col0)];
   chunks<T, DK, true>(a, s, head, col0, i * seg.tokens, min((i + 1) * seg.tokens, s.len), st, m);
   if (i == seg.count - 1 && s.slot >= 0) {
     float *to = a.state_out + (s.slot * a.h + head) * DK * a.dv;
