@@ -1165,8 +1165,8 @@ int dx_linear_attn(const void *q, const void *k, const void *v, const float *dec
           "linear_attn: row strides must cover heads * dim and be multiples of %ld elements", (long)vec);
   const int64_t most_stride = INT64_C(1) << 24;
   SUPPORTED(q_row_stride < most_stride && k_row_stride < most_stride && v_row_stride < most_stride &&
-                out_row_stride < most_stride,
-            "linear_attn: row strides of 2^24 elements or more");
+                out_row_stride < most_stride && decay_row_stride < most_stride / 4,
+            "linear_attn: row strides of 2^24 elements or more (decay: 2^22)");
   REQUIRE(decay_row_stride == 0 || decay_row_stride >= num_heads, "linear_attn: decay rows of %ld for %d heads",
           (long)decay_row_stride, num_heads);
   REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(state_in) && aligned16(state_out),

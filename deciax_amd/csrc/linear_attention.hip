@@ -322,39 +322,39 @@ struct Tile {
   } decay[2];  // this chunk's and the next one's
 };
 
-// A chunk's rows on their way from memory. A row's place is a uniform address and 32 bits a lane (strides are below 2^24).
+// A chunk's rows as a buffer of n of them: rows behind them read as zeros and are not written, without a branch. An offset
+// stays below 2^31, since strides are below 2^24.
+DX_DEVICE __amdgpu_buffer_rsrc_t rows_of(const uint16_t *first, int n, long stride) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)first, (short)0, (int)(n * stride * 2), 0x00020000);
+}
+
+// A chunk's rows on their way from memory.
 template <int DK, int NC, bool OUT>
 struct Fetched {
   static constexpr int KI = DK / 32, VI = 2 * NC, KR = THREADS / (DK / 8), VR = THREADS / (8 * NC);  // loads, rows a load
   u32x4 q[OUT ? KI : 1], k[KI], v[VI];
-  float g;
 
-  DX_DEVICE static u32x4 at(const uint16_t *base, uint32_t bytes) {
-    return *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(base) + bytes);
-  }
-
-  DX_DEVICE void load(const LinearAttn &a, long row, int n, int head, int kh, int col0, int tid) {
-    const u32x4 none = {0, 0, 0, 0};
+  DX_DEVICE void load(const LinearAttn &a, long row, int n, int head, int kh, int col0, uint32_t tid) {
+#if defined(__HIP_DEVICE_COMPILE__)
     const uint32_t kr = tid / (DK / 8), kc = 16 * (tid % (DK / 8)), vr = tid / (8 * NC), vc = 16 * (tid % (8 * NC));
-    const uint32_t qo = 2 * kr * (uint32_t)a.qs + kc, ko = 2 * kr * (uint32_t)a.ks + kc, vo = 2 * vr * (uint32_t)a.vs + vc;
-    const uint16_t *qp = static_cast<const uint16_t *>(a.q) + row * a.qs + kh * DK;
-    const uint16_t *kp = static_cast<const uint16_t *>(a.k) + row * a.ks + kh * DK;
-    const uint16_t *vp = static_cast<const uint16_t *>(a.v) + row * a.vs + head * a.dv + col0;
+    const uint32_t qs = 2 * (uint32_t)a.qs, ks = 2 * (uint32_t)a.ks, vs = 2 * (uint32_t)a.vs;
+    const auto qp = rows_of(static_cast<const uint16_t *>(a.q) + row * a.qs + kh * DK, n, a.qs);
+    const auto kp = rows_of(static_cast<const uint16_t *>(a.k) + row * a.ks + kh * DK, n, a.ks);
+    const auto vp = rows_of(static_cast<const uint16_t *>(a.v) + row * a.vs + head * a.dv + col0, n, a.vs);
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
-      const bool in = (int)kr + KR * i < n;
-      if (OUT) q[i] = in ? at(qp + (long)(KR * i) * a.qs, qo) : none;
-      k[i] = in ? at(kp + (long)(KR * i) * a.ks, ko) : none;
+      if (OUT) q[i] = __builtin_amdgcn_raw_buffer_load_b128(qp, (kr + KR * i) * qs + kc, 0, 0);
+      k[i] = __builtin_amdgcn_raw_buffer_load_b128(kp, (kr + KR * i) * ks + kc, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < VI; ++i) v[i] = (int)vr + VR * i < n ? at(vp + (long)(VR * i) * a.vs, vo) : none;
-    if (tid < 64) g = tid < n ? a.decay[(row + tid) * a.ds + head] : 0.f;
+    for (int i = 0; i < VI; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(vp, (vr + VR * i) * vs + vc, 0, 0);
+#endif
   }
 
   // The first wave's: what the chunk's decays come to. The state is 2^x times what the registers hold: a chunk moves x, and
   // the registers are shifted by whole powers of two when x leaves [-8, 8]. So no rounding of a decay is ever multiplied
   // in, and a head that forgets slowly has nothing to multiply.
-  DX_DEVICE double sums(typename Tile<DK, NC>::Decay &d, double x, float log2_scale) const {
+  DX_DEVICE static double sums(typename Tile<DK, NC>::Decay &d, float g, double x, float log2_scale) {
     const int lane = threadIdx.x;
     double sum = (double)decay_of(g) * 1.4426950408889634;
 #pragma unroll
@@ -377,16 +377,16 @@ struct Fetched {
     return x;
   }
 
-  DX_DEVICE void store(Tile<DK, NC> &m, int tid) const {
+  DX_DEVICE void store(Tile<DK, NC> &m, uint32_t tid) const {
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
-      const int at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
+      const uint32_t at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
       if (OUT) *reinterpret_cast<u32x4 *>(m.q + place<DK>(r, c)) = q[i];
       *reinterpret_cast<u32x4 *>(m.k + place<DK>(r, c)) = k[i];
     }
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
-      const int at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
+      const uint32_t at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
       *reinterpret_cast<u32x4 *>(m.v + place<COLS * NC>(r, c)) = v[i];
     }
   }
@@ -403,17 +403,36 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
   double total = 0.0, next = 0.0, rest = 0.0;  // next: the first wave's, behind the chunk that it has summed last
   Fetched<DK, NC, OUT> f;
   f.load(a, s.start + t0, min(N, t1 - t0), head, kh, col0, threadIdx.x);
-  if (wave == 0) next = f.sums(m.decay[0], 0.0, log2_scale);
+  // g of a chunk's tokens, a chunk earlier than its rows, so that no sum of them waits for the rows
+  auto decay = [&](int t) {
+    float g = 0.f;
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int n = max(min(N, t1 - t), 0), lane = threadIdx.x & 63;
+    const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)(a.decay + (s.start + t) * a.ds + head), (short)0,
+                                                        n > 0 ? (int)((n - 1) * a.ds + 1) * 4 : 0, 0x00020000);
+    g = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, 4 * (uint32_t)lane * (uint32_t)a.ds, 0, 0));
+#endif
+    return g;
+  };
+  auto sums = [&](typename Tile<DK, NC>::Decay &d, float g, int t, double x) {
+    return Fetched<DK, NC, OUT>::sums(d, t + (int)threadIdx.x < t1 ? g : 0.f, x, log2_scale);  // rows of stride 0 have no end
+  };
+  float g1 = decay(t0), g2 = decay(t0 + N);
+  if (wave == 0) next = sums(m.decay[0], g1, t0, 0.0);
+  // waited for here: the loop's own wait for these rows is then not one for the outputs stored before it
+  __builtin_amdgcn_s_waitcnt(0x0f70);
   int par = 0;
   for (int t = t0; t < t1; t += N, par ^= 1) {
     const int n = min(N, t1 - t);
     const long row = s.start + t;
-    int tid = threadIdx.x;
+    uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // places in LDS are found again for every chunk: held over all of them they take registers
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
     f.store(m, tid);
     lds_barrier();
-    if (t + N < t1) f.load(a, row + N, min(N, t1 - t - N), head, kh, col0, tid);
+    g1 = g2;
+    g2 = decay(t + 2 * N);
+    f.load(a, row + N, max(min(N, t1 - t - N), 0), head, kh, col0, tid);  // none behind the last chunk
     const typename Tile<DK, NC>::Decay &d = m.decay[par];
     total += d.total;
     floatx4 o[4][NC];
@@ -477,7 +496,7 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
             for (int y = 0; y < NC; ++y) o[i][y] = mfma16(sf[y][z], qx[i], o[i][y]);
       }
     }
-    if (wave == 0 && t + N < t1) next = f.sums(m.decay[par ^ 1], next, log2_scale);
+    if (wave == 0 && t + N < t1) next = sums(m.decay[par ^ 1], g1, t + N, next);
     lds_barrier();
     bf16x8 vf[2][NC];
 #pragma unroll
@@ -526,15 +545,16 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
               }
           }
       }
+#if defined(__HIP_DEVICE_COMPILE__)
+      const auto out = rows_of(static_cast<uint16_t *>(a.out) + row * a.os + head * a.dv + col0, n, a.os);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (16 * i + c < n) {
-          uint16_t *base = static_cast<uint16_t *>(a.out) + (row + 16 * i) * a.os + head * a.dv + col0 + 16 * NC * wave;
-          char *out = reinterpret_cast<char *>(base) + 2 * ((uint32_t)c * (uint32_t)a.os + 4 * g);
 #pragma unroll
-          for (int y = 0; y < NC; ++y)
-            *reinterpret_cast<u32x2 *>(out + 32 * y) = u32x2{pack_bf2(o[i][y][0], o[i][y][1]), pack_bf2(o[i][y][2], o[i][y][3])};
-        }
+        for (int y = 0; y < NC; ++y)
+          __builtin_amdgcn_raw_buffer_store_b64(
+              u32x2{pack_bf2(o[i][y][0], o[i][y][1]), pack_bf2(o[i][y][2], o[i][y][3])}, out,
+              2 * ((uint32_t)(16 * i + c) * (uint32_t)a.os + 16 * (NC * wave + y) + 4 * g), 0, 0);
+#endif
     }
     const int shift = __builtin_amdgcn_readfirstlane(d.shift);
     if (shift != 0)

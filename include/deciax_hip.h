@@ -699,8 +699,8 @@ int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
  * tokens keeps its state. One token a sequence and whole prompts take the same
  * call; results do not depend on the batch. A NaN or infinity in a token's row
  * does not reach earlier tokens. max_seq_len bounds the grid: longer device
- * lengths are cut to it. Row strides stay below 2^24 elements. Workspace size
- * from dx_linear_attn_workspace. */
+ * lengths are cut to it. Row strides stay below 2^24 elements, decay's
+ * below 2^22. Workspace size from dx_linear_attn_workspace. */
 int dx_linear_attn(const void *q, const void *k, const void *v,
                    const float *decay, void *out, const float *state_in,
                    float *state_out, const int32_t *seq_start,

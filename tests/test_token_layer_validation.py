@@ -101,7 +101,7 @@ def test_qk_norm_rope(bad, want) -> None:
     (dict(scale=math.nan), INVALID), (dict(scale=math.inf), INVALID), (dict(seqs=5), INVALID), (dict(qs=248), INVALID),
     (dict(ks=260), INVALID), (dict(vs=248), INVALID), (dict(os=252), INVALID), (dict(ds=3), INVALID),
     (dict(ds=-4), INVALID), (dict(qs=1 << 24), UNSUPPORTED), (dict(ks=1 << 24), UNSUPPORTED),
-    (dict(vs=1 << 24), UNSUPPORTED), (dict(os=1 << 24), UNSUPPORTED), (dict(q=ODD), INVALID), (dict(s_in=ODD), INVALID), (dict(s_out=ODD), INVALID),
+    (dict(vs=1 << 24), UNSUPPORTED), (dict(os=1 << 24), UNSUPPORTED), (dict(ds=1 << 22), UNSUPPORTED), (dict(q=ODD), INVALID), (dict(s_in=ODD), INVALID), (dict(s_out=ODD), INVALID),
     (dict(out=P), INVALID), (dict(seqs=3, most=2000, ws_bytes=1000), INVALID), (dict(seqs=3, most=2000, ws=None), INVALID),
     (dict(seqs=3, most=2000, ws=ODD), INVALID), (dict(), OK), (dict(ds=0), OK), (dict(ws=None, ws_bytes=0), OK)])
 def test_linear_attention(bad, want) -> None:
