@@ -35,6 +35,17 @@ DX_DEVICE Sequence sequence(const LinearAttn &a, int b) {
   return s;
 }
 
+// The head and the first column of a workgroup that has W of them. Those that read the same rows of q and k are hk apart
+// in the grid: where hk is a multiple of 8, on the same XCD, whose L2 holds the rows.
+struct Unit {
+  int head, col0;
+};
+template <int W>
+DX_DEVICE Unit unit(const LinearAttn &a) {
+  const int kh = blockIdx.x % a.hk, rest = blockIdx.x / a.hk, blocks = a.dv / W;
+  return Unit{kh * (a.h / a.hk) + rest / blocks, rest % blocks * W};
+}
+
 DX_DEVICE float decay_of(float g) { return g < NO_DECAY_BELOW ? NO_DECAY_BELOW : g; }
 
 template <typename T>
@@ -457,7 +468,8 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int at = 32 * b + 16 * j + 4 * g + r;
-            p[4 * j + r] = at <= 16 * wave + c ? w[j][r] * fast_exp2((float)(mine - d.sum[at])) : 0.f;
+            const float weight = w[j][r] * fast_exp2((float)(mine - d.sum[at]));  // before the choice: no branch around it
+            p[4 * j + r] = at <= 16 * wave + c ? weight : 0.f;
           }
         bf16x8 parts[2];
         split(p, parts);
@@ -618,8 +630,8 @@ DX_DEVICE long tile_at(const LinearAttn &a, int x, int y, int r, int col0) {
 template <int DK, int NC>
 __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
   __shared__ __align__(16) Tile<DK, NC> m;
-  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / (COLS * NC);
-  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * (COLS * NC);
+  const int b = blockIdx.z, i = blockIdx.y;
+  const auto [head, col0] = unit<COLS * NC>(a);
   const Sequence s = sequence(a, b);
   const la::Segments seg = la::segments(s.len);
   if (s.len <= la::STEP || i >= seg.count - 1) return;
@@ -643,8 +655,8 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) segment_bf16_kerne
 template <int DK, int NC>
 __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
   __shared__ __align__(16) Tile<DK, NC> m;
-  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / (COLS * NC);
-  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * (COLS * NC);
+  const int b = blockIdx.z, i = blockIdx.y;
+  const auto [head, col0] = unit<COLS * NC>(a);
   const Sequence s = sequence(a, b);
   if (s.len <= la::STEP) {
     if (i > 0) return;
@@ -688,8 +700,8 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(
 template <typename T, int DK>
 __global__ void __launch_bounds__(THREADS) segment_kernel(LinearAttn a, float *parts, double *sums, int most) {
   __shared__ Chunk<DK> m;
-  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / COLS;
-  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * COLS;
+  const int b = blockIdx.z, i = blockIdx.y;
+  const auto [head, col0] = unit<COLS>(a);
   const Sequence s = sequence(a, b);
   const la::Segments seg = la::segments(s.len);
   if (s.len <= la::STEP || i >= seg.count - 1) return;
@@ -733,8 +745,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(LinearAttn a, float *part
 template <typename T, int DK>
 __global__ void __launch_bounds__(THREADS) chunk_kernel(LinearAttn a, const float *parts, int most) {
   __shared__ Chunk<DK> m;
-  const int b = blockIdx.z, i = blockIdx.y, blocks = a.dv / COLS;
-  const int head = blockIdx.x / blocks, col0 = blockIdx.x % blocks * COLS;
+  const int b = blockIdx.z, i = blockIdx.y;
+  const auto [head, col0] = unit<COLS>(a);
   const Sequence s = sequence(a, b);
   if (s.len <= la::STEP) {
     if (i == 0) step_body<T, DK>(a, s, head, col0, &m.q[0][0]);
