@@ -291,6 +291,14 @@ DX_DEVICE bf16x8 both(s16x4 x, s16x4 y) {
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// Queries lie in the order in which two tiles of the state are eight k of a lane: chunk 4 u + g of a row has the dimensions
+// 32 u + 4 g .. and 32 u + 16 + 4 g .. (one read), where the four dimensions h of a row are half (h >> 2) & 1 of chunk
+// 4 u + (h & 3).
+template <int W>
+DX_DEVICE int q_half(int r, int h) {
+  return place<W>(r, 4 * (h >> 3) + (h & 3)) + ((h >> 2) & 1) * 4;
+}
+
 // Columns 16 t .. of the rows 32 a + 4 g .. and 32 a + 16 + 4 g .. as eight k.
 template <int W>
 DX_DEVICE bf16x8 columns(const uint16_t *rows, int a, int t, int lane) {
@@ -318,6 +326,19 @@ DX_DEVICE void split(const float (&x)[8], bf16x8 (&out)[N]) {
     }
     out[n] = as_bf16x8(w);
   }
+}
+
+// Asks for N times one matrix instruction and V others of the vector unit, in the block between two barriers of the
+// schedule: each runs while the other does.
+template <int N, int V>
+DX_DEVICE void interleave() {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+  }
+#endif
 }
 
 template <int DK, int NC>
@@ -392,7 +413,10 @@ struct Fetched {
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       const uint32_t at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
-      if (OUT) *reinterpret_cast<u32x4 *>(m.q + place<DK>(r, c)) = q[i];
+      if (OUT) {  // by halves: see q_half
+        *reinterpret_cast<u32x2 *>(m.q + q_half<DK>(r, 2 * c)) = u32x2{q[i][0], q[i][1]};
+        *reinterpret_cast<u32x2 *>(m.q + q_half<DK>(r, 2 * c + 1)) = u32x2{q[i][2], q[i][3]};
+      }
       *reinterpret_cast<u32x4 *>(m.k + place<DK>(r, c)) = k[i];
     }
 #pragma unroll
@@ -408,6 +432,7 @@ template <int DK, int NC, bool OUT>
 DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col0, int t0, int t1,
                        floatx4 (&st)[DK / 16][NC], Tile<DK, NC> &m) {
   constexpr int N = 64, W = COLS * NC;
+  constexpr bool AHEAD = DK < 256;  // operands are made ready while others are multiplied; at 256 registers are short
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kh = head / (a.h / a.hk);
   const float log2_scale = log2f(a.scale);
@@ -451,26 +476,36 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
       bf16x8 qf[DK / 32];
 #pragma unroll
       for (int u = 0; u < DK / 32; ++u)
-        qf[u] = as_bf16x8(*reinterpret_cast<const u32x4 *>(m.q + place<DK>(16 * wave + c, 4 * u + g)));
+        qf[u] = both(*reinterpret_cast<const s16x4 *>(m.q + q_half<DK>(16 * wave + c, 8 * u + 2 * g)),
+                     *reinterpret_cast<const s16x4 *>(m.q + q_half<DK>(16 * wave + c, 8 * u + 2 * g + 1)));
       const double mine = d.sum[16 * wave + c] + log2_scale;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         if (2 * b > wave) break;
+        bf16x8 kf[DK / 32][2];  // all reads at once
+        double sum[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int u = 0; u < DK / 32; ++u)
+            kf[u][j] = as_bf16x8(*reinterpret_cast<const u32x4 *>(m.k + place<DK>(32 * b + 16 * j + c, 4 * u + g)));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[4 * j + r] = d.sum[32 * b + 16 * j + 4 * g + r];
+        }
+        __builtin_amdgcn_sched_barrier(0);
         floatx4 w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
         for (int u = 0; u < DK / 32; ++u)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)  // the second is hidden for the even waves' last: 0 by the mask below
-            w[j] = mfma16(as_bf16x8(*reinterpret_cast<const u32x4 *>(m.k + place<DK>(32 * b + 16 * j + c, 4 * u + g))), qf[u], w[j]);
+          for (int j = 0; j < 2; ++j) w[j] = mfma16(kf[u][j], qf[u], w[j]);  // keys behind the queries: 0 below
         float p[8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int e = 0; e < 8; ++e) p[e] = fast_exp2((float)(mine - sum[e]));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int at = 32 * b + 16 * j + 4 * g + r;
-            const float weight = w[j][r] * fast_exp2((float)(mine - d.sum[at]));  // before the choice: no branch around it
-            p[4 * j + r] = at <= 16 * wave + c ? weight : 0.f;
-          }
+        for (int e = 0; e < 8; ++e) {
+          const float weight = w[e >> 2][e & 3] * p[e];  // before the choice: no branch around it
+          p[e] = 32 * b + 16 * (e >> 2) + 4 * g + (e & 3) <= 16 * wave + c ? weight : 0.f;
+        }
         bf16x8 parts[2];
         split(p, parts);
 #pragma unroll
@@ -480,10 +515,12 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int y = 0; y < NC; ++y) o[i][y] = floatx4{0, 0, 0, 0};
+      // Two tiles of the state at a time: while the matrix cores multiply one pair, the next is split and its queries read.
+      bf16x8 sf[2][NC][2], qx[2][4];
+      auto ready = [&](int u, int at) {
 #pragma unroll
-      for (int u = 0; u < DK / 32; ++u) {
-        __builtin_amdgcn_sched_barrier(0);  // what is read ahead has to fit the registers
-        bf16x8 sf[NC][2], qx[4];
+        for (int i = 0; i < 4; ++i)
+          qx[at][i] = as_bf16x8(*reinterpret_cast<const u32x4 *>(m.q + place<DK>(16 * i + c, 4 * u + g)));
 #pragma unroll
         for (int y = 0; y < NC; ++y) {
           float pair[8];
@@ -492,36 +529,85 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
             pair[r] = st[2 * u][y][r];
             pair[4 + r] = st[2 * u + 1][y][r];
           }
-          split(pair, sf[y]);
+          split(pair, sf[at][y]);
         }
+      };
+      ready(0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint16_t *p0 = m.q + place<DK>(16 * i + c, 4 * u + (g >> 1)) + (g & 1) * 4;
-          const uint16_t *p1 = m.q + place<DK>(16 * i + c, 4 * u + 2 + (g >> 1)) + (g & 1) * 4;
-          qx[i] = both(*reinterpret_cast<const s16x4 *>(p0), *reinterpret_cast<const s16x4 *>(p1));
-        }
+      for (int u = 0; u < DK / 32; ++u) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (u + 1 < DK / 32) ready(u + 1, (u + 1) & 1);
 #pragma unroll
         for (int z = 0; z < 2; ++z)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int y = 0; y < NC; ++y) o[i][y] = mfma16(sf[y][z], qx[i], o[i][y]);
+            for (int y = 0; y < NC; ++y) o[i][y] = mfma16(sf[u & 1][y][z], qx[u & 1][i], o[i][y]);
+        if (u + 1 < DK / 32) interleave<8 * NC, 3>();
       }
     }
     if (wave == 0 && t + N < t1) next = sums(m.decay[par ^ 1], g1, t + N, next);
     lds_barrier();
+    const int shift = __builtin_amdgcn_readfirstlane(d.shift);
+    if (shift != 0)
+#pragma unroll
+      for (int u = 0; u < DK / 16; ++u)
+#pragma unroll
+        for (int y = 0; y < NC; ++y)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[u][y][r] = ldexpf(st[u][y][r], shift);
     bf16x8 vf[2][NC];
+    floatx4 weight[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int y = 0; y < NC; ++y) vf[b][y] = columns<W>(m.v, b, NC * wave + y, lane);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) weight[b][j] = *reinterpret_cast<const floatx4 *>(d.to_end + 32 * b + 16 * j + 4 * g);
+    }
+    const bf16x8 nothing = as_bf16x8(u32x4{0, 0, 0, 0});
+    floatx4 sum = {0, 0, 0, 0};  // 0 times each value: NaN where one is no finite number
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int y = 0; y < NC; ++y) vf[b][y] = columns<W>(m.v, b, NC * wave + y, lane);
-    if constexpr (OUT) {
-      const bf16x8 nothing = as_bf16x8(u32x4{0, 0, 0, 0});
-      floatx4 sum = {0, 0, 0, 0};  // 0 times each value: NaN where one is no finite number
+      for (int y = 0; y < NC; ++y) sum = mfma16(nothing, vf[b][y], sum);
+    const bool lost = __any(sum[0] != 0.f);
+    // A weight of 0 would carry a later token's infinity or NaN to an earlier one: such values are left out of the products,
+    // and what they reach is NaN.
+    int first = N;  // of the wave's column lane % (16 NC): the first token whose value is lost
+    if (lost) {
+      for (int j = 0; j < N; ++j) {
+        const int col = 16 * NC * wave + lane % (16 * NC);
+        if (first == N && (m.v[place<W>(j, col >> 3) + (col & 7)] & 0x7f80) == 0x7f80) first = j;
+      }
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int y = 0; y < NC; ++y) sum = mfma16(nothing, vf[b][y], sum);
+        for (int y = 0; y < NC; ++y) {
+          u32x4 x = __builtin_bit_cast(u32x4, vf[b][y]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] &= ((x[e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((x[e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+          vf[b][y] = as_bf16x8(x);
+        }
+    }
+    bf16x8 wv[2][NC][3];
+    auto weigh = [&](int b) {
+#pragma unroll
+      for (int y = 0; y < NC; ++y) {
+        const u32x4 raw = __builtin_bit_cast(u32x4, vf[b][y]);
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[2 * e] = lo_bf(raw[e]) * weight[b][e >> 1][(2 * e) & 3];
+          p[2 * e + 1] = hi_bf(raw[e]) * weight[b][e >> 1][(2 * e + 1) & 3];
+        }
+        split(p, wv[b][y]);
+      }
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    if (AHEAD) weigh(0);
+    if constexpr (OUT) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float from = d.from_start[16 * i + c];
@@ -530,33 +616,26 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[i][y][r] *= from;
       }
-      if (!__any(sum[0] != 0.f)) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int z = 0; z < 2; ++z)
+        for (int z = 0; z < 2; ++z)
 #pragma unroll
-            for (int i = 2 * b; i < 4; ++i) {
-              const bf16x8 p = as_bf16x8(m.p[i][b][z][lane]);
+          for (int i = 2 * b; i < 4; ++i) {
+            const bf16x8 p = as_bf16x8(m.p[i][b][z][lane]);
 #pragma unroll
-              for (int y = 0; y < NC; ++y) o[i][y] = mfma16(vf[b][y], p, o[i][y]);
-            }
-      } else {  // a weight of 0 would carry a later token's infinity or NaN to this one
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j <= 16 * i + c; ++j) {
-            const int other = c + 16 * ((j & 15) >> 2), e = (j & 3) + 4 * ((j >> 4) & 1);
-            float p = 0.f;
-            for (int z = 0; z < 2; ++z) p += bf2f(reinterpret_cast<const uint16_t *>(&m.p[i][j >> 5][z][other])[e]);
-#pragma unroll
-            for (int y = 0; y < NC; ++y)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int col = 16 * (NC * wave + y) + 4 * g + r;
-                o[i][y][r] = fmaf(p, bf2f(m.v[place<W>(j, col >> 3) + (col & 7)]), o[i][y][r]);
-              }
+            for (int y = 0; y < NC; ++y) o[i][y] = mfma16(vf[b][y], p, o[i][y]);
           }
-      }
+      if (AHEAD) interleave<12 * NC, 5>();
+      if (lost)
+#pragma unroll
+        for (int y = 0; y < NC; ++y)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = __shfl(first, 16 * y + 4 * g + r, 64);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i][y][r] = 16 * i + c >= at ? NAN : o[i][y][r];
+          }
 #if defined(__HIP_DEVICE_COMPILE__)
       const auto out = rows_of(static_cast<uint16_t *>(a.out) + row * a.os + head * a.dv + col0, n, a.os);
 #pragma unroll
@@ -568,34 +647,13 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
               2 * ((uint32_t)(16 * i + c) * (uint32_t)a.os + 16 * (NC * wave + y) + 4 * g), 0, 0);
 #endif
     }
-    const int shift = __builtin_amdgcn_readfirstlane(d.shift);
-    if (shift != 0)
-#pragma unroll
-      for (int u = 0; u < DK / 16; ++u)
-#pragma unroll
-        for (int y = 0; y < NC; ++y)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) st[u][y][r] = ldexpf(st[u][y][r], shift);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      bf16x8 wv[NC][3];
-      const floatx4 w0 = *reinterpret_cast<const floatx4 *>(d.to_end + 32 * b + 4 * g);
-      const floatx4 w1 = *reinterpret_cast<const floatx4 *>(d.to_end + 32 * b + 16 + 4 * g);
-#pragma unroll
-      for (int y = 0; y < NC; ++y) {
-        const u32x4 raw = __builtin_bit_cast(u32x4, vf[b][y]);
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[2 * e] = lo_bf(raw[e]) * (e < 2 ? w0[2 * e] : w1[2 * e - 4]);
-          p[2 * e + 1] = hi_bf(raw[e]) * (e < 2 ? w0[2 * e + 1] : w1[2 * e - 3]);
-        }
-        split(p, wv[y]);
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (!AHEAD || b == 0) weigh(AHEAD ? 1 : b);
       constexpr int AT_ONCE = 2;
 #pragma unroll
       for (int u0 = 0; u0 < DK / 16; u0 += AT_ONCE) {
-        __builtin_amdgcn_sched_barrier(0);
         bf16x8 kt[AT_ONCE];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) kt[u] = columns<DK>(m.k, b, u0 + u, lane);
@@ -604,9 +662,19 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #pragma unroll
           for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
-            for (int y = 0; y < NC; ++y) st[u0 + u][y] = mfma16(kt[u], wv[y][z], st[u0 + u][y]);
+            for (int y = 0; y < NC; ++y) st[u0 + u][y] = mfma16(kt[u], wv[b][y][z], st[u0 + u][y]);
       }
+      if (AHEAD && b == 0) interleave<DK / 16 * 3 * NC, 3>();
     }
+    if (lost)
+#pragma unroll
+      for (int y = 0; y < NC; ++y) {
+        const float gone = __shfl(first, 16 * y + c, 64) < N ? NAN : 0.f;
+#pragma unroll
+        for (int u = 0; u < DK / 16; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[u][y][r] += gone;
+      }
     rest = d.rest;
     lds_barrier();
   }
