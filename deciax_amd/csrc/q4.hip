@@ -146,6 +146,89 @@ linear_q4_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes
   }
 }
 
+// Up to 16 rows: x stays in registers (TPW tiles of its columns a wave), and the workgroup walks tiles of 16 rows of W, one
+// in `gridDim.x`: the next one's codes are on their way while this one's are multiplied. Same sums as linear_q4_kernel.
+template <int TPW, int SPG, typename OUT>
+__global__ void __launch_bounds__(THREADS)
+linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
+                     OUT *__restrict__ y, int m, int n, int k, long ldx, long ldy) {
+  constexpr int GROUPS = 4 / SPG;
+  __shared__ __align__(16) float parts[2][WAVES][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, q = lane >> 4;
+  const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4, groups = k / (32 * SPG);
+  const int mine = (tiles_k - wave + WAVES - 1) / WAVES;  // tiles of this wave, TPW at most
+
+  u32x4 raw[TPW];
+  uint32_t word[TPW][GROUPS];
+  auto load = [&](int tile) {
+    const u32x4 *cp = codes + ((long)tile * tiles_k + wave) * 64;
+    const uint32_t *wp = words + (long)tile * groups * 16;
+#pragma unroll
+    for (int d = 0; d < TPW; ++d)
+      if (d < mine) {
+        raw[d] = cp[d * (WAVES * 64) + lane];
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) word[d][g] = wp[min((wave + d * WAVES) * GROUPS + g, groups - 1) * 16 + c];
+      }
+  };
+  load(blockIdx.x);
+  u32x4 xf[TPW][4];
+  const uint16_t *xr = x + min(c, m - 1) * ldx + 8 * q;  // rows behind the last: not stored
+#pragma unroll
+  for (int d = 0; d < TPW; ++d)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int col = (wave + d * WAVES) * 128 + 32 * s;
+      xf[d][s] = u32x4{0, 0, 0, 0};  // columns behind the last
+      if (col < k) xf[d][s] = *reinterpret_cast<const u32x4 *>(xr + col);
+    }
+  const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  int buffer = 0;
+  for (int tile = blockIdx.x; tile < tiles_n; tile += gridDim.x, buffer ^= 1) {
+    floatx4 sum = {0, 0, 0, 0};
+    const int next = tile + (int)gridDim.x;
+#pragma unroll
+    for (int d = 0; d < TPW; ++d) {
+      if (d >= mine) break;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        if ((wave + d * WAVES) * GROUPS + g >= groups) break;
+        floatx4 acc = {0, 0, 0, 0}, xs = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
+          xs = mfma16(xf[d][s], ones, xs);
+          acc = mfma16(xf[d][s], halves(raw[d][s]), acc);
+        }
+        const float s2 = 2.f * scale_of(word[d][g]), off = -8.f - 0.5f * zero_of(word[d][g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = fmaf(s2, fmaf(off, xs[e], acc[e]), sum[e]);
+      }
+    }
+    if (next < tiles_n) load(next);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) parts[buffer][wave][64 * e + lane] = sum[e];  // row 4 q + e
+    // what this buffer held is read before the barrier of the tile between
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int at = threadIdx.x;
+    if (at < 16 * m) {
+      const int o = 16 * tile + (at & 15);
+      const int from = 64 * ((at >> 4) & 3) + 16 * (at >> 6) + (at & 15);
+      float v = parts[buffer][0][from];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v += parts[buffer][w][from];
+      if (o < n) {
+        if constexpr (sizeof(OUT) == 2)
+          y[(long)(at >> 4) * ldy + o] = f2bf(v);
+        else
+          y[(long)(at >> 4) * ldy + o] = v;
+      }
+    }
+  }
+}
+
 // A wave lays out one tile: lane 16 q + r the codes of row r that linear_q4_kernel reads there. Once a weight, not tuned.
 struct Place {
   int row, col;  // of the lane's first value of step 0
@@ -298,8 +381,27 @@ hipError_t run(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, 
   return hipGetLastError();
 }
 
+template <int TPW, int SPG>
+hipError_t run_few(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
+  constexpr int MOST = 512;  // workgroups: two a CU
+  const int tiles = dx_ceil_div(w.n, 16), each = dx_ceil_div(tiles, MOST);
+  const dim3 grid((unsigned)dx_ceil_div(tiles, each));
+  const u32x4 *codes = static_cast<const u32x4 *>(w.codes);
+  if (f32)
+    linear_q4_few_kernel<TPW, SPG, float>
+        <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<float *>(y), (int)m, w.n, w.k, ldx, ldy);
+  else
+    linear_q4_few_kernel<TPW, SPG, uint16_t>
+        <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<uint16_t *>(y), (int)m, w.n, w.k, ldx, ldy);
+  return hipGetLastError();
+}
+
 template <int SPG>
 hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
+  const int tiles = dx_ceil_div(w.k, 128 * WAVES);  // of a wave
+  if (m <= 16 && tiles <= 2) return run_few<2, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 16 && tiles <= 4) return run_few<4, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 16 && tiles <= 6) return run_few<6, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16) return run<1, 1, SPG, 4>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 32) return run<2, 1, SPG, 2>(w, x, y, m, ldx, ldy, f32, s);
   return run<4, 4, SPG, 1>(w, x, y, m, ldx, ldy, f32, s);
