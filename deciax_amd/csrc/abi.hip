@@ -1080,6 +1080,7 @@ int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y, 
   REQUIRE(out_dtype == DX_BF16 || out_dtype == DX_F32, "linear_q4: unknown out dtype %d", out_dtype);
   REQUIRE(x_row_stride >= k && x_row_stride % 8 == 0 && y_row_stride >= n,
           "linear_q4: row strides must cover the rows, x's be a multiple of 8");
+  SUPPORTED(x_row_stride < 1 << 24, "linear_q4: x rows of %ld elements, below 2^24", (long)x_row_stride);
   REQUIRE(aligned16(x) && reinterpret_cast<uintptr_t>(y) % (out_dtype == DX_BF16 ? 2 : 4) == 0,
           "linear_q4: x must be 16-byte aligned, y to its type");
   if (m == 0) return DX_OK;

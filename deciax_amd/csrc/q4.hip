@@ -146,87 +146,154 @@ linear_q4_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes
   }
 }
 
-// Up to 16 rows: x stays in registers (TPW tiles of its columns a wave), and the workgroup walks tiles of 16 rows of W, one
-// in `gridDim.x`: the next one's codes are on their way while this one's are multiplied. Same sums as linear_q4_kernel.
+// Reads of a weight's tiles t and groups of one tile row, and of x, as buffers: what lies behind the last column reads as 0,
+// without a branch, so that every load stays on its way until it is used.
+struct TileRow {
+  __amdgpu_buffer_rsrc_t codes, words;
+};
+DX_DEVICE TileRow tile_row(const u32x4 *codes, const uint32_t *words, long tile, int tiles_k, int groups) {
+  return TileRow{__builtin_amdgcn_make_buffer_rsrc((void *)(codes + tile * tiles_k * 64), (short)0, tiles_k * 1024, 0x00020000),
+                 __builtin_amdgcn_make_buffer_rsrc((void *)(words + tile * groups * 16), (short)0, groups * 64, 0x00020000)};
+}
+DX_DEVICE u32x4 load16(__amdgpu_buffer_rsrc_t from, uint32_t bytes) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_raw_buffer_load_b128(from, bytes, 0, 0);
+#else
+  return u32x4{};
+#endif
+}
+DX_DEVICE uint32_t load4(__amdgpu_buffer_rsrc_t from, uint32_t bytes) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_raw_buffer_load_b32(from, bytes, 0, 0);
+#else
+  return 0;
+#endif
+}
+
+// A tile's codes and words.
+template <int GROUPS>
+struct Codes {
+  u32x4 raw;
+  uint32_t word[GROUPS];
+  DX_DEVICE void load(const TileRow &from, uint32_t t, int lane) {
+    raw = load16(from.codes, t * 1024 + lane * 16);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) word[g] = load4(from.words, (t * GROUPS + g) * 64 + (lane & 15) * 4);
+  }
+};
+
+// Columns 128 t .. of this lane's row of x, of which `row` are the bytes before it.
+struct Columns {
+  u32x4 step[4];
+  DX_DEVICE void load(__amdgpu_buffer_rsrc_t x, uint32_t row, uint32_t t, uint32_t k, int lane) {
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s) {
+      const uint32_t col = 128 * t + 32 * s;
+      step[s] = load16(x, col < k ? row + 2 * (col + 8 * (lane >> 4)) : 0x7fffffffu);
+    }
+  }
+};
+
+template <int SPG>
+DX_DEVICE void multiply(const Codes<4 / SPG> &w, const Columns &x, floatx4 &sum) {
+  const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+  for (int g = 0; g < 4 / SPG; ++g) {
+    floatx4 acc = {0, 0, 0, 0}, xs = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
+      xs = mfma16(x.step[s], ones, xs);
+      acc = mfma16(x.step[s], halves(w.raw[s]), acc);
+    }
+    const float s2 = 2.f * scale_of(w.word[g]), off = -8.f - 0.5f * zero_of(w.word[g]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = fmaf(s2, fmaf(off, xs[e], acc[e]), sum[e]);
+  }
+}
+
+// The waves' sums of a tile, added in their order and stored. The next tile takes the other buffer: what this one held is
+// read before its barrier.
+template <typename OUT>
+DX_DEVICE void join(float (&parts)[WAVES][256], const floatx4 &sum, OUT *y, int tile, int m, int n, long ldy) {
+  const int at = threadIdx.x, lane = at & 63;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) parts[at >> 6][64 * e + lane] = sum[e];  // row 4 (lane / 16) + e
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (at >= 16 * m) return;
+  const int o = 16 * tile + (at & 15), from = 64 * ((at >> 4) & 3) + 16 * (at >> 6) + (at & 15);
+  float v = parts[0][from];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) v += parts[w][from];
+  if (o >= n) return;
+  if constexpr (sizeof(OUT) == 2)
+    y[(long)(at >> 4) * ldy + o] = f2bf(v);
+  else
+    y[(long)(at >> 4) * ldy + o] = v;
+}
+
+// Up to 16 rows, TPW tiles of columns a wave: x stays in registers, and the workgroup walks tiles of 16 rows of W, one in
+// `gridDim.x`; the next one's codes are on their way while this one's are multiplied. Same sums as linear_q4_kernel.
 template <int TPW, int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
                      OUT *__restrict__ y, int m, int n, int k, long ldx, long ldy) {
-  constexpr int GROUPS = 4 / SPG;
   __shared__ __align__(16) float parts[2][WAVES][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, q = lane >> 4;
   const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4, groups = k / (32 * SPG);
-  const int mine = (tiles_k - wave + WAVES - 1) / WAVES;  // tiles of this wave, TPW at most
-
-  u32x4 raw[TPW];
-  uint32_t word[TPW][GROUPS];
-  auto load = [&](int tile) {
-    const u32x4 *cp = codes + ((long)tile * tiles_k + wave) * 64;
-    const uint32_t *wp = words + (long)tile * groups * 16;
+  Codes<4 / SPG> w[TPW];
+  TileRow from = tile_row(codes, words, blockIdx.x, tiles_k, groups);
 #pragma unroll
-    for (int d = 0; d < TPW; ++d)
-      if (d < mine) {
-        raw[d] = cp[d * (WAVES * 64) + lane];
+  for (int d = 0; d < TPW; ++d) w[d].load(from, wave + d * WAVES, lane);
+  const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)x, (short)0, (int)(((m - 1) * ldx + k) * 2), 0x00020000);
+  const uint32_t row = min(lane & 15, m - 1) * (uint32_t)ldx * 2;  // rows behind the last: not stored
+  Columns xs[TPW];
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) word[d][g] = wp[min((wave + d * WAVES) * GROUPS + g, groups - 1) * 16 + c];
-      }
-  };
-  load(blockIdx.x);
-  u32x4 xf[TPW][4];
-  const uint16_t *xr = x + min(c, m - 1) * ldx + 8 * q;  // rows behind the last: not stored
-#pragma unroll
-  for (int d = 0; d < TPW; ++d)
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int col = (wave + d * WAVES) * 128 + 32 * s;
-      xf[d][s] = u32x4{0, 0, 0, 0};  // columns behind the last
-      if (col < k) xf[d][s] = *reinterpret_cast<const u32x4 *>(xr + col);
-    }
-  const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  for (int d = 0; d < TPW; ++d) xs[d].load(rows, row, wave + d * WAVES, k, lane);
   int buffer = 0;
   for (int tile = blockIdx.x; tile < tiles_n; tile += gridDim.x, buffer ^= 1) {
     floatx4 sum = {0, 0, 0, 0};
     const int next = tile + (int)gridDim.x;
+    from = tile_row(codes, words, min(next, tiles_n - 1), next < tiles_n ? tiles_k : 0, next < tiles_n ? groups : 0);
 #pragma unroll
     for (int d = 0; d < TPW; ++d) {
-      if (d >= mine) break;
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        if ((wave + d * WAVES) * GROUPS + g >= groups) break;
-        floatx4 acc = {0, 0, 0, 0}, xs = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
-          xs = mfma16(xf[d][s], ones, xs);
-          acc = mfma16(xf[d][s], halves(raw[d][s]), acc);
-        }
-        const float s2 = 2.f * scale_of(word[d][g]), off = -8.f - 0.5f * zero_of(word[d][g]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = fmaf(s2, fmaf(off, xs[e], acc[e]), sum[e]);
-      }
+      multiply<SPG>(w[d], xs[d], sum);
+      w[d].load(from, wave + d * WAVES, lane);
     }
-    if (next < tiles_n) load(next);
+    join(parts[buffer], sum, y, tile, m, n, ldy);
+  }
+}
+
+// Up to 16 rows and more columns than that: one tile of W a workgroup, codes four tiles ahead and x two.
+template <int SPG, typename OUT>
+__global__ void __launch_bounds__(THREADS)
+linear_q4_long_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
+                      OUT *__restrict__ y, int m, int n, int k, long ldx, long ldy) {
+  constexpr int AHEAD = 4, X_AHEAD = 2;
+  __shared__ __align__(16) float parts[WAVES][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles_k = (k + 127) >> 7, groups = k / (32 * SPG);
+  const TileRow from = tile_row(codes, words, blockIdx.x, tiles_k, groups);
+  const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)x, (short)0, (int)(((m - 1) * ldx + k) * 2), 0x00020000);
+  const uint32_t row = min(lane & 15, m - 1) * (uint32_t)ldx * 2;
+  Codes<4 / SPG> w[AHEAD];
+  Columns xs[X_AHEAD];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) parts[buffer][wave][64 * e + lane] = sum[e];  // row 4 q + e
-    // what this buffer held is read before the barrier of the tile between
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const int at = threadIdx.x;
-    if (at < 16 * m) {
-      const int o = 16 * tile + (at & 15);
-      const int from = 64 * ((at >> 4) & 3) + 16 * (at >> 6) + (at & 15);
-      float v = parts[buffer][0][from];
+  for (int d = 0; d < AHEAD; ++d) w[d].load(from, wave + d * WAVES, lane);
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) v += parts[buffer][w][from];
-      if (o < n) {
-        if constexpr (sizeof(OUT) == 2)
-          y[(long)(at >> 4) * ldy + o] = f2bf(v);
-        else
-          y[(long)(at >> 4) * ldy + o] = v;
-      }
+  for (int d = 0; d < X_AHEAD; ++d) xs[d].load(rows, row, wave + d * WAVES, k, lane);
+  floatx4 sum = {0, 0, 0, 0};
+  for (int t = wave; t < tiles_k; t += AHEAD * WAVES) {
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {  // tiles behind the last add 0
+      const int at = t + d * WAVES;
+      multiply<SPG>(w[d], xs[d % X_AHEAD], sum);
+      w[d].load(from, at + AHEAD * WAVES, lane);
+      xs[d % X_AHEAD].load(rows, row, at + X_AHEAD * WAVES, k, lane);
     }
   }
+  join(parts, sum, y, blockIdx.x, m, n, ldy);
 }
 
 // A wave lays out one tile: lane 16 q + r the codes of row r that linear_q4_kernel reads there. Once a weight, not tuned.
@@ -397,12 +464,25 @@ hipError_t run_few(const Q4Weight &w, const uint16_t *x, void *y, long m, long l
 }
 
 template <int SPG>
+hipError_t run_long(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
+  const dim3 grid((unsigned)dx_ceil_div(w.n, 16));
+  const u32x4 *codes = static_cast<const u32x4 *>(w.codes);
+  if (f32)
+    linear_q4_long_kernel<SPG, float>
+        <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<float *>(y), (int)m, w.n, w.k, ldx, ldy);
+  else
+    linear_q4_long_kernel<SPG, uint16_t>
+        <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<uint16_t *>(y), (int)m, w.n, w.k, ldx, ldy);
+  return hipGetLastError();
+}
+
+template <int SPG>
 hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
   const int tiles = dx_ceil_div(w.k, 128 * WAVES);  // of a wave
   if (m <= 16 && tiles <= 2) return run_few<2, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16 && tiles <= 4) return run_few<4, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16 && tiles <= 6) return run_few<6, SPG>(w, x, y, m, ldx, ldy, f32, s);
-  if (m <= 16) return run<1, 1, SPG, 4>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 16) return run_long<SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 32) return run<2, 1, SPG, 2>(w, x, y, m, ldx, ldy, f32, s);
   return run<4, 4, SPG, 1>(w, x, y, m, ldx, ldy, f32, s);
 }

@@ -73,7 +73,7 @@ def test_malformed_weights_are_refused(make, bad, want) -> None:
     (values(w=None), INVALID), (values(w=BYTE), INVALID), (values(ldw=255), INVALID),
     (linear(x=None), INVALID), (linear(y=None), INVALID), (linear(x=ODD), INVALID), (linear(y=BYTE), INVALID),
     (linear(m=-1), INVALID), (linear(m=(1 << 20) + 1), UNSUPPORTED), (linear(ldx=248), INVALID),
-    (linear(ldx=260), INVALID), (linear(ldy=7), INVALID), (linear(dtype=5), INVALID), (linear(), OK)])
+    (linear(ldx=260), INVALID), (linear(ldx=1 << 24), UNSUPPORTED), (linear(ldy=7), INVALID), (linear(dtype=5), INVALID), (linear(), OK)])
 def test_q4(call, want) -> None:
     check(call, want)
 
