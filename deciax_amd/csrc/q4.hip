@@ -182,28 +182,45 @@ struct Codes {
   }
 };
 
-// Columns 128 t .. of this lane's row of x, of which `row` are the bytes before it.
+// Columns 128 t .. of 16 rows of x. Read as they are multiplied, a lane its row, 16 rows' pieces of 64 bytes would take four
+// times as long as whole rows of 256: so 16 lanes read a row, and the wave turns the tile in LDS, chunk c of row r at c ^ r.
 struct Columns {
-  u32x4 step[4];
-  DX_DEVICE void load(__amdgpu_buffer_rsrc_t x, uint32_t row, uint32_t t, uint32_t k, int lane) {
+  u32x4 part[4];
+  // at: the rows' bytes before their columns; rows behind the last stand for it and are not stored.
+  DX_DEVICE static void places(uint32_t (&at)[4], int m, long ldx, int lane) {
 #pragma unroll
-    for (uint32_t s = 0; s < 4; ++s) {
-      const uint32_t col = 128 * t + 32 * s;
-      step[s] = load16(x, col < k ? row + 2 * (col + 8 * (lane >> 4)) : 0x7fffffffu);
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * i + (lane >> 4);
+      at[i] = min(r, m - 1) * (uint32_t)ldx * 2 + 16 * ((lane & 15) ^ r);
     }
+  }
+  DX_DEVICE void load(__amdgpu_buffer_rsrc_t x, const uint32_t (&at)[4], int t, int k, int lane) {
+    const int left = k - 128 * t;  // columns, at most 0 behind the last tile
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = 8 * ((lane & 15) ^ (4 * i + (lane >> 4)));
+      part[i] = load16(x, col < left ? at[i] + 256 * t : 0x7fffffffu);
+    }
+  }
+  DX_DEVICE void turn(u32x4 *lds, u32x4 (&step)[4], int lane) const {
+    const int c = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[64 * i + lane] = part[i];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) step[s] = lds[16 * c + ((4 * s + q) ^ c)];
   }
 };
 
 template <int SPG>
-DX_DEVICE void multiply(const Codes<4 / SPG> &w, const Columns &x, floatx4 &sum) {
+DX_DEVICE void multiply(const Codes<4 / SPG> &w, const u32x4 (&x)[4], floatx4 &sum) {
   const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
   for (int g = 0; g < 4 / SPG; ++g) {
     floatx4 acc = {0, 0, 0, 0}, xs = {0, 0, 0, 0};
 #pragma unroll
     for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
-      xs = mfma16(x.step[s], ones, xs);
-      acc = mfma16(x.step[s], halves(w.raw[s]), acc);
+      xs = mfma16(x[s], ones, xs);
+      acc = mfma16(x[s], halves(w.raw[s]), acc);
     }
     const float s2 = 2.f * scale_of(w.word[g]), off = -8.f - 0.5f * zero_of(w.word[g]);
 #pragma unroll
@@ -240,6 +257,7 @@ __global__ void __launch_bounds__(THREADS)
 linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
                      OUT *__restrict__ y, int m, int n, int k, long ldx, long ldy) {
   __shared__ __align__(16) float parts[2][WAVES][256];
+  __shared__ u32x4 turned[WAVES][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4, groups = k / (32 * SPG);
   Codes<4 / SPG> w[TPW];
@@ -247,10 +265,14 @@ linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ c
 #pragma unroll
   for (int d = 0; d < TPW; ++d) w[d].load(from, wave + d * WAVES, lane);
   const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)x, (short)0, (int)(((m - 1) * ldx + k) * 2), 0x00020000);
-  const uint32_t row = min(lane & 15, m - 1) * (uint32_t)ldx * 2;  // rows behind the last: not stored
-  Columns xs[TPW];
+  uint32_t at[4];
+  Columns::places(at, m, ldx, lane);
+  Columns read[TPW];
 #pragma unroll
-  for (int d = 0; d < TPW; ++d) xs[d].load(rows, row, wave + d * WAVES, k, lane);
+  for (int d = 0; d < TPW; ++d) read[d].load(rows, at, wave + d * WAVES, k, lane);
+  u32x4 xs[TPW][4];
+#pragma unroll
+  for (int d = 0; d < TPW; ++d) read[d].turn(turned[wave], xs[d], lane);
   int buffer = 0;
   for (int tile = blockIdx.x; tile < tiles_n; tile += gridDim.x, buffer ^= 1) {
     floatx4 sum = {0, 0, 0, 0};
@@ -265,32 +287,37 @@ linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ c
   }
 }
 
-// Up to 16 rows and more columns than that: one tile of W a workgroup, codes four tiles ahead and x two.
+// Up to 16 rows and more columns than that: one tile of W a workgroup, codes eight tiles ahead and x two.
 template <int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_long_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
                       OUT *__restrict__ y, int m, int n, int k, long ldx, long ldy) {
-  constexpr int AHEAD = 4, X_AHEAD = 2;
+  constexpr int AHEAD = 8, X_AHEAD = 2;
   __shared__ __align__(16) float parts[WAVES][256];
+  __shared__ u32x4 turned[WAVES][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_k = (k + 127) >> 7, groups = k / (32 * SPG);
   const TileRow from = tile_row(codes, words, blockIdx.x, tiles_k, groups);
   const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)x, (short)0, (int)(((m - 1) * ldx + k) * 2), 0x00020000);
-  const uint32_t row = min(lane & 15, m - 1) * (uint32_t)ldx * 2;
+  uint32_t at[4];
+  Columns::places(at, m, ldx, lane);
   Codes<4 / SPG> w[AHEAD];
   Columns xs[X_AHEAD];
 #pragma unroll
   for (int d = 0; d < AHEAD; ++d) w[d].load(from, wave + d * WAVES, lane);
 #pragma unroll
-  for (int d = 0; d < X_AHEAD; ++d) xs[d].load(rows, row, wave + d * WAVES, k, lane);
+  for (int d = 0; d < X_AHEAD; ++d) xs[d].load(rows, at, wave + d * WAVES, k, lane);
   floatx4 sum = {0, 0, 0, 0};
   for (int t = wave; t < tiles_k; t += AHEAD * WAVES) {
 #pragma unroll
     for (int d = 0; d < AHEAD; ++d) {  // tiles behind the last add 0
-      const int at = t + d * WAVES;
-      multiply<SPG>(w[d], xs[d % X_AHEAD], sum);
-      w[d].load(from, at + AHEAD * WAVES, lane);
-      xs[d % X_AHEAD].load(rows, row, at + X_AHEAD * WAVES, k, lane);
+      const int tile = t + d * WAVES;
+      __builtin_amdgcn_sched_barrier(0);  // one tile after the other: turned all at once they take the registers
+      u32x4 step[4];
+      xs[d % X_AHEAD].turn(turned[wave], step, lane);
+      xs[d % X_AHEAD].load(rows, at, tile + X_AHEAD * WAVES, k, lane);
+      multiply<SPG>(w[d], step, sum);
+      w[d].load(from, tile + AHEAD * WAVES, lane);
     }
   }
   join(parts, sum, y, blockIdx.x, m, n, ldy);
