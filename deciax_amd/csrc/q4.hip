@@ -27,125 +27,15 @@ DX_DEVICE u32x4 halves(uint32_t w) {
 DX_DEVICE float scale_of(uint32_t word) { return __uint_as_float(word & ~15u); }
 DX_DEVICE float zero_of(uint32_t word) { return (float)(word & 15u); }
 
-// y = x W^T. A workgroup has 16 MT rows of x and 16 NT rows of W, wave w the tiles w, w + 8, .. of their columns; the
-// eight partial sums are added in their order. So the order of a sum goes by k alone, and a row of y depends on its row of
-// x alone, whatever MT and NT are.
+// y = x W^T on 16x16x32 products (first operand x: lane l has row l % 16 and the columns 8 (l / 16) .. of a step of 32; second
+// W, the same; the result's lane l has column l % 16, rows 4 (l / 16) + e).
+//
+// Eight sums are taken: of the tiles 0, 8, 16, .. of the columns, of 1, 9, 17, .., and so on, each in this order, and added
+// in theirs. So the order of a sum goes by k alone, and a row of y depends on its row of x alone, whichever kernel has it:
+// up to 64 rows the eight waves of a workgroup have a sum each, beyond a wave takes them one after the other.
 //
 // The products are of x and 8 + code / 2, both exact: with X the group's sum of x (one more product, by ones),
 // sum x (code - zero) = 2 (sum x (8 + code / 2) - (8 + zero / 2) X), the difference rounded once, and only then the scale.
-template <int MT, int NT, int SPG, int DEPTH, typename OUT>
-__global__ void __launch_bounds__(THREADS)
-linear_q4_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
-                 OUT *__restrict__ y, long m, int n, int k, long ldx, long ldy) {
-  constexpr int GROUPS = 4 / SPG;  // of a tile's columns
-  __shared__ float parts[WAVES][16][16 * NT + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 15, q = lane >> 4;
-  const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4, groups = k / (32 * SPG);
-  const int n0 = blockIdx.x * NT;
-  const long m0 = (long)blockIdx.y * (16 * MT);
-
-  const uint16_t *xr[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) xr[i] = x + min(m0 + 16 * i + c, m - 1) * ldx + 8 * q;  // rows behind the last: not stored
-  const u32x4 *cp[NT];
-  const uint32_t *wp[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const long tile = min(n0 + j, tiles_n - 1);
-    cp[j] = codes + tile * tiles_k * 64 + lane;
-    wp[j] = words + tile * groups * 16 + c;
-  }
-  const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-  floatx4 sum[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) sum[i][j] = floatx4{0, 0, 0, 0};
-
-  u32x4 raw[DEPTH][NT];
-  uint32_t word[DEPTH][NT][GROUPS];
-  auto load = [&](int t, int d) {
-    if (t >= tiles_k) return;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      raw[d][j] = cp[j][(long)t * 64];
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) word[d][j][g] = wp[j][(long)min(t * GROUPS + g, groups - 1) * 16];
-    }
-  };
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) load(wave + d * WAVES, d);
-  for (int t0 = wave; t0 < tiles_k; t0 += DEPTH * WAVES) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int t = t0 + d * WAVES;
-      if (t >= tiles_k) break;
-      const int steps = min(4, (k - t * 128) >> 5);  // of 32 columns; whole groups
-      u32x4 xf[4][MT];
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (s < steps)
-#pragma unroll
-          for (int i = 0; i < MT; ++i) xf[s][i] = *reinterpret_cast<const u32x4 *>(xr[i] + t * 128 + 32 * s);
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        if (g * SPG >= steps) break;
-        floatx4 acc[MT][NT], xs[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          xs[i] = floatx4{0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i) xs[i] = mfma16(xf[s][i], ones, xs[i]);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const u32x4 b = halves(raw[d][j][s]);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(xf[s][i], b, acc[i][j]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float s2 = 2.f * scale_of(word[d][j][g]), off = -8.f - 0.5f * zero_of(word[d][j][g]);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[i][j][e] = fmaf(s2, fmaf(off, xs[i][e], acc[i][j][e]), sum[i][j][e]);
-        }
-      }
-      load(t + DEPTH * WAVES, d);
-    }
-  }
-
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    if (i > 0) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) parts[wave][4 * q + e][16 * j + c] = sum[i][j][e];
-    __syncthreads();
-    for (int at = threadIdx.x; at < 256 * NT; at += THREADS) {
-      const int row = at / (16 * NT), col = at % (16 * NT);
-      const long r = m0 + 16 * i + row;
-      const int o = n0 * 16 + col;
-      if (r >= m || o >= n) continue;
-      float v = parts[0][row][col];
-#pragma unroll
-      for (int w = 1; w < WAVES; ++w) v += parts[w][row][col];
-      if constexpr (sizeof(OUT) == 2)
-        y[r * ldy + o] = f2bf(v);
-      else
-        y[r * ldy + o] = v;
-    }
-  }
-}
-
 // Reads of a weight's tiles t and groups of one tile row, and of x, as buffers: what lies behind the last column reads as 0,
 // without a branch, so that every load stays on its way until it is used.
 struct TileRow {
@@ -211,20 +101,37 @@ struct Columns {
   }
 };
 
-template <int SPG>
-DX_DEVICE void multiply(const Codes<4 / SPG> &w, const u32x4 (&x)[4], floatx4 &sum) {
+template <int MT, int NT, int SPG>
+DX_DEVICE void multiply(const Codes<4 / SPG> (&w)[NT], const u32x4 (&x)[MT][4], floatx4 (&sum)[MT][NT]) {
   const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
   for (int g = 0; g < 4 / SPG; ++g) {
-    floatx4 acc = {0, 0, 0, 0}, xs = {0, 0, 0, 0};
+    floatx4 acc[MT][NT], xs[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      xs[i] = floatx4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int s = g * SPG; s < (g + 1) * SPG; ++s) {
-      xs = mfma16(x[s], ones, xs);
-      acc = mfma16(x[s], halves(w.raw[s]), acc);
-    }
-    const float s2 = 2.f * scale_of(w.word[g]), off = -8.f - 0.5f * zero_of(w.word[g]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] = fmaf(s2, fmaf(off, xs[e], acc[e]), sum[e]);
+      for (int i = 0; i < MT; ++i) xs[i] = mfma16(x[i][s], ones, xs[i]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const u32x4 b = halves(w[j].raw[s]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(x[i][s], b, acc[i][j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const float s2 = 2.f * scale_of(w[j].word[g]), off = -8.f - 0.5f * zero_of(w[j].word[g]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[i][j][e] = fmaf(s2, fmaf(off, xs[i][e], acc[i][j][e]), sum[i][j][e]);
+    }
   }
 }
 
@@ -260,30 +167,30 @@ linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ c
   __shared__ u32x4 turned[WAVES][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4, groups = k / (32 * SPG);
-  Codes<4 / SPG> w[TPW];
+  Codes<4 / SPG> w[TPW][1];
   TileRow from = tile_row(codes, words, blockIdx.x, tiles_k, groups);
 #pragma unroll
-  for (int d = 0; d < TPW; ++d) w[d].load(from, wave + d * WAVES, lane);
+  for (int d = 0; d < TPW; ++d) w[d][0].load(from, wave + d * WAVES, lane);
   const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)x, (short)0, (int)(((m - 1) * ldx + k) * 2), 0x00020000);
   uint32_t at[4];
   Columns::places(at, m, ldx, lane);
   Columns read[TPW];
 #pragma unroll
   for (int d = 0; d < TPW; ++d) read[d].load(rows, at, wave + d * WAVES, k, lane);
-  u32x4 xs[TPW][4];
+  u32x4 xs[TPW][1][4];
 #pragma unroll
-  for (int d = 0; d < TPW; ++d) read[d].turn(turned[wave], xs[d], lane);
+  for (int d = 0; d < TPW; ++d) read[d].turn(turned[wave], xs[d][0], lane);
   int buffer = 0;
   for (int tile = blockIdx.x; tile < tiles_n; tile += gridDim.x, buffer ^= 1) {
-    floatx4 sum = {0, 0, 0, 0};
+    floatx4 sum[1][1] = {{{0, 0, 0, 0}}};
     const int next = tile + (int)gridDim.x;
     from = tile_row(codes, words, min(next, tiles_n - 1), next < tiles_n ? tiles_k : 0, next < tiles_n ? groups : 0);
 #pragma unroll
     for (int d = 0; d < TPW; ++d) {
-      multiply<SPG>(w[d], xs[d], sum);
-      w[d].load(from, wave + d * WAVES, lane);
+      multiply<1, 1, SPG>(w[d], xs[d], sum);
+      w[d][0].load(from, wave + d * WAVES, lane);
     }
-    join(parts[buffer], sum, y, tile, m, n, ldy);
+    join(parts[buffer], sum[0][0], y, tile, m, n, ldy);
   }
 }
 
@@ -301,27 +208,172 @@ linear_q4_long_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ 
   const auto rows = __builtin_amdgcn_make_buffer_rsrc((void *)x, (short)0, (int)(((m - 1) * ldx + k) * 2), 0x00020000);
   uint32_t at[4];
   Columns::places(at, m, ldx, lane);
-  Codes<4 / SPG> w[AHEAD];
+  Codes<4 / SPG> w[AHEAD][1];
   Columns xs[X_AHEAD];
 #pragma unroll
-  for (int d = 0; d < AHEAD; ++d) w[d].load(from, wave + d * WAVES, lane);
+  for (int d = 0; d < AHEAD; ++d) w[d][0].load(from, wave + d * WAVES, lane);
 #pragma unroll
   for (int d = 0; d < X_AHEAD; ++d) xs[d].load(rows, at, wave + d * WAVES, k, lane);
-  floatx4 sum = {0, 0, 0, 0};
+  floatx4 sum[1][1] = {{{0, 0, 0, 0}}};
   for (int t = wave; t < tiles_k; t += AHEAD * WAVES) {
 #pragma unroll
     for (int d = 0; d < AHEAD; ++d) {  // tiles behind the last add 0
       const int tile = t + d * WAVES;
       __builtin_amdgcn_sched_barrier(0);  // one tile after the other: turned all at once they take the registers
-      u32x4 step[4];
-      xs[d % X_AHEAD].turn(turned[wave], step, lane);
+      u32x4 step[1][4];
+      xs[d % X_AHEAD].turn(turned[wave], step[0], lane);
       xs[d % X_AHEAD].load(rows, at, tile + X_AHEAD * WAVES, k, lane);
-      multiply<SPG>(w[d], step, sum);
-      w[d].load(from, tile + AHEAD * WAVES, lane);
+      multiply<1, 1, SPG>(w[d], step, sum);
+      w[d][0].load(from, tile + AHEAD * WAVES, lane);
     }
   }
-  join(parts, sum, y, blockIdx.x, m, n, ldy);
+  join(parts, sum[0][0], y, blockIdx.x, m, n, ldy);
 }
+
+// What a wave holds of 16 MT rows and 16 NT columns: the codes of two tiles, x of one on its way.
+template <int MT, int NT, int SPG>
+struct Block {
+  TileRow from[NT];
+  __amdgpu_buffer_rsrc_t rows[MT];
+  Codes<4 / SPG> w[2][NT];
+  Columns read[MT];
+  uint32_t at[4];  // of whole tiles of rows; those that are not whole have their last rows' places cut below
+  int m[MT], k, lane;
+  long ldx;
+
+  DX_DEVICE Block(const uint16_t *x, const u32x4 *codes, const uint32_t *words, long m0, long m, int tile0, int n, int k,
+                  int groups, long ldx)
+      : k(k), lane(threadIdx.x & 63), ldx(ldx) {
+    const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) from[j] = tile_row(codes, words, min(tile0 + j, tiles_n - 1), tiles_k, groups);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const long first = min(m0 + 16 * i, m - 1);
+      const int left = (int)min(m - first, 16L);
+      rows[i] = __builtin_amdgcn_make_buffer_rsrc((void *)(x + first * ldx), (short)0, (int)(((left - 1) * ldx + k) * 2),
+                                                  0x00020000);
+    }
+    Columns::places(at, 16, ldx, lane);  // rows behind the last lie behind the buffer: they read as 0 and are not stored
+  }
+  DX_DEVICE void load_x(int t) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) read[i].load(rows[i], at, t, k, lane);
+  }
+  DX_DEVICE void load_w(int set, int t) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[set][j].load(from[j], t, lane);
+  }
+  // One tile of columns, while the next one's x and the codes of `next` come.
+  DX_DEVICE void step(int set, int next, u32x4 *turned, floatx4 (&sum)[MT][NT]) {
+    u32x4 x[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) read[i].turn(turned, x[i], lane);
+    load_x(next);
+    load_w(set ^ 1, next);
+    multiply<MT, NT, SPG>(w[set], x, sum);
+  }
+};
+
+// 17 to 64 rows: the eight waves' sums of 16 MT rows and 16 NT columns.
+template <int MT, int NT, int SPG, typename OUT>
+__global__ void __launch_bounds__(THREADS)
+linear_q4_some_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
+                      OUT *__restrict__ y, long m, int n, int k, long ldx, long ldy) {
+  __shared__ float parts[WAVES][16][16 * NT + 1];
+  __shared__ u32x4 turned[WAVES][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles_k = (k + 127) >> 7;
+  const long m0 = (long)blockIdx.y * (16 * MT);
+  Block<MT, NT, SPG> b(x, codes, words, m0, m, blockIdx.x * NT, n, k, k / (32 * SPG), ldx);
+  floatx4 sum[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sum[i][j] = floatx4{0, 0, 0, 0};
+  b.load_w(0, wave);
+  b.load_x(wave);
+  for (int t = wave; t < tiles_k; t += 2 * WAVES) {
+    b.step(0, t + WAVES, turned[wave], sum);
+    b.step(1, t + 2 * WAVES, turned[wave], sum);  // behind the last tile it adds 0
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    if (i > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) parts[wave][4 * (lane >> 4) + e][16 * j + (lane & 15)] = sum[i][j][e];
+    __syncthreads();
+    for (int at = threadIdx.x; at < 256 * NT; at += THREADS) {
+      const int row = at / (16 * NT), col = at % (16 * NT), o = blockIdx.x * NT * 16 + col;
+      const long r = m0 + 16 * i + row;
+      if (r >= m || o >= n) continue;
+      float v = parts[0][row][col];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v += parts[w][row][col];
+      if constexpr (sizeof(OUT) == 2)
+        y[r * ldy + o] = f2bf(v);
+      else
+        y[r * ldy + o] = v;
+    }
+  }
+}
+
+// More rows: four waves of 16 MT rows each and the same 16 NT columns, each with all eight sums, one after the other.
+template <int MT, int NT, int SPG, typename OUT>
+__global__ void __launch_bounds__(256, 2)
+linear_q4_many_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
+                      OUT *__restrict__ y, long m, int n, int k, long ldx, long ldy) {
+  __shared__ u32x4 turned[4][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles_k = (k + 127) >> 7;
+  const long m0 = ((long)blockIdx.y * 4 + wave) * (16 * MT);
+  if (m0 >= m) return;
+  Block<MT, NT, SPG> b(x, codes, words, m0, m, blockIdx.x * NT, n, k, k / (32 * SPG), ldx);
+  floatx4 sum[MT][NT], total[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sum[i][j] = total[i][j] = floatx4{0, 0, 0, 0};
+  int t = 0;
+  auto one = [&](int set) {
+    const bool last = t + WAVES >= tiles_k;  // of its sum
+    const int next = !last ? t + WAVES : t % WAVES + 1 < WAVES ? t % WAVES + 1 : tiles_k;
+    b.step(set, next, turned[wave], sum);
+    if (last) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          total[i][j] += sum[i][j];
+          sum[i][j] = floatx4{0, 0, 0, 0};
+        }
+    }
+    t = next;
+  };
+  b.load_w(0, 0);
+  b.load_x(0);
+  for (int i = 0; i < tiles_k; i += 2) {
+    one(0);
+    if (i + 1 < tiles_k) one(1);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const long r = m0 + 16 * i + 4 * (lane >> 4) + e;
+        const int o = (blockIdx.x * NT + j) * 16 + (lane & 15);
+        if (r >= m || o >= n) continue;
+        if constexpr (sizeof(OUT) == 2)
+          y[r * ldy + o] = f2bf(total[i][j][e]);
+        else
+          y[r * ldy + o] = total[i][j][e];
+      }
+}
+
 
 // A wave lays out one tile: lane 16 q + r the codes of row r that linear_q4_kernel reads there. Once a weight, not tuned.
 struct Place {
@@ -462,16 +514,29 @@ q4_values_kernel(const u32x4 *__restrict__ codes, const uint32_t *__restrict__ w
   }
 }
 
-template <int MT, int NT, int SPG, int DEPTH>
-hipError_t run(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
+template <int MT, int NT, int SPG>
+hipError_t run_some(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
   const dim3 grid((unsigned)dx_ceil_div(w.n, 16 * NT), (unsigned)dx_ceil_div(m, 16 * MT));
   const u32x4 *codes = static_cast<const u32x4 *>(w.codes);
   if (f32)
-    linear_q4_kernel<MT, NT, SPG, DEPTH, float>
+    linear_q4_some_kernel<MT, NT, SPG, float>
         <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<float *>(y), m, w.n, w.k, ldx, ldy);
   else
-    linear_q4_kernel<MT, NT, SPG, DEPTH, uint16_t>
+    linear_q4_some_kernel<MT, NT, SPG, uint16_t>
         <<<grid, dim3(THREADS), 0, s>>>(x, codes, w.words, static_cast<uint16_t *>(y), m, w.n, w.k, ldx, ldy);
+  return hipGetLastError();
+}
+
+template <int MT, int NT, int SPG>
+hipError_t run_many(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
+  const dim3 grid((unsigned)dx_ceil_div(w.n, 16 * NT), (unsigned)dx_ceil_div(m, 64 * MT));
+  const u32x4 *codes = static_cast<const u32x4 *>(w.codes);
+  if (f32)
+    linear_q4_many_kernel<MT, NT, SPG, float>
+        <<<grid, dim3(256), 0, s>>>(x, codes, w.words, static_cast<float *>(y), m, w.n, w.k, ldx, ldy);
+  else
+    linear_q4_many_kernel<MT, NT, SPG, uint16_t>
+        <<<grid, dim3(256), 0, s>>>(x, codes, w.words, static_cast<uint16_t *>(y), m, w.n, w.k, ldx, ldy);
   return hipGetLastError();
 }
 
@@ -510,8 +575,8 @@ hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long l
   if (m <= 16 && tiles <= 4) return run_few<4, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16 && tiles <= 6) return run_few<6, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16) return run_long<SPG>(w, x, y, m, ldx, ldy, f32, s);
-  if (m <= 32) return run<2, 1, SPG, 2>(w, x, y, m, ldx, ldy, f32, s);
-  return run<4, 4, SPG, 1>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 64) return run_some<2, 1, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  return run_many<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
 }
 
 inline long tiles_of(const Q4Weight &w) { return (long)dx_ceil_div(w.n, 16) * dx_ceil_div(w.k, 128); }
