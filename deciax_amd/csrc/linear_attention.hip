@@ -352,6 +352,7 @@ struct Tile {
     int shift;
     double total, rest;  // of g; of the state's scale behind the chunk
   } decay[2];  // this chunk's and the next one's
+  int lost[2];  // whether a value is no finite number
 };
 
 // A chunk's rows as a buffer of n of them: rows behind them read as zeros and are not written, without a branch. An offset
@@ -409,7 +410,7 @@ struct Fetched {
     return x;
   }
 
-  DX_DEVICE void store(Tile<DK, NC> &m, uint32_t tid) const {
+  DX_DEVICE void store(Tile<DK, NC> &m, uint32_t tid, int par) const {
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       const uint32_t at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
@@ -424,21 +425,25 @@ struct Fetched {
       const uint32_t at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
       *reinterpret_cast<u32x4 *>(m.v + place<COLS * NC>(r, c)) = v[i];
     }
+    const bf16x8 nothing = as_bf16x8(u32x4{0, 0, 0, 0});
+    floatx4 sum = {0, 0, 0, 0};  // 0 times each value: NaN where one is no finite number
+#pragma unroll
+    for (int i = 0; i < VI; ++i) sum = mfma16(nothing, as_bf16x8(v[i]), sum);
+    if (sum[0] != 0.f) m.lost[par] = 1;
   }
 };
 
-// Tokens [t0, t1) of a sequence from the state st on; OUT: with their outputs. Returns the sum of their g, in powers of two.
+// Tokens [t0, t1) of a sequence from the state st on, the first chunk's rows on their way; OUT: with their outputs. Returns
+// the sum of their g, in powers of two.
 template <int DK, int NC, bool OUT>
 DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col0, int t0, int t1,
-                       floatx4 (&st)[DK / 16][NC], Tile<DK, NC> &m) {
+                       floatx4 (&st)[DK / 16][NC], Fetched<DK, NC, OUT> &f, Tile<DK, NC> &m) {
   constexpr int N = 64, W = COLS * NC;
   constexpr bool AHEAD = DK < 256;  // operands are made ready while others are multiplied; at 256 registers are short
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kh = head / (a.h / a.hk);
   const float log2_scale = log2f(a.scale);
   double total = 0.0, next = 0.0, rest = 0.0;  // next: the first wave's, behind the chunk that it has summed last
-  Fetched<DK, NC, OUT> f;
-  f.load(a, s.start + t0, min(N, t1 - t0), head, kh, col0, threadIdx.x);
   // g of a chunk's tokens, a chunk earlier than its rows, so that no sum of them waits for the rows
   auto decay = [&](int t) {
     float g = 0.f;
@@ -455,22 +460,39 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
   };
   float g1 = decay(t0), g2 = decay(t0 + N);
   if (wave == 0) next = sums(m.decay[0], g1, t0, 0.0);
+  if (threadIdx.x < 2) m.lost[threadIdx.x] = 0;
   // waited for here: the loop's own wait for these rows is then not one for the outputs stored before it
   __builtin_amdgcn_s_waitcnt(0x0f70);
+  lds_barrier();
   int par = 0;
   for (int t = t0; t < t1; t += N, par ^= 1) {
     const int n = min(N, t1 - t);
     const long row = s.start + t;
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // places in LDS are found again for every chunk: held over all of them they take registers
+    tid &= THREADS - 1;
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-    f.store(m, tid);
+    f.store(m, tid, par);
     lds_barrier();
     g1 = g2;
     g2 = decay(t + 2 * N);
     f.load(a, row + N, max(min(N, t1 - t - N), 0), head, kh, col0, tid);  // none behind the last chunk
     const typename Tile<DK, NC>::Decay &d = m.decay[par];
     total += d.total;
+    // A weight of 0 would carry a later token's infinity or NaN to an earlier one: such values are taken out of the wave's
+    // columns, and what they reach is NaN.
+    const bool lost = __builtin_amdgcn_readfirstlane(m.lost[par]) != 0;
+    int first = N;  // of the wave's column lane % (16 NC): the first token whose value is lost
+    if (lost) {
+      const int col = 16 * NC * wave + lane % (16 * NC);
+      for (int j = N - 1; j >= 0; --j) {
+        uint16_t &v = m.v[place<W>(j, col >> 3) + (col & 7)];
+        if ((v & 0x7f80) == 0x7f80) {
+          first = j;
+          v = 0;  // by all lanes of a column alike
+        }
+      }
+    }
     floatx4 o[4][NC];
     if constexpr (OUT) {
       bf16x8 qf[DK / 32];
@@ -565,32 +587,6 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #pragma unroll
       for (int j = 0; j < 2; ++j) weight[b][j] = *reinterpret_cast<const floatx4 *>(d.to_end + 32 * b + 16 * j + 4 * g);
     }
-    const bf16x8 nothing = as_bf16x8(u32x4{0, 0, 0, 0});
-    floatx4 sum = {0, 0, 0, 0};  // 0 times each value: NaN where one is no finite number
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int y = 0; y < NC; ++y) sum = mfma16(nothing, vf[b][y], sum);
-    const bool lost = __any(sum[0] != 0.f);
-    // A weight of 0 would carry a later token's infinity or NaN to an earlier one: such values are left out of the products,
-    // and what they reach is NaN.
-    int first = N;  // of the wave's column lane % (16 NC): the first token whose value is lost
-    if (lost) {
-      for (int j = 0; j < N; ++j) {
-        const int col = 16 * NC * wave + lane % (16 * NC);
-        if (first == N && (m.v[place<W>(j, col >> 3) + (col & 7)] & 0x7f80) == 0x7f80) first = j;
-      }
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int y = 0; y < NC; ++y) {
-          u32x4 x = __builtin_bit_cast(u32x4, vf[b][y]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[e] &= ((x[e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((x[e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
-          vf[b][y] = as_bf16x8(x);
-        }
-    }
     bf16x8 wv[2][NC][3];
     auto weigh = [&](int b) {
 #pragma unroll
@@ -626,7 +622,13 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #pragma unroll
             for (int y = 0; y < NC; ++y) o[i][y] = mfma16(vf[b][y], p, o[i][y]);
           }
-      if (AHEAD) interleave<12 * NC, 5>();
+      if (AHEAD) {
+        interleave<12 * NC, 5>();
+#pragma unroll
+        for (int y = 0; y < NC; ++y)
+#pragma unroll
+          for (int z = 0; z < 3; ++z) asm volatile("" ::"v"(__builtin_bit_cast(u32x4, wv[0][y][z])));  // here, not below
+      }
       if (lost)
 #pragma unroll
         for (int y = 0; y < NC; ++y)
@@ -676,6 +678,7 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
           for (int r = 0; r < 4; ++r) st[u][y][r] += gone;
       }
     rest = d.rest;
+    if (tid == 0) m.lost[par] = 0;
     lds_barrier();
   }
   const Factor scale = factor_of(rest * 0.6931471805599453);
@@ -703,12 +706,14 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) segment_bf16_kerne
   const Sequence s = sequence(a, b);
   const la::Segments seg = la::segments(s.len);
   if (s.len <= la::STEP || i >= seg.count - 1) return;
+  Fetched<DK, NC, false> f;
+  f.load(a, s.start + i * seg.tokens, 64, head, head / (a.h / a.hk), col0, threadIdx.x);
   floatx4 st[DK / 16][NC];
 #pragma unroll
   for (int x = 0; x < DK / 16; ++x)
 #pragma unroll
     for (int y = 0; y < NC; ++y) st[x][y] = floatx4{0, 0, 0, 0};
-  const double total = tiles<DK, NC, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, m);
+  const double total = tiles<DK, NC, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, f, m);
   const long unit = ((long)b * most + i) * a.h + head;
   float *to = parts + unit * DK * a.dv;
 #pragma unroll
@@ -738,6 +743,9 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(
   if (i >= seg.count) return;
   const float *from = seg.count > 1 ? parts + (((long)b * most + i) * a.h + head) * DK * a.dv
                       : s.slot >= 0 ? a.state_in + (s.slot * a.h + head) * DK * a.dv : nullptr;
+  const int t0 = i * seg.tokens, t1 = min(t0 + seg.tokens, s.len);
+  Fetched<DK, NC, true> f;
+  f.load(a, s.start + t0, min(64, t1 - t0), head, head / (a.h / a.hk), col0, threadIdx.x);
   floatx4 st[DK / 16][NC];
 #pragma unroll
   for (int x = 0; x < DK / 16; ++x)
@@ -750,7 +758,7 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(
       for (int y = 0; y < NC; ++y)
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[x][y][r] = from[tile_at<NC>(a, x, y, r, col0)];
-  tiles<DK, NC, true>(a, s, head, col0, i * seg.tokens, min((i + 1) * seg.tokens, s.len), st, m);
+  tiles<DK, NC, true>(a, s, head, col0, t0, t1, st, f, m);
   if (i == seg.count - 1 && s.slot >= 0) {
     float *to = a.state_out + (s.slot * a.h + head) * DK * a.dv;
 #pragma unroll
