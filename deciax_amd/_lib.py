@@ -198,8 +198,16 @@ def check(status: int, what: str) -> None:
     raise RuntimeError(f"{what}: {msg}")
 
 
+_FUNCTIONS: dict[str, Any] = {}  # of the library, looked up once: a third of a small call's time on the host
+
+
 def call(name: str, *args: Any) -> None:
-    check(getattr(lib(), name)(*args), name)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(lib(), name)
+    status = fn(*args)
+    if status != DX_OK:
+        check(status, name)
 
 
 def device_arch(device: int = 0) -> str:

@@ -110,9 +110,8 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(HeadRope a) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 hipError_t run(const HeadRope &a, hipStream_t s) {
-  constexpr int ROWS = 4;
   const dim3 grid((unsigned)dx_ceil_div(a.rows, ROWS));
   if (a.interleaved)
     qk_norm_rope_kernel<T, D, ROWS, true><<<grid, dim3(THREADS), 0, s>>>(a);
@@ -121,11 +120,17 @@ hipError_t run(const HeadRope &a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Up to 1024 rows a workgroup has one: four of them would leave CUs without work.
+template <typename T, int D>
+hipError_t by_rows(const HeadRope &a, hipStream_t s) {
+  return a.rows <= 1024 ? run<T, D, 1>(a, s) : run<T, D, 4>(a, s);
+}
+
 template <typename T>
 hipError_t by_dim(const HeadRope &a, hipStream_t s) {
-  if (a.d == 64) return run<T, 64>(a, s);
-  if (a.d == 128) return run<T, 128>(a, s);
-  return run<T, 256>(a, s);
+  if (a.d == 64) return by_rows<T, 64>(a, s);
+  if (a.d == 128) return by_rows<T, 128>(a, s);
+  return by_rows<T, 256>(a, s);
 }
 
 }  // namespace

@@ -932,21 +932,21 @@ class Q4Weight:
     groups = property(lambda self: self._arrays[1])
 
     def __init__(self, codes: torch.Tensor, groups: torch.Tensor, n: int, k: int) -> None:
-        if n < 1 or k < 1 or groups.dim() != 3 or groups.shape[1] < 1 or k % groups.shape[1]:
-            raise ValueError("Q4Weight: groups must be [ceil(n / 16), k / group, 16]")
-        tiles = -(-n // 16)
-        if codes.shape != (tiles, -(-k // 128), 64, 16) or groups.shape != (tiles, groups.shape[1], 16):
-            raise ValueError(f"Q4Weight: codes {tuple(codes.shape)} and groups {tuple(groups.shape)} are not those of a "
-                             f"weight of {n} x {k}")
-        index = codes.get_device()
+        tiles, index = (n + 15) // 16, codes.get_device()
+        shape = groups.shape
+        if n < 1 or k < 1 or len(shape) != 3 or shape[1] < 1 or k % shape[1] or shape[0] != tiles or shape[2] != 16 or \
+                codes.shape != (tiles, (k + 127) // 128, 64, 16):
+            raise ValueError(f"Q4Weight: codes {tuple(codes.shape)} and groups {tuple(shape)} are not those of a weight of "
+                             f"{n} x {k}: [ceil(n / 16), ceil(k / 128), 64, 16] and [ceil(n / 16), k / group, 16]")
+        group = k // shape[1]
+        if group not in (32, 64, 128):
+            raise ValueError(f"Q4Weight: groups of {group}, not 32, 64 or 128")
         if codes.dtype != torch.uint8 or not codes.is_contiguous():
             raise ValueError("Q4Weight: codes must be contiguous uint8")
         if groups.dtype != torch.int32 or groups.get_device() != index or not groups.is_contiguous():
             raise ValueError("Q4Weight: groups must be contiguous int32 on the codes' device")
         self._arrays = codes, groups
-        self.n, self.k, self.group, self.index = n, k, k // groups.shape[1], index
-        if self.group not in (32, 64, 128):
-            raise ValueError(f"Q4Weight: groups of {self.group}, not 32, 64 or 128")
+        self.n, self.k, self.group, self.index = n, k, group, index
         self._at = codes.data_ptr(), groups.data_ptr()
 
 
@@ -960,8 +960,15 @@ def _q4_empty(n: int, k: int, group: int, device: torch.device) -> Q4Weight:
 
 def _stride(t: torch.Tensor, name: str, width: int) -> int:
     """Row stride of a 2-D view; one row has no next one."""
-    stride = _rows(t, name) if t.shape[1] > 1 else t.stride(0)
-    return stride if t.shape[0] > 1 else -(-width // 8) * 8
+    stride, step = t.stride()
+    if step != 1 and t.shape[1] > 1:
+        raise ValueError(f"{name} rows must be contiguous")
+    return stride if t.shape[0] > 1 else (width + 7) // 8 * 8
+
+
+def _spans_meet(a: int, a_bytes: int, b: int, b_bytes: int) -> bool:
+    """Whether two stretches of memory share a byte."""
+    return a < b + b_bytes and b < a + a_bytes
 
 
 def quantize_q4(w: torch.Tensor, *, group: int = 128) -> Q4Weight:
@@ -1128,7 +1135,9 @@ def qk_norm_rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
             raise ValueError(f"qk_norm_rope: out must be {dtype} [>= {rows}, >= {width}] on x's device, got {out.dtype} "
                              f"{tuple(out.shape)} on {out.device}")
         os = _stride(out, "out", width)
-        if (out.data_ptr(), os) != (x.data_ptr(), xs) and _meet(out, x):
+        size, a, b = x.element_size(), x.data_ptr(), out.data_ptr()
+        if rows > 0 and (a, xs) != (b, os) and _spans_meet(a, ((rows - 1) * xs + width) * size, b,
+                                                           ((rows - 1) * os + width) * size):
             raise ValueError("qk_norm_rope: out must be x itself or have memory of its own")
     if rows == 0 or width == 0:
         return out
@@ -1155,17 +1164,20 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     rows, kw, vw = q.shape[0], num_k_heads * k_dim, num_heads * v_dim
     if num_k_heads < 1 or num_heads < 1 or num_heads % num_k_heads:
         raise ValueError(f"linear_attention: num_heads {num_heads} must be a positive multiple of num_k_heads {num_k_heads}")
+    strides = []
     for t, name, width in ((q, "q", kw), (k, "k", kw), (v, "v", vw)):
-        if t.dim() != 2 or t.dtype != dtype or t.get_device() != index or t.shape[0] != rows or t.shape[1] < width:
+        shape = t.shape
+        if len(shape) != 2 or t.dtype != dtype or t.get_device() != index or shape[0] != rows or shape[1] < width:
             raise ValueError(f"linear_attention: {name} must be {dtype} [{rows}, >= {width}] on q's device, got {t.dtype} "
-                             f"{tuple(t.shape)} on {t.device}")
+                             f"{tuple(shape)} on {t.device}")
+        strides.append(_stride(t, name, width))
     if decay.dtype != F32 or decay.get_device() != index or decay.shape != (rows, num_heads) or \
             (num_heads > 1 and decay.stride(1) != 1):
         raise ValueError(f"linear_attention: decay must be fp32 [{rows}, {num_heads}] on q's device, heads side by side")
-    shape = (num_heads, k_dim, v_dim)
+    states = state.shape[0] if state.dim() == 4 else -1
     for t, name in ((state, "state"), (state_out, "state_out")):
-        if t is not None and (t.dtype != F32 or t.get_device() != index or t.dim() != 4 or t.shape[1:] != shape or
-                              not t.is_contiguous() or t.shape != state.shape):
+        if t is not None and (t.dtype != F32 or t.get_device() != index or t.shape != (states, num_heads, k_dim, v_dim) or
+                              not t.is_contiguous()):
             raise ValueError(f"linear_attention: {name} must be contiguous fp32 [states, {num_heads}, {k_dim}, {v_dim}] on "
                              f"q's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
     seqs = seq_start.shape[0] if seq_start.dim() == 1 else -1
@@ -1173,8 +1185,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
         if t is not None and (t.dtype != torch.int32 or t.get_device() != index or t.shape != (seqs,) or
                               not t.is_contiguous()):
             raise ValueError(f"linear_attention: {name} must be contiguous int32 [sequences] on q's device")
-    if state_index is None and state.shape[0] < seqs:
-        raise ValueError(f"linear_attention: {state.shape[0]} states for {seqs} sequences")
+    if state_index is None and states < seqs:
+        raise ValueError(f"linear_attention: {states} states for {seqs} sequences")
     if out is None:
         out = torch.empty((rows, vw), dtype=dtype, device=q.device)
     elif out.dim() != 2 or out.dtype != dtype or out.get_device() != index or out.shape[0] < rows or out.shape[1] < vw:
@@ -1182,21 +1194,23 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
                          f"{tuple(out.shape)} on {out.device}")
     elif _meet(out, q) or _meet(out, k) or _meet(out, v):
         raise ValueError("linear_attention: out must not meet q, k or v")
-    if state_out is None:
-        state_out = state
-    elif state_out.data_ptr() != state.data_ptr() and _meet(state, state_out):
+    s_in = state.data_ptr()
+    s_out = s_in if state_out is None else state_out.data_ptr()
+    size = 4 * states * num_heads * k_dim * v_dim
+    if s_in != s_out and _spans_meet(s_in, size, s_out, size):
         raise ValueError("linear_attention: state_out must be state itself or have memory of its own")
     if seqs == 0:
         return out
-    ds = decay.stride(0) if rows > 1 else num_heads
-    ws = _bytes(_lib.lib().dx_linear_attn_workspace(seqs, max_seq_len, num_heads, k_dim, v_dim), q.device)
-    spare = ws.data_ptr()  # stands in for the arrays of no rows or no states, which have no address
+    need = _lib.lib().dx_linear_attn_workspace(seqs, max_seq_len, num_heads, k_dim, v_dim)
+    spare = 0
+    if need > 0 or rows == 0 or states == 0:  # arrays of no rows or no states have no address: the workspace stands in
+        ws = _bytes(need, q.device)
+        spare, need = ws.data_ptr(), ws.numel()
     _call_on(index, "dx_linear_attn", q.data_ptr() or spare, k.data_ptr() or spare, v.data_ptr() or spare,
-             decay.data_ptr() or spare, out.data_ptr() or spare + 16, state.data_ptr() or spare,
-             state_out.data_ptr() or spare, seq_start.data_ptr(), seq_len.data_ptr(), _ptr(state_index), seqs, max_seq_len,
-             state.shape[0], rows, num_k_heads, num_heads, k_dim, v_dim, _stride(q, "q", kw), _stride(k, "k", kw),
-             _stride(v, "v", vw), ds, _stride(out, "out", vw), scale, DX_BF16 if dtype == BF16 else DX_F32, spare,
-             ws.numel())
+             decay.data_ptr() or spare, out.data_ptr() or spare + 16, s_in or spare, s_out or spare, seq_start.data_ptr(),
+             seq_len.data_ptr(), _ptr(state_index), seqs, max_seq_len, states, rows, num_k_heads, num_heads, k_dim, v_dim,
+             *strides, decay.stride(0) if rows > 1 else num_heads, _stride(out, "out", vw), scale,
+             DX_BF16 if dtype == BF16 else DX_F32, spare or None, need)
     return out
 
 
