@@ -344,7 +344,7 @@ DX_DEVICE void interleave() {
 template <int DK, int NC>
 struct Tile {
   static constexpr int TOKENS = 64, W = COLS * NC;
-  uint16_t q[TOKENS * DK], k[TOKENS * DK], v[TOKENS * W];
+  uint16_t q[TOKENS * (DK > W ? DK : W)], k[TOKENS * DK], v[TOKENS * W];  // q: behind the products with it, outputs
   u32x4 p[4][2][2][64];  // [16 queries][32 keys][part][lane]
   struct Decay {
     double sum[TOKENS];  // of g, in powers of two
@@ -638,15 +638,26 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i][y][r] = 16 * i + c >= at ? NAN : o[i][y][r];
           }
-#if defined(__HIP_DEVICE_COMPILE__)
-      const auto out = rows_of(static_cast<uint16_t *>(a.out) + row * a.os + head * a.dv + col0, n, a.os);
+      // The wave's outputs through its own part of q: stored as they lie, 8 bytes a lane in pieces of 32, they took an
+      // eighth of the kernel's time. Chunk x of row r at x ^ f(r), over banks of 16 chunks.
+      constexpr int CH = 2 * NC, LINE = 16 / CH;  // chunks of a row, rows of a line of banks
+      uint16_t *own = m.q + wave * (N * CH * 8);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int y = 0; y < NC; ++y)
-          __builtin_amdgcn_raw_buffer_store_b64(
-              u32x2{pack_bf2(o[i][y][0], o[i][y][1]), pack_bf2(o[i][y][2], o[i][y][3])}, out,
-              2 * ((uint32_t)(16 * i + c) * (uint32_t)a.os + 16 * (NC * wave + y) + 4 * g), 0, 0);
+        for (int y = 0; y < NC; ++y) {
+          const int r = 16 * i + c, x = 2 * y + (g >> 1);
+          *reinterpret_cast<u32x2 *>(own + (r * CH + (x ^ (r / LINE % CH))) * 8 + (g & 1) * 4) =
+              u32x2{pack_bf2(o[i][y][0], o[i][y][1]), pack_bf2(o[i][y][2], o[i][y][3])};
+        }
+#if defined(__HIP_DEVICE_COMPILE__)
+      const auto out = rows_of(static_cast<uint16_t *>(a.out) + row * a.os + head * a.dv + col0, n, a.os);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const uint32_t r = (64 * i + lane) / CH, x = lane % CH;
+        __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4 *>(own + (r * CH + (x ^ (r / LINE % CH))) * 8),
+                                               out, 2 * (r * (uint32_t)a.os + 16 * NC * wave + 8 * x), 0, 0);
+      }
 #endif
     }
 #pragma unroll
