@@ -70,13 +70,15 @@ DX_DEVICE Factor factor_of(double g) {
 }
 DX_DEVICE float times(float x, Factor f) { return fmaf(x, f.hi, x * f.lo); }
 
-// Token by token: thread 16 r + c has four columns and the rows r, r + 16, ..
+// Token by token: thread 16 r + c of 256 has four columns and the rows r, r + 16, ..
+template <int DK>
+constexpr int STEP_LDS = 2 * DK + 4 * COLS;  // floats
 template <typename T, int DK>
 DX_DEVICE void step_body(const LinearAttn &a, const Sequence &s, int head, int col0, float *lds) {
   constexpr int R = DK / 16;
   float *kq = lds;                    // [2][DK]
   float *part = lds + 2 * DK;         // [4 waves][COLS]
-  const int tid = threadIdx.x, c = tid & 15, r = tid >> 4, wave = tid >> 6;
+  const int tid = threadIdx.x % THREADS, c = tid & 15, r = tid >> 4, wave = tid >> 6;
   const int kh = head / (a.h / a.hk);
   const long at = ((s.slot * a.h + head) * DK + r) * (long)a.dv + col0 + 4 * c;
   floatx4 st[R];
@@ -124,7 +126,7 @@ DX_DEVICE void step_body(const LinearAttn &a, const Sequence &s, int head, int c
 
 template <typename T, int DK>
 __global__ void __launch_bounds__(THREADS) step_kernel(LinearAttn a) {
-  __shared__ __align__(16) float lds[2 * DK + 4 * COLS];
+  __shared__ __align__(16) float lds[STEP_LDS<DK>];
   const int blocks = a.dv / COLS;
   step_body<T, DK>(a, sequence(a, blockIdx.y), blockIdx.x / blocks, blockIdx.x % blocks * COLS, lds);
 }
@@ -341,9 +343,9 @@ DX_DEVICE void interleave() {
 #endif
 }
 
-template <int DK, int NC>
+template <int DK, int NC, int WAVES>
 struct Tile {
-  static constexpr int TOKENS = 64, W = COLS * NC;
+  static constexpr int TOKENS = 64, W = 16 * NC * WAVES;
   uint16_t q[TOKENS * (DK > W ? DK : W)], k[TOKENS * DK], v[TOKENS * W];  // q: behind the products with it, outputs
   u32x4 p[4][2][2][64];  // [16 queries][32 keys][part][lane]
   struct Decay {
@@ -362,14 +364,16 @@ DX_DEVICE __amdgpu_buffer_rsrc_t rows_of(const uint16_t *first, int n, long stri
 }
 
 // A chunk's rows on their way from memory.
-template <int DK, int NC, bool OUT>
+template <int DK, int NC, int WAVES, bool OUT>
 struct Fetched {
-  static constexpr int KI = DK / 32, VI = 2 * NC, KR = THREADS / (DK / 8), VR = THREADS / (8 * NC);  // loads, rows a load
+  using Shared = Tile<DK, NC, WAVES>;
+  static constexpr int THREADS = 64 * WAVES, W = Shared::W;
+  static constexpr int KR = THREADS / (DK / 8), VR = THREADS / (W / 8), KI = 64 / KR, VI = 64 / VR;  // rows a load, loads
   u32x4 q[OUT ? KI : 1], k[KI], v[VI];
 
   DX_DEVICE void load(const LinearAttn &a, long row, int n, int head, int kh, int col0, uint32_t tid) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const uint32_t kr = tid / (DK / 8), kc = 16 * (tid % (DK / 8)), vr = tid / (8 * NC), vc = 16 * (tid % (8 * NC));
+    const uint32_t kr = tid / (DK / 8), kc = 16 * (tid % (DK / 8)), vr = tid / (W / 8), vc = 16 * (tid % (W / 8));
     const uint32_t qs = 2 * (uint32_t)a.qs, ks = 2 * (uint32_t)a.ks, vs = 2 * (uint32_t)a.vs;
     const auto qp = rows_of(static_cast<const uint16_t *>(a.q) + row * a.qs + kh * DK, n, a.qs);
     const auto kp = rows_of(static_cast<const uint16_t *>(a.k) + row * a.ks + kh * DK, n, a.ks);
@@ -387,7 +391,7 @@ struct Fetched {
   // The first wave's: what the chunk's decays come to. The state is 2^x times what the registers hold: a chunk moves x, and
   // the registers are shifted by whole powers of two when x leaves [-8, 8]. So no rounding of a decay is ever multiplied
   // in, and a head that forgets slowly has nothing to multiply.
-  DX_DEVICE static double sums(typename Tile<DK, NC>::Decay &d, float g, double x, float log2_scale) {
+  DX_DEVICE static double sums(typename Shared::Decay &d, float g, double x, float log2_scale) {
     const int lane = threadIdx.x;
     double sum = (double)decay_of(g) * 1.4426950408889634;
 #pragma unroll
@@ -410,7 +414,7 @@ struct Fetched {
     return x;
   }
 
-  DX_DEVICE void store(Tile<DK, NC> &m, uint32_t tid, int par) const {
+  DX_DEVICE void store(Shared &m, uint32_t tid, int par) const {
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       const uint32_t at = tid + THREADS * i, r = at / (DK / 8), c = at % (DK / 8);
@@ -422,8 +426,8 @@ struct Fetched {
     }
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
-      const uint32_t at = tid + THREADS * i, r = at / (8 * NC), c = at % (8 * NC);
-      *reinterpret_cast<u32x4 *>(m.v + place<COLS * NC>(r, c)) = v[i];
+      const uint32_t at = tid + THREADS * i, r = at / (W / 8), c = at % (W / 8);
+      *reinterpret_cast<u32x4 *>(m.v + place<W>(r, c)) = v[i];
     }
     const bf16x8 nothing = as_bf16x8(u32x4{0, 0, 0, 0});
     floatx4 sum = {0, 0, 0, 0};  // 0 times each value: NaN where one is no finite number
@@ -435,10 +439,10 @@ struct Fetched {
 
 // Tokens [t0, t1) of a sequence from the state st on, the first chunk's rows on their way; OUT: with their outputs. Returns
 // the sum of their g, in powers of two.
-template <int DK, int NC, bool OUT>
+template <int DK, int NC, int WAVES, bool OUT>
 DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col0, int t0, int t1,
-                       floatx4 (&st)[DK / 16][NC], Fetched<DK, NC, OUT> &f, Tile<DK, NC> &m) {
-  constexpr int N = 64, W = COLS * NC;
+                       floatx4 (&st)[DK / 16][NC], Fetched<DK, NC, WAVES, OUT> &f, Tile<DK, NC, WAVES> &m) {
+  constexpr int N = 64, W = Tile<DK, NC, WAVES>::W;
   constexpr bool AHEAD = DK < 256;  // operands are made ready while others are multiplied; at 256 registers are short
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kh = head / (a.h / a.hk);
@@ -455,8 +459,8 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
 #endif
     return g;
   };
-  auto sums = [&](typename Tile<DK, NC>::Decay &d, float g, int t, double x) {
-    return Fetched<DK, NC, OUT>::sums(d, t + (int)threadIdx.x < t1 ? g : 0.f, x, log2_scale);  // rows of stride 0 have no end
+  auto sums = [&](typename Tile<DK, NC, WAVES>::Decay &d, float g, int t, double x) {
+    return Fetched<DK, NC, WAVES, OUT>::sums(d, t + (int)threadIdx.x < t1 ? g : 0.f, x, log2_scale);  // rows of stride 0 have no end
   };
   float g1 = decay(t0), g2 = decay(t0 + N);
   if (wave == 0) next = sums(m.decay[0], g1, t0, 0.0);
@@ -470,14 +474,14 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
     const long row = s.start + t;
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // places in LDS are found again for every chunk: held over all of them they take registers
-    tid &= THREADS - 1;
+    tid &= 64 * WAVES - 1;
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
     f.store(m, tid, par);
     lds_barrier();
     g1 = g2;
     g2 = decay(t + 2 * N);
     f.load(a, row + N, max(min(N, t1 - t - N), 0), head, kh, col0, tid);  // none behind the last chunk
-    const typename Tile<DK, NC>::Decay &d = m.decay[par];
+    const typename Tile<DK, NC, WAVES>::Decay &d = m.decay[par];
     total += d.total;
     // A weight of 0 would carry a later token's infinity or NaN to an earlier one: such values are taken out of the wave's
     // columns, and what they reach is NaN.
@@ -495,43 +499,51 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
     }
     floatx4 o[4][NC];
     if constexpr (OUT) {
+      const int mine = wave & 3;  // its 16 queries; eight waves share them by 32 keys
       bf16x8 qf[DK / 32];
 #pragma unroll
       for (int u = 0; u < DK / 32; ++u)
-        qf[u] = both(*reinterpret_cast<const s16x4 *>(m.q + q_half<DK>(16 * wave + c, 8 * u + 2 * g)),
-                     *reinterpret_cast<const s16x4 *>(m.q + q_half<DK>(16 * wave + c, 8 * u + 2 * g + 1)));
-      const double mine = d.sum[16 * wave + c] + log2_scale;
+        qf[u] = both(*reinterpret_cast<const s16x4 *>(m.q + q_half<DK>(16 * mine + c, 8 * u + 2 * g)),
+                     *reinterpret_cast<const s16x4 *>(m.q + q_half<DK>(16 * mine + c, 8 * u + 2 * g + 1)));
+      const double upto = d.sum[16 * mine + c] + log2_scale;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        if (2 * b > wave) break;
-        bf16x8 kf[DK / 32][2];  // all reads at once
+        if (2 * b > mine) break;
+        if (WAVES == 8 && b != wave >> 2) continue;
         double sum[8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int u = 0; u < DK / 32; ++u)
-            kf[u][j] = as_bf16x8(*reinterpret_cast<const u32x4 *>(m.k + place<DK>(32 * b + 16 * j + c, 4 * u + g)));
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum[4 * j + r] = d.sum[32 * b + 16 * j + 4 * g + r];
-        }
-        __builtin_amdgcn_sched_barrier(0);
         floatx4 w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        constexpr int AT_ONCE = DK / 32 < 4 ? DK / 32 : 4;  // reads on their way together
 #pragma unroll
-        for (int u = 0; u < DK / 32; ++u)
+        for (int u0 = 0; u0 < DK / 32; u0 += AT_ONCE) {
+          bf16x8 kf[AT_ONCE][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) w[j] = mfma16(kf[u][j], qf[u], w[j]);  // keys behind the queries: 0 below
+          for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              kf[u][j] = as_bf16x8(
+                  *reinterpret_cast<const u32x4 *>(m.k + place<DK>(32 * b + 16 * j + c, 4 * (u0 + u) + g)));
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) w[j] = mfma16(kf[u][j], qf[u0 + u], w[j]);  // keys behind the queries: 0 below
+        }
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = fast_exp2((float)(mine - sum[e]));
+        for (int e = 0; e < 8; ++e) p[e] = fast_exp2((float)(upto - sum[e]));
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float weight = w[e >> 2][e & 3] * p[e];  // before the choice: no branch around it
-          p[e] = 32 * b + 16 * (e >> 2) + 4 * g + (e & 3) <= 16 * wave + c ? weight : 0.f;
+          p[e] = 32 * b + 16 * (e >> 2) + 4 * g + (e & 3) <= 16 * mine + c ? weight : 0.f;
         }
         bf16x8 parts[2];
         split(p, parts);
 #pragma unroll
-        for (int z = 0; z < 2; ++z) m.p[wave][b][z][lane] = __builtin_bit_cast(u32x4, parts[z]);
+        for (int z = 0; z < 2; ++z) m.p[mine][b][z][lane] = __builtin_bit_cast(u32x4, parts[z]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -709,22 +721,22 @@ DX_DEVICE long tile_at(const LinearAttn &a, int x, int y, int r, int col0) {
   return (long)(16 * x + 4 * (lane >> 4) + r) * a.dv + col0 + 16 * (NC * (threadIdx.x >> 6) + y) + (lane & 15);
 }
 
-template <int DK, int NC>
-__global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
-  __shared__ __align__(16) Tile<DK, NC> m;
+template <int DK, int NC, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
+  __shared__ __align__(16) Tile<DK, NC, WAVES> m;
   const int b = blockIdx.z, i = blockIdx.y;
-  const auto [head, col0] = unit<COLS * NC>(a);
+  const auto [head, col0] = unit<16 * NC * WAVES>(a);
   const Sequence s = sequence(a, b);
   const la::Segments seg = la::segments(s.len);
   if (s.len <= la::STEP || i >= seg.count - 1) return;
-  Fetched<DK, NC, false> f;
+  Fetched<DK, NC, WAVES, false> f;
   f.load(a, s.start + i * seg.tokens, 64, head, head / (a.h / a.hk), col0, threadIdx.x);
   floatx4 st[DK / 16][NC];
 #pragma unroll
   for (int x = 0; x < DK / 16; ++x)
 #pragma unroll
     for (int y = 0; y < NC; ++y) st[x][y] = floatx4{0, 0, 0, 0};
-  const double total = tiles<DK, NC, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, f, m);
+  const double total = tiles<DK, NC, WAVES, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, f, m);
   const long unit = ((long)b * most + i) * a.h + head;
   float *to = parts + unit * DK * a.dv;
 #pragma unroll
@@ -736,17 +748,19 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) segment_bf16_kerne
   if (col0 == 0 && threadIdx.x == 0) sums[unit] = total * 0.6931471805599453;
 }
 
-template <int DK, int NC>
-__global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
-  __shared__ __align__(16) Tile<DK, NC> m;
+template <int DK, int NC, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
+  __shared__ __align__(16) Tile<DK, NC, WAVES> m;
   const int b = blockIdx.z, i = blockIdx.y;
-  const auto [head, col0] = unit<COLS * NC>(a);
+  const auto [head, col0] = unit<16 * NC * WAVES>(a);
   const Sequence s = sequence(a, b);
   if (s.len <= la::STEP) {
     if (i > 0) return;
-    for (int y = 0; y < NC; ++y) {
-      if (y > 0) __syncthreads();
-      step_body<uint16_t, DK>(a, s, head, col0 + COLS * y, reinterpret_cast<float *>(&m));
+    // 256 threads have COLS columns: the workgroup's halves side by side, or one after the other
+    const int half = threadIdx.x / THREADS;
+    for (int y = half; y < 16 * NC * WAVES / COLS; y += 64 * WAVES / THREADS) {
+      if (y > half) __syncthreads();
+      step_body<uint16_t, DK>(a, s, head, col0 + COLS * y, reinterpret_cast<float *>(&m) + half * STEP_LDS<DK>);
     }
     return;
   }
@@ -755,7 +769,7 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(
   const float *from = seg.count > 1 ? parts + (((long)b * most + i) * a.h + head) * DK * a.dv
                       : s.slot >= 0 ? a.state_in + (s.slot * a.h + head) * DK * a.dv : nullptr;
   const int t0 = i * seg.tokens, t1 = min(t0 + seg.tokens, s.len);
-  Fetched<DK, NC, true> f;
+  Fetched<DK, NC, WAVES, true> f;
   f.load(a, s.start + t0, min(64, t1 - t0), head, head / (a.h / a.hk), col0, threadIdx.x);
   floatx4 st[DK / 16][NC];
 #pragma unroll
@@ -769,7 +783,7 @@ __global__ void __launch_bounds__(THREADS, DK == 256 ? 1 : 2) chunk_bf16_kernel(
       for (int y = 0; y < NC; ++y)
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[x][y][r] = from[tile_at<NC>(a, x, y, r, col0)];
-  tiles<DK, NC, true>(a, s, head, col0, t0, t1, st, f, m);
+  tiles<DK, NC, WAVES, true>(a, s, head, col0, t0, t1, st, f, m);
   if (i == seg.count - 1 && s.slot >= 0) {
     float *to = a.state_out + (s.slot * a.h + head) * DK * a.dv;
 #pragma unroll
@@ -871,11 +885,13 @@ hipError_t run(const LinearAttn &a, hipStream_t s) {
   const int most = la::most_segments(a.max_len);
   const bool two = sizeof(T) == 2 && a.dv > COLS;  // columns of a workgroup: 2 COLS, which read each row of q and k once
   if (two) x /= 2;
-  const dim3 grid(x, most, a.num_seqs), before(x, most - 1, a.num_seqs), block(THREADS);
+  // 2 COLS columns: four waves of 32, two workgroups a CU; at DK 256, where one fills the registers, eight of 16
+  constexpr int NC = DK == 256 ? 1 : 2, WAVES = DK == 256 ? 8 : 4;
+  const dim3 grid(x, most, a.num_seqs), before(x, most - 1, a.num_seqs), block(THREADS), wide(64 * WAVES);
   if (most > 1) {
     if constexpr (sizeof(T) == 2) {
-      if (two) segment_bf16_kernel<DK, 2><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
-      else segment_bf16_kernel<DK, 1><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
+      if (two) segment_bf16_kernel<DK, NC, WAVES><<<before, wide, 0, s>>>(a, a.parts, a.sums, most);
+      else segment_bf16_kernel<DK, 1, 4><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
     } else {
       segment_kernel<T, DK><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
     }
@@ -883,8 +899,8 @@ hipError_t run(const LinearAttn &a, hipStream_t s) {
     join_kernel<<<dim3(y, a.h, a.num_seqs), block, 0, s>>>(a, a.parts, a.sums, most);
   }
   if constexpr (sizeof(T) == 2) {
-    if (two) chunk_bf16_kernel<DK, 2><<<grid, block, 0, s>>>(a, a.parts, most);
-    else chunk_bf16_kernel<DK, 1><<<grid, block, 0, s>>>(a, a.parts, most);
+    if (two) chunk_bf16_kernel<DK, NC, WAVES><<<grid, wide, 0, s>>>(a, a.parts, most);
+    else chunk_bf16_kernel<DK, 1, 4><<<grid, block, 0, s>>>(a, a.parts, most);
   } else {
     chunk_kernel<T, DK><<<grid, block, 0, s>>>(a, a.parts, most);
   }
