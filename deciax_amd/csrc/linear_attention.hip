@@ -131,122 +131,227 @@ __global__ void __launch_bounds__(THREADS) step_kernel(LinearAttn a) {
   step_body<T, DK>(a, sequence(a, blockIdx.y), blockIdx.x / blocks, blockIdx.x % blocks * COLS, lds);
 }
 
-// Chunks of 32 tokens with fp32 products (v_mfma_f32_16x16x4_f32: lane l has row or column l % 16 of an operand and k
-// l / 16, and of the result column l % 16, rows 4 (l / 16) + r).
+// A barrier for what went through LDS alone: loads of the next chunk stay on their way.
+DX_DEVICE void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ------------------------------------------------------------------------------------------ fp32, chunks of 32 tokens
+//
+// fp32 products (v_mfma_f32_16x16x4_f32: lane l has row or column l % 16 of an operand and k l / 16, and of the result
+// column l % 16, rows 4 (l / 16) + r). Four products take 16 k, of which group l / 16 has 4 (l / 16) .. + 3: rows of LDS are
+// read 16 bytes a lane, and a result tile is the four second operands of the next product as it lies. Wave w has the
+// columns 16 w .. of the state, in registers.
 DX_DEVICE floatx4 mfma_f32(float x, float y, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0); }
+
+// Rows as a buffer of n of them: those behind read as zeros and are not written, without a branch. An offset stays below
+// 2^31, since strides are below 2^24.
+DX_DEVICE __amdgpu_buffer_rsrc_t rows_of(const void *first, int n, long stride_bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)first, (short)0, (int)(n * stride_bytes), 0x00020000);
+}
+
+// What a chunk's decays come to, found by one wave: lane i has token i. Powers of two.
+struct Sums {
+  double upto, end;  // of this lane's token and of the chunk
+};
+template <int N>
+DX_DEVICE Sums sum_of(float g) {
+  const int lane = threadIdx.x & 63;
+  double sum = (double)decay_of(g) * 1.4426950408889634;
+#pragma unroll
+  for (int off = 1; off < N; off <<= 1) {
+    const double y = __shfl_up(sum, off, 64);
+    if (lane >= off) sum += y;
+  }
+  return Sums{sum, __shfl(sum, N - 1, 64)};
+}
 
 template <int DK>
 struct Chunk {
-  static constexpr int TOKENS = 32, W = DK + 4, VW = COLS + 4, PW = TOKENS + 4;
-  float q[TOKENS][W], k[TOKENS][W], v[TOKENS][VW], p[TOKENS][PW], s[DK][VW];
-  double sum[TOKENS];
-  float from_start[TOKENS], to_end[TOKENS];  // e^G_i, e^(G_C - G_j)
-  Factor all;
-  int lost;  // whether a value is no finite number
+  static constexpr int TOKENS = 32, W = DK + 4, VW = COLS + 4, PW = TOKENS + 4;  // rows 16 bytes on: on other banks
+  float q[TOKENS][W], k[TOKENS][W], v[TOKENS][VW], p[TOKENS][PW];
+  struct Decay {
+    double sum[TOKENS], total;
+    float from_start[TOKENS], to_end[TOKENS];  // 2^G_i, 2^(G_C - G_j)
+    Factor all;
+  } decay[2];  // this chunk's and the next one's
+  int lost[2];  // whether a value is no finite number
 };
 
 // The wave's columns of the state: tile i has rows 16 i + 4 (l / 16) + r, column 16 wave + l % 16.
-template <int DK>
 DX_DEVICE long state_at(const LinearAttn &a, int i, int r, int col0) {
   const int lane = threadIdx.x & 63;
   return (long)(16 * i + 4 * (lane >> 4) + r) * a.dv + col0 + 16 * (threadIdx.x >> 6) + (lane & 15);
 }
 
-// Tokens [t0, t1) of a sequence from the state st on; OUT: with their outputs. Returns the sum of their g.
-template <typename T, int DK, bool OUT>
+// A chunk's rows on their way from memory.
+template <int DK, bool OUT>
+struct FetchedF32 {
+  static constexpr int KI = DK / 32, KR = 4 * THREADS / DK, VR = 4 * THREADS / COLS;  // loads of q and k; rows a load
+  floatx4 q[OUT ? KI : 1], k[KI], v[2];
+
+  DX_DEVICE void load(const LinearAttn &a, long row, int n, int head, int kh, int col0) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t tid = threadIdx.x, kr = tid / (DK / 4), kc = 16 * (tid % (DK / 4)), vr = tid / 16, vc = 16 * (tid % 16);
+    const uint32_t qs = 4 * (uint32_t)a.qs, ks = 4 * (uint32_t)a.ks, vs = 4 * (uint32_t)a.vs;
+    const auto qp = rows_of(static_cast<const float *>(a.q) + row * a.qs + kh * DK, n, 4 * a.qs);
+    const auto kp = rows_of(static_cast<const float *>(a.k) + row * a.ks + kh * DK, n, 4 * a.ks);
+    const auto vp = rows_of(static_cast<const float *>(a.v) + row * a.vs + head * a.dv + col0, n, 4 * a.vs);
+    auto at = [](__amdgpu_buffer_rsrc_t from, uint32_t bytes) {
+      return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(from, bytes, 0, 0));
+    };
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      if (OUT) q[i] = at(qp, (kr + KR * i) * qs + kc);
+      k[i] = at(kp, (kr + KR * i) * ks + kc);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v[i] = at(vp, (vr + VR * i) * vs + vc);
+#endif
+  }
+
+  DX_DEVICE void store(Chunk<DK> &m, int par) const {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      const int r = tid / (DK / 4) + KR * i, c = 4 * (tid % (DK / 4));
+      if (OUT) *reinterpret_cast<floatx4 *>(&m.q[r][c]) = q[i];
+      *reinterpret_cast<floatx4 *>(&m.k[r][c]) = k[i];
+    }
+    bool lost = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<floatx4 *>(&m.v[tid / 16 + VR * i][4 * (tid % 16)]) = v[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lost |= !(fabsf(v[i][e]) < INFINITY);
+    }
+    if (lost) m.lost[par] = 1;
+  }
+};
+
+// Tokens [t0, t1) of a sequence from the state st on; OUT: with their outputs. Returns the sum of their g, in powers of two.
+template <int DK, bool OUT>
 DX_DEVICE double chunks(const LinearAttn &a, const Sequence &s, int head, int col0, int t0, int t1, floatx4 (&st)[DK / 16],
                         Chunk<DK> &m) {
   constexpr int N = Chunk<DK>::TOKENS;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int kh = head / (a.h / a.hk);
+  auto decay = [&](int t) { return wave == 1 && lane < N && t + lane < t1 ? a.decay[(s.start + t + lane) * a.ds + head] : 0.f; };
+  auto sums = [&](typename Chunk<DK>::Decay &d, float x) {
+    const Sums sum = sum_of<N>(x);
+    if (lane < N) {
+      d.sum[lane] = sum.upto;
+      d.from_start[lane] = exp2f((float)sum.upto);
+      d.to_end[lane] = exp2f((float)(sum.end - sum.upto));
+    }
+    if (lane == 0) {
+      d.all = factor_of(sum.end * 0.6931471805599453);
+      d.total = sum.end;
+    }
+  };
+  FetchedF32<DK, OUT> f;
+  f.load(a, s.start + t0, min(N, t1 - t0), head, kh, col0);
+  float next = decay(t0);
+  if (wave == 1) sums(m.decay[0], next);
+  next = decay(t0 + N);
+  if (tid < 2) m.lost[tid] = 0;
+  __syncthreads();
   double total = 0.0;
-  for (int t = t0; t < t1; t += N) {
+  int par = 0;
+  for (int t = t0; t < t1; t += N, par ^= 1) {
     const int n = min(N, t1 - t);
     const long row = s.start + t;
-    __syncthreads();
-    if (tid == 0) m.lost = 0;
-    __syncthreads();
-    for (int i = tid; i < N * DK; i += THREADS) {
-      const int j = i / DK, d = i % DK;
-      if (OUT) m.q[j][d] = j < n ? value(static_cast<const T *>(a.q) + (row + j) * a.qs + kh * DK + d) : 0.f;
-      m.k[j][d] = j < n ? value(static_cast<const T *>(a.k) + (row + j) * a.ks + kh * DK + d) : 0.f;
+    f.store(m, par);
+    lds_barrier();
+    f.load(a, row + N, max(min(N, t1 - t - N), 0), head, kh, col0);  // none behind the last chunk
+    const typename Chunk<DK>::Decay &d = m.decay[par];
+    total += d.total;
+    floatx4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (wave == 1) {  // whose tile of the weights is that of later tokens
+      sums(m.decay[par ^ 1], next);
+      next = decay(t + 2 * N);
     }
-    for (int i = tid; i < N * COLS; i += THREADS) {
-      const int j = i / COLS, d = i % COLS;
-      const float x = j < n ? value(static_cast<const T *>(a.v) + (row + j) * a.vs + head * a.dv + col0 + d) : 0.f;
-      m.v[j][d] = x;
-      if (!(fabsf(x) < INFINITY)) m.lost = 1;
-    }
-    if (wave == 0) {
-      double x = lane < n ? (double)decay_of(a.decay[(row + lane) * a.ds + head]) : 0.0;
-#pragma unroll
-      for (int off = 1; off < N; off <<= 1) {
-        const double y = __shfl_up(x, off, 64);
-        if (lane >= off) x += y;
-      }
-      const double end = __shfl(x, N - 1, 64);
-      if (lane < N) {
-        m.sum[lane] = x;
-        m.from_start[lane] = expf((float)x);
-        m.to_end[lane] = expf((float)(end - x));
-      }
-      if (lane == 0) m.all = factor_of(end);
-    }
-    __syncthreads();
-    total += m.sum[N - 1];
     if constexpr (OUT) {
-      {
-        const int i0 = 16 * (wave >> 1), j0 = 16 * (wave & 1);  // the wave's tile of the weights
-        floatx4 p = {0, 0, 0, 0};
-        if (i0 >= j0)
-          for (int d = 0; d < DK; d += 4) p = mfma_f32(m.q[i0 + c][d + g], m.k[j0 + c][d + g], p);
+      const int i0 = 16 * (wave >> 1), j0 = 16 * (wave & 1);
+      floatx4 p[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      if (wave != 1)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = i0 + 4 * g + r, j = j0 + c;
-          m.p[i][j] = j <= i ? p[r] * expf((float)(m.sum[i] - m.sum[j])) : 0.f;
+        for (int x = 0; x < DK; x += 16) {
+          const floatx4 qx = *reinterpret_cast<const floatx4 *>(&m.q[i0 + c][x + 4 * g]);
+          const floatx4 kx = *reinterpret_cast<const floatx4 *>(&m.k[j0 + c][x + 4 * g]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e & 1] = mfma_f32(qx[e], kx[e], p[e & 1]);
         }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = i0 + 4 * g + r, j = j0 + c;
+        const float weight = (p[0][r] + p[1][r]) * exp2f((float)(d.sum[i] - d.sum[j]));
+        m.p[i][j] = j <= i ? weight : 0.f;
       }
-      // the state's columns of this wave are written and read by it alone
 #pragma unroll
-      for (int i = 0; i < DK / 16; ++i)
+      for (int x = 0; x < DK / 16; ++x)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m.s[16 * i + 4 * g + r][16 * wave + c] = st[i][r];
-      floatx4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-      for (int d = 0; d < DK; d += 4) {
-        const float y = m.s[d + g][16 * wave + c];
+        for (int i = 0; i < 2; ++i) {
+          const floatx4 qx = *reinterpret_cast<const floatx4 *>(&m.q[16 * i + c][16 * x + 4 * g]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) o[i] = mfma_f32(m.q[16 * i + c][d + g], y, o[i]);
-      }
-      __syncthreads();
-      const bool lost = m.lost;
+          for (int e = 0; e < 4; ++e) o[i] = mfma_f32(qx[e], st[x][e], o[i]);
+        }
+    }
+    lds_barrier();
+    float v[2][4];  // rows 16 j + 4 g + e of the wave's columns
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[i][r] *= m.from_start[16 * i + 4 * g + r];
-        if (!lost) {
-          for (int j = 0; j < N; j += 4) o[i] = mfma_f32(m.p[16 * i + c][j + g], m.v[j + g][16 * wave + c], o[i]);
-        } else {  // a weight of 0 would carry a later token's infinity or NaN to this one
+      for (int e = 0; e < 4; ++e) v[j][e] = m.v[16 * j + 4 * g + e][16 * wave + c];
+    if constexpr (OUT) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[i][r] *= d.from_start[16 * i + 4 * g + r];
+      if (!m.lost[par]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const floatx4 px = *reinterpret_cast<const floatx4 *>(&m.p[16 * i + c][16 * j + 4 * g]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i] = mfma_f32(px[e], v[j][e], o[i]);
+          }
+      } else {  // a weight of 0 would carry a later token's infinity or NaN to this one
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
           for (int r = 0; r < 4; ++r)
             for (int j = 0; j <= 16 * i + 4 * g + r; ++j)
               o[i][r] = fmaf(m.p[16 * i + 4 * g + r][j], m.v[j][16 * wave + c], o[i][r]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = 16 * i + 4 * g + r;
-          if (j < n) put(static_cast<T *>(a.out) + (row + j) * a.os + head * a.dv + col0 + 16 * wave + c, a.scale * o[i][r]);
-        }
       }
+#if defined(__HIP_DEVICE_COMPILE__)
+      const auto out = rows_of(static_cast<float *>(a.out) + row * a.os + head * a.dv + col0, n, 4 * a.os);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(a.scale * o[i][r]), out,
+                                                4 * ((16 * i + 4 * g + r) * (uint32_t)a.os + 16 * wave + c), 0, 0);
+#endif
     }
-    const Factor all = m.all;
+    const Factor all = d.all;
 #pragma unroll
     for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) st[i][r] = times(st[i][r], all);
-    for (int j = 0; j < N; j += 4) {
-      const float y = m.v[j + g][16 * wave + c] * m.to_end[j + g];
 #pragma unroll
-      for (int i = 0; i < DK / 16; ++i) st[i] = mfma_f32(m.k[j + g][16 * i + c], y, st[i]);
-    }
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y = v[j][e] * d.to_end[16 * j + 4 * g + e];
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) st[i] = mfma_f32(m.k[16 * j + 4 * g + e][16 * i + c], y, st[i]);
+      }
+    lds_barrier();
+    if (tid == 0) m.lost[par] = 0;  // set again behind the next chunk's barriers
   }
   return total;
 }
@@ -272,13 +377,6 @@ DX_DEVICE s16x4 read_transposed(const uint16_t *p) {
 #else
   return s16x4{};
 #endif
-}
-
-// A barrier for what went through LDS alone: loads of the next chunk stay on their way.
-DX_DEVICE void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 
 // Rows of W values in 16-byte chunks, chunk c of row r at c ^ f(r): 16 rows' reads of one chunk, and eight rows' transposed
@@ -357,12 +455,6 @@ struct Tile {
   int lost[2];  // whether a value is no finite number
 };
 
-// A chunk's rows as a buffer of n of them: rows behind them read as zeros and are not written, without a branch. An offset
-// stays below 2^31, since strides are below 2^24.
-DX_DEVICE __amdgpu_buffer_rsrc_t rows_of(const uint16_t *first, int n, long stride) {
-  return __builtin_amdgcn_make_buffer_rsrc((void *)first, (short)0, (int)(n * stride * 2), 0x00020000);
-}
-
 // A chunk's rows on their way from memory.
 template <int DK, int NC, int WAVES, bool OUT>
 struct Fetched {
@@ -375,9 +467,9 @@ struct Fetched {
 #if defined(__HIP_DEVICE_COMPILE__)
     const uint32_t kr = tid / (DK / 8), kc = 16 * (tid % (DK / 8)), vr = tid / (W / 8), vc = 16 * (tid % (W / 8));
     const uint32_t qs = 2 * (uint32_t)a.qs, ks = 2 * (uint32_t)a.ks, vs = 2 * (uint32_t)a.vs;
-    const auto qp = rows_of(static_cast<const uint16_t *>(a.q) + row * a.qs + kh * DK, n, a.qs);
-    const auto kp = rows_of(static_cast<const uint16_t *>(a.k) + row * a.ks + kh * DK, n, a.ks);
-    const auto vp = rows_of(static_cast<const uint16_t *>(a.v) + row * a.vs + head * a.dv + col0, n, a.vs);
+    const auto qp = rows_of(static_cast<const uint16_t *>(a.q) + row * a.qs + kh * DK, n, 2 * a.qs);
+    const auto kp = rows_of(static_cast<const uint16_t *>(a.k) + row * a.ks + kh * DK, n, 2 * a.ks);
+    const auto vp = rows_of(static_cast<const uint16_t *>(a.v) + row * a.vs + head * a.dv + col0, n, 2 * a.vs);
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       if (OUT) q[i] = __builtin_amdgcn_raw_buffer_load_b128(qp, (kr + KR * i) * qs + kc, 0, 0);
@@ -393,13 +485,7 @@ struct Fetched {
   // in, and a head that forgets slowly has nothing to multiply.
   DX_DEVICE static double sums(typename Shared::Decay &d, float g, double x, float log2_scale) {
     const int lane = threadIdx.x;
-    double sum = (double)decay_of(g) * 1.4426950408889634;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double y = __shfl_up(sum, off, 64);
-      if (lane >= off) sum += y;
-    }
-    const double end = __shfl(sum, 63, 64);
+    const auto [sum, end] = sum_of<64>(g);
     d.sum[lane] = sum;
     d.from_start[lane] = fast_exp2((float)(sum + x + log2_scale));
     x += end;
@@ -663,7 +749,7 @@ DX_DEVICE double tiles(const LinearAttn &a, const Sequence &s, int head, int col
               u32x2{pack_bf2(o[i][y][0], o[i][y][1]), pack_bf2(o[i][y][2], o[i][y][3])};
         }
 #if defined(__HIP_DEVICE_COMPILE__)
-      const auto out = rows_of(static_cast<uint16_t *>(a.out) + row * a.os + head * a.dv + col0, n, a.os);
+      const auto out = rows_of(static_cast<uint16_t *>(a.out) + row * a.os + head * a.dv + col0, n, 2 * a.os);
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const uint32_t r = (64 * i + lane) / CH, x = lane % CH;
@@ -798,8 +884,8 @@ __global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) chunk_bf16_kern
 // ------------------------------------------------------------------------------------------ segments
 
 // What each segment but the last adds to the state, and the sum of its g.
-template <typename T, int DK>
-__global__ void __launch_bounds__(THREADS) segment_kernel(LinearAttn a, float *parts, double *sums, int most) {
+template <int DK>
+__global__ void __launch_bounds__(THREADS) segment_f32_kernel(LinearAttn a, float *parts, double *sums, int most) {
   __shared__ Chunk<DK> m;
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<COLS>(a);
@@ -809,14 +895,14 @@ __global__ void __launch_bounds__(THREADS) segment_kernel(LinearAttn a, float *p
   floatx4 st[DK / 16];
 #pragma unroll
   for (int x = 0; x < DK / 16; ++x) st[x] = floatx4{0, 0, 0, 0};
-  const double total = chunks<T, DK, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, m);
+  const double total = chunks<DK, false>(a, s, head, col0, i * seg.tokens, (i + 1) * seg.tokens, st, m);
   const long unit = ((long)b * most + i) * a.h + head;
   float *to = parts + unit * DK * a.dv;
 #pragma unroll
   for (int x = 0; x < DK / 16; ++x)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) to[state_at<DK>(a, x, r, col0)] = st[x][r];
-  if (col0 == 0 && threadIdx.x == 0) sums[unit] = total;
+    for (int r = 0; r < 4; ++r) to[state_at(a, x, r, col0)] = st[x][r];
+  if (col0 == 0 && threadIdx.x == 0) sums[unit] = total * 0.6931471805599453;
 }
 
 // In the place of each segment's part the state that it starts from. Four values a thread.
@@ -843,14 +929,14 @@ __global__ void __launch_bounds__(THREADS) join_kernel(LinearAttn a, float *part
   }
 }
 
-template <typename T, int DK>
-__global__ void __launch_bounds__(THREADS) chunk_kernel(LinearAttn a, const float *parts, int most) {
+template <int DK>
+__global__ void __launch_bounds__(THREADS) chunk_f32_kernel(LinearAttn a, const float *parts, int most) {
   __shared__ Chunk<DK> m;
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<COLS>(a);
   const Sequence s = sequence(a, b);
   if (s.len <= la::STEP) {
-    if (i == 0) step_body<T, DK>(a, s, head, col0, &m.q[0][0]);
+    if (i == 0) step_body<float, DK>(a, s, head, col0, &m.q[0][0]);
     return;
   }
   const la::Segments seg = la::segments(s.len);
@@ -864,14 +950,14 @@ __global__ void __launch_bounds__(THREADS) chunk_kernel(LinearAttn a, const floa
 #pragma unroll
     for (int x = 0; x < DK / 16; ++x)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) st[x][r] = from[state_at<DK>(a, x, r, col0)];
-  chunks<T, DK, true>(a, s, head, col0, i * seg.tokens, min((i + 1) * seg.tokens, s.len), st, m);
+      for (int r = 0; r < 4; ++r) st[x][r] = from[state_at(a, x, r, col0)];
+  chunks<DK, true>(a, s, head, col0, i * seg.tokens, min((i + 1) * seg.tokens, s.len), st, m);
   if (i == seg.count - 1 && s.slot >= 0) {
     float *to = a.state_out + (s.slot * a.h + head) * DK * a.dv;
 #pragma unroll
     for (int x = 0; x < DK / 16; ++x)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) to[state_at<DK>(a, x, r, col0)] = st[x][r];
+      for (int r = 0; r < 4; ++r) to[state_at(a, x, r, col0)] = st[x][r];
   }
 }
 
@@ -893,7 +979,7 @@ hipError_t run(const LinearAttn &a, hipStream_t s) {
       if (two) segment_bf16_kernel<DK, NC, WAVES><<<before, wide, 0, s>>>(a, a.parts, a.sums, most);
       else segment_bf16_kernel<DK, 1, 4><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
     } else {
-      segment_kernel<T, DK><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
+      segment_f32_kernel<DK><<<before, block, 0, s>>>(a, a.parts, a.sums, most);
     }
     const unsigned y = (unsigned)dx_ceil_div((long)a.dk * a.dv, 4 * THREADS);
     join_kernel<<<dim3(y, a.h, a.num_seqs), block, 0, s>>>(a, a.parts, a.sums, most);
@@ -902,7 +988,7 @@ hipError_t run(const LinearAttn &a, hipStream_t s) {
     if (two) chunk_bf16_kernel<DK, NC, WAVES><<<grid, wide, 0, s>>>(a, a.parts, most);
     else chunk_bf16_kernel<DK, 1, 4><<<grid, block, 0, s>>>(a, a.parts, most);
   } else {
-    chunk_kernel<T, DK><<<grid, block, 0, s>>>(a, a.parts, most);
+    chunk_f32_kernel<DK><<<grid, block, 0, s>>>(a, a.parts, most);
   }
   return hipGetLastError();
 }

@@ -575,7 +575,8 @@ hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long l
   if (m <= 16 && tiles <= 4) return run_few<4, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16 && tiles <= 6) return run_few<6, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16) return run_long<SPG>(w, x, y, m, ldx, ldy, f32, s);
-  if (m <= 64) return run_some<2, 1, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  // workgroups of 128 rows and 64 columns where there is one for every CU
+  if ((long)dx_ceil_div(w.n, 64) * dx_ceil_div(m, 128) < 256) return run_some<2, 1, SPG>(w, x, y, m, ldx, ldy, f32, s);
   return run_many<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
 }
 
