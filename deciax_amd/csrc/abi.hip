@@ -1124,7 +1124,7 @@ struct LinearAttnWorkspace {
 
 // INT64_MAX: no workspace is large enough.
 LinearAttnWorkspace linear_attn_workspace(int64_t seqs, int32_t max_len, int64_t heads, int64_t dk, int64_t dv) {
-  const int64_t most = la::most_segments(max_len);
+  const int64_t most = la::most_segments(max_len, la::limit((int)dk));
   if (most <= 1 || seqs <= 0) return {0, 0};
   if ((double)seqs * most * heads * dk * dv * 4 > 4e18) return {INT64_MAX, INT64_MAX};
   const int64_t units = seqs * most * heads;

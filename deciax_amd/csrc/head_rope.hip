@@ -123,7 +123,7 @@ hipError_t run(const HeadRope &a, hipStream_t s) {
 // Up to 1024 rows a workgroup has one: four of them would leave CUs without work.
 template <typename T, int D>
 hipError_t by_rows(const HeadRope &a, hipStream_t s) {
-  return a.rows <= 1024 ? run<T, D, 1>(a, s) : run<T, D, 4>(a, s);
+  return a.rows <= 1024 || (a.hq + a.hkv) * D >= 4096 ? run<T, D, 1>(a, s) : run<T, D, 4>(a, s);
 }
 
 template <typename T>

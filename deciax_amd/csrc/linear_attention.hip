@@ -813,7 +813,7 @@ __global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) segment_bf16_ke
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<16 * NC * WAVES>(a);
   const Sequence s = sequence(a, b);
-  const la::Segments seg = la::segments(s.len);
+  const la::Segments seg = la::segments(s.len, la::limit(DK));
   if (s.len <= la::STEP || i >= seg.count - 1) return;
   Fetched<DK, NC, WAVES, false> f;
   f.load(a, s.start + i * seg.tokens, 64, head, head / (a.h / a.hk), col0, threadIdx.x);
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) chunk_bf16_kern
     }
     return;
   }
-  const la::Segments seg = la::segments(s.len);
+  const la::Segments seg = la::segments(s.len, la::limit(DK));
   if (i >= seg.count) return;
   const float *from = seg.count > 1 ? parts + (((long)b * most + i) * a.h + head) * DK * a.dv
                       : s.slot >= 0 ? a.state_in + (s.slot * a.h + head) * DK * a.dv : nullptr;
@@ -890,8 +890,8 @@ __global__ void __launch_bounds__(THREADS) segment_f32_kernel(LinearAttn a, floa
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<COLS>(a);
   const Sequence s = sequence(a, b);
-  const la::Segments seg = la::segments(s.len);
-  if (s.len <= la::STEP || i >= seg.count - 1) return;
+  const la::Segments seg = la::segments(s.len, la::limit(DK));
+  if (s.len <= la::STEP_F32 || i >= seg.count - 1) return;
   floatx4 st[DK / 16];
 #pragma unroll
   for (int x = 0; x < DK / 16; ++x) st[x] = floatx4{0, 0, 0, 0};
@@ -909,9 +909,9 @@ __global__ void __launch_bounds__(THREADS) segment_f32_kernel(LinearAttn a, floa
 __global__ void __launch_bounds__(THREADS) join_kernel(LinearAttn a, float *parts, const double *sums, int most) {
   const int b = blockIdx.z, head = blockIdx.y;
   const Sequence s = sequence(a, b);
-  const la::Segments seg = la::segments(s.len);
+  const la::Segments seg = la::segments(s.len, la::limit(a.dk));
   const long size = (long)a.dk * a.dv, at = ((long)blockIdx.x * THREADS + threadIdx.x) * 4;
-  if (s.len <= la::STEP || seg.count == 1 || at >= size) return;
+  if (seg.count == 1 || at >= size) return;
   floatx4 st = {0, 0, 0, 0};
   if (s.slot >= 0) st = *reinterpret_cast<const floatx4 *>(a.state_in + (s.slot * a.h + head) * size + at);
   for (int i = 0; i < seg.count; ++i) {
@@ -935,11 +935,11 @@ __global__ void __launch_bounds__(THREADS) chunk_f32_kernel(LinearAttn a, const 
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<COLS>(a);
   const Sequence s = sequence(a, b);
-  if (s.len <= la::STEP) {
+  if (s.len <= la::STEP_F32) {
     if (i == 0) step_body<float, DK>(a, s, head, col0, &m.q[0][0]);
     return;
   }
-  const la::Segments seg = la::segments(s.len);
+  const la::Segments seg = la::segments(s.len, la::limit(DK));
   if (i >= seg.count) return;
   const float *from = seg.count > 1 ? parts + (((long)b * most + i) * a.h + head) * DK * a.dv
                       : s.slot >= 0 ? a.state_in + (s.slot * a.h + head) * DK * a.dv : nullptr;
@@ -964,12 +964,13 @@ __global__ void __launch_bounds__(THREADS) chunk_f32_kernel(LinearAttn a, const 
 template <typename T, int DK>
 hipError_t run(const LinearAttn &a, hipStream_t s) {
   unsigned x = (unsigned)(a.h * (a.dv / COLS));
-  if (a.max_len <= la::STEP) {
+  if (a.max_len <= (sizeof(T) == 2 ? la::STEP : la::STEP_F32)) {
     step_kernel<T, DK><<<dim3(x, a.num_seqs), dim3(THREADS), 0, s>>>(a);
     return hipGetLastError();
   }
-  const int most = la::most_segments(a.max_len);
-  const bool two = sizeof(T) == 2 && a.dv > COLS;  // columns of a workgroup: 2 COLS, which read each row of q and k once
+  const int most = la::most_segments(a.max_len, la::limit(DK));
+  // columns of a workgroup: 2 COLS, which read each row of q and k once, where COLS would make more workgroups than CUs
+  const bool two = sizeof(T) == 2 && a.dv > COLS && (long)x * most * a.num_seqs > 256;
   if (two) x /= 2;
   // 2 COLS columns: four waves of 32, two workgroups a CU; at DK 256, where one fills the registers, eight of 16
   constexpr int NC = DK == 256 ? 1 : 2, WAVES = DK == 256 ? 8 : 4;

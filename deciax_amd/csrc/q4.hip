@@ -542,8 +542,8 @@ hipError_t run_many(const Q4Weight &w, const uint16_t *x, void *y, long m, long 
 
 template <int TPW, int SPG>
 hipError_t run_few(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
-  constexpr int MOST = 512;  // workgroups: two a CU
-  const int tiles = dx_ceil_div(w.n, 16), each = dx_ceil_div(tiles, MOST);
+  const int tiles = dx_ceil_div(w.n, 16), most = TPW <= 4 && tiles > 2048 ? 512 : 256;
+  const int each = dx_ceil_div(tiles, most);
   const dim3 grid((unsigned)dx_ceil_div(tiles, each));
   const u32x4 *codes = static_cast<const u32x4 *>(w.codes);
   if (f32)
@@ -574,9 +574,13 @@ hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long l
   if (m <= 16 && tiles <= 2) return run_few<2, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16 && tiles <= 4) return run_few<4, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16 && tiles <= 6) return run_few<6, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 16 && tiles <= 8) return run_few<8, SPG>(w, x, y, m, ldx, ldy, f32, s);
   if (m <= 16) return run_long<SPG>(w, x, y, m, ldx, ldy, f32, s);
   // workgroups of 128 rows and 64 columns where there is one for every CU
-  if ((long)dx_ceil_div(w.n, 64) * dx_ceil_div(m, 128) < 256) return run_some<2, 1, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 64 || (long)dx_ceil_div(w.n, 64) * dx_ceil_div(m, 128) < 256) {
+    if ((long)dx_ceil_div(w.n, 32) * dx_ceil_div(m, 32) <= 256) return run_some<2, 2, SPG>(w, x, y, m, ldx, ldy, f32, s);
+    return run_some<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  }
   return run_many<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
 }
 

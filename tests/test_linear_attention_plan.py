@@ -14,20 +14,25 @@ PROGRAM = r'''
 #include <cstdio>
 #include <initializer_list>
 #include "linear_attention_plan.h"
-int main() {
+int sweep(int limit) {
   int most = 0;
   for (long len = 0; len <= (1L << 30); len += len < 70000 ? 1 : len / 977) {
-    const la::Segments s = la::segments((int)len);
-    if (s.count < 1 || s.tokens < 64 || s.tokens % 64) return printf("%ld: %d segments of %d\n", len, s.count, s.tokens), 1;
+    const la::Segments s = la::segments((int)len, limit);
+    if (s.count < 1 || s.tokens < 64 || s.tokens % 64) return printf("%ld: %d segments of %d\n", len, s.count, s.tokens);
     // every token in a segment, none of them empty but that of no tokens
     if ((long)s.tokens * s.count < len || (s.count > 1 && (long)s.tokens * (s.count - 1) >= len))
-      return printf("%ld: %d segments of %d\n", len, s.count, s.tokens), 1;
+      return printf("%ld: %d segments of %d\n", len, s.count, s.tokens);
     most = s.count > most ? s.count : most;
-    if (most > la::most_segments((int)len)) return printf("%ld: %d, room for %d\n", len, most, la::most_segments((int)len)), 1;
+    const int room = la::most_segments((int)len, limit);
+    if (most > room || room > limit) return printf("%ld: %d, room for %d\n", len, most, room);
   }
-  for (int len : {0, 1, la::STEP, 512, 513, 1 << 30}) {
-    const la::Segments s = la::segments(len);
-    printf("%d %d %d %d\n", len, s.tokens, s.count, la::most_segments(len));
+  return 0;
+}
+int main() {
+  if (la::limit(64) != la::limit(128) || sweep(la::limit(64)) || sweep(la::limit(256))) return 1;
+  for (int len : {0, 1, la::STEP, la::ONE, la::ONE + 1, 1 << 30}) {
+    const la::Segments s = la::segments(len, la::limit(128));
+    printf("%d %d %d %d\n", len, s.tokens, s.count, la::most_segments(len, la::limit(128)));
   }
   return 0;
 }
