@@ -70,7 +70,8 @@ DX_DEVICE Factor factor_of(double g) {
 }
 DX_DEVICE float times(float x, Factor f) { return fmaf(x, f.hi, x * f.lo); }
 
-// Token by token: thread 16 r + c of 256 has four columns and the rows r, r + 16, ..
+// Token by token: thread 16 r + c of 256 has four columns and the rows r, r + 16, .., all fp32. Bound by the state, read and
+// written once: 48 sequences of 1 token, 32 heads of 128 by 128 (202 MB) 42 us, 4.8 TB/s.
 template <int DK>
 constexpr int STEP_LDS = 2 * DK + 4 * COLS;  // floats
 template <typename T, int DK>
@@ -143,7 +144,8 @@ DX_DEVICE void lds_barrier() {
 // fp32 products (v_mfma_f32_16x16x4_f32: lane l has row or column l % 16 of an operand and k l / 16, and of the result
 // column l % 16, rows 4 (l / 16) + r). Four products take 16 k, of which group l / 16 has 4 (l / 16) .. + 3: rows of LDS are
 // read 16 bytes a lane, and a result tile is the four second operands of the next product as it lies. Wave w has the
-// columns 16 w .. of the state, in registers.
+// columns 16 w .. of the state, in registers. Bound by the chain of a sequence's chunks, of which one is about 2.3 us at keys of
+// 64 dimensions: rows are asked for a chunk ahead. 4161 tokens of 3 heads of 64 by 256 75 us; 5 of 3 to 37 tokens 10.
 DX_DEVICE floatx4 mfma_f32(float x, float y, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0); }
 
 // Rows as a buffer of n of them: those behind read as zeros and are not written, without a branch. An offset stays below
@@ -365,6 +367,12 @@ DX_DEVICE double chunks(const LinearAttn &a, const Sequence &s, int head, int co
 //     two bf16 parts, since every wave needs all of it.
 //   O^T += S^T Q^T: two tiles of S are eight k of a lane as they lie, again as two bf16 parts; Q is read by the same rows.
 //   S = K^T (w V): both read transposed; w V, w = e^(G_C - G_j), as three bf16 parts: the state keeps fp32's precision.
+// P and S as one part each would be off by 2^-8 of the mass of an output, which the output's own rounding does not hide.
+//
+// Bound by the wave's own instructions: at keys of 128 dimensions the matrix unit is busy 31% of the time and the vector
+// unit 45% (splitting into parts, decays, addresses), rarely both at once, and the chain of a chunk's phases leaves no more
+// than a tenth idle. 12 sequences of 517 to 16384 tokens, 46000 in all, 32 heads of 128 by 128: 672 us, of which 400 here, 190
+// the segments' own part, 70 the join; without the products for the state 115 less, without stores of outputs 90.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -808,7 +816,8 @@ DX_DEVICE long tile_at(const LinearAttn &a, int x, int y, int r, int col0) {
 }
 
 template <int DK, int NC, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
+__global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2)
+segment_bf16_kernel(LinearAttn a, float *parts, double *sums, int most) {
   __shared__ __align__(16) Tile<DK, NC, WAVES> m;
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<16 * NC * WAVES>(a);
@@ -835,7 +844,8 @@ __global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) segment_bf16_ke
 }
 
 template <int DK, int NC, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2) chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
+__global__ void __launch_bounds__(64 * WAVES, DK == 256 ? 1 : 2)
+chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
   __shared__ __align__(16) Tile<DK, NC, WAVES> m;
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<16 * NC * WAVES>(a);
@@ -905,7 +915,7 @@ __global__ void __launch_bounds__(THREADS) segment_f32_kernel(LinearAttn a, floa
   if (col0 == 0 && threadIdx.x == 0) sums[unit] = total * 0.6931471805599453;
 }
 
-// In the place of each segment's part the state that it starts from. Four values a thread.
+// In the place of each segment's part the state that it starts from. Four values a thread; bound by the parts' bytes.
 __global__ void __launch_bounds__(THREADS) join_kernel(LinearAttn a, float *parts, const double *sums, int most) {
   const int b = blockIdx.z, head = blockIdx.y;
   const Sequence s = sequence(a, b);
@@ -969,10 +979,13 @@ hipError_t run(const LinearAttn &a, hipStream_t s) {
     return hipGetLastError();
   }
   const int most = la::most_segments(a.max_len, la::limit(DK));
-  // columns of a workgroup: 2 COLS, which read each row of q and k once, where COLS would make more workgroups than CUs
+  // Columns of a workgroup: 2 COLS share the rows of q and k and their weights, but where COLS make no more workgroups than
+  // there are CUs they are faster (32 heads of 128 by 128, 200 tokens: 1 sequence 20 us against 24, 4 22 and 26, 5 29 and
+  // 27; 12 of 3000 648 and 534). A column's sums are the same.
   const bool two = sizeof(T) == 2 && a.dv > COLS && (long)x * most * a.num_seqs > 256;
   if (two) x /= 2;
-  // 2 COLS columns: four waves of 32, two workgroups a CU; at DK 256, where one fills the registers, eight of 16
+  // 2 COLS columns: four waves of 32, two workgroups a CU (12 of 3000: 534 us, eight waves of 16 597); at DK 256, where one
+  // fills the registers, eight of 16 (2111 tokens 86 us, four of 32 101)
   constexpr int NC = DK == 256 ? 1 : 2, WAVES = DK == 256 ? 8 : 4;
   const dim3 grid(x, most, a.num_seqs), before(x, most - 1, a.num_seqs), block(THREADS), wide(64 * WAVES);
   if (most > 1) {

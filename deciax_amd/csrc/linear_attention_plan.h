@@ -4,8 +4,9 @@
 
 namespace la {
 
-// Up to STEP tokens (STEP_F32 in fp32) a sequence goes token by token: 1 to 2.4 us each, where a chunk costs the same for 1 token and 64. Measured, heads of 128 by 128: 32 of them 7.7 and 8.6 us at 5 and
-// 6 tokens against 9.8 in a chunk, and 24 sequences 26.3 and 27.9 against 28.2; fp32, 24 sequences of 8: 31 against 57.
+// Up to STEP tokens (STEP_F32 in fp32) a sequence goes token by token, 1 to 2.4 us each, where a chunk takes the same for
+// 1 token and 64. Measured at heads of 128 by 128: 32 of them 7.7 and 8.6 us at 5 and 6 tokens against 9.8 in a chunk, 24
+// sequences 26.3 and 27.9 against 28.2; in fp32, 24 sequences of 8 tokens 31 against 57.
 //
 // Beyond, in chunks. A segment's end state needs its start state only at the end, so segments of a long sequence run side
 // by side: their own part first, then the join, then their outputs, which is the work of the states twice. One segment up

@@ -32,10 +32,12 @@ DX_DEVICE float zero_of(uint32_t word) { return (float)(word & 15u); }
 //
 // Eight sums are taken: of the tiles 0, 8, 16, .. of the columns, of 1, 9, 17, .., and so on, each in this order, and added
 // in theirs. So the order of a sum goes by k alone, and a row of y depends on its row of x alone, whichever kernel has it:
-// up to 64 rows the eight waves of a workgroup have a sum each, beyond a wave takes them one after the other.
+// with few rows the eight waves of a workgroup have a sum each, with many a wave takes them one after the other.
 //
 // The products are of x and 8 + code / 2, both exact: with X the group's sum of x (one more product, by ones),
 // sum x (code - zero) = 2 (sum x (8 + code / 2) - (8 + zero / 2) X), the difference rounded once, and only then the scale.
+// All sums in fp32. An infinity or a NaN in a row of x makes that row of y NaN.
+//
 // Reads of a weight's tiles t and groups of one tile row, and of x, as buffers: what lies behind the last column reads as 0,
 // without a branch, so that every load stays on its way until it is used.
 struct TileRow {
@@ -158,7 +160,10 @@ DX_DEVICE void join(float (&parts)[WAVES][256], const floatx4 &sum, OUT *y, int 
 }
 
 // Up to 16 rows, TPW tiles of columns a wave: x stays in registers, and the workgroup walks tiles of 16 rows of W, one in
-// `gridDim.x`; the next one's codes are on their way while this one's are multiplied. Same sums as linear_q4_kernel.
+// `gridDim.x`; the next one's codes are on their way while this one's are multiplied. Bound by the reads of the codes, once
+// there are enough: 4 rows x 256000 x 3584 (481 MB) 91 us, 5.3 TB/s; 1 x 28672 x 3584 12.2 us, half of them the first
+// tile's latency and the launch; 1 x 3584 x 4096 4.3 us, where an empty launch takes 3.4. Without x in registers each tile
+// reads it again: 166 us for the first.
 template <int TPW, int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
@@ -194,12 +199,15 @@ linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ c
   }
 }
 
-// Up to 16 rows and more columns than that: one tile of W a workgroup, codes eight tiles ahead and x two.
+// Up to 16 rows and more columns than that: one tile of W a workgroup, codes and x two tiles ahead. Bound by the chain of
+// a wave's tiles (a load's way, the turn, the products): 13 x 3585 x 14336 with groups of 32 11.2 us of 30 MB, 16 x 28672 x
+// 9216 36 us (3.8 TB/s). Codes further ahead take the registers of a second workgroup a CU and unroll more code: four tiles
+// 12.9 and 51 us, eight 13.2 and 66. One ahead 12.4 and 36.5.
 template <int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_long_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
                       OUT *__restrict__ y, int m, int n, int k, long ldx, long ldy) {
-  constexpr int AHEAD = 8, X_AHEAD = 2;
+  constexpr int AHEAD = 2;
   __shared__ __align__(16) float parts[WAVES][256];
   __shared__ u32x4 turned[WAVES][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -209,20 +217,20 @@ linear_q4_long_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ 
   uint32_t at[4];
   Columns::places(at, m, ldx, lane);
   Codes<4 / SPG> w[AHEAD][1];
-  Columns xs[X_AHEAD];
+  Columns xs[AHEAD];
 #pragma unroll
   for (int d = 0; d < AHEAD; ++d) w[d][0].load(from, wave + d * WAVES, lane);
 #pragma unroll
-  for (int d = 0; d < X_AHEAD; ++d) xs[d].load(rows, at, wave + d * WAVES, k, lane);
+  for (int d = 0; d < AHEAD; ++d) xs[d].load(rows, at, wave + d * WAVES, k, lane);
   floatx4 sum[1][1] = {{{0, 0, 0, 0}}};
   for (int t = wave; t < tiles_k; t += AHEAD * WAVES) {
 #pragma unroll
     for (int d = 0; d < AHEAD; ++d) {  // tiles behind the last add 0
       const int tile = t + d * WAVES;
-      __builtin_amdgcn_sched_barrier(0);  // one tile after the other: turned all at once they take the registers
+      __builtin_amdgcn_sched_barrier(0);  // one tile after the other: both turned at once 12.7 us for 11.2
       u32x4 step[1][4];
-      xs[d % X_AHEAD].turn(turned[wave], step[0], lane);
-      xs[d % X_AHEAD].load(rows, at, tile + X_AHEAD * WAVES, k, lane);
+      xs[d % AHEAD].turn(turned[wave], step[0], lane);
+      xs[d % AHEAD].load(rows, at, tile + AHEAD * WAVES, k, lane);
       multiply<1, 1, SPG>(w[d], step, sum);
       w[d][0].load(from, tile + AHEAD * WAVES, lane);
     }
@@ -275,7 +283,8 @@ struct Block {
   }
 };
 
-// 17 to 64 rows: the eight waves' sums of 16 MT rows and 16 NT columns.
+// More rows: the eight waves' sums of 16 MT rows and 16 NT columns. Bound by the x that each workgroup reads from L2 and turns
+// and by its waves' chains: 64 rows x 28672 x 3584 41 us, 128 x 3584 x 14336 27, 64 x 8192 x 3584 12.
 template <int MT, int NT, int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_some_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
@@ -320,7 +329,11 @@ linear_q4_some_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ 
   }
 }
 
-// More rows: four waves of 16 MT rows each and the same 16 NT columns, each with all eight sums, one after the other.
+// Many rows: four waves of 16 MT rows each and the same 16 NT columns, each with all eight sums, one after the other. Bound
+// by the vector unit: per tile and wave 128 instructions make the codes bf16 and 32 MT NT / SPG apply the zeros and scales,
+// 4 cycles each, beside 40 products of 16 cycles. 2048 x 8192 x 3584 200 us (600 TFLOP/s); 611 rows with groups of 64 82 us,
+// in 640 workgroups where 512 fit at once (the library's product of bf16 weights of that size takes 40). Larger tiles lose the second
+// workgroup of a CU: 16 MT x 16 NT of 64 x 32, 64 x 64 and 32 x 128 take 125, 125 and 135 us for those 82.
 template <int MT, int NT, int SPG, typename OUT>
 __global__ void __launch_bounds__(256, 2)
 linear_q4_many_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
@@ -374,8 +387,8 @@ linear_q4_many_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ 
       }
 }
 
-
-// A wave lays out one tile: lane 16 q + r the codes of row r that linear_q4_kernel reads there. Once a weight, not tuned.
+// A wave lays out one tile: lane 16 q + r the codes that the products read as its.
+// Once a weight, so it is not tuned.
 struct Place {
   int row, col;  // of the lane's first value of step 0
   bool in;       // the row exists
@@ -540,6 +553,9 @@ hipError_t run_many(const Q4Weight &w, const uint16_t *x, void *y, long m, long 
   return hipGetLastError();
 }
 
+// Two workgroups a CU where their registers fit (up to four tiles of x a wave) and each still has four tiles of W or more;
+// else one, with more of them: 40000 columns of 2048 9.7 us with two and 10.6 with one, 256000 of 3584 92 and 101, but 8192
+// of 3584 6.2 and 5.6.
 template <int TPW, int SPG>
 hipError_t run_few(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
   const int tiles = dx_ceil_div(w.n, 16), most = TPW <= 4 && tiles > 2048 ? 512 : 256;
@@ -568,20 +584,28 @@ hipError_t run_long(const Q4Weight &w, const uint16_t *x, void *y, long m, long 
   return hipGetLastError();
 }
 
+// Up to 16 rows: x in registers up to 8192 columns (28672 rows of W: 2048 columns 7.7 us against 11.8 with x read again,
+// 8192 23 against 28), but where each workgroup has one tile of W anyway and more than 4096 columns not (3584 rows of W and
+// 8192 columns, 16 rows of x: 7.7 against 6.6 read as it is multiplied; 2048 columns 3.4 against 3.7).
+//
+// More: tiles of 128 x 64 where there is one for every CU and more than half of their rows are in use, else eight waves a
+// tile (us of the one and the other: 128 x 16384 x 3584 34 and 39, 128 x 28672 x 3584 51 and 73, 611 x 8192 x 3584 85 and
+// 102, but 200 x 3584 x 4096 37 and 18, 64 x 28672 x 3584 43 and 40). These of 32 x 64, or of 32 x 32 where the smaller ones
+// are no more than the CUs (17 x 3584 x 4096 9.5 and 8.4, 32 x 8192 x 3584 10.0 and 8.5, but 64 x 8192 x 3584 11.7 and 14.5).
 template <int SPG>
 hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
   const int tiles = dx_ceil_div(w.k, 128 * WAVES);  // of a wave
-  if (m <= 16 && tiles <= 2) return run_few<2, SPG>(w, x, y, m, ldx, ldy, f32, s);
-  if (m <= 16 && tiles <= 4) return run_few<4, SPG>(w, x, y, m, ldx, ldy, f32, s);
-  if (m <= 16 && tiles <= 6) return run_few<6, SPG>(w, x, y, m, ldx, ldy, f32, s);
-  if (m <= 16 && tiles <= 8) return run_few<8, SPG>(w, x, y, m, ldx, ldy, f32, s);
-  if (m <= 16) return run_long<SPG>(w, x, y, m, ldx, ldy, f32, s);
-  // workgroups of 128 rows and 64 columns where there is one for every CU
-  if (m <= 64 || (long)dx_ceil_div(w.n, 64) * dx_ceil_div(m, 128) < 256) {
-    if ((long)dx_ceil_div(w.n, 32) * dx_ceil_div(m, 32) <= 256) return run_some<2, 2, SPG>(w, x, y, m, ldx, ldy, f32, s);
-    return run_some<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  if (m <= 16) {
+    if (tiles <= 2) return run_few<2, SPG>(w, x, y, m, ldx, ldy, f32, s);
+    if (tiles <= 4) return run_few<4, SPG>(w, x, y, m, ldx, ldy, f32, s);
+    if (tiles <= 6 && w.n > 4096) return run_few<6, SPG>(w, x, y, m, ldx, ldy, f32, s);
+    if (tiles <= 8 && w.n > 4096) return run_few<8, SPG>(w, x, y, m, ldx, ldy, f32, s);
+    return run_long<SPG>(w, x, y, m, ldx, ldy, f32, s);
   }
-  return run_many<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  const bool many = m > 64 && (long)dx_ceil_div(w.n, 64) * dx_ceil_div(m, 128) >= 256;
+  if (many) return run_many<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  if ((long)dx_ceil_div(w.n, 32) * dx_ceil_div(m, 32) <= 256) return run_some<2, 2, SPG>(w, x, y, m, ldx, ldy, f32, s);
+  return run_some<2, 4, SPG>(w, x, y, m, ldx, ldy, f32, s);
 }
 
 inline long tiles_of(const Q4Weight &w) { return (long)dx_ceil_div(w.n, 16) * dx_ceil_div(w.k, 128); }
