@@ -1155,7 +1155,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     [rows, >= Hk * Dk] and v [rows, >= H * Dv], bf16 or fp32, g = decay [rows, H] fp32 (log decays, <= 0; rows may be one
     row expanded), states fp32 [states, H, Dk, Dv]. Sequence b goes on from state[state_index[b]] (default: b) and leaves
     its state in `state_out` (default: `state` itself). One token a sequence and whole prompts take the same call. Returns
-    [rows, H * Dv]; rows of no sequence are not written, `out` must not meet q, k or v."""
+    [rows, H * Dv]; rows of no sequence are not written, `out` must not meet what the call reads or its states."""
     dtype, index = q.dtype, q.get_device()
     if dtype not in (BF16, F32):
         raise ValueError(f"linear_attention: q must be bf16 or fp32, got {dtype}")
@@ -1192,8 +1192,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     elif out.dim() != 2 or out.dtype != dtype or out.get_device() != index or out.shape[0] < rows or out.shape[1] < vw:
         raise ValueError(f"linear_attention: out must be {dtype} [>= {rows}, >= {vw}] on q's device, got {out.dtype} "
                          f"{tuple(out.shape)} on {out.device}")
-    elif _meet(out, q) or _meet(out, k) or _meet(out, v):
-        raise ValueError("linear_attention: out must not meet q, k or v")
+    elif any(_meet(out, t) for t in (q, k, v, decay, state, state_out) if t is not None):
+        raise ValueError("linear_attention: out must not meet q, k, v, decay or a state")
     s_in = state.data_ptr()
     s_out = s_in if state_out is None else state_out.data_ptr()
     size = 4 * states * num_heads * k_dim * v_dim

@@ -320,3 +320,26 @@ def test_refusals() -> None:
         call(s=big[:3], state_out=big[1:4])
     assert call(starts=i32([]), lengths=i32([]), s=s[:0], most=0).shape == (8, 256)
     assert call(q=q[:0], k=q[:0], v=v[:0], g=g[:0], lengths=i32([0, 0])).shape == (0, 256)
+
+
+@pytest.mark.parametrize("dk,dv,h", [(64, 128, 4), (128, 128, 4), (256, 128, 3), (128, 256, 2), (256, 256, 2)])
+def test_large_batches_are_their_sequences(dk: int, dv: int, h: int) -> None:
+    """Workgroups of twice the columns, where a batch has more of them than there are CUs: the same results to the bit."""
+    say(f"linear_attention in a batch of many heads {dk} x {dv}")
+    lengths = [1, 5, 6, 7, 40, 64, 65, 0, 769, 130] + [17 + b % 40 for b in range(256 * 64 // (h * dv))]
+    c = Case(12, lengths, 1, h, dk, dv, "bf16")
+    assert h * dv // 64 * len(lengths) > 256
+    out, state = c.run()
+    for b, n in enumerate(lengths[:12]):
+        one, s = c.run(rows=[b])
+        rows = slice(c.starts[b], c.starts[b] + n)
+        assert np.array_equal(one[rows], out[rows]) and np.array_equal(s[c.index[b]], state[c.index[b]]), n
+    small = Case(13, [7, 8, 9, 16, 769, 1041], 1, h, dk, dv, "bf16")
+    small.check(*small.run())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_lengths_around_a_rule(dtype: str) -> None:
+    say(f"linear_attention lengths around the rules {dtype}")
+    c = Case(14, [4, 5, 6, 7, 8, 9, 10, 767, 768, 769, 832, 961, 1024], 1, 1, 64, 64, dtype)
+    c.check(*c.run())

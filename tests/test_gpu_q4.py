@@ -214,3 +214,26 @@ def test_refusals() -> None:
                 lambda: K.pack_q4(x.byte(), x[:, :2], x[:, :1].byte()), lambda: K.pack_q4(x.byte(), x[:, :1])):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("n,k,group", [(16400, 160, 32), (33000, 96, 32), (4200, 5248, 128), (4200, 8192, 64),
+                                       (4200, 8320, 64), (5000, 3200, 32)])
+def test_rows_of_weights_do_not_depend_on_their_number(n: int, k: int, group: int) -> None:
+    """Kernels are chosen by the rows of x and of the weight; a result is the same to the bit whichever ran."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"linear_q4 of {n} rows of weights, k {k}")
+    r = rng(n + k)
+    parts = weight(r, n, k, group)
+    w, part = packed(*parts), packed(*(t[:48] for t in parts))
+    x = bf16_np(r.normal(size=(300, k)))
+    dev = to_dev(x)
+    want = K.linear_q4(dev, w, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    check(to_np(want[:4, :48]), x[:4], tuple(t[:48] for t in parts), False)
+    check(to_np(want[:2]), x[:2], parts, False)
+    for m in (1, 16, 17, 40, 64, 65, 128, 129, 257, 300):
+        assert torch.equal(K.linear_q4(dev[:m], w, out_dtype=torch.float32), want[:m]), m
+        assert torch.equal(K.linear_q4(dev[:m], part, out_dtype=torch.float32), want[:m, :48]), m
