@@ -1027,7 +1027,7 @@ int validate_q4(const void *codes, const void *groups, int32_t n, int32_t k, int
   REQUIRE(n > 0 && k > 0, "%s: a weight of %d x %d", what, n, k);
   SUPPORTED(group == 32 || group == 64 || group == 128, "%s: groups of %d, not 32, 64 or 128", what, group);
   SUPPORTED(k % group == 0, "%s: k = %d must be a multiple of the group %d", what, k, group);
-  SUPPORTED(n <= 1 << 24 && k <= 1 << 24 && (int64_t)n * k <= INT64_C(1) << 40, "%s: a weight of %d x %d", what, n, k);
+  SUPPORTED(n <= 1 << 24 && k <= 1 << 24 && (int64_t)n * k <= INT64_C(1) << 36, "%s: a weight of %d x %d", what, n, k);
   REQUIRE(aligned16(codes) && aligned16(groups), "%s: codes and groups must be 16-byte aligned", what);
   *out = Q4Weight{const_cast<void *>(codes), static_cast<uint32_t *>(const_cast<void *>(groups)), n, k, group};
   return DX_OK;
@@ -1109,7 +1109,7 @@ int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions, const do
           "qk_norm_rope: x, out and norms must be 16-byte aligned");
   REQUIRE(reinterpret_cast<uintptr_t>(inv_freq) % 8 == 0, "qk_norm_rope: inv_freq not aligned to its type");
   REQUIRE(!q_norm || eps >= 0.f, "qk_norm_rope: eps must be >= 0");
-  SUPPORTED(rows <= INT64_C(1) << 31, "qk_norm_rope: %ld rows beyond the launch grid", (long)rows);
+  SUPPORTED(rows < 1 << 24, "qk_norm_rope: %ld rows beyond the launch grid", (long)rows);
   if (rows == 0 || width == 0) return DX_OK;
   const HeadRope a{x, q_norm, k_norm, out, positions, inv_freq, rows, x_row_stride, out_row_stride,
                    num_q_heads, num_kv_heads, head_dim, rotary_dim / 2, eps, attention_factor, interleaved != 0};

@@ -630,7 +630,8 @@ int64_t dx_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top);
  * 1, 3, 5, 7. Missing rows and columns have code 0.
  * groups: 32-bit words [ceil(n / 16)][k / group][16], the scale (a bf16 or fp16
  * number) as fp32 with the zero in its lowest four bits; missing rows 0.
- * No counterpart in the reference, whose weights are bf16.
+ * n and k up to 2^24, n k up to 2^36. No counterpart in the reference, whose
+ * weights are bf16.
  *
  * dx_q4_quantize: from bf16 rows. A group's range, widened to hold 0, is cut
  * into 15 steps: scale = bf16((hi - lo) / 15), zero = round(-lo / scale), code =
@@ -654,10 +655,10 @@ int dx_q4_values(const void *codes, const void *groups, float *w,
 /* y[m, n] = x W^T for bf16 rows x and a weight in 4 bits, as dx_linear
  * (src/deciax/nn.py:11-19): exact products, fp32 sums, one rounding to out_dtype
  * (DX_BF16 or DX_F32). The order of a sum goes by k alone: a row of y depends on
- * its row of x, whatever m is. n is any size, y rows need no alignment, x rows lie
- * less than 2^24 elements apart. A row of
- * x with an infinity or a NaN, or whose sums of 16 x over a group pass fp32's
- * range, gives infinities or NaN in its own row of y. */
+ * its row of x, whatever m (up to 2^20) is. n is any size, y rows need no
+ * alignment, x rows lie less than 2^24 elements apart. A row of x with an
+ * infinity or a NaN, or whose sums of 16 x over a group pass fp32's range, gives
+ * infinities or NaN in its own row of y. */
 int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y,
                  int64_t m, int32_t n, int32_t k, int32_t group,
                  int64_t x_row_stride, int64_t y_row_stride, int32_t out_dtype,
@@ -672,8 +673,8 @@ int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y,
  * dimensions j and j + rotary_dim / 2, or 2 j and 2 j + 1 when `interleaved`.
  * Replaces the q / k norms and the partial rotation of
  * src/deciax/models/qwen3_5/text.py:75-91 and `apply_rope`
- * (src/deciax/nn.py:35-44). rotary_dim is a multiple of 16 up to head_dim;
- * fp32 throughout, rounded once to dtype. out is x itself (same row stride) or
+ * (src/deciax/nn.py:35-44). rotary_dim is a multiple of 16 up to head_dim, rows
+ * less than 2^24; fp32 throughout, rounded once to dtype. out is x itself (same row stride) or
  * memory that does not meet it. */
 int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
                     const double *inv_freq, const void *q_norm,
@@ -699,7 +700,8 @@ int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
  * state_out is state_in itself or memory that does not meet it; a sequence of no
  * tokens keeps its state. One token a sequence and whole prompts take the same
  * call; results do not depend on the batch. A NaN or infinity in a token's row
- * does not reach earlier tokens. max_seq_len bounds the grid: longer device
+ * does not reach earlier tokens, one of v no other column; from there on what it
+ * reaches is infinite or NaN. max_seq_len bounds the grid: longer device
  * lengths are cut to it. Row strides stay below 2^24 elements, decay's
  * below 2^22. Workspace size from dx_linear_attn_workspace. */
 int dx_linear_attn(const void *q, const void *k, const void *v,

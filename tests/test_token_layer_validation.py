@@ -62,7 +62,8 @@ def check(call, want: int) -> None:
     (dict(codes=None), INVALID), (dict(groups=None), INVALID), (dict(codes=ODD), INVALID), (dict(groups=ODD), INVALID),
     (dict(n=0), INVALID), (dict(n=-3), INVALID), (dict(k=0), INVALID), (dict(group=16), UNSUPPORTED),
     (dict(group=0), UNSUPPORTED), (dict(group=256), UNSUPPORTED), (dict(k=192), UNSUPPORTED),
-    (dict(n=(1 << 24) + 1), UNSUPPORTED), (dict(k=1 << 25), UNSUPPORTED), (dict(n=1 << 24, k=1 << 17), UNSUPPORTED)])
+    (dict(n=(1 << 24) + 1), UNSUPPORTED), (dict(k=1 << 25), UNSUPPORTED), (dict(n=1 << 24, k=1 << 17), UNSUPPORTED),
+    (dict(n=1 << 23, k=1 << 14), UNSUPPORTED)])
 def test_malformed_weights_are_refused(make, bad, want) -> None:
     check(make(**bad), want)
 
@@ -85,7 +86,7 @@ def test_q4(call, want) -> None:
     (dict(rot=8), UNSUPPORTED), (dict(rot=128), UNSUPPORTED), (dict(xs=376), INVALID), (dict(os=376), INVALID),
     (dict(xs=388), INVALID), (dict(os=388), INVALID), (dict(x=ODD), INVALID), (dict(out=ODD), INVALID),
     (dict(qn=ODD, kn=P), INVALID), (dict(freq=ctypes.c_void_p(0x10004)), INVALID), (dict(qn=P, kn=P, eps=-1.0), INVALID),
-    (dict(qn=P, kn=P, eps=math.nan), INVALID), (dict(rows=(1 << 31) + 1), UNSUPPORTED), (dict(), OK),
+    (dict(qn=P, kn=P, eps=math.nan), INVALID), (dict(rows=(1 << 31) + 1), UNSUPPORTED), (dict(rows=1 << 24), UNSUPPORTED), (dict(), OK),
     (dict(rows=5, hq=0, hkv=0), OK), (dict(xs=388, os=388, dtype=_lib.DX_F32), OK)])
 def test_qk_norm_rope(bad, want) -> None:
     check(turn(**bad), want)
