@@ -1052,7 +1052,9 @@ def rope_frequencies(rotary_dim: int, *, theta: float = 10000.0, scaling: Mappin
      "attention_factor": 0.1 ln f + 1}   pairs that turn less than beta_slow times within n positions divided by f, those
         that turn more than beta_fast times kept, a ramp over j between
     {"rope_type": "llama3", "factor": f, "original_max_position_embeddings": n, "low_freq_factor": 1,
-     "high_freq_factor": 4}   the same, with a ramp over the number of turns"""
+     "high_freq_factor": 4}   the same, with a ramp over the number of turns
+
+    Other entries are refused: what they change is not known here."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rope_frequencies: rotary_dim {rotary_dim} must be even and positive")
     if not theta > 0:
@@ -1062,8 +1064,16 @@ def rope_frequencies(rotary_dim: int, *, theta: float = 10000.0, scaling: Mappin
     options = dict(scaling or {})
     kind = options.get("rope_type", options.get("type", "default"))
     factor, attention = float(options.get("factor", 1.0)), 1.0
-    if kind not in ("default", "linear", "yarn", "llama3"):
+    context = ("factor", "original_max_position_embeddings")
+    known = {"default": (), "linear": ("factor",), "yarn": (*context, "beta_fast", "beta_slow", "attention_factor"),
+             "llama3": (*context, "low_freq_factor", "high_freq_factor")}
+    if kind not in known:
         raise ValueError(f"rope_frequencies: unknown rope_type {kind!r}")
+    others = sorted(set(options) - {"rope_type", "type", *known[kind]})
+    if others:
+        raise ValueError(f"rope_frequencies: {kind} does not know {', '.join(others)}")
+    if kind == "yarn" and not theta > 1:
+        raise ValueError(f"rope_frequencies: yarn needs a theta above 1, got {theta}")
     if not factor >= 1.0:
         raise ValueError(f"rope_frequencies: factor must be >= 1, got {factor}")
     if kind == "linear":

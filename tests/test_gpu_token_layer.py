@@ -151,3 +151,77 @@ def test_steps_from_a_graph() -> None:
         for name in want:
             assert torch.equal(got[name], want[name]), (i, name)
         captured.check(got, np.array(now), [0, 1, 2], [1, 1, 1], [c + 1 for c in now])
+
+
+def far_rows(rows: int, stride: int, last: int, width: int):
+    """A bf16 buffer of more than 2^31 elements whose last rows hold values; the rest is not written."""
+    import torch
+
+    x = torch.empty((rows, stride), dtype=torch.bfloat16, device="cuda")
+    assert rows * stride > 2 ** 31
+    x[-last:, :width] = to_dev(bf16_np(rng(last).normal(size=(last, width))))
+    return x
+
+
+def test_weights_beyond_32_bit_offsets() -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("linear_q4 of a weight of 4.8 GB")
+    n, k = 2_300_000, 4096
+    r = torch.Generator(device="cuda").manual_seed(1)
+    tiles = n // 16
+    codes = torch.empty((tiles, k // 128, 64, 16), dtype=torch.uint8, device="cuda")
+    assert codes.numel() > 2 ** 32
+    codes[-20:] = torch.randint(0, 256, (20, k // 128, 64, 16), dtype=torch.uint8, device="cuda", generator=r)
+    groups = torch.zeros((tiles, k // 128, 16), dtype=torch.int32, device="cuda")
+    groups[-20:] = torch.rand((20, k // 128, 16), device="cuda", generator=r).to(torch.bfloat16).float().view(torch.int32) | 7
+    w, part = K.Q4Weight(codes, groups, n, k), K.Q4Weight(codes[-20:].clone(), groups[-20:].clone(), 320, k)
+    x = to_dev(bf16_np(rng(5).normal(size=(70, k))))
+    for m in (1, 20, 70):
+        got, want = K.linear_q4(x[:m], w), K.linear_q4(x[:m], part)
+        assert torch.equal(got[:, -320:], want) and (got[:, :1000] == 0).all(), m
+
+
+def test_rows_beyond_32_bit_offsets() -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("token layer rows beyond 2^31 elements")
+    x = far_rows(150_000, 16384, 40, 512)
+    w = q4.packed(*q4.weight(rng(6), 300, 512, 128))
+    out = K.linear_q4(x[:, :512], w)
+    assert torch.equal(out[-40:], K.linear_q4(x[-40:, :512].contiguous(), w))
+    freq, _ = K.rope_frequencies(64)
+    positions = torch.arange(150_000, dtype=torch.int32, device="cuda")
+    kw = dict(num_q_heads=6, num_kv_heads=2, head_dim=64)
+    want = K.qk_norm_rope(x[-40:, :512].clone(), positions[-40:].clone(), freq, **kw)
+    K.qk_norm_rope(x, positions, freq, **kw)
+    assert torch.equal(x[-40:, :512], want)
+    g = -torch.rand((150_000, 2), device="cuda")
+    mixer_kw = dict(num_k_heads=1, num_heads=2, k_dim=64, v_dim=64, scale=0.125)
+
+    def run(x, g, start: int, state, **more):
+        return K.linear_attention(x[:, :64], x[:, 64:128], x[:, 128:256], g, state, i32([start]), i32([40]), 40, **mixer_kw,
+                                  **more)
+
+    state, near = (torch.zeros((1, 2, 64, 64), device="cuda") for _ in range(2))
+    room = torch.empty((150_000, 16384), dtype=torch.bfloat16, device="cuda")
+    run(x, g, 150_000 - 40, state, out=room[:, :128])
+    want = run(x[-40:, :256].contiguous(), g[-40:].contiguous(), 0, near)
+    assert torch.equal(room[-40:, :128], want) and torch.equal(state, near)
+    del room, x
+    pool = torch.empty((70_000, 2, 128, 128), device="cuda")
+    assert pool.numel() > 2 ** 31
+    y = to_dev(bf16_np(rng(7).normal(size=(900, 512))))
+    for n in (1, 50, 900):  # token by token, one segment, more of them
+        pool[-1] = 0.5
+        near = torch.full((1, 2, 128, 128), 0.5, device="cuda")
+        outs = [K.linear_attention(y[:n, :128], y[:n, 128:256], y[:n, 256:], g[:n], s, i32([0]), i32([n]), n, num_k_heads=1,
+                                   num_heads=2, k_dim=128, v_dim=128, scale=0.1, state_index=i32([len(s) - 1]))
+                for s in (pool, near)]
+        assert torch.equal(*outs) and torch.equal(pool[-1], near[0]), n
+    del pool
+    torch.cuda.empty_cache()

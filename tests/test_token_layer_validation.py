@@ -169,3 +169,20 @@ def test_rope_frequencies() -> None:
                 dict(rotary_dim=64, scaling={"rope_type": "linear", "factor": 0.5})):
         with pytest.raises(ValueError, match="rope_frequencies"):
             K.rope_frequencies(**bad, device="cpu")
+
+
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "default", "factor": 2.0}, {"rope_type": "linear", "factor": 2.0, "beta_fast": 32},
+    {"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 4096, "mscale": 0.7},
+    {"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 4096, "truncate": False},
+    {"rope_type": "llama3", "factor": 2.0, "original_max_position_embeddings": 4096, "beta_fast": 32},
+    {"rope_type": "dynamic", "factor": 2.0}, {"rope_type": "linear", "factor": 0.5}, {"rope_type": "yarn", "factor": 2.0}])
+def test_rope_scaling_that_is_not_known_is_refused(scaling) -> None:
+    with pytest.raises(ValueError, match="rope_frequencies"):
+        K.rope_frequencies(64, scaling=scaling, device="cpu")
+
+
+def test_yarn_needs_a_base_above_one() -> None:
+    with pytest.raises(ValueError, match="theta"):
+        K.rope_frequencies(64, theta=1.0, device="cpu", scaling={"type": "yarn", "factor": 2.0,
+                                                                 "original_max_position_embeddings": 4096})
