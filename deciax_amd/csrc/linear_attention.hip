@@ -489,15 +489,16 @@ struct Fetched {
   }
 
   // The first wave's: what the chunk's decays come to. The state is 2^x times what the registers hold: a chunk moves x, and
-  // the registers are shifted by whole powers of two when x leaves [-8, 8]. So no rounding of a decay is ever multiplied
-  // in, and a head that forgets slowly has nothing to multiply.
+  // the registers are shifted by whole powers of two when x leaves [0, 1). So no rounding of a decay is ever multiplied
+  // in, and a head that forgets slowly has hardly anything to multiply. With x below 0 the registers, and v times its
+  // weight on the way to them, would pass fp32's range where the state does not.
   DX_DEVICE static double sums(typename Shared::Decay &d, float g, double x, float log2_scale) {
     const int lane = threadIdx.x;
     const auto [sum, end] = sum_of<64>(g);
     d.sum[lane] = sum;
     d.from_start[lane] = fast_exp2((float)(sum + x + log2_scale));
     x += end;
-    const double whole = x < -8.0 || x > 8.0 ? rint(x) : 0.0;
+    const double whole = x < 0.0 || x >= 1.0 ? floor(x) : 0.0;
     x -= whole;
     d.to_end[lane] = fast_exp2((float)(end - sum - x));
     if (lane == 0) {

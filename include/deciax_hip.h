@@ -701,7 +701,12 @@ int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
  * tokens keeps its state. One token a sequence and whole prompts take the same
  * call; results do not depend on the batch. A NaN or infinity in a token's row
  * does not reach earlier tokens, one of v no other column; from there on what it
- * reaches is infinite or NaN. max_seq_len bounds the grid: longer device
+ * reaches is infinite or NaN. Sequences of more than 6 tokens (fp32: 8) go in
+ * chunks of 64 (32), whose sums are taken before their decays: a product of a q
+ * with the k of an earlier token of its chunk, or with the state that the chunk
+ * starts from, has to stay within fp32's range, with scale and without, and
+ * for bf16 rows states and products with k within bf16's; v may be any finite
+ * number. max_seq_len bounds the grid: longer device
  * lengths are cut to it. Row strides stay below 2^24 elements, decay's
  * below 2^22. Workspace size from dx_linear_attn_workspace. */
 int dx_linear_attn(const void *q, const void *k, const void *v,

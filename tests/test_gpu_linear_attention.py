@@ -343,3 +343,21 @@ def test_lengths_around_a_rule(dtype: str) -> None:
     say(f"linear_attention lengths around the rules {dtype}")
     c = Case(14, [4, 5, 6, 7, 8, 9, 10, 767, 768, 769, 832, 961, 1024], 1, 1, 64, 64, dtype)
     c.check(*c.run())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("rate", [0.0, 1e-3, 0.08, 1.0])
+def test_largest_values_stay_finite(rate: float, dk: int, dv: int, dtype: str) -> None:
+    """Values up to bf16's largest number, keys so small that the states and all sums stay below 2^-4 of fp32's range: what
+    is finite token by token is finite in chunks and segments, whatever the state has been scaled by in between."""
+    say(f"linear_attention largest values, rate {rate}, {dk} x {dv} {dtype}")
+    c = Case(15, [3, 40, 64, 65, 200, 900], 1, 2, dk, dv, dtype)
+    most = float.fromhex("0x1.fep127")
+    c.v = np.where(np.abs(c.v) > 0.5, np.sign(c.v) * most, bf16_np(c.v.clip(-1, 1) * 2.0 ** 126)).astype(np.float32)
+    c.k = bf16_np(c.k * 2.0 ** -20)
+    c.state = (c.state * 2.0 ** 108).astype(np.float32)
+    c.decay = (-rate * np.ones_like(c.decay)).astype(np.float32)
+    out, state = c.run()
+    assert np.isfinite(out[:, :2 * dv]).all() and np.isfinite(state).all()
+    c.check(out, state)
