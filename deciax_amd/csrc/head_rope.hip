@@ -2,7 +2,8 @@
 //
 // Per head: u = x / sqrt(mean x^2 + eps) (1 + w) (without norm weights u = x), then the first 2 `pairs` dimensions turn by
 // position * inv_freq[j]: pairs (j, j + pairs), or neighbours (2 j, 2 j + 1); cos and sin times `factor`. fp32 throughout,
-// rounded once. The angle is taken in 64 bits, as a share of a turn: in fp32 it is off by 0.06 at position 10^6.
+// rounded once. The angle is taken in 64 bits, as a share of a turn: in fp32 it is off by 0.06 at position 10^6. What fp32
+// cannot hold of the share turns its cosine and sine on: else each is off by up to 2^-23.3, whatever its own size.
 #include "common.h"
 #include "kernels.h"
 
@@ -56,9 +57,10 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(HeadRope a) {
     const int r = i / pairs, j = i - r * pairs;
     double t = (double)a.positions[row0 + r] * a.inv_freq[j] * 0.15915494309189535;  // turns: by 1 / (2 pi)
     t -= rint(t);
+    const float angle = (float)(2.0 * t), rest = (float)(2.0 * t - angle) * 3.14159274f;
     float s, c;
-    sincospif((float)(2.0 * t), &s, &c);
-    turns[r][j] = float2{c * a.factor, s * a.factor};
+    sincospif(angle, &s, &c);
+    turns[r][j] = float2{fmaf(-s, rest, c) * a.factor, fmaf(c, rest, s) * a.factor};
   }
   const int part = threadIdx.x % LANES, dim = 8 * part;
   float wq[8], wk[8];

@@ -164,3 +164,28 @@ def test_refusals() -> None:
                 dict(out=x.float()), dict(x=x[:, 4:], hq=3), dict(x=x[:, 1::2][:, :128], hq=1, hkv=1)):
         with pytest.raises(ValueError):
             call(**bad)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_cosines_and_sines_keep_their_own_precision(layout: str) -> None:
+    """Pairs (1, 0) turn to (cos, sin), whose small values beside a multiple of a quarter turn are as exact as the large ones.
+    sincospi's cosine and sine are off by 2 u of themselves, the angle behind its fp32 number by a product and a sum: under
+    8 u. The angle itself: three roundings of 2^-53 of at most 20000 radians, 7e-12."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"qk_norm_rope cosines and sines, {layout}")
+    rows, pairs = 5000, 32
+    freq, _ = K.rope_frequencies(2 * pairs, theta=500.0)
+    x = np.zeros((rows, 2, pairs) if layout == "half" else (rows, pairs, 2), np.float32)
+    (x[:, 0] if layout == "half" else x[..., 0])[:] = 1.0
+    positions = rng(6).integers(0, 20000, rows)
+    got = K.qk_norm_rope(to_dev(x.reshape(rows, -1), "f32"), i32(positions), freq, num_q_heads=1, num_kv_heads=0, head_dim=64,
+                         layout=layout)
+    torch.cuda.synchronize()
+    angle = positions[:, None] * freq.cpu().numpy()
+    want = np.stack([np.cos(angle), np.sin(angle)], 1 if layout == "half" else 2).reshape(rows, -1)
+    off = np.abs(to_np(got) - want)
+    tol = 8 * U * np.abs(want) + 7e-12
+    assert (off <= tol).all(), (float((off / tol).max()), float(off.max() / U))
