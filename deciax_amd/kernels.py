@@ -1054,7 +1054,8 @@ def rope_frequencies(rotary_dim: int, *, theta: float = 10000.0, scaling: Mappin
     {"rope_type": "llama3", "factor": f, "original_max_position_embeddings": n, "low_freq_factor": 1,
      "high_freq_factor": 4}   the same, with a ramp over the number of turns
 
-    Other entries are refused: what they change is not known here."""
+    A number here is its entry's default, also where that is None; f and n have to be there. Other entries are refused: what
+    they change is not known here."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rope_frequencies: rotary_dim {rotary_dim} must be even and positive")
     if not theta > 0:
@@ -1063,7 +1064,6 @@ def rope_frequencies(rotary_dim: int, *, theta: float = 10000.0, scaling: Mappin
     inv_freq = theta ** (-2.0 * pair / rotary_dim)
     options = dict(scaling or {})
     kind = options.get("rope_type", options.get("type", "default"))
-    factor, attention = float(options.get("factor", 1.0)), 1.0
     context = ("factor", "original_max_position_embeddings")
     known = {"default": (), "linear": ("factor",), "yarn": (*context, "beta_fast", "beta_slow", "attention_factor"),
              "llama3": (*context, "low_freq_factor", "high_freq_factor")}
@@ -1074,29 +1074,46 @@ def rope_frequencies(rotary_dim: int, *, theta: float = 10000.0, scaling: Mappin
         raise ValueError(f"rope_frequencies: {kind} does not know {', '.join(others)}")
     if kind == "yarn" and not theta > 1:
         raise ValueError(f"rope_frequencies: yarn needs a theta above 1, got {theta}")
+
+    def number(name: str, default: float | None = None) -> float:
+        """An entry; None stands for its default, and one without a default has to be there."""
+        value = options.get(name)
+        if value is None and default is not None:
+            return default
+        try:
+            value = float(value)
+        except (TypeError, ValueError):
+            value = math.nan
+        if not math.isfinite(value):
+            raise ValueError(f"rope_frequencies: {kind} needs a number for {name}, got {options.get(name)!r}")
+        return value
+
+    factor, attention = 1.0 if kind == "default" else number("factor"), 1.0
     if not factor >= 1.0:
         raise ValueError(f"rope_frequencies: factor must be >= 1, got {factor}")
     if kind == "linear":
         inv_freq = inv_freq / factor
     elif kind in ("yarn", "llama3"):
-        if "original_max_position_embeddings" not in options:
-            raise ValueError(f"rope_frequencies: {kind} needs original_max_position_embeddings")
-        length = float(options["original_max_position_embeddings"])
-        turns = length * inv_freq / (2 * math.pi)
+        length = number("original_max_position_embeddings")
+        if not length > 0:
+            raise ValueError(f"rope_frequencies: original_max_position_embeddings must be > 0, got {length}")
         if kind == "yarn":
+            fast, slow = number("beta_fast", 32.0), number("beta_slow", 1.0)
+            if not fast >= slow > 0:
+                raise ValueError(f"rope_frequencies: need beta_fast >= beta_slow > 0, got {fast} and {slow}")
+
             # pair j turns `beta` times within the length at j = rotary_dim ln(length / (2 pi beta)) / (2 ln theta)
             def at(beta: float) -> float:
                 return rotary_dim * math.log(length / (2 * math.pi * beta)) / (2 * math.log(theta))
 
-            low = max(math.floor(at(float(options.get("beta_fast", 32.0)))), 0)
-            high = min(math.ceil(at(float(options.get("beta_slow", 1.0)))), rotary_dim - 1)
+            low, high = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary_dim - 1)
             keep = 1.0 - ((pair - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
-            given = options.get("attention_factor")
-            attention = 0.1 * math.log(factor) + 1.0 if given is None else float(given)
+            attention = number("attention_factor", 0.1 * math.log(factor) + 1.0)
         else:
-            least, most = float(options.get("low_freq_factor", 1.0)), float(options.get("high_freq_factor", 4.0))
+            least, most = number("low_freq_factor", 1.0), number("high_freq_factor", 4.0)
             if not most > least:
                 raise ValueError("rope_frequencies: high_freq_factor must be above low_freq_factor")
+            turns = length * inv_freq / (2 * math.pi)
             keep = ((turns - least) / (most - least)).clamp(0.0, 1.0)
         inv_freq = inv_freq * (keep + (1.0 - keep) / factor)
     return inv_freq.to(device), attention

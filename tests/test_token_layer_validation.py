@@ -186,3 +186,34 @@ def test_yarn_needs_a_base_above_one() -> None:
     with pytest.raises(ValueError, match="theta"):
         K.rope_frequencies(64, theta=1.0, device="cpu", scaling={"type": "yarn", "factor": 2.0,
                                                                  "original_max_position_embeddings": 4096})
+
+
+CONTEXT = {"original_max_position_embeddings": 4096}
+
+
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "linear"}, {"rope_type": "yarn", **CONTEXT}, {"rope_type": "llama3", **CONTEXT},
+    {"rope_type": "linear", "factor": None}, {"type": "yarn", "factor": None, **CONTEXT},
+    {"rope_type": "linear", "factor": math.nan}, {"rope_type": "linear", "factor": math.inf},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": None},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 0},
+    {"rope_type": "llama3", "factor": 4.0, "original_max_position_embeddings": -4096},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": math.nan},
+    {"rope_type": "yarn", "factor": 4.0, "beta_slow": 0, **CONTEXT},
+    {"rope_type": "yarn", "factor": 4.0, "beta_fast": 1, "beta_slow": 32, **CONTEXT},
+    {"rope_type": "yarn", "factor": 4.0, "attention_factor": math.nan, **CONTEXT},
+    {"rope_type": "llama3", "factor": 4.0, "low_freq_factor": math.nan, **CONTEXT},
+    {"rope_type": "linear", "factor": "four"}], ids=str)
+def test_rope_scaling_without_its_numbers_is_refused(scaling) -> None:
+    """A factor that is not there is not 1: positions would mean something else than they did in training."""
+    with pytest.raises(ValueError, match="rope_frequencies"):
+        K.rope_frequencies(64, scaling=scaling, device="cpu")
+
+
+@pytest.mark.parametrize("name,entries", [("yarn", ("beta_fast", "beta_slow", "attention_factor")),
+                                          ("llama3", ("low_freq_factor", "high_freq_factor"))])
+def test_rope_scaling_entries_of_none_are_their_defaults(name: str, entries) -> None:
+    some = {"rope_type": name, "factor": 4.0, **CONTEXT}
+    want, one = K.rope_frequencies(64, scaling=some, device="cpu")
+    got, two = K.rope_frequencies(64, scaling=some | dict.fromkeys(entries), device="cpu")
+    assert torch.equal(got, want) and one == two
