@@ -46,6 +46,15 @@ hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
 int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
+// Whether one of n rows of `width` bytes, `stride` bytes apart, shares a byte with a block of memory.
+bool rows_meet(const void *rows, int64_t n, int64_t stride, int64_t width, const void *block, int64_t bytes) {
+  if (n <= 0 || width <= 0 || bytes <= 0) return false;
+  const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(block) - reinterpret_cast<uintptr_t>(rows));
+  // the first row that ends behind the block's start
+  const int64_t r = at < width ? 0 : stride > 0 ? (at - width) / stride + 1 : n;
+  return r < n && r * stride < at + bytes;
+}
+
 // Key-mask words per sequence: whole 64-key tiles, since a tile's second 32-key block may start past the
 // sequence's last key.
 int32_t key_mask_words(int64_t max_seq_len) { return (int32_t)(align_up(max_seq_len, 64) / 32); }
@@ -1178,6 +1187,26 @@ int dx_linear_attn(const void *q, const void *k, const void *v, const float *dec
           (long)w.total);
   REQUIRE(w.total == 0 || (workspace && aligned16(workspace)), "linear_attn: needs a 16-byte aligned workspace");
   if (num_seqs == 0) return DX_OK;
+  // What is written, against what is read: the rows and the decays by their strides, since states may lie between them.
+  const double all_states = 4.0 * num_states * num_heads * k_dim * v_dim;
+  const int64_t states = all_states < 4e18 ? (int64_t)all_states : INT64_C(1) << 61, size = 16 / vec;
+  REQUIRE(state_out == state_in || !rows_meet(state_in, 1, 0, states, state_out, states),
+          "linear_attn: state_out must be state_in itself or memory that does not meet it");
+  REQUIRE(!rows_meet(q, rows, q_row_stride * size, kw * size, state_out, states) &&
+              !rows_meet(k, rows, k_row_stride * size, kw * size, state_out, states) &&
+              !rows_meet(v, rows, v_row_stride * size, vw * size, state_out, states) &&
+              !rows_meet(decay, rows, decay_row_stride * 4, num_heads * 4, state_out, states),
+          "linear_attn: state_out must not meet q, k, v or decay");
+  REQUIRE(!rows_meet(out, rows, out_row_stride * size, vw * size, state_in, states) &&
+              !rows_meet(out, rows, out_row_stride * size, vw * size, state_out, states),
+          "linear_attn: out must not meet the states");
+  // decays one behind the other; others may have rows of `out` between them
+  const int64_t decays = decay_row_stride > num_heads ? 0 : 4 * (decay_row_stride > 0 && rows > 0 ? rows : 1) * num_heads;
+  REQUIRE(!rows_meet(out, rows, out_row_stride * size, vw * size, decay, decays), "linear_attn: out must not meet decay");
+  for (const int32_t *ints : {seq_start, seq_len, state_index})
+    REQUIRE(!ints || (!rows_meet(state_out, 1, 0, states, ints, 4 * (int64_t)num_seqs) &&
+                      !rows_meet(out, rows, out_row_stride * size, vw * size, ints, 4 * (int64_t)num_seqs)),
+            "linear_attn: out and state_out must not meet the sequences' starts, lengths or indices");
   LinearAttn a{q, k, v, out, decay, state_in, state_out, seq_start, seq_len, state_index, rows, q_row_stride,
                k_row_stride, v_row_stride, out_row_stride, decay_row_stride, num_seqs, max_seq_len, num_states,
                num_k_heads, num_heads, k_dim, v_dim, scale, static_cast<float *>(workspace),

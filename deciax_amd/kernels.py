@@ -1182,7 +1182,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     [rows, >= Hk * Dk] and v [rows, >= H * Dv], bf16 or fp32, g = decay [rows, H] fp32 (log decays, <= 0; rows may be one
     row expanded), states fp32 [states, H, Dk, Dv]. Sequence b goes on from state[state_index[b]] (default: b) and leaves
     its state in `state_out` (default: `state` itself). One token a sequence and whole prompts take the same call. Returns
-    [rows, H * Dv]; rows of no sequence are not written, `out` must not meet what the call reads or its states."""
+    [rows, H * Dv]; rows of no sequence are not written, `out` must not meet what the call reads or its states, nor the states
+    that it writes what it reads."""
     dtype, index = q.dtype, q.get_device()
     if dtype not in (BF16, F32):
         raise ValueError(f"linear_attention: q must be bf16 or fp32, got {dtype}")

@@ -697,7 +697,8 @@ int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
  * `rows` has none) and the state state_index[b] of num_states (null: b) of
  * state_in, state_out: [num_states][num_heads][k_dim][v_dim]; an index outside
  * starts from zeros and is not kept, and no two sequences may share one.
- * state_out is state_in itself or memory that does not meet it; a sequence of no
+ * state_out is state_in itself or memory that does not meet it, and neither out
+ * nor state_out meets anything else that the call reads; a sequence of no
  * tokens keeps its state. One token a sequence and whole prompts take the same
  * call; results do not depend on the batch. A NaN or infinity in a token's row
  * does not reach earlier tokens, one of v no other column; from there on what it

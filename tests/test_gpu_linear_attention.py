@@ -361,3 +361,35 @@ def test_largest_values_stay_finite(rate: float, dk: int, dv: int, dtype: str) -
     out, state = c.run()
     assert np.isfinite(out[:, :2 * dv]).all() and np.isfinite(state).all()
     c.check(out, state)
+
+
+def test_states_between_the_rows() -> None:
+    """States may lie in the same stretch of memory as the rows, but not on one of them, nor on the decays."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say("linear_attention states between rows")
+    r = rng(16)
+    n, d = 40, 64
+    room = torch.zeros((n, 3 * d + d * d), device="cuda")
+    room[:, :3 * d] = torch.from_numpy(r.normal(size=(n, 3 * d)).astype(np.float32))
+    q, k, v = room[:, :3 * d].split(d, 1)
+    g = torch.from_numpy(-r.random((n, 1)).astype(np.float32)).cuda()
+    kw = dict(num_k_heads=1, num_heads=1, k_dim=d, v_dim=d, scale=0.125)
+    args = (i32([0]), i32([n]), n)
+    want_state = torch.zeros((1, 1, d, d), device="cuda")
+    want = K.linear_attention(q, k, v, g, want_state, *args, **kw)
+    state = room[7, 3 * d:].view(1, 1, d, d)  # behind the seventh row's values, in front of the eighth's
+    before = room[:, :3 * d].clone()
+    got = K.linear_attention(q, k, v, g, state, *args, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(state, want_state) and torch.equal(room[:, :3 * d], before)
+    flat = room.view(-1)
+    for at in (7 * room.shape[1] + 3 * d - 4, 7 * room.shape[1] + 3 * d + 4, 0):
+        with pytest.raises(ValueError, match="meet"):
+            K.linear_attention(q, k, v, g, flat[at:at + d * d].view(1, 1, d, d), *args, **kw)
+    rows = torch.zeros((1, 1, d, d), device="cuda")
+    with pytest.raises(ValueError, match="meet"):
+        K.linear_attention(q, k, v, rows.view(-1, 1)[:n], rows, *args, **kw)
+    assert torch.equal(room[:, :3 * d], before)

@@ -217,3 +217,26 @@ def test_rope_scaling_entries_of_none_are_their_defaults(name: str, entries) -> 
     want, one = K.rope_frequencies(64, scaling=some, device="cpu")
     got, two = K.rope_frequencies(64, scaling=some | dict.fromkeys(entries), device="cpu")
     assert torch.equal(got, want) and one == two
+
+
+def at(offset: int) -> ctypes.c_void_p:
+    return ctypes.c_void_p(0x10000000 + offset)
+
+
+# q, k, v: 100 rows of 512 bytes, 4 KB apart; decay 100 rows of 16; 4 states of 128 KB
+ROWS = 100 * 4096
+ARRAYS = dict(q=at(0), k=at(512), v=at(1024), decay=at(ROWS), s_in=at(2 * ROWS), s_out=at(2 * ROWS), start=at(4 * ROWS),
+              length=at(4 * ROWS + 64), index=at(4 * ROWS + 128), out=at(5 * ROWS), qs=2048, ks=2048, vs=2048, seqs=2, most=40)
+STATES = 4 * 4 * 128 * 64 * 4
+
+
+@pytest.mark.parametrize("meeting", [
+    dict(s_out=at(0)), dict(s_out=at(ROWS - 4096 + 512 - 16)), dict(s_out=at(16 - STATES)), dict(s_out=at(512 + 256)),
+    dict(s_out=at(ROWS - 4096 + 1024 + 512 - 16)), dict(s_out=at(ROWS)), dict(s_out=at(ROWS + 1600 - 16)),
+    dict(s_in=at(0), s_out=at(0)), dict(s_out=at(2 * ROWS + STATES - 16)), dict(s_out=at(2 * ROWS - STATES + 16)),
+    dict(s_out=at(4 * ROWS)), dict(s_out=at(4 * ROWS + 64)), dict(s_out=at(4 * ROWS + 128)),
+    dict(out=at(2 * ROWS)), dict(out=at(2 * ROWS + STATES - 16)), dict(s_out=at(5 * ROWS + 99 * 512 + 496)),
+    dict(out=at(ROWS)), dict(out=at(4 * ROWS)), dict(out=at(4 * ROWS + 128))], ids=str)
+def test_linear_attention_does_not_write_over_what_it_reads(meeting) -> None:
+    check(attend(**ARRAYS | meeting), INVALID)
+    assert b"meet" in _lib.lib().dx_last_error()
