@@ -1093,6 +1093,10 @@ int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y, 
   REQUIRE(aligned16(x) && reinterpret_cast<uintptr_t>(y) % (out_dtype == DX_BF16 ? 2 : 4) == 0,
           "linear_q4: x must be 16-byte aligned, y to its type");
   if (m == 0) return DX_OK;
+  const int64_t size = out_dtype == DX_BF16 ? 2 : 4, tiles = align_up(n, 16) / 16;
+  REQUIRE(!rows_meet(y, m, y_row_stride * size, n * size, codes, tiles * (align_up(k, 128) * 8)) &&
+              !rows_meet(y, m, y_row_stride * size, n * size, groups, tiles * (k / group) * 64),
+          "linear_q4: y must not meet the weight");
   return check_launch(dx_linear_q4_launch(q, static_cast<const uint16_t *>(x), y, m, x_row_stride, y_row_stride,
                                           out_dtype == DX_F32, as_stream(stream)),
                       "linear_q4 launch");

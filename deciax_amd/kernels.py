@@ -1017,7 +1017,7 @@ def linear_q4(x: torch.Tensor, weight: Q4Weight, *, out: torch.Tensor | None = N
               out_dtype: torch.dtype = BF16) -> torch.Tensor:
     """`x @ w.T` for bf16 rows x [m, k] and a weight in 4 bits: `linear` of the numbers that it stands for, with exact
     products and fp32 sums, rounded once to `out_dtype` (bf16 or fp32; see dx_linear_q4). A row of the result depends on
-    its row of x alone. `out` must not meet x."""
+    its row of x alone. `out` must not meet x or the weight."""
     index, n, k = weight.index, weight.n, weight.k
     if index < 0:
         raise ValueError("linear_q4: the weight must be in device (HIP) memory")

@@ -656,7 +656,8 @@ int dx_q4_values(const void *codes, const void *groups, float *w,
  * (src/deciax/nn.py:11-19): exact products, fp32 sums, one rounding to out_dtype
  * (DX_BF16 or DX_F32). The order of a sum goes by k alone: a row of y depends on
  * its row of x, whatever m (up to 2^20) is. n is any size, y rows need no
- * alignment, x rows lie less than 2^24 elements apart. A row of x with an
+ * alignment and must not meet the weight, x rows lie less than 2^24 elements
+ * apart. A row of x with an
  * infinity or a NaN, or whose sums of 16 x over a group pass fp32's range, gives
  * infinities or NaN in its own row of y. */
 int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y,

@@ -237,3 +237,15 @@ def test_rows_of_weights_do_not_depend_on_their_number(n: int, k: int, group: in
     for m in (1, 16, 17, 40, 64, 65, 128, 129, 257, 300):
         assert torch.equal(K.linear_q4(dev[:m], w, out_dtype=torch.float32), want[:m]), m
         assert torch.equal(K.linear_q4(dev[:m], part, out_dtype=torch.float32), want[:m, :48]), m
+
+
+def test_products_over_the_weight_are_refused() -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    w = K.quantize_q4(torch.zeros((64, 256), dtype=torch.bfloat16, device="cuda"))
+    x = torch.zeros((4, 256), dtype=torch.bfloat16, device="cuda")
+    for out in (w.codes.view(-1)[:512].view(torch.bfloat16).view(4, 64), w.groups.view(-1)[:256].view(torch.float32).view(4, 64)):
+        with pytest.raises(ValueError, match="meet"):
+            K.linear_q4(x, w, out=out, out_dtype=out.dtype)

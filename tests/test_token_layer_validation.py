@@ -240,3 +240,16 @@ STATES = 4 * 4 * 128 * 64 * 4
 def test_linear_attention_does_not_write_over_what_it_reads(meeting) -> None:
     check(attend(**ARRAYS | meeting), INVALID)
     assert b"meet" in _lib.lib().dx_last_error()
+
+
+# 100 rows of x and y, 4 KB apart; codes of 8 x 256 are 2 KB (two tiles), their groups 128 bytes
+PRODUCT = dict(x=at(0), y=at(2 * ROWS), codes=at(ROWS), groups=at(ROWS + 2048), m=100, ldx=2048, ldy=2048)
+
+
+@pytest.mark.parametrize("meeting", [
+    dict(y=at(ROWS)), dict(y=at(ROWS + 2048)), dict(y=at(ROWS - 99 * 4096)), dict(y=at(ROWS + 2048 - 99 * 4096 + 120)),
+    dict(y=at(ROWS + 2046)), dict(codes=at(2 * ROWS)), dict(groups=at(2 * ROWS + 5 * 4096)),
+    dict(codes=at(2 * ROWS + 4096 - 2032)), dict(y=at(ROWS + 2040), dtype=_lib.DX_F32, ldy=1024)], ids=str)
+def test_products_are_not_written_over_the_weight(meeting) -> None:
+    check(linear(**PRODUCT | meeting), INVALID)
+    assert b"meet" in _lib.lib().dx_last_error()
