@@ -171,7 +171,7 @@ DX_DEVICE Sums sum_of(float g) {
 }
 
 template <int DK>
-struct Chunk {
+struct alignas(16) Chunk {
   static constexpr int TOKENS = 32, W = DK + 4, VW = COLS + 4, PW = TOKENS + 4;  // rows 16 bytes on: on other banks
   float q[TOKENS][W], k[TOKENS][W], v[TOKENS][VW], p[TOKENS][PW];
   struct Decay {
@@ -180,7 +180,10 @@ struct Chunk {
     Factor all;
   } decay[2];  // this chunk's and the next one's
   int lost[2];  // whether a value is no finite number
+  static_assert(W % 4 == 0 && VW % 4 == 0 && PW % 4 == 0, "rows are read and written 16 bytes at a time");
 };
+static_assert(alignof(Chunk<64>) % 16 == 0 && alignof(Chunk<128>) % 16 == 0 && alignof(Chunk<256>) % 16 == 0,
+              "rows are read and written 16 bytes at a time");
 
 // The wave's columns of the state: tile i has rows 16 i + 4 (l / 16) + r, column 16 wave + l % 16.
 DX_DEVICE long state_at(const LinearAttn &a, int i, int r, int col0) {
@@ -897,7 +900,7 @@ chunk_bf16_kernel(LinearAttn a, const float *parts, int most) {
 // What each segment but the last adds to the state, and the sum of its g.
 template <int DK>
 __global__ void __launch_bounds__(THREADS) segment_f32_kernel(LinearAttn a, float *parts, double *sums, int most) {
-  __shared__ Chunk<DK> m;
+  __shared__ __align__(16) Chunk<DK> m;
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<COLS>(a);
   const Sequence s = sequence(a, b);
@@ -953,7 +956,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(LinearAttn a, float *part
 
 template <int DK>
 __global__ void __launch_bounds__(THREADS) chunk_f32_kernel(LinearAttn a, const float *parts, int most) {
-  __shared__ Chunk<DK> m;
+  __shared__ __align__(16) Chunk<DK> m;
   const int b = blockIdx.z, i = blockIdx.y;
   const auto [head, col0] = unit<COLS>(a);
   const Sequence s = sequence(a, b);
