@@ -246,12 +246,11 @@ struct Block {
   Codes<4 / SPG> w[2][NT];
   Columns read[MT];
   uint32_t at[4];  // of whole tiles of rows; those that are not whole have their last rows' places cut below
-  int m[MT], k, lane;
-  long ldx;
+  int k, lane;
 
   DX_DEVICE Block(const uint16_t *x, const u32x4 *codes, const uint32_t *words, long m0, long m, int tile0, int n, int k,
                   int groups, long ldx)
-      : k(k), lane(threadIdx.x & 63), ldx(ldx) {
+      : k(k), lane(threadIdx.x & 63) {
     const int tiles_k = (k + 127) >> 7, tiles_n = (n + 15) >> 4;
 #pragma unroll
     for (int j = 0; j < NT; ++j) from[j] = tile_row(codes, words, min(tile0 + j, tiles_n - 1), tiles_k, groups);
