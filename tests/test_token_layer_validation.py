@@ -253,3 +253,23 @@ PRODUCT = dict(x=at(0), y=at(2 * ROWS), codes=at(ROWS), groups=at(ROWS + 2048), 
 def test_products_are_not_written_over_the_weight(meeting) -> None:
     check(linear(**PRODUCT | meeting), INVALID)
     assert b"meet" in _lib.lib().dx_last_error()
+
+
+@pytest.mark.parametrize("dim,theta,context,factor,fast,slow", [
+    (64, 1e6, 4096, 8.0, 32.0, 1.0), (128, 1e4, 4096, 4.0, 32.0, 1.0), (256, 1e4, 8192, 2.5, 24.0, 2.0), (16, 500.0, 64, 3.0, 32.0, 1.0),
+    (128, 1e6, 1 << 20, 16.0, 32.0, 1.0)])
+def test_yarn_ramps_over_the_pairs(dim, theta, context, factor, fast, slow) -> None:
+    """From the last pair that turns `beta_fast` times within the length, or the first of all, to the first one that turns no
+    more than `beta_slow` times (counted on beyond the rotated pairs, up to the dimension before the last) the share of the
+    frequencies that is divided by the factor grows by the same step from pair to pair."""
+    turns = [context * theta ** (-2 * j / dim) / (2 * math.pi) for j in range(dim)]
+    low = max([j for j in range(dim) if turns[j] >= fast], default=0)
+    high = min([j for j in range(dim) if turns[j] <= slow], default=dim - 1)
+    assert high > low
+    got, _ = K.rope_frequencies(dim, theta=theta, device="cpu", scaling={
+        "rope_type": "yarn", "factor": factor, "original_max_position_embeddings": context, "beta_fast": fast, "beta_slow": slow})
+    assert got.shape == (dim // 2,)
+    for j, f in enumerate(got.tolist()):
+        share = min(max((j - low) / (high - low), 0.0), 1.0)
+        want = theta ** (-2 * j / dim) * ((1 - share) + share / factor)
+        assert abs(f - want) < 1e-12 * want, j
