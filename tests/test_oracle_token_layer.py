@@ -76,3 +76,17 @@ def test_recurrence_is_the_weighted_sum() -> None:
     first, s1 = oracle.linear_attention(q[:4], k[:4], v[:4], g[:4], s0, 0.5)
     second, s2 = oracle.linear_attention(q[4:], k[4:], v[4:], g[4:], s1, 0.5)
     assert np.allclose(np.concatenate([first, second]), out) and np.allclose(s2, s)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_only_cut_codes_are_further_than_half_a_step(group: int) -> None:
+    """A code between 0 and 15 is the nearest one, up to the division's rounding to fp32. One that is cut to 15: range and zero
+    together pass 15 by the scale's rounding, 15 2^-8 / (1 - 2^-8) of a step, and by the zero's, half a step."""
+    w = bf16_np(rng(group + 1).normal(size=(400, 2 * group)) * np.exp(rng(group + 2).normal(size=(400, 1))))
+    code, scale, zero = oracle.quantise_q4(w, group)
+    steps = w.reshape(400, 2, group) / scale[..., None].astype(np.float64)
+    off = np.abs(code.reshape(steps.shape) - zero[..., None].astype(np.float64) - steps)
+    whole = np.rint(steps) + zero[..., None]
+    cut = (whole < 0) | (whole > 15)
+    assert (off[~cut] <= 0.5 + 16 * 2.0 ** -24).all() and (off[cut] <= 0.5 + 15 / 255 + 16 * 2.0 ** -24).all()
+    assert cut.any() and off[~cut].max() > 0.49
