@@ -249,3 +249,53 @@ def test_products_over_the_weight_are_refused() -> None:
     for out in (w.codes.view(-1)[:256].view(torch.bfloat16).view(2, 64), w.groups.view(-1)[:128].view(torch.float32).view(2, 64)):
         with pytest.raises(ValueError, match="meet"):
             K.linear_q4(x[:2], w, out=out, out_dtype=out.dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k,group", [
+    (128, 16400, 3584, 64), (129, 8200, 3584, 32), (130, 8192, 3584, 128), (257, 5500, 1344, 64), (300, 5450, 1344, 32),
+    (70, 16390, 1024, 128), (65, 16384, 1152, 128), (200, 8193, 14336, 128), (129, 8192, 14336, 32)])
+def test_many_rows_of_large_weights(m: int, n: int, k: int, group: int, dtype: str) -> None:
+    """A tile of 128 by 64 for every CU: all eight sums in one wave, some with a tile more than others. Against the oracle
+    at the edges of the tiles, and to the bit what the same rows give where the eight sums are eight waves'."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"linear_q4 many rows {m} x {n} x {k} group {group} {dtype}")
+    assert m > 64 and -(-n // 64) * -(-m // 128) >= 256
+    r = rng(m + n + k)
+    parts = weight(r, n, k, group)
+    w = packed(*parts)
+    x = bf16_np(r.normal(size=(m, k)) * np.exp(r.normal(size=k) * 0.5))
+    dev = to_dev(x)
+    t = torch.bfloat16 if dtype == "bf16" else torch.float32
+    room = torch.full((m + 1, n + 3), 5.0, dtype=t, device="cuda")
+    out = K.linear_q4(dev, w, out=room[:m, 1:n + 1], out_dtype=t)
+    torch.cuda.synchronize()
+    rows = sorted({0, 15, 16, 31, 32, 63, 64, m // 2, m - 1} & set(range(m)))
+    cols = sorted({0, 15, 16, 63, 64, n // 2, n // 2 + 1, n - 17, n - 1})
+    check(to_np(out)[np.ix_(rows, cols)], x[rows], tuple(p[cols] for p in parts), dtype == "bf16")
+    for at in (0, m - 64, m - 16):
+        few = K.linear_q4(dev[at:at + 64], w, out_dtype=t)
+        assert torch.equal(few, out[at:at + len(few)]), at
+    assert (room[m] == 5).all() and (room[:, 0] == 5).all() and (room[:, n + 1:] == 5).all()
+
+
+@pytest.mark.parametrize("group,k", [(32, 2080), (64, 1344), (128, 3584)])
+def test_rows_of_large_weights_do_not_depend_on_the_batch(group: int, k: int) -> None:
+    """As above for 300 rows of weights: with 16400 the rows of a batch pass through every kernel."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"linear_q4 rows alone and in batches, 16400 rows of weights, group {group}")
+    r = rng(group + 1)
+    w = packed(*weight(r, 16400, k, group))
+    x = to_dev(bf16_np(r.normal(size=(300, k))))
+    want = K.linear_q4(x, w, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    for m in (1, 2, 16, 17, 32, 33, 48, 64, 65, 66, 100, 128, 129, 192, 193, 256, 257, 299):
+        for at in (0, 300 - m):
+            got = K.linear_q4(x[at:at + m], w, out_dtype=torch.float32)
+            assert torch.equal(got, want[at:at + m]), (m, at)
