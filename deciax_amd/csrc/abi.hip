@@ -1124,6 +1124,13 @@ int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions, const do
   REQUIRE(!q_norm || eps >= 0.f, "qk_norm_rope: eps must be >= 0");
   SUPPORTED(rows < 1 << 24, "qk_norm_rope: %ld rows beyond the launch grid", (long)rows);
   if (rows == 0 || width == 0) return DX_OK;
+  const int64_t size = 16 / vec, norm_bytes = q_norm ? head_dim * size : 0;
+  auto out_meets = [&](const void *p, int64_t bytes) {
+    return rows_meet(out, rows, out_row_stride * size, width * size, p, bytes);
+  };
+  REQUIRE(!out_meets(positions, 4 * rows) && !out_meets(inv_freq, 4 * (int64_t)rotary_dim) &&
+              !out_meets(q_norm, norm_bytes) && !out_meets(k_norm, norm_bytes),
+          "qk_norm_rope: out must not meet positions, inv_freq or norms");
   const HeadRope a{x, q_norm, k_norm, out, positions, inv_freq, rows, x_row_stride, out_row_stride,
                    num_q_heads, num_kv_heads, head_dim, rotary_dim / 2, eps, attention_factor, interleaved != 0};
   return check_launch(dx_qk_norm_rope_launch(a, dtype == DX_F32, as_stream(stream)), "qk_norm_rope launch");

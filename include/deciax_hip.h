@@ -676,7 +676,7 @@ int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y,
  * src/deciax/models/qwen3_5/text.py:75-91 and `apply_rope`
  * (src/deciax/nn.py:35-44). rotary_dim is a multiple of 16 up to head_dim, rows
  * less than 2^24; fp32 throughout, rounded once to dtype. out is x itself (same row stride) or
- * memory that does not meet it. */
+ * memory that does not meet it, and meets nothing else that the call reads. */
 int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
                     const double *inv_freq, const void *q_norm,
                     const void *k_norm, int64_t rows, int32_t num_q_heads,

@@ -273,3 +273,16 @@ def test_yarn_ramps_over_the_pairs(dim, theta, context, factor, fast, slow) -> N
         share = min(max((j - low) / (high - low), 0.0), 1.0)
         want = theta ** (-2 * j / dim) * ((1 - share) + share / factor)
         assert abs(f - want) < 1e-12 * want, j
+
+
+# 100 rows of 384 of x and out, 4 KB apart; 100 positions, 32 frequencies, norms of 64
+TURNED = dict(x=at(0), out=at(ROWS), pos=at(2 * ROWS), freq=at(2 * ROWS + 512), qn=at(2 * ROWS + 1024), kn=at(2 * ROWS + 1152),
+              rows=100, xs=2048, os=2048)
+
+
+@pytest.mark.parametrize("meeting", [
+    dict(out=at(2 * ROWS)), dict(out=at(2 * ROWS - 99 * 4096 + 384)), dict(pos=at(ROWS - 396)), dict(freq=at(ROWS + 760)),
+    dict(qn=at(ROWS + 4096 - 112)), dict(kn=at(ROWS + 99 * 4096 + 752)), dict(x=at(ROWS), pos=at(ROWS + 764))], ids=str)
+def test_turned_heads_are_not_written_over_what_is_read(meeting) -> None:
+    check(turn(**TURNED | meeting), INVALID)
+    assert b"meet" in _lib.lib().dx_last_error()
