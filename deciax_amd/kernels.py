@@ -1229,6 +1229,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
         raise ValueError("linear_attention: state_out must be state itself or have memory of its own")
     if seqs == 0:
         return out
+    if not 0 <= max_seq_len < 1 << 31:  # a C int would hold another number
+        raise ValueError(f"linear_attention: max_seq_len {max_seq_len} out of range")
     need = _lib.lib().dx_linear_attn_workspace(seqs, max_seq_len, num_heads, k_dim, v_dim)
     spare = 0
     if need > 0 or rows == 0 or states == 0:  # arrays of no rows or no states have no address: the workspace stands in

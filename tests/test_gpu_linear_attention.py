@@ -393,3 +393,14 @@ def test_states_between_the_rows() -> None:
     with pytest.raises(ValueError, match="meet"):
         K.linear_attention(q, k, v, rows.view(-1, 1)[:n], rows, *args, **kw)
     assert torch.equal(room[:, :3 * d], before)
+
+
+@pytest.mark.parametrize("most", [-1, 2 ** 31, 2 ** 32 + 5, 2 ** 40])
+def test_bounds_that_the_c_entry_cannot_hold_are_refused(most: int) -> None:
+    import torch
+
+    from deciax_amd import kernels as K
+
+    x, g, s = torch.zeros((8, 64), device="cuda"), torch.zeros((8, 1), device="cuda"), torch.zeros((1, 1, 64, 64), device="cuda")
+    with pytest.raises(ValueError, match="max_seq_len"):
+        K.linear_attention(x, x, x, g, s, i32([0]), i32([8]), most, num_k_heads=1, num_heads=1, k_dim=64, v_dim=64, scale=0.1)
