@@ -659,7 +659,8 @@ int dx_q4_values(const void *codes, const void *groups, float *w,
  * alignment and must not meet the weight, x rows lie less than 2^24 elements
  * apart. A row of x with an
  * infinity or a NaN, or whose sums of 16 x over a group pass fp32's range, gives
- * infinities or NaN in its own row of y. */
+ * infinities or NaN in its own row of y, a scale of 2^127 or more in its own
+ * column. */
 int dx_linear_q4(const void *x, const void *codes, const void *groups, void *y,
                  int64_t m, int32_t n, int32_t k, int32_t group,
                  int64_t x_row_stride, int64_t y_row_stride, int32_t out_dtype,

@@ -299,3 +299,26 @@ def test_rows_of_large_weights_do_not_depend_on_the_batch(group: int, k: int) ->
         for at in (0, 300 - m):
             got = K.linear_q4(x[at:at + m], w, out_dtype=torch.float32)
             assert torch.equal(got, want[at:at + m]), (m, at)
+
+
+@pytest.mark.parametrize("m", [3, 40, 130])
+def test_largest_scales(m: int) -> None:
+    """Scales below 2^127 are numbers like others; larger ones are lost in their own column of the result alone."""
+    import torch
+
+    from deciax_amd import kernels as K
+
+    say(f"linear_q4 scales of 2^126, {m} rows")
+    r = rng(13)
+    parts = weight(r, 8200, 256, 64)
+    parts[1][5], parts[1][17, 2] = 2.0 ** 126, -(2.0 ** 126)
+    x = bf16_np(r.normal(size=(m, 256)) * 2.0 ** -20)
+    got = K.linear_q4(to_dev(x), packed(*parts), out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    cols = [0, 4, 5, 6, 17, 18, 8199]
+    check(to_np(got)[:, cols], x, tuple(p[cols] for p in parts), False)
+    parts[1][5, 1] = 2.0 ** 127
+    lost = K.linear_q4(to_dev(x), packed(*parts), out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    other = torch.arange(8200, device="cuda") != 5
+    assert torch.equal(lost[:, other], got[:, other])
