@@ -46,7 +46,9 @@ DX_DEVICE void store8(T *p, const float (&x)[8]) {
 // A workgroup takes ROWS rows: their cosines and sines once into LDS, then eight dimensions of a head a thread, a head's
 // D / 8 lanes side by side. A row may be read and written in place: a lane writes what it read, and takes its partner's
 // half from the partner's registers. Bound by the bytes of the rows, each read and written once: 70471 rows of 24 heads of
-// 256 (1.73 GB) 312 us, 5.5 TB/s. A small call is the launch and one chain of loads: 48 rows 5.4 us.
+// 256 (1.73 GB), a quarter of each turned, 311 us, 5.6 TB/s. Turned whole 467: a lane reads eight cosines and sines in a row,
+// and the lanes' reads meet on the same banks of LDS (72% of its cycles). A small call is the launch and one chain of
+// loads: 48 rows 4.9 us, with norms 5.4.
 template <typename T, int D, int ROWS, bool INTERLEAVED>
 __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(HeadRope a) {
   constexpr int LANES = D / 8;
@@ -123,9 +125,9 @@ hipError_t run(const HeadRope &a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// One row a workgroup up to 1024 rows (four would leave CUs without work: 48 rows of 24 heads of 256 5.4 us against 13.4)
-// and where a row keeps the threads busy twice or more (70000 rows 460 us against 467). Narrow rows share the start: 30000
-// of 20 heads of 128 78 us one by one and 61 four at a time, of 6 heads of 64 25 and 14.
+// One row a workgroup up to 1024 rows (four would leave CUs without work: 24 heads of 256, 48 rows 5.4 us against 13.4, 1024
+// 11.2 and 16.0) and where a row keeps the threads busy twice or more (70471 rows, turned whole, 469 us against 471). Narrow
+// rows share the start: 30000 of 20 heads of 128 84 us one by one and 66 four at a time, of 6 heads of 64 28 and 16.
 template <typename T, int D>
 hipError_t by_rows(const HeadRope &a, hipStream_t s) {
   return a.rows <= 1024 || (a.hq + a.hkv) * D >= 4096 ? run<T, D, 1>(a, s) : run<T, D, 4>(a, s);

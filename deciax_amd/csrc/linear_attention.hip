@@ -144,8 +144,9 @@ DX_DEVICE void lds_barrier() {
 // fp32 products (v_mfma_f32_16x16x4_f32: lane l has row or column l % 16 of an operand and k l / 16, and of the result
 // column l % 16, rows 4 (l / 16) + r). Four products take 16 k, of which group l / 16 has 4 (l / 16) .. + 3: rows of LDS are
 // read 16 bytes a lane, and a result tile is the four second operands of the next product as it lies. Wave w has the
-// columns 16 w .. of the state, in registers. Bound by the chain of a sequence's chunks, of which one is about 2.3 us at keys of
-// 64 dimensions: rows are asked for a chunk ahead. 4161 tokens of 3 heads of 64 by 256 75 us; 5 of 3 to 37 tokens 10.
+// columns 16 w .. of the state, in registers. Bound by the chain of a sequence's chunks, of which one is 2.3 to 2.9 us at keys of
+// 64 dimensions: rows are asked for a chunk ahead. 4161 tokens of 3 heads of 64 by 256 60 us, 2111 of 32 heads of 128 by 128
+// 144; 5 sequences of 3 to 37 tokens 10.
 DX_DEVICE floatx4 mfma_f32(float x, float y, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0); }
 
 // Rows as a buffer of n of them: those behind read as zeros and are not written, without a branch. An offset stays below
@@ -370,12 +371,14 @@ DX_DEVICE double chunks(const LinearAttn &a, const Sequence &s, int head, int co
 //     two bf16 parts, since every wave needs all of it.
 //   O^T += S^T Q^T: two tiles of S are eight k of a lane as they lie, again as two bf16 parts; Q is read by the same rows.
 //   S = K^T (w V): both read transposed; w V, w = e^(G_C - G_j), as three bf16 parts: the state keeps fp32's precision.
-// P and S as one part each would be off by 2^-8 of the mass of an output, which the output's own rounding does not hide.
+// P and S as one part each would be off by 2^-8 of the mass of an output (its sums of absolute values), which the output's own
+// rounding does not hide. As two they are off by up to 2^-16 of it: below that rounding unless the terms cancel to less than
+// 2^-8 of them. A third part of both would be some 29% more products.
 //
-// Bound by the wave's own instructions: at keys of 128 dimensions the matrix unit is busy 31% of the time and the vector
-// unit 45% (splitting into parts, decays, addresses), rarely both at once, and the chain of a chunk's phases leaves no more
-// than a tenth idle. 12 sequences of 517 to 16384 tokens, 46000 in all, 32 heads of 128 by 128: 672 us, of which 400 here, 190
-// the segments' own part, 70 the join; without the products for the state 115 less, without stores of outputs 90.
+// Bound by the wave's own instructions: at keys of 128 dimensions the matrix unit is busy 32% of the time and the vector
+// unit 46% (splitting into parts, decays, addresses), both at once 11%; at keys of 256, whose one workgroup a CU has no
+// other beside it, 21%, 27% and 5%. 12 sequences of 517 to 16384 tokens, 46000 in all, 32 heads of 128 by 128: 660 us, of which
+// 400 here, 195 the segments' own part, 60 the join; without the products for the state 115 less, without stores of outputs 90.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -920,8 +923,8 @@ __global__ void __launch_bounds__(THREADS) segment_f32_kernel(LinearAttn a, floa
 }
 
 // In the place of each segment's part the state that it starts from. Four values a thread, four parts on their way together
-// (eight ask for parts that are not there: 40.9 us for 40.0 at 1024 tokens), the decays found once a workgroup; bound by the
-// bytes of the parts: 12 sequences of 517 to 16384 tokens 60 us. Part after part, 8192 tokens take 131 us in all for 123.
+// (eight ask for parts that are not there: 41.3 us in all for 40.3 at 1024 tokens), the decays found once a workgroup; bound
+// by the bytes of the parts: 12 sequences of 517 to 16384 tokens 60 us. Part after part, 8192 tokens take 122 us in all for 121.
 __global__ void __launch_bounds__(THREADS) join_kernel(LinearAttn a, float *parts, const double *sums, int most) {
   constexpr int AT_ONCE = 4;
   __shared__ Factor decay[la::MOST_SEGMENTS];
@@ -995,12 +998,12 @@ hipError_t run(const LinearAttn &a, hipStream_t s) {
   }
   const int most = la::most_segments(a.max_len, la::limit(DK));
   // Columns of a workgroup: 2 COLS share the rows of q and k and their weights, but where COLS make no more workgroups than
-  // there are CUs they are faster (32 heads of 128 by 128, 200 tokens: 1 sequence 20 us against 24, 4 22 and 26, 5 29 and
-  // 27; 12 of 3000 648 and 534). A column's sums are the same.
+  // there are CUs they are faster (32 heads of 128 by 128, 200 tokens: 1 sequence 20 us against 24, 4 22 and 26, 5 28 and
+  // 27; 12 of 3000 727 and 586). A column's sums are the same.
   const bool two = sizeof(T) == 2 && a.dv > COLS && (long)x * most * a.num_seqs > 256;
   if (two) x /= 2;
-  // 2 COLS columns: four waves of 32, two workgroups a CU (12 of 3000: 534 us, eight waves of 16 597); at DK 256, where one
-  // fills the registers, eight of 16 (2111 tokens 86 us, four of 32 101)
+  // 2 COLS columns: four waves of 32, two workgroups a CU (12 of 3000: 581 us, eight waves of 16 664); at DK 256, where one
+  // fills the registers, eight of 16 (2111 tokens 80 us, four of 32 91)
   constexpr int NC = DK == 256 ? 1 : 2, WAVES = DK == 256 ? 8 : 4;
   const dim3 grid(x, most, a.num_seqs), before(x, most - 1, a.num_seqs), block(THREADS), wide(64 * WAVES);
   if (most > 1) {

@@ -161,9 +161,9 @@ DX_DEVICE void join(float (&parts)[WAVES][256], const floatx4 &sum, OUT *y, int 
 
 // Up to 16 rows, TPW tiles of columns a wave: x stays in registers, and the workgroup walks tiles of 16 rows of W, one in
 // `gridDim.x`; the next one's codes are on their way while this one's are multiplied. Bound by the reads of the codes, once
-// there are enough: 4 rows x 256000 x 3584 (481 MB) 91 us, 5.3 TB/s; 1 x 28672 x 3584 12.2 us, half of them the first
-// tile's latency and the launch; 1 x 3584 x 4096 4.3 us, where an empty launch takes 3.4. Without x in registers each tile
-// reads it again: 166 us for the first.
+// there are enough: 4 rows x 256000 x 3584 (481 MB) 92 us, 5.2 TB/s; 1 x 28672 x 3584 12.0 us, half of them the first
+// tile's latency and the launch; 1 x 3584 x 4096 4.3 us, where an empty launch takes 3.4. Read again for each tile of W, x
+// takes the first to 189 us.
 template <int TPW, int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
@@ -200,9 +200,9 @@ linear_q4_few_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ c
 }
 
 // Up to 16 rows and more columns than that: one tile of W a workgroup, codes and x two tiles ahead. Bound by the chain of
-// a wave's tiles (a load's way, the turn, the products): 13 x 3585 x 14336 with groups of 32 11.2 us of 30 MB, 16 x 28672 x
-// 9216 36 us (3.8 TB/s). Codes further ahead take the registers of a second workgroup a CU and unroll more code: four tiles
-// 12.9 and 51 us, eight 13.2 and 66. One ahead 12.4 and 36.5.
+// a wave's tiles (a load's way, the turn, the products): 13 x 3585 x 14336 with groups of 32 11.4 us of 30 MB, 16 x 28672 x
+// 9216 37 us (3.8 TB/s). Codes further ahead take the registers of a second workgroup a CU and unroll more code: four tiles
+// 14.1 and 57 us, eight 15.5 and 79. One ahead 12.6 and 38.2.
 template <int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_long_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
@@ -227,7 +227,7 @@ linear_q4_long_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ 
 #pragma unroll
     for (int d = 0; d < AHEAD; ++d) {  // tiles behind the last add 0
       const int tile = t + d * WAVES;
-      __builtin_amdgcn_sched_barrier(0);  // one tile after the other: both turned at once 12.7 us for 11.2
+      __builtin_amdgcn_sched_barrier(0);  // one tile after the other: both turned at once a tenth more
       u32x4 step[1][4];
       xs[d % AHEAD].turn(turned[wave], step[0], lane);
       xs[d % AHEAD].load(rows, at, tile + AHEAD * WAVES, k, lane);
@@ -283,7 +283,8 @@ struct Block {
 };
 
 // More rows: the eight waves' sums of 16 MT rows and 16 NT columns. Bound by the x that each workgroup reads from L2 and turns
-// and by its waves' chains: 64 rows x 28672 x 3584 41 us, 128 x 3584 x 14336 27, 64 x 8192 x 3584 12.
+// for only 16 NT columns and by its waves' short chains: 17 to 32 rows x 28672 x 3584 22 us, 33 to 64, which read and make the
+// codes bf16 twice, 41 (bf16 weights of that size would take 37 to read); 64 x 8192 x 3584 10.5, 128 x 3584 x 14336 27.
 template <int MT, int NT, int SPG, typename OUT>
 __global__ void __launch_bounds__(THREADS)
 linear_q4_some_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ codes, const uint32_t *__restrict__ words,
@@ -330,7 +331,7 @@ linear_q4_some_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ 
 
 // Many rows: four waves of 16 MT rows each and the same 16 NT columns, each with all eight sums, one after the other. Bound
 // by the vector unit: per tile and wave 128 instructions make the codes bf16 and 32 MT NT / SPG apply the zeros and scales,
-// 4 cycles each, beside 40 products of 16 cycles. 2048 x 8192 x 3584 200 us (600 TFLOP/s); 611 rows with groups of 64 82 us,
+// 4 cycles each, beside 40 products of 16 cycles. 2048 x 8192 x 3584 190 us (630 TFLOP/s); 611 rows with groups of 64 82 us,
 // in 640 workgroups where 512 fit at once (the library's product of bf16 weights of that size takes 40). Larger tiles lose the second
 // workgroup of a CU: 16 MT x 16 NT of 64 x 32, 64 x 64 and 32 x 128 take 125, 125 and 135 us for those 82.
 template <int MT, int NT, int SPG, typename OUT>
@@ -387,7 +388,8 @@ linear_q4_many_kernel(const uint16_t *__restrict__ x, const u32x4 *__restrict__ 
 }
 
 // A wave lays out one tile: lane 16 q + r the codes that the products read as its.
-// Once a weight, so it is not tuned.
+// Once a weight, so it is not tuned: one of 28672 x 3584 is quantised in 70 us, packed from a byte a code in 192 and read as
+// fp32 in 108, where the bytes alone take 46, 28 and 83.
 struct Place {
   int row, col;  // of the lane's first value of step 0
   bool in;       // the row exists
@@ -553,8 +555,8 @@ hipError_t run_many(const Q4Weight &w, const uint16_t *x, void *y, long m, long 
 }
 
 // Two workgroups a CU where their registers fit (up to four tiles of x a wave) and each still has four tiles of W or more;
-// else one, with more of them: 40000 columns of 2048 9.7 us with two and 10.6 with one, 256000 of 3584 92 and 101, but 8192
-// of 3584 6.2 and 5.6.
+// else one, with more of them: 40000 columns of 2048 9.9 us with two and 10.9 with one, 256000 of 3584 96 and 108, but 8192
+// of 3584 6.4 and 5.8.
 template <int TPW, int SPG>
 hipError_t run_few(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
   const int tiles = dx_ceil_div(w.n, 16), most = TPW <= 4 && tiles > 2048 ? 512 : 256;
@@ -583,14 +585,14 @@ hipError_t run_long(const Q4Weight &w, const uint16_t *x, void *y, long m, long 
   return hipGetLastError();
 }
 
-// Up to 16 rows: x in registers up to 8192 columns (28672 rows of W: 2048 columns 7.7 us against 11.8 with x read again,
-// 8192 23 against 28), but where each workgroup has one tile of W anyway and more than 4096 columns not (3584 rows of W and
-// 8192 columns, 16 rows of x: 7.7 against 6.6 read as it is multiplied; 2048 columns 3.4 against 3.7).
+// Up to 16 rows: x in registers up to 8192 columns (28672 rows of W: 2048 columns 8.6 us against 13.0 with x read again,
+// 8192 28 against 33), but where each workgroup has one tile of W anyway and more than 4096 columns not (3584 rows of W and
+// 8192 columns, 16 rows of x: 7.3 against 6.8 read as it is multiplied; 2048 columns 3.6 against 3.7).
 //
 // More: tiles of 128 x 64 where there is one for every CU and more than half of their rows are in use, else eight waves a
-// tile (us of the one and the other: 128 x 16384 x 3584 34 and 39, 128 x 28672 x 3584 51 and 73, 611 x 8192 x 3584 85 and
-// 102, but 200 x 3584 x 4096 37 and 18, 64 x 28672 x 3584 43 and 40). These of 32 x 64, or of 32 x 32 where the smaller ones
-// are no more than the CUs (17 x 3584 x 4096 9.5 and 8.4, 32 x 8192 x 3584 10.0 and 8.5, but 64 x 8192 x 3584 11.7 and 14.5).
+// tile (us of the one and the other: 128 x 16384 x 3584 37 and 39, 128 x 28672 x 3584 50 and 73, 611 x 8192 x 3584 83 and
+// 100, but 200 x 3584 x 4096 37 and 18, 64 x 28672 x 3584 43 and 41). These of 32 x 64, or of 32 x 32 where the smaller ones
+// are no more than the CUs (17 x 3584 x 4096 9.4 and 8.0, 32 x 8192 x 3584 10.0 and 8.5, but 64 x 8192 x 3584 10.9 and 12.9).
 template <int SPG>
 hipError_t by_rows(const Q4Weight &w, const uint16_t *x, void *y, long m, long ldx, long ldy, bool f32, hipStream_t s) {
   const int tiles = dx_ceil_div(w.k, 128 * WAVES);  // of a wave
