@@ -710,9 +710,10 @@ int dx_qk_norm_rope(const void *x, void *out, const int32_t *positions,
  * starts from, has to stay within fp32's range, with scale and without, and
  * for bf16 rows states and products with k within bf16's; v may be any finite
  * number. There bf16 rows' outputs are off by up to 2^-16 of the same sums of
- * absolute values, beside their own rounding; states keep fp32's precision.
- * max_seq_len bounds the grid: longer device
- * lengths are cut to it. Row strides stay below 2^24 elements, decay's
+ * absolute values, beside their own rounding; states keep fp32's precision for
+ * values of v from 2^-100 on. A decay of less than 2^-126 between two tokens of
+ * a chunk counts as 0. max_seq_len bounds the grid: longer device lengths are
+ * cut to it. Row strides stay below 2^24 elements, decay's
  * below 2^22. Workspace size from dx_linear_attn_workspace. */
 int dx_linear_attn(const void *q, const void *k, const void *v,
                    const float *decay, void *out, const float *state_in,

@@ -404,3 +404,14 @@ def test_bounds_that_the_c_entry_cannot_hold_are_refused(most: int) -> None:
     x, g, s = torch.zeros((8, 64), device="cuda"), torch.zeros((8, 1), device="cuda"), torch.zeros((1, 1, 64, 64), device="cuda")
     with pytest.raises(ValueError, match="max_seq_len"):
         K.linear_attention(x, x, x, g, s, i32([0]), i32([8]), most, num_k_heads=1, num_heads=1, k_dim=64, v_dim=64, scale=0.1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_small_values_keep_their_precision(dtype: str) -> None:
+    """Values around 2^-100 beside large keys: the parts that they are split into are numbers of full precision still."""
+    say(f"linear_attention small values {dtype}")
+    c = Case(17, [5, 64, 200, 900], 1, 2, 64, 128, dtype)
+    c.v = np.sign(c.v) * bf16_np((np.abs(c.v) + 1) * 2.0 ** -100)
+    c.k = bf16_np(c.k * 2.0 ** 50)
+    c.state = (c.state * 2.0 ** -50).astype(np.float32)
+    c.check(*c.run())
